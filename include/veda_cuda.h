@@ -232,6 +232,45 @@ int veda_cross_entropy(const void* logits, int64_t ldl, const int64_t* targets, 
 int veda_mean_f64(const float* v, int64_t n, float* out, double* out_f64, veda_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------- */
+/* The loss head without stored logits: cross_entropy(matmul_nt(x, w), targets)              */
+/* (src/libs/autograd/Variable.cpp:325-346, Loss.cpp:18-103) with the vocabulary in pieces.   */
+/* x [rows, dim] and w [vocab, dim] in dtype, targets [rows]. A row whose target is           */
+/* ignore_index, or lies outside [0, vocab), is not counted: its loss and gradients are 0. A  */
+/* target outside the vocabulary that is not ignore_index also sets *status (device int, may  */
+/* be NULL) to VEDA_ERR_OUT_OF_RANGE. With no counted row the loss and the gradients are 0.   */
+/*   fwd: lse[r] = log sum_v exp z[r, v], row_loss[r] = lse[r] - z[r, t_r], loss[0] = the mean  */
+/*        over the counted rows, all fp32; lse and loss may be NULL. What a row that is not     */
+/*        counted holds (NaN included) reaches no other row and no gradient.                    */
+/*   bwd: with q = exp(z - lse) - onehot(t) and coef = upstream[0] / counted rows (upstream:  */
+/*        device float, NULL = 1), dx = coef q w in dtype (overwritten) and dw = coef q^T x + */
+/*        beta_dw dw in dtype_dw (VEDA_F32, or VEDA_BF16 for bf16 operands; beta_dw 0 or 1).  */
+/*        lse is the forward's. dx or dw may be NULL. In bf16, q is rounded to bf16 before    */
+/*        the gradient products, as veda_cross_entropy's dlogits are.                         */
+/* Operands: any pitch >= dim and any element-aligned base; where a base is not 16-byte       */
+/* aligned or a pitch no multiple of 8 (bf16; always for fp32) an operand is laid out in the  */
+/* workspace first. The workspace (256-byte aligned, contents undefined before and after) is  */
+/* sized by veda_linear_cross_entropy_workspace; pass a pitch of 1 for an operand whose base  */
+/* is not 16-byte aligned. The largest size with backward = 0 and 1 serves both calls. Results */
+/* repeat bit for bit. fp32 operands are multiplied on the tensor cores as pairs of fp16      */
+/* values (22 bits); magnitudes below 2^-39 of an operand's largest, and of q below 2^-38,    */
+/* are lost.                                                                                  */
+/* ---------------------------------------------------------------------------------------- */
+size_t veda_linear_cross_entropy_workspace(int64_t rows, int64_t vocab, int64_t dim, int64_t ldx,
+                                           int64_t ldw, int dtype, int backward);
+int veda_linear_cross_entropy_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                  const int64_t* targets, int64_t ignore_index, float* row_loss,
+                                  float* lse, float* loss, int64_t rows, int64_t vocab, int64_t dim,
+                                  void* workspace, size_t workspace_bytes, int* status, int dtype,
+                                  veda_stream_t stream);
+int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                  const int64_t* targets, int64_t ignore_index, const float* lse,
+                                  const float* upstream, void* dx, int64_t lddx, void* dw,
+                                  int64_t lddw, int dtype_dw, float beta_dw, int64_t rows,
+                                  int64_t vocab, int64_t dim, void* workspace,
+                                  size_t workspace_bytes, int* status, int dtype,
+                                  veda_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------- */
 /* Embedding (autograd::embedding, src/libs/autograd/NonLinear.cpp:203-254).                  */
 /* ---------------------------------------------------------------------------------------- */
 /* out[p] = table[ids[p]], bit-exact. An id outside [0, vocab) writes zeros and sets *status

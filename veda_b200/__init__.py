@@ -69,6 +69,11 @@ SIGNATURES = {
                              _p]),
     "veda_cross_entropy": (_i, [_p, _i64, _p, _p, _p, _i64, _i64, _i64, _f, _p, _i, _p]),
     "veda_mean_f64": (_i, [_p, _i64, _p, _p, _p]),
+    "veda_linear_cross_entropy_workspace": (_sz, [_i64, _i64, _i64, _i64, _i64, _i, _i]),
+    "veda_linear_cross_entropy_fwd": (_i, [_p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _i64,
+                                           _p, _sz, _p, _i, _p]),
+    "veda_linear_cross_entropy_bwd": (_i, [_p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _i64,
+                                           _i, _f, _i64, _i64, _i64, _p, _sz, _p, _i, _p]),
     "veda_embedding_fwd": (_i, [_p, _i64, _p, _i64, _i64, _p, _i64, _p, _i, _p]),
     "veda_embedding_bwd": (_i, [_p, _i64, _p, _i64, _i64, _i64, _p, _i, _p, _sz, _i, _p]),
     "veda_embedding_bwd_workspace": (_sz, [_i64]),

@@ -1,0 +1,1169 @@
+// The loss head in one operator: z = x W^T over the vocabulary, softmax cross-entropy against the
+// targets, and the gradients of x and W, without the [rows, vocab] logits ever being stored.
+//
+// The composition autograd::matmul_nt + autograd::cross_entropy of the reference
+// (src/libs/autograd/Variable.cpp:325-346, Loss.cpp:18-103), which keeps logits, log-probabilities
+// and probabilities of the whole block. With lse_n = log sum_v exp z_nv and the rows whose target
+// is counted:
+//   forward   loss_n = lse_n - z_n[t_n], loss = mean over the counted rows. One pass over 256 x 256
+//             logit tiles in tensor memory; a thread owns a row and keeps the running maximum and
+//             the running sum of exponentials (fp32, log2 units) over a strip of tiles, so a row
+//             leaves (max, sum) pairs only, which a second launch merges.
+//   backward  q = exp(z - lse) - onehot(t), formed piece by piece of the vocabulary from z computed
+//             again (the price of not keeping it), dx = coef q W, dW = coef q^T x with
+//             coef = upstream / counted rows. A piece of q stays in L2: the launch that multiplies
+//             piece c into dx and dW computes piece c + 1 beside it.
+// q is stored without coef, so its largest entry, about -1 at the target, keeps its bits when
+// rounded to bf16 whatever the row count; coef is applied to the fp32 sums. The sums over the
+// vocabulary (dx) are held in an fp32 buffer, added piece by piece in order: no atomics meet on an
+// element within a launch, so results repeat bit for bit.
+//
+// fp32 operands: each is split into two fp16 planes, value 2^e = hi + lo (22 bits, e chosen from
+// the tensor's largest finite value), and a product becomes hi hi + hi lo + lo hi on the same tiles
+// with three times the k-blocks; lo lo is below the 22nd bit. fp32 CUDA-core products run at a
+// twentieth of the tensor cores' rate, so three tensor products are still far cheaper.
+#include "pair_mma.cuh"
+
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cfloat>
+
+namespace veda::cuda
+{
+int* device_status_ptr();
+
+namespace lce
+{
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kQScale = 8192.0f;   // of the split q planes: |q| <= 1 becomes at most 2^13
+
+// 2^x with the hardware approximation (relative error ~2^-22; -inf -> 0)
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Device scalars of a call: what turns a tile's sum into a logit, and the gradients' factors. The
+// powers of two stay apart from coef: their product with it could be subnormal where dx is not.
+struct Scalars
+{
+    float z;                // 2^-(ex + ew) of split operands, else 1
+    float coef;             // upstream / counted rows
+    float unit_dx, unit_dw; // 2^-(13 + ew), 2^-(13 + ex) of split operands, else 1
+    float x, w;             // 2^ex, 2^ew of split operands
+};
+
+struct Params
+{
+    CUtensorMap x, w;        // operands [rows, dim], [vocab, dim]; plane 1: the lo halves
+    CUtensorMap q_in;        // piece of q read by the gradient products
+    CUtensorMap q_out;       // piece of q written (store boxes)
+    CUtensorMap dx, dw;      // fp32 sums of dx; dW (store boxes)
+    int rows, vocab, dim;
+    int segments;            // products per pair of operands: 1, or 3 (split)
+    int is_bf16;
+    int num_m;               // row tiles
+    // logits of this launch: vocabulary rows v0 .. v0 + 256 num_n
+    int v0, num_n, strip;
+    // gradient products of this launch: q_in holds vocabulary rows g0 .. g0 + gcols
+    int g0, gcols, num_d, dw_tiles, dx_tiles;
+    int dx_add;              // dx sums: 0 store, 1 add
+    int dw_mode;             // 0: from registers; 1: TMA store; 2: TMA add (fp32)
+    int dw_f32, dw_beta;
+    void* dw_ptr;
+    int64_t lddw;
+    const Scalars* scalars;
+    const int64_t* targets;
+    int64_t ignore;
+    const float* lse;
+    float2* parts;           // [strip slots][rows] running (max, sum)
+    float* target_logit;     // [rows]
+    int* status;
+};
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b)
+{
+    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b)
+{
+    const __half2 t = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
+__device__ __forceinline__ float f16_lo(uint32_t w)
+{
+    return __low2float(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ float f16_hi(uint32_t w)
+{
+    return __high2float(*reinterpret_cast<const __half2*>(&w));
+}
+
+// A row's counted target, -1 for a row that is ignored, out of the vocabulary or past the end.
+__device__ __forceinline__ int counted_target(const Params& p, int row)
+{
+    if (row >= p.rows)
+    {
+        return -1;
+    }
+    const int64_t t = p.targets[row];
+    return t == p.ignore || t < 0 || t >= p.vocab ? -1 : static_cast<int>(t);
+}
+
+// The operand planes of segment s of a split product: hi hi, hi lo, lo hi.
+__device__ __forceinline__ void planes_of(int segment, int& za, int& zb)
+{
+    za = segment == 2 ? 1 : 0;
+    zb = segment == 1 ? 1 : 0;
+}
+
+// ---- forward: running (max, sum) per row over strips of logit tiles ---------------------------
+struct StatsWork
+{
+    using Params = lce::Params;
+    struct Tile
+    {
+        bool skip, first, last, a_mn, b_mn;
+        int kbs, mb, nb, slot;
+        uint32_t idesc;
+    };
+    struct State
+    {
+        float m, s;
+        int target;
+    };
+
+    // Strips run with the row tile fastest: the clusters working at one time share a few strips of
+    // the head, which therefore comes from HBM once, while the rows stay in L2.
+    static __device__ __forceinline__ bool tile(const Params& p, int cid, int clusters, int i, Tile& t)
+    {
+        const int strips = (p.num_n + p.strip - 1) / p.strip;
+        const int unit = cid + i / p.strip * clusters;
+        if (unit >= strips * p.num_m)
+        {
+            return false;
+        }
+        const int sub = i % p.strip;
+        t.slot = unit / p.num_m;
+        t.mb = unit - t.slot * p.num_m;
+        t.nb = t.slot * p.strip + sub;
+        t.skip = t.nb >= p.num_n;
+        t.first = sub == 0;
+        t.last = sub == p.strip - 1 || t.nb == p.num_n - 1;
+        t.kbs = (p.dim + pair::kBK - 1) / pair::kBK * p.segments;
+        t.a_mn = t.b_mn = false;
+        t.idesc = pair::idesc(p.is_bf16 != 0, false, false);
+        return true;
+    }
+
+    static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, int kb,
+                                                    pair::Piece& a, pair::Piece& b)
+    {
+        const int per = (p.dim + pair::kBK - 1) / pair::kBK;
+        const int seg = kb / per;
+        const int k = (kb - seg * per) * pair::kBK;
+        int za, zb;
+        planes_of(seg, za, zb);
+        a = {&p.x, k, t.mb * pair::kTile + rank * 128, za};
+        b = {&p.w, k, p.v0 + t.nb * pair::kTile + rank * 128, zb};
+    }
+
+    static __device__ __forceinline__ void before(const Params& p, const Tile& t, State& s, int row0, int,
+                                                  int lane)
+    {
+        if (t.first)
+        {
+            s.m = -INFINITY;
+            s.s = 0.0f;
+            s.target = counted_target(p, t.mb * pair::kTile + row0 + lane);
+        }
+    }
+
+    template <int COLS>
+    static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, State& s, uint32_t taddr,
+                                                    int row0, int col0, pair::Staging&, int lane)
+    {
+        if (t.mb * pair::kTile + row0 >= p.rows)
+        {
+            return;
+        }
+        const int row = t.mb * pair::kTile + row0 + lane;
+        const int first = p.v0 + t.nb * pair::kTile + col0;
+        const float zs = p.segments > 1 ? p.scalars->z : 1.0f;
+#pragma unroll 1
+        for (int c = 0; c < COLS; c += 32)
+        {
+            const int left = p.vocab - first - c;   // columns of this chunk inside the vocabulary
+            if (left <= 0)
+            {
+                break;
+            }
+            uint32_t r[32];
+            tc::tmem_ld32(taddr + static_cast<uint32_t>(c), r);
+            float z[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+            {
+                z[j] = __uint_as_float(r[j]);
+            }
+            if (p.segments > 1)
+            {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) z[j] *= zs;
+            }
+            if (left < 32)
+            {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) z[j] = j < left ? z[j] : -INFINITY;
+            }
+            const int at = s.target - first - c;
+            if (__any_sync(0xFFFFFFFFu, at >= 0 && at < 32))
+            {
+                float zt = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) zt = j == at ? z[j] : zt;
+                if (at >= 0 && at < 32)
+                {
+                    p.target_logit[row] = zt;
+                }
+            }
+            float mx[4] = {z[0], z[1], z[2], z[3]};
+#pragma unroll
+            for (int j = 4; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], z[j]);
+            const float m = fmaxf(s.m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e);
+            // a row of -inf so far: any finite reference gives exponentials of 0, and NaN stays NaN
+            const float ref = m == -INFINITY ? 0.0f : m;
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum[j & 3] += ex2(fmaf(z[j], kLog2e, -ref));
+            s.s = s.s * ex2(s.m - ref) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+            s.m = m;
+        }
+        if (t.last && row < p.rows)
+        {
+            const int halves = pair::kTile / COLS;
+            p.parts[static_cast<int64_t>(t.slot * halves + col0 / COLS) * p.rows + row] = make_float2(s.m, s.s);
+        }
+    }
+};
+
+// ---- backward: the next piece of q beside the current piece's two products --------------------
+struct GradWork
+{
+    using Params = lce::Params;
+    enum Kind { kDw, kDx, kQ };
+    struct Tile
+    {
+        bool skip, a_mn, b_mn;
+        int kind, kbs, mb, nb;
+        uint32_t idesc;
+    };
+    struct State
+    {
+        float lse2, keep;
+        int target;
+    };
+
+    // Longest tiles first: dW (k runs over the rows), dx (over the piece), then q (over dim).
+    static __device__ __forceinline__ bool tile(const Params& p, int cid, int clusters, int i, Tile& t)
+    {
+        int u = cid + i * clusters;
+        t.skip = false;
+        const bool bf = p.is_bf16 != 0;
+        if (u < p.dw_tiles)
+        {
+            t.kind = kDw;
+            t.mb = u / p.num_d;
+            t.nb = u - t.mb * p.num_d;
+            t.kbs = (p.rows + pair::kBK - 1) / pair::kBK * p.segments;
+            t.a_mn = t.b_mn = true;
+            t.idesc = pair::idesc(bf, true, true);
+            return true;
+        }
+        u -= p.dw_tiles;
+        if (u < p.dx_tiles)
+        {
+            t.kind = kDx;
+            t.mb = u / p.num_d;
+            t.nb = u - t.mb * p.num_d;
+            t.kbs = (p.gcols + pair::kBK - 1) / pair::kBK * p.segments;
+            t.a_mn = false;
+            t.b_mn = true;
+            t.idesc = pair::idesc(bf, false, true);
+            return true;
+        }
+        u -= p.dx_tiles;
+        if (u >= p.num_m * p.num_n)
+        {
+            return false;
+        }
+        t.kind = kQ;
+        t.nb = u / p.num_m;
+        t.mb = u - t.nb * p.num_m;
+        t.kbs = (p.dim + pair::kBK - 1) / pair::kBK * p.segments;
+        t.a_mn = t.b_mn = false;
+        t.idesc = pair::idesc(bf, false, false);
+        return true;
+    }
+
+    static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, int kb,
+                                                    pair::Piece& a, pair::Piece& b)
+    {
+        const int per = p.segments > 1 ? t.kbs / p.segments : t.kbs;
+        const int seg = p.segments > 1 ? kb / per : 0;
+        const int k = (kb - seg * per) * pair::kBK;
+        const int m = t.mb * pair::kTile + rank * 128, n = t.nb * pair::kTile + rank * 128;
+        int za, zb;
+        planes_of(seg, za, zb);
+        if (t.kind == kDw)
+        {
+            a = {&p.q_in, m, k, za};
+            b = {&p.x, n, k, zb};
+        }
+        else if (t.kind == kDx)
+        {
+            a = {&p.q_in, k, m, za};
+            b = {&p.w, n, p.g0 + k, zb};
+        }
+        else
+        {
+            a = {&p.x, k, m, za};
+            b = {&p.w, k, p.v0 + n, zb};
+        }
+    }
+
+    static __device__ __forceinline__ void before(const Params& p, const Tile& t, State& s, int row0, int,
+                                                  int lane)
+    {
+        if (t.kind == kQ)
+        {
+            const int row = t.mb * pair::kTile + row0 + lane;
+            s.target = counted_target(p, row);
+            s.lse2 = s.target >= 0 ? p.lse[row] * kLog2e : 0.0f;
+        }
+    }
+
+    template <int COLS>
+    static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, State& s, uint32_t taddr,
+                                                    int row0, int col0, pair::Staging& st, int lane)
+    {
+        if (t.kind == kQ)
+        {
+            epilogue_q<COLS>(p, t, s, taddr, row0, col0, st, lane);
+        }
+        else
+        {
+            epilogue_grad<COLS>(p, t, taddr, row0, col0, st, lane);
+        }
+    }
+
+    // q of the tile's rows, 64 columns at a time: 0 in ignored rows and past the vocabulary.
+    template <int COLS>
+    static __device__ __forceinline__ void epilogue_q(const Params& p, const Tile& t, const State& s,
+                                                      uint32_t taddr, int row0, int col0, pair::Staging& st,
+                                                      int lane)
+    {
+        const int trow = t.mb * pair::kTile + row0;
+        if (trow >= p.rows)
+        {
+            return;
+        }
+        const float zs = p.segments > 1 ? p.scalars->z * kLog2e : kLog2e;
+        const float scale = p.segments > 1 ? kQScale : 1.0f;
+#pragma unroll 1
+        for (int c = 0; c < COLS; c += 64)
+        {
+            const int col = t.nb * pair::kTile + col0 + c;   // within the piece
+            const int left = p.vocab - p.v0 - col;
+            uint32_t hi[32], lo[32];
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+            {
+                uint32_t r[32];
+                tc::tmem_ld32(taddr + static_cast<uint32_t>(c + 32 * half), r);
+                const int at = s.target - p.v0 - col - 32 * half;
+                const bool plain = left >= 64 && !__any_sync(0xFFFFFFFFu, s.target < 0 || (at >= 0 && at < 32));
+                float q[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) q[j] = ex2(fmaf(__uint_as_float(r[j]), zs, -s.lse2));
+                if (!plain)
+                {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                    {
+                        const float v = j == at ? q[j] - 1.0f : q[j];
+                        q[j] = s.target >= 0 && 32 * half + j < left ? v : 0.0f;
+                    }
+                }
+                if (p.segments > 1)
+                {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                    {
+                        const float a = q[2 * j] * scale, b = q[2 * j + 1] * scale;
+                        const uint32_t h = pack_f16(a, b);
+                        hi[16 * half + j] = h;
+                        lo[16 * half + j] = pack_f16(a - f16_lo(h), b - f16_hi(h));
+                    }
+                }
+                else
+                {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) hi[16 * half + j] = pack_bf16(q[2 * j], q[2 * j + 1]);
+                }
+            }
+            send(p, hi, col, trow, 0, st, lane);
+            if (p.segments > 1)
+            {
+                send(p, lo, col, trow, 1, st, lane);
+            }
+        }
+    }
+
+    static __device__ __forceinline__ void send(const Params& p, const uint32_t (&w)[32], int col, int row,
+                                                int plane, pair::Staging& st, int lane)
+    {
+        uint8_t* buf = st.buffer(lane);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+        {
+            *reinterpret_cast<uint4*>(buf + tc::sw128_offset(lane, k)) =
+                make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+        }
+        tc::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0)
+        {
+            tc::tma_store_3d(&p.q_out, buf, col, row, plane);
+            tc::bulk_commit_group();
+        }
+        st.sent();
+    }
+
+    // dx: the fp32 sums as they are. dW: times coef, rounded once to its type.
+    template <int COLS>
+    static __device__ __forceinline__ void epilogue_grad(const Params& p, const Tile& t, uint32_t taddr,
+                                                         int row0, int col0, pair::Staging& st, int lane)
+    {
+        const bool dw = t.kind == kDw;
+        const int trow = t.mb * pair::kTile + row0;   // within the piece for dW
+        if (trow >= (dw ? p.gcols : p.rows))
+        {
+            return;
+        }
+        const float coef = dw ? p.scalars->coef : 1.0f, unit = dw ? p.scalars->unit_dw : 1.0f;
+        const bool f32 = !dw || p.dw_f32;
+        const int step = f32 ? 32 : 64;
+        const int mode = dw ? p.dw_mode : 1 + p.dx_add;
+        const int orow = dw ? p.g0 + trow : trow;
+#pragma unroll 1
+        for (int c = 0; c < COLS; c += step)
+        {
+            const int col = t.nb * pair::kTile + col0 + c;
+            if (col >= p.dim)
+            {
+                break;
+            }
+            uint32_t r[32], r2[32];
+            tc::tmem_ld32(taddr + static_cast<uint32_t>(c), r);
+            if (!f32)
+            {
+                tc::tmem_ld32(taddr + static_cast<uint32_t>(c + 32), r2);
+            }
+            if (mode == 0)
+            {
+                store_direct(p, r, orow + lane, col, trow + lane, unit, coef);
+                if (!f32)
+                {
+                    store_direct(p, r2, orow + lane, col + 32, trow + lane, unit, coef);
+                }
+                continue;
+            }
+            uint8_t* buf = st.buffer(lane);
+            if (f32)
+            {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                {
+                    float4 o = make_float4(__uint_as_float(r[4 * k]), __uint_as_float(r[4 * k + 1]),
+                                           __uint_as_float(r[4 * k + 2]), __uint_as_float(r[4 * k + 3]));
+                    if (dw)
+                    {
+                        o = make_float4(o.x * unit * coef, o.y * unit * coef, o.z * unit * coef, o.w * unit * coef);
+                    }
+                    *reinterpret_cast<float4*>(buf + tc::sw128_offset(lane, k)) = o;
+                }
+            }
+            else
+            {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                    {
+                        const int j = 8 * (k & 3) + 2 * q;
+                        const uint32_t a = k < 4 ? r[j] : r2[j], b = k < 4 ? r[j + 1] : r2[j + 1];
+                        w[q] = pack_bf16(__uint_as_float(a) * coef, __uint_as_float(b) * coef);
+                    }
+                    *reinterpret_cast<uint4*>(buf + tc::sw128_offset(lane, k)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            tc::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0)
+            {
+                const CUtensorMap* map = dw ? &p.dw : &p.dx;
+                if (mode == 2)
+                {
+                    pair::reduce_add_3d(map, buf, col, orow, 0);
+                }
+                else
+                {
+                    tc::tma_store_3d(map, buf, col, orow, 0);
+                }
+                tc::bulk_commit_group();
+            }
+            st.sent();
+        }
+    }
+
+    // A dW row piece whose pitch or base TMA cannot describe, or bf16 accumulation.
+    static __device__ __forceinline__ void store_direct(const Params& p, const uint32_t (&r)[32], int row,
+                                                        int col, int piece_row, float unit, float coef)
+    {
+        if (piece_row >= p.gcols)
+        {
+            return;
+        }
+        const int64_t at = static_cast<int64_t>(row) * p.lddw + col;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+        {
+            if (col + j < p.dim)
+            {
+                float v = __uint_as_float(r[j]) * unit * coef;
+                if (p.dw_f32)
+                {
+                    float* d = static_cast<float*>(p.dw_ptr) + at + j;
+                    *d = p.dw_beta ? *d + v : v;
+                }
+                else
+                {
+                    bf16* d = static_cast<bf16*>(p.dw_ptr) + at + j;
+                    *d = __float2bfloat16_rn(p.dw_beta ? __bfloat162float(*d) + v : v);
+                }
+            }
+        }
+    }
+};
+
+// ---- the small launches around them ------------------------------------------------------------
+constexpr int kMaxBlocks = 296;   // partial maxima of an operand
+
+__device__ __forceinline__ bool counted(int64_t t, int64_t ignore, int64_t vocab)
+{
+    return t != ignore && t >= 0 && t < vocab;
+}
+
+// Largest finite magnitude of the counted rows of x (blocks below gx) and of w (the others) as one
+// partial per block.
+__global__ void __launch_bounds__(256)
+absmax_kernel(const float* __restrict__ x, int64_t ldx, int64_t rows, const float* __restrict__ w, int64_t ldw,
+              int64_t vocab, int64_t dim, const int64_t* __restrict__ targets, int64_t ignore, int gx,
+              float* __restrict__ part)
+{
+    __shared__ float warp_part[8];
+    dep_wait();
+    dep_release();
+    const bool is_w = static_cast<int>(blockIdx.x) >= gx;
+    const float* m = is_w ? w : x;
+    const int64_t ld = is_w ? ldw : ldx, n = is_w ? vocab : rows;
+    const int64_t b = is_w ? blockIdx.x - gx : blockIdx.x, blocks = is_w ? gridDim.x - gx : gx;
+    float top = 0.0f;
+    for (int64_t r = b * 8 + threadIdx.x / 32; r < n; r += blocks * 8)
+    {
+        if (!is_w && !counted(targets[r], ignore, vocab))
+        {
+            continue;
+        }
+        for (int64_t c = threadIdx.x & 31; c < dim; c += 32)
+        {
+            const float v = fabsf(m[r * ld + c]);
+            top = v <= FLT_MAX ? fmaxf(top, v) : top;
+        }
+    }
+    top = warp_max(top);
+    if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x == 0)
+    {
+        for (int k = 1; k < 8; ++k) top = fmaxf(top, warp_part[k]);
+        part[blockIdx.x] = top;
+    }
+}
+
+// 2^e that brings a largest magnitude into [2^13, 2^14), clamped so that 2^e and 2^-e are normal
+// (a tensor of magnitudes below 2^-113 keeps fewer bits).
+__device__ __forceinline__ float split_scale(float top)
+{
+    if (top == 0.0f)
+    {
+        return 1.0f;
+    }
+    int e;
+    frexpf(top, &e);   // top = f 2^e, f in [1/2, 1)
+    e = 14 - e;
+    return ldexpf(1.0f, e < -120 ? -120 : e > 120 ? 120 : e);
+}
+
+// The call's scalars: split scales from the partial maxima, and upstream / counted rows.
+__global__ void __launch_bounds__(1024)
+scalars_kernel(const int64_t* __restrict__ targets, int64_t ignore, int64_t rows, int64_t vocab,
+               const float* __restrict__ upstream, const float* __restrict__ part, int gx, int gw,
+               Scalars* out, int* status)
+{
+    __shared__ int counts[32];
+    __shared__ float tops[2];
+    dep_wait();
+    dep_release();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int n = 0, bad = 0;
+    for (int64_t i = threadIdx.x; i < rows; i += blockDim.x)
+    {
+        const int64_t t = targets[i];
+        if (t != ignore)
+        {
+            t >= 0 && t < vocab ? ++n : ++bad;
+        }
+    }
+    n = __reduce_add_sync(0xFFFFFFFFu, n);
+    if (__any_sync(0xFFFFFFFFu, bad != 0) && lane == 0 && status != nullptr)
+    {
+        *status = VEDA_ERR_OUT_OF_RANGE;
+    }
+    if (lane == 0) counts[warp] = n;
+    if (part != nullptr && warp < 2)
+    {
+        float top = 0.0f;
+        for (int i = lane; i < (warp == 0 ? gx : gw); i += 32) top = fmaxf(top, part[(warp == 0 ? 0 : gx) + i]);
+        top = warp_max(top);
+        if (lane == 0) tops[warp] = top;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0)
+    {
+        int total = 0;
+        for (int k = 0; k < 32; ++k) total += counts[k];
+        // no counted row: the loss and every gradient are zero
+        const float coef = total > 0 ? (upstream != nullptr ? *upstream : 1.0f) / static_cast<float>(total) : 0.0f;
+        Scalars s{1.0f, coef, 1.0f, 1.0f, 1.0f, 1.0f};
+        if (part != nullptr)
+        {
+            s.x = split_scale(tops[0]);
+            s.w = split_scale(tops[1]);
+            s.z = 1.0f / s.x / s.w;
+            s.unit_dx = 1.0f / kQScale / s.w;
+            s.unit_dw = 1.0f / kQScale / s.x;
+        }
+        *out = s;
+    }
+}
+
+// Operand planes of x (blocks below gx) and w with a pitch of a multiple of 8 elements: a bf16 copy,
+// or the two fp16 halves of an fp32 operand. clear: rows of x that are not counted become zeros, so
+// that what padding holds (NaN included) meets q = 0 in dW's product as 0.
+template <typename T>
+__global__ void __launch_bounds__(256)
+pack_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, const T* __restrict__ w, int64_t ldw,
+            int64_t vocab, int64_t dim, const int64_t* __restrict__ targets, int64_t ignore, bool clear, int gx,
+            uint16_t* __restrict__ px, uint16_t* __restrict__ pw, int64_t ldp, const Scalars* __restrict__ scalars)
+{
+    dep_wait();
+    dep_release();
+    const bool is_w = static_cast<int>(blockIdx.x) >= gx;
+    const T* m = is_w ? w : x;
+    uint16_t* out = is_w ? pw : px;
+    const int64_t ld = is_w ? ldw : ldx, n = is_w ? vocab : rows;
+    const int64_t b = is_w ? blockIdx.x - gx : blockIdx.x, blocks = is_w ? gridDim.x - gx : gx;
+    const float scale = sizeof(T) == 4 ? (is_w ? scalars->w : scalars->x) : 1.0f;
+    for (int64_t r = b * 8 + threadIdx.x / 32; r < n; r += blocks * 8)
+    {
+        const bool keep = is_w || !clear || counted(targets[r], ignore, vocab);
+        for (int64_t c = threadIdx.x & 31; c < dim; c += 32)
+        {
+            if constexpr (sizeof(T) == 2)
+            {
+                out[r * ldp + c] = keep ? __bfloat16_as_ushort(m[r * ld + c]) : uint16_t{0};
+            }
+            else
+            {
+                const float v = keep ? m[r * ld + c] * scale : 0.0f;
+                const __half h = __float2half_rn(v);
+                out[r * ldp + c] = __half_as_ushort(h);
+                out[(n + r) * ldp + c] = __half_as_ushort(__float2half_rn(v - __half2float(h)));
+            }
+        }
+    }
+}
+
+// Merges a row's (max, sum) pairs in slot order: lse = ln 2 (max + log2 sum), loss = lse - z[target].
+__global__ void __launch_bounds__(256)
+merge_kernel(const float2* __restrict__ parts, int slots, int64_t rows, int64_t vocab,
+             const int64_t* __restrict__ targets, int64_t ignore, const float* __restrict__ target_logit,
+             float* __restrict__ row_loss, float* __restrict__ lse, int* status)
+{
+    // 32 rows a block, eight slices of the slots
+    __shared__ float2 part[8][32];
+    dep_wait();
+    dep_release();
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+    float m = -INFINITY, s = 0.0f;
+    auto add = [&](float2 o) {
+        const float top = fmaxf(m, o.x);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        s = s * ex2(m - ref) + o.y * ex2(o.x - ref);
+        m = top;
+    };
+    if (row < rows)
+    {
+        for (int k = slice; k < slots; k += 8) add(parts[static_cast<int64_t>(k) * rows + row]);
+    }
+    part[slice][lane] = make_float2(m, s);
+    __syncthreads();
+    if (slice != 0 || row >= rows)
+    {
+        return;
+    }
+    for (int k = 1; k < 8; ++k) add(part[k][lane]);
+    const float l = (m + log2f(s)) * kLn2;
+    if (lse != nullptr) lse[row] = l;
+    const int64_t t = targets[row];
+    const bool inside = t >= 0 && t < vocab;
+    if (t != ignore && !inside && status != nullptr)
+    {
+        *status = VEDA_ERR_OUT_OF_RANGE;
+    }
+    row_loss[row] = t != ignore && inside ? l - target_logit[row] : 0.0f;
+}
+
+// Mean of the counted rows' losses, summed in double in a fixed order; 0 when none is counted.
+__global__ void __launch_bounds__(1024)
+mean_kernel(const float* __restrict__ row_loss, const int64_t* __restrict__ targets, int64_t ignore, int64_t rows,
+            int64_t vocab, float* loss)
+{
+    __shared__ double sums[32];
+    __shared__ int counts[32];
+    dep_wait();
+    dep_release();
+    double s = 0.0;
+    int n = 0;
+    for (int64_t i = threadIdx.x; i < rows; i += blockDim.x)
+    {
+        const int64_t t = targets[i];
+        if (t != ignore && t >= 0 && t < vocab)
+        {
+            s += static_cast<double>(row_loss[i]);
+            ++n;
+        }
+    }
+    s = warp_sum(s);
+    n = __reduce_add_sync(0xFFFFFFFFu, n);
+    if ((threadIdx.x & 31) == 0)
+    {
+        sums[threadIdx.x >> 5] = s;
+        counts[threadIdx.x >> 5] = n;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0)
+    {
+        int total = counts[0];
+        s = sums[0];
+        for (int k = 1; k < 32; ++k)
+        {
+            s += sums[k];
+            total += counts[k];
+        }
+        *loss = total > 0 ? static_cast<float>(s / total) : 0.0f;
+    }
+}
+
+// dx = coef x the fp32 sums.
+template <typename T>
+__global__ void __launch_bounds__(256)
+finish_dx_kernel(const float* __restrict__ acc, int64_t lda, T* __restrict__ dx, int64_t lddx, int64_t rows,
+                 int64_t dim, const Scalars* __restrict__ scalars)
+{
+    dep_wait();
+    dep_release();
+    const float coef = scalars->coef, unit = scalars->unit_dx;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32; r < rows; r += static_cast<int64_t>(gridDim.x) * 8)
+    {
+        for (int64_t c = threadIdx.x & 31; c < dim; c += 32)
+        {
+            dx[r * lddx + c] = from_f32<T>(acc[r * lda + c] * unit * coef);
+        }
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------
+int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// Where a call's scratch lies in its workspace (offsets in bytes, each a multiple of 256).
+struct Layout
+{
+    int planes;
+    int64_t ldp;          // pitch of the operand planes (elements)
+    int64_t piece;        // columns of a piece of q (a multiple of 256)
+    int64_t ld_acc;       // pitch of the fp32 dx sums
+    int strip, slots;     // forward: tiles a strip, strips
+    size_t scalars, part, px, pw, parts, target_logit, q, acc, total;
+};
+
+// Tiles per strip: up to 8, by the number of tile times the busiest of `clusters` clusters runs;
+// longer strips win ties (fewer partial pairs). 8192 rows x 151936: 8 (33 rounds of 8 against 257 of
+// 1, within 3 %, an eighth of the pairs); a single row tile: 1 (9 rounds against 16 with 8).
+int choose_strip(int num_m, int num_n, int clusters)
+{
+    int best = 1;
+    int64_t best_time = INT64_MAX;
+    for (int s = 1; s <= 8; s *= 2)
+    {
+        const int64_t units = static_cast<int64_t>((num_n + s - 1) / s) * num_m;
+        const int64_t time = (units + clusters - 1) / clusters * s;
+        if (time * 32 <= best_time * 33 || best_time == INT64_MAX)
+        {
+            best = s;
+            best_time = std::min(time, best_time);
+        }
+    }
+    return best;
+}
+
+Layout layout(int64_t rows, int64_t vocab, int64_t dim, bool pack_x, bool pack_w, int dtype, bool backward)
+{
+    Layout l{};
+    size_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const size_t here = at;
+        at += static_cast<size_t>(round_up(bytes, 256));
+        return here;
+    };
+    l.planes = dtype == VEDA_F32 ? 2 : 1;
+    l.ldp = round_up(dim, 8);
+    l.scalars = take(sizeof(Scalars));
+    l.part = take(2 * kMaxBlocks * 4);
+    l.px = take(pack_x ? l.planes * rows * l.ldp * 2 : 0);
+    l.pw = take(pack_w ? l.planes * vocab * l.ldp * 2 : 0);
+    const int num_n = static_cast<int>((vocab + 255) / 256), num_m = static_cast<int>((rows + 255) / 256);
+    if (!backward)
+    {
+        // at most 74 clusters on a B200; fewer (reserved SMs) only change which strip is best
+        l.strip = choose_strip(num_m, num_n, 74);
+        l.slots = (num_n + l.strip - 1) / l.strip;
+        l.parts = take(static_cast<int64_t>(l.slots) * 2 * rows * 8);
+        l.target_logit = take(rows * 4);
+    }
+    else
+    {
+        // two pieces of q of about 32 MB each, so that both, the dx sums and x stay in L2
+        const int64_t fit = (int64_t{32} << 20) / (rows * 2 * l.planes) / 256 * 256;
+        l.piece = std::min(round_up(vocab, 256), std::max<int64_t>(256, fit));
+        l.q = take(2 * l.planes * rows * l.piece * 2);
+        l.ld_acc = round_up(dim, 4);
+        l.acc = take(rows * l.ld_acc * 4);
+    }
+    l.total = at;
+    return l;
+}
+
+struct Call
+{
+    const void *x, *w;
+    int64_t ldx, ldw, rows, vocab, dim;
+    int dtype;
+    bool pack_x, pack_w, backward;
+    Layout l;
+    char* ws;
+    Scalars* scalars() const { return reinterpret_cast<Scalars*>(ws + l.scalars); }
+};
+
+bool needs_pack(const void* m, int64_t ld, int dtype) { return dtype == VEDA_F32 || !aligned16(m) || ld % 8 != 0; }
+
+unsigned pack_blocks(int64_t rows)
+{
+    return static_cast<unsigned>(std::min<int64_t>((rows + 7) / 8, kMaxBlocks));
+}
+
+// fp32: the largest magnitudes. Then the scalars, then the operand planes where the operands cannot
+// be read in place, and the operands' tensor maps.
+int prepare(const Call& c, const int64_t* targets, int64_t ignore, const float* upstream, int* status,
+            bool scalars, Params& p, cudaStream_t s)
+{
+    float* part = nullptr;
+    const unsigned gx = pack_blocks(c.rows), gw = pack_blocks(c.vocab);
+    if (c.dtype == VEDA_F32)
+    {
+        part = reinterpret_cast<float*>(c.ws + c.l.part);
+        const int rc = launch("veda_linear_cross_entropy", absmax_kernel, dim3(gx + gw), dim3(256), 0, s,
+                              static_cast<const float*>(c.x), c.ldx, c.rows, static_cast<const float*>(c.w), c.ldw,
+                              c.vocab, c.dim, targets, ignore, static_cast<int>(gx), part);
+        if (rc != VEDA_OK) return rc;
+    }
+    if (scalars || part != nullptr)
+    {
+        const int rc = launch("veda_linear_cross_entropy", scalars_kernel, dim3(1), dim3(1024), 0, s, targets, ignore,
+                              c.rows, c.vocab, upstream, static_cast<const float*>(part), static_cast<int>(gx),
+                              static_cast<int>(gw), c.scalars(), status);
+        if (rc != VEDA_OK) return rc;
+    }
+    const void *px = c.x, *pw = c.w;
+    int64_t ldx = c.ldx, ldw = c.ldw;
+    if (c.pack_x || c.pack_w)
+    {
+        auto* ox = reinterpret_cast<uint16_t*>(c.ws + c.l.px);
+        auto* ow = reinterpret_cast<uint16_t*>(c.ws + c.l.pw);
+        const unsigned bx = c.pack_x ? gx : 0, bw = c.pack_w ? gw : 0;
+        const int rc =
+            c.dtype == VEDA_F32
+                ? launch("veda_linear_cross_entropy", pack_kernel<float>, dim3(bx + bw), dim3(256), 0, s,
+                         static_cast<const float*>(c.x), c.ldx, c.rows, static_cast<const float*>(c.w), c.ldw,
+                         c.vocab, c.dim, targets, ignore, c.backward, static_cast<int>(bx), ox, ow, c.l.ldp,
+                         static_cast<const Scalars*>(c.scalars()))
+                : launch("veda_linear_cross_entropy", pack_kernel<bf16>, dim3(bx + bw), dim3(256), 0, s,
+                         static_cast<const bf16*>(c.x), c.ldx, c.rows, static_cast<const bf16*>(c.w), c.ldw,
+                         c.vocab, c.dim, targets, ignore, c.backward, static_cast<int>(bx), ox, ow, c.l.ldp,
+                         static_cast<const Scalars*>(c.scalars()));
+        if (rc != VEDA_OK) return rc;
+        if (c.pack_x)
+        {
+            px = ox;
+            ldx = c.l.ldp;
+        }
+        if (c.pack_w)
+        {
+            pw = ow;
+            ldw = c.l.ldp;
+        }
+    }
+    const bool bf = c.dtype == VEDA_BF16;
+    if (!pair::make_map3(&p.x, px, 2, bf, c.dim, c.rows, c.l.planes, ldx, c.rows * ldx, 64, 64) ||
+        !pair::make_map3(&p.w, pw, 2, bf, c.dim, c.vocab, c.l.planes, ldw, c.vocab * ldw, 64, 64))
+    {
+        return fail(VEDA_ERR_CUDA, "veda_linear_cross_entropy: tensor map creation failed");
+    }
+    p.rows = static_cast<int>(c.rows);
+    p.vocab = static_cast<int>(c.vocab);
+    p.dim = static_cast<int>(c.dim);
+    p.segments = bf ? 1 : 3;
+    p.is_bf16 = bf;
+    p.num_m = static_cast<int>((c.rows + 255) / 256);
+    p.num_d = static_cast<int>((c.dim + 255) / 256);
+    p.scalars = c.scalars();
+    p.targets = targets;
+    p.ignore = ignore;
+    p.status = device_status_ptr();
+    return VEDA_OK;
+}
+
+// Common checks; fills c and its layout.
+int check(Call& c, void* workspace, size_t bytes, bool backward, const char* name)
+{
+    c.backward = backward;
+    c.pack_x = backward || needs_pack(c.x, c.ldx, c.dtype);
+    c.pack_w = needs_pack(c.w, c.ldw, c.dtype);
+    c.l = layout(c.rows, c.vocab, c.dim, c.pack_x, c.pack_w, c.dtype, backward);
+    if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 || bytes < c.l.total)
+    {
+        return fail(VEDA_ERR_INVALID_ARGUMENT,
+                    std::string(name) + ": workspace too small or not 256-byte aligned (see "
+                                        "veda_linear_cross_entropy_workspace; a base that is not 16-byte aligned "
+                                        "needs the size of a pitch that is no multiple of 8)");
+    }
+    c.ws = static_cast<char*>(workspace);
+    return VEDA_OK;
+}
+
+constexpr int64_t kLimit = (1ll << 31) - 512;   // tile coordinates are 32-bit
+
+} // namespace lce
+} // namespace veda::cuda
+
+using namespace veda::cuda;
+
+extern "C" size_t veda_linear_cross_entropy_workspace(int64_t rows, int64_t vocab, int64_t dim, int64_t ldx,
+                                                      int64_t ldw, int dtype, int backward)
+{
+    if (rows <= 0 || vocab <= 0 || dim <= 0 || rows > lce::kLimit || vocab > lce::kLimit || dim > lce::kLimit ||
+        !valid_dtype(dtype))
+    {
+        return 0;
+    }
+    return lce::layout(rows, vocab, dim, backward != 0 || dtype == VEDA_F32 || ldx % 8 != 0, dtype == VEDA_F32 || ldw % 8 != 0, dtype,
+                       backward != 0)
+        .total;
+}
+
+extern "C" int veda_linear_cross_entropy_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                             const int64_t* targets, int64_t ignore_index, float* row_loss, float* lse,
+                                             float* loss, int64_t rows, int64_t vocab, int64_t dim, void* workspace,
+                                             size_t workspace_bytes, int* status, int dtype, veda_stream_t stream)
+{
+    VEDA_REQUIRE(valid_dtype(dtype), "unknown dtype");
+    VEDA_REQUIRE(rows >= 0 && vocab > 0 && dim > 0, "bad shape");
+    VEDA_REQUIRE(rows <= lce::kLimit && vocab <= lce::kLimit && dim <= lce::kLimit, "an extent does not fit 31 bits");
+    VEDA_REQUIRE(ldx >= dim && ldw >= dim, "leading dimension smaller than dim");
+    if (rows == 0)
+    {
+        // nothing to average over: 0, as for a batch of ignored rows
+        if (loss != nullptr && cudaMemsetAsync(loss, 0, sizeof(float), stream) != cudaSuccess)
+        {
+            return fail(VEDA_ERR_CUDA, "veda_linear_cross_entropy_fwd: clearing the loss failed");
+        }
+        return VEDA_OK;
+    }
+    VEDA_REQUIRE(x != nullptr && w != nullptr && targets != nullptr && row_loss != nullptr, "null pointer");
+    lce::Call c{x, w, ldx, ldw, rows, vocab, dim, dtype};
+    int rc = lce::check(c, workspace, workspace_bytes, false, "veda_linear_cross_entropy_fwd");
+    if (rc != VEDA_OK) return rc;
+    const int clusters = pair::clusters_available<lce::StatsWork, 4>();
+    if (clusters < 1)
+    {
+        return fail(VEDA_ERR_UNSUPPORTED, "veda_linear_cross_entropy_fwd: no CTA pair fits on this device");
+    }
+    lce::Params p{};
+    rc = lce::prepare(c, targets, ignore_index, nullptr, nullptr, false, p, stream);
+    if (rc != VEDA_OK) return rc;
+    p.num_n = static_cast<int>((vocab + 255) / 256);
+    p.strip = c.l.strip;
+    p.parts = reinterpret_cast<float2*>(c.ws + c.l.parts);
+    p.target_logit = reinterpret_cast<float*>(c.ws + c.l.target_logit);
+    const int64_t units = static_cast<int64_t>(c.l.slots) * p.num_m;
+    VEDA_REQUIRE(units <= lce::kLimit, "too many tiles");
+    rc = pair::launch_pair<lce::StatsWork, 4>("veda_linear_cross_entropy_fwd", p,
+                                              static_cast<int>(std::min<int64_t>(units, clusters)), stream);
+    if (rc != VEDA_OK) return rc;
+    rc = launch("veda_linear_cross_entropy_fwd (merge)", lce::merge_kernel, dim3(static_cast<unsigned>((rows + 31) / 32)),
+                dim3(256), 0, stream, static_cast<const float2*>(p.parts), c.l.slots, rows, vocab, targets, ignore_index,
+                static_cast<const float*>(p.target_logit), row_loss, lse, status);
+    if (rc != VEDA_OK || loss == nullptr) return rc;
+    return launch("veda_linear_cross_entropy_fwd (mean)", lce::mean_kernel, dim3(1), dim3(1024), 0, stream,
+                  static_cast<const float*>(row_loss), targets, ignore_index, rows, vocab, loss);
+}
+
+extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                             const int64_t* targets, int64_t ignore_index, const float* lse,
+                                             const float* upstream, void* dx, int64_t lddx, void* dw, int64_t lddw,
+                                             int dtype_dw, float beta_dw, int64_t rows, int64_t vocab, int64_t dim,
+                                             void* workspace, size_t workspace_bytes, int* status, int dtype,
+                                             veda_stream_t stream)
+{
+    VEDA_REQUIRE(valid_dtype(dtype) && valid_dtype(dtype_dw), "unknown dtype");
+    VEDA_REQUIRE(dtype == VEDA_BF16 || dtype_dw == VEDA_F32, "fp32 operands have an fp32 weight gradient");
+    VEDA_REQUIRE(rows >= 0 && vocab > 0 && dim > 0, "bad shape");
+    VEDA_REQUIRE(rows <= lce::kLimit && vocab <= lce::kLimit && dim <= lce::kLimit, "an extent does not fit 31 bits");
+    VEDA_REQUIRE(ldx >= dim && ldw >= dim, "leading dimension smaller than dim");
+    VEDA_REQUIRE((dx == nullptr || lddx >= dim) && (dw == nullptr || lddw >= dim),
+                 "gradient leading dimension smaller than dim");
+    VEDA_REQUIRE(beta_dw == 0.0f || beta_dw == 1.0f, "beta_dw must be 0 (overwrite) or 1 (accumulate)");
+    if (rows == 0)
+    {
+        if (dw != nullptr && beta_dw == 0.0f &&
+            cudaMemset2DAsync(dw, lddw * dtype_size(dtype_dw), 0, dim * dtype_size(dtype_dw), vocab, stream) != cudaSuccess)
+        {
+            return fail(VEDA_ERR_CUDA, "veda_linear_cross_entropy_bwd: clearing dw failed");
+        }
+        return VEDA_OK;
+    }
+    VEDA_REQUIRE(x != nullptr && w != nullptr && targets != nullptr && lse != nullptr, "null pointer");
+    if (dx == nullptr && dw == nullptr)
+    {
+        return VEDA_OK;
+    }
+    lce::Call c{x, w, ldx, ldw, rows, vocab, dim, dtype};
+    int rc = lce::check(c, workspace, workspace_bytes, true, "veda_linear_cross_entropy_bwd");
+    if (rc != VEDA_OK) return rc;
+    const int clusters = pair::clusters_available<lce::GradWork, 4>();
+    if (clusters < 1)
+    {
+        return fail(VEDA_ERR_UNSUPPORTED, "veda_linear_cross_entropy_bwd: no CTA pair fits on this device");
+    }
+    lce::Params p{};
+    rc = lce::prepare(c, targets, ignore_index, upstream, status, true, p, stream);
+    if (rc != VEDA_OK) return rc;
+    const int64_t piece = c.l.piece, plane = rows * piece;
+    const bool bf = dtype == VEDA_BF16;
+    CUtensorMap q_load[2], q_store[2];
+    bool ok = true;
+    for (int b = 0; b < 2; ++b)
+    {
+        char* q = c.ws + c.l.q + static_cast<size_t>(b) * c.l.planes * plane * 2;
+        ok = ok && pair::make_map3(&q_load[b], q, 2, bf, piece, rows, c.l.planes, piece, plane, 64, 64) &&
+             pair::make_map3(&q_store[b], q, 2, bf, piece, rows, c.l.planes, piece, plane, 64, 32);
+    }
+    float* acc = reinterpret_cast<float*>(c.ws + c.l.acc);
+    ok = ok && pair::make_map3(&p.dx, acc, 4, false, dim, rows, 1, c.l.ld_acc, rows * c.l.ld_acc, 32, 32);
+    p.dw_f32 = dtype_dw == VEDA_F32;
+    p.dw_beta = beta_dw != 0.0f;
+    p.dw_ptr = dw;
+    p.lddw = lddw;
+    if (dw != nullptr)
+    {
+        const int es = p.dw_f32 ? 4 : 2;
+        const bool fits = aligned16(dw) && lddw * es % 16 == 0 && !(p.dw_beta && !p.dw_f32);
+        if (fits && pair::make_map3(&p.dw, dw, es, !p.dw_f32, dim, vocab, 1, lddw, vocab * lddw, 128 / es, 32))
+        {
+            p.dw_mode = p.dw_beta ? 2 : 1;
+        }
+    }
+    if (!ok)
+    {
+        return fail(VEDA_ERR_CUDA, "veda_linear_cross_entropy_bwd: tensor map creation failed");
+    }
+    p.lse = lse;
+    // launch c: q of piece c, and the products of piece c - 1
+    const int64_t pieces = (vocab + piece - 1) / piece;
+    for (int64_t k = 0; k <= pieces; ++k)
+    {
+        p.num_n = 0;
+        p.dw_tiles = p.dx_tiles = 0;
+        if (k < pieces)
+        {
+            p.v0 = static_cast<int>(k * piece);
+            p.num_n = static_cast<int>((std::min(piece, vocab - k * piece) + 255) / 256);
+            p.q_out = q_store[k & 1];
+        }
+        if (k > 0)
+        {
+            p.g0 = static_cast<int>((k - 1) * piece);
+            p.gcols = static_cast<int>(std::min(piece, vocab - (k - 1) * piece));
+            p.q_in = q_load[(k - 1) & 1];
+            p.dw_tiles = dw != nullptr ? (p.gcols + 255) / 256 * p.num_d : 0;
+            p.dx_tiles = dx != nullptr ? p.num_m * p.num_d : 0;
+            p.dx_add = k > 1;
+        }
+        const int64_t units = static_cast<int64_t>(p.num_m) * p.num_n + p.dw_tiles + p.dx_tiles;
+        rc = pair::launch_pair<lce::GradWork, 4>("veda_linear_cross_entropy_bwd", p,
+                                                 static_cast<int>(std::min<int64_t>(units, clusters)), stream);
+        if (rc != VEDA_OK) return rc;
+    }
+    if (dx == nullptr)
+    {
+        return VEDA_OK;
+    }
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((rows + 7) / 8, 8ll * sm_count()));
+    return bf ? launch("veda_linear_cross_entropy_bwd (dx)", lce::finish_dx_kernel<bf16>, dim3(blocks), dim3(256), 0,
+                       stream, static_cast<const float*>(acc), c.l.ld_acc, static_cast<bf16*>(dx), lddx, rows, dim,
+                       static_cast<const lce::Scalars*>(c.scalars()))
+              : launch("veda_linear_cross_entropy_bwd (dx)", lce::finish_dx_kernel<float>, dim3(blocks), dim3(256), 0,
+                       stream, static_cast<const float*>(acc), c.l.ld_acc, static_cast<float*>(dx), lddx, rows, dim,
+                       static_cast<const lce::Scalars*>(c.scalars()));
+}

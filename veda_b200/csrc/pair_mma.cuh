@@ -1,0 +1,366 @@
+// A persistent CTA-pair tensor-core kernel over a list of 256 x 256 output tiles, with the list and
+// the epilogue supplied by a Work type: the mainloop of the loss head (linear_ce.cu) and of the
+// Newton-Schulz products (newton_schulz.cu).
+//
+// A cluster of two CTAs computes a tile with tcgen05.mma.cta_group::2 (M 256, N 256, K 16; 16-bit
+// operands, fp32 accumulators in TMEM). Each CTA stages its own 128 rows of A and 128 columns of B
+// (32 KB per 64-deep k-block, six stages), the even CTA issues the products, two 256-column
+// accumulators alternate so that a tile's epilogue runs under the next tile's products. Operands are
+// read through 3-D tensor maps (column, row, plane) with 64 x 64 boxes, so one map serves an operand
+// in both orders: K-major (two boxes down the rows) and MN-major (two boxes along the columns).
+// Loads carry no multicast. Every wait is bounded (tc::mbar_wait).
+//
+// Work provides
+//   struct Params                      the kernel's argument (tensor maps, pointers, sizes, status)
+//   struct Tile { bool skip; int kbs; uint32_t idesc; bool a_mn, b_mn; ... }
+//   bool tile(p, cid, clusters, i, t)  the i-th tile of cluster cid; false at the end of its list
+//   void operands(p, t, rank, kb, a, b)  where k-block kb's operand pieces of CTA `rank` lie
+//   void epilogue(p, t, state, ...)    one warp's 32 rows x COLS columns of the finished tile
+// All roles walk the same list, so tile() must depend on its arguments and on Params alone.
+#pragma once
+
+#include "tc_common.cuh"
+
+namespace veda::cuda::pair
+{
+
+constexpr int kTile = 256;   // tile rows and columns of a CTA pair
+constexpr int kBK = 64;      // k-block: 64 16-bit values, one 128-byte swizzle row
+
+template <int EPI_WARPS_>
+struct Cfg
+{
+    static constexpr int EPI_WARPS = EPI_WARPS_;   // 4, or 8 with half the columns each
+    static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+    static constexpr int STAGES = EPI_WARPS == 8 ? 5 : 6;
+    static constexpr int OPERAND = 128 * kBK * 2;   // one CTA's half of an operand's k-block
+    static constexpr int STAGE = 2 * OPERAND;
+    static constexpr int STAGE_TILE = 32 * 128;     // epilogue staging: 32 rows x 128 bytes
+    static constexpr int STAGING = EPI_WARPS * 2 * STAGE_TILE;
+    static constexpr int SMEM = STAGES * STAGE + STAGING + 1024 + 256;
+};
+
+// A 128 x 64 operand piece: the tensor map and the coordinates of its first 64 x 64 box; the second
+// lies 64 rows further down (K-major) or 64 columns further right (MN-major).
+struct Piece
+{
+    const CUtensorMap* map;
+    int x, y, z;
+};
+
+// kind::f16 instruction descriptor: fp32 accumulators, A and B both bf16 or both fp16.
+__host__ __device__ constexpr uint32_t idesc(bool is_bf16, bool a_mn, bool b_mn)
+{
+    const uint32_t type = is_bf16 ? 1u : 0u;
+    return (1u << 4) | (type << 7) | (type << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
+           (static_cast<uint32_t>(kTile >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
+}
+
+__device__ __forceinline__ uint32_t cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// shared::cluster address of a shared variable at the same place in CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(tc::smem_u32(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(tc::smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+__device__ __forceinline__ void reduce_add_3d(const CUtensorMap* map, const void* src, int x, int y, int z)
+{
+    asm volatile(
+        "cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+            reinterpret_cast<uint64_t>(map)),
+        "r"(tc::smem_u32(src)), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+__device__ __forceinline__ void mma2(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(desc), "r"(accumulate));
+}
+__device__ __forceinline__ void commit2(uint64_t* bar)
+{
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(tc::smem_u32(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+
+// One warp's staging tiles (two of 32 rows x 128 bytes): buffer() waits until the bulk group that
+// used the next one has read it and gives the tile; sent() counts the group just committed by lane 0.
+struct Staging
+{
+    uint8_t* base;
+    uint32_t count = 0;
+    __device__ __forceinline__ uint8_t* buffer(int lane)
+    {
+        if (count >= 2)
+        {
+            if (lane == 0)
+            {
+                tc::bulk_wait_group_read<1>();
+            }
+            __syncwarp();
+        }
+        return base + (count & 1) * Cfg<4>::STAGE_TILE;
+    }
+    __device__ __forceinline__ void sent() { ++count; }
+};
+
+template <class Work, int EPI_WARPS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI_WARPS>::THREADS, 1)
+pair_kernel(const __grid_constant__ typename Work::Params p)
+{
+    using namespace tc;
+    using C_ = Cfg<EPI_WARPS>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint8_t* sa = smem;
+    uint8_t* sb = smem + C_::STAGES * C_::OPERAND;
+    uint8_t* staging = sb + C_::STAGES * C_::OPERAND;
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + C_::STAGING);
+    uint64_t* empty = full + C_::STAGES;
+    uint64_t* tfull = empty + C_::STAGES;
+    uint64_t* tempty = tfull + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+    volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int cid = static_cast<int>(blockIdx.x >> 1);
+    const int clusters = static_cast<int>(gridDim.x >> 1);
+
+    if (threadIdx.x == 0)
+    {
+        *abort = 0;
+        for (int s = 0; s < C_::STAGES; ++s)
+        {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b)
+        {
+            mbar_init(&tfull[b], 1);
+            mbar_init(&tempty[b], 2 * EPI_WARPS);   // the epilogue warps of both CTAs
+        }
+        mbar_fence_init();
+    }
+    if (warp == 1)
+    {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(tmem_slot)),
+                     "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    fence_before();
+    __syncthreads();
+    cluster_sync();   // both CTAs' barriers exist before any signal crosses
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+    dep_wait();
+    dep_release();
+
+    typename Work::Tile t;
+    if (warp == 0 && lane == 0)
+    {
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int i = 0; Work::tile(p, cid, clusters, i, t); ++i)
+        {
+            if (t.skip)
+            {
+                continue;
+            }
+            for (int kb = 0; kb < t.kbs; ++kb)
+            {
+                Piece a, b;
+                Work::operands(p, t, static_cast<int>(rank), kb, a, b);
+                mbar_wait(&empty[stage], phase ^ 1, p.status, abort);
+                if (rank == 0)
+                {
+                    mbar_expect_tx(&full[stage], 2 * C_::STAGE);   // both CTAs' halves
+                }
+                const uint32_t bar = peer_addr(&full[stage], 0);
+                uint8_t* ad = sa + stage * C_::OPERAND;
+                uint8_t* bd = sb + stage * C_::OPERAND;
+                load_box(ad, a.map, bar, a.x, a.y, a.z);
+                load_box(ad + C_::OPERAND / 2, a.map, bar, a.x + (t.a_mn ? 64 : 0), a.y + (t.a_mn ? 0 : 64), a.z);
+                load_box(bd, b.map, bar, b.x, b.y, b.z);
+                load_box(bd + C_::OPERAND / 2, b.map, bar, b.x + (t.b_mn ? 64 : 0), b.y + (t.b_mn ? 0 : 64), b.z);
+                if (++stage == C_::STAGES)
+                {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+    }
+    else if (warp == 1 && lane == 0 && rank == 0)
+    {
+        int stage = 0, it = 0;
+        uint32_t phase = 0;
+        for (int i = 0; Work::tile(p, cid, clusters, i, t); ++i)
+        {
+            if (t.skip)
+            {
+                continue;
+            }
+            const int buf = it & 1;
+            mbar_wait(&tempty[buf], ((it >> 1) & 1) ^ 1, p.status, abort);
+            fence_after();
+            const uint32_t d = tmem + static_cast<uint32_t>(buf * kTile);
+            const uint32_t astep = t.a_mn ? 2048 : 32, bstep = t.b_mn ? 2048 : 32;
+            const uint32_t albo = t.a_mn ? kBK * 128 : 16, blbo = t.b_mn ? kBK * 128 : 16;
+            for (int kb = 0; kb < t.kbs; ++kb)
+            {
+                mbar_wait(&full[stage], phase, p.status, abort);
+                fence_after();
+                const uint32_t ab = smem_u32(sa + stage * C_::OPERAND);
+                const uint32_t bb = smem_u32(sb + stage * C_::OPERAND);
+#pragma unroll
+                for (int kk = 0; kk < kBK / 16; ++kk)
+                {
+                    mma2(d, smem_desc(ab + kk * astep, albo, 1024), smem_desc(bb + kk * bstep, blbo, 1024),
+                         t.idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+                }
+                commit2(&empty[stage]);
+                if (++stage == C_::STAGES)
+                {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            commit2(&tfull[buf]);
+            ++it;
+        }
+    }
+    else if (warp >= 2)
+    {
+        const int quarter = warp & 3;   // the TMEM lanes this warp may read
+        constexpr int COLS = kTile / (EPI_WARPS / 4);
+        const int col0 = ((warp - 2) >> 2) * COLS;
+        const uint32_t release = peer_addr(&tempty[0], 0);
+        Staging st{staging + (warp - 2) * 2 * C_::STAGE_TILE};
+        typename Work::State state;
+        int it = 0;
+        for (int i = 0; Work::tile(p, cid, clusters, i, t); ++i)
+        {
+            if (t.skip)
+            {
+                continue;
+            }
+            const int buf = it & 1;
+            const int row0 = static_cast<int>(rank) * 128 + quarter * 32;   // within the tile
+            Work::before(p, t, state, row0, col0, lane);
+            mbar_wait(&tfull[buf], (it >> 1) & 1, p.status, abort);
+            fence_after();
+            const uint32_t base = tmem + static_cast<uint32_t>(buf * kTile + col0) +
+                                  (static_cast<uint32_t>(quarter * 32) << 16);
+            Work::template epilogue<COLS>(p, t, state, base, row0, col0, st, lane);
+            fence_before();
+            __syncwarp();
+            if (lane == 0)
+            {
+                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                                 release + static_cast<uint32_t>(buf * 8))
+                             : "memory");
+            }
+            ++it;
+        }
+        if (lane == 0)
+        {
+            bulk_wait_group<0>();   // staged output fully written before the CTA's memory goes
+        }
+    }
+    fence_before();
+    __syncthreads();
+    cluster_sync();   // no CTA leaves while its peer may still read its operands or barriers
+    if (warp == 1)
+    {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------
+// A tensor map over `planes` row-major matrices of `rows` x `cols` (element size es: 2 for 16-bit,
+// 4 for fp32), rows ld elements and planes `plane` elements apart, with boxes of bx x by and the
+// 128-byte swizzle (or none). The base must be 16-byte aligned, ld and plane multiples of 16 bytes.
+bool make_map3(CUtensorMap* map, const void* base, int es, bool is_bf16, int64_t cols, int64_t rows,
+               int64_t planes, int64_t ld, int64_t plane, uint32_t bx, uint32_t by, bool swizzle = true);
+
+// Clusters of the kernel that the current device can hold at once, capped by the SMs that
+// veda_set_reserved_sms leaves (0: none fit). Cached per device.
+template <class Work, int EPI_WARPS>
+int clusters_available()
+{
+    constexpr int kDevices = 64;
+    static std::atomic<int> cached[kDevices];   // 0: not asked yet, else clusters + 1
+    int device = 0;
+    cudaGetDevice(&device);
+    if (device < 0 || device >= kDevices)
+    {
+        return 0;
+    }
+    int have = cached[device].load(std::memory_order_acquire);
+    if (have == 0)
+    {
+        auto kernel = pair_kernel<Work, EPI_WARPS>;
+        int n = 0;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<EPI_WARPS>::SMEM) ==
+            cudaSuccess)
+        {
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(2 * (sm_count() / 2));
+            cfg.blockDim = dim3(Cfg<EPI_WARPS>::THREADS);
+            cfg.dynamicSmemBytes = Cfg<EPI_WARPS>::SMEM;
+            cudaLaunchAttribute attr{};
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = 2;
+            attr.val.clusterDim.y = 1;
+            attr.val.clusterDim.z = 1;
+            cfg.attrs = &attr;
+            cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess)
+            {
+                n = 0;
+            }
+            cudaGetLastError();
+        }
+        have = n + 1;
+        cached[device].store(have, std::memory_order_release);
+    }
+    const int cap = compute_sms() / 2;
+    return have - 1 < cap ? have - 1 : cap;
+}
+
+template <class Work, int EPI_WARPS>
+int launch_pair(const char* what, const typename Work::Params& p, int clusters, cudaStream_t s)
+{
+    return launch(what, pair_kernel<Work, EPI_WARPS>, dim3(2 * clusters), dim3(Cfg<EPI_WARPS>::THREADS),
+                  Cfg<EPI_WARPS>::SMEM, s, p);
+}
+
+} // namespace veda::cuda::pair
