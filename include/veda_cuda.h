@@ -337,6 +337,43 @@ int veda_adamw_step_dev(float* master, float* m, float* v, float* g, void* lowp,
                         int write_grad, veda_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------- */
+/* Orthogonalisation by Newton-Schulz products, and the Muon step (no counterpart in the      */
+/* reference, whose optimiser is AdamW).                                                      */
+/* ---------------------------------------------------------------------------------------- */
+/* Per matrix of the batch: X = g / (|g|_F + eps), then `steps` times X <- a X + (b S + c S^2) X
+ * with S = X X^T, taken on the smaller side; out = X. dtype is that of g and out. The usual
+ * coefficients are 3.4445, -4.7750, 2.0315 with 5 steps, which bring every singular value that is
+ * not tiny to about 1; others must keep the singular values of X, and |a|, |b| + |c|, below 16.
+ * bf16 matrices are multiplied in fp16 from an X held in two fp16 values (22 bits); fp32 ones as
+ * pairs of fp16 values throughout. Row r, column c of matrix k is g[k stride_g + r ldg + c], any
+ * alignment; out may be g. A zero matrix stays zero; a matrix that is not finite gives NaN in
+ * itself alone. The workspace (256-byte aligned, contents undefined before and after) is sized by
+ * veda_orthogonalize_workspace (0 for an empty or refused shape). batch <= 2^15, rows and cols <=
+ * 2^20. Results repeat bit for bit and do not depend on the batch a matrix is in. */
+size_t veda_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, int dtype);
+int veda_orthogonalize(const void* g, int64_t ldg, int64_t stride_g, void* out, int64_t ldo,
+                       int64_t stride_o, int64_t batch, int64_t rows, int64_t cols, int steps,
+                       float a, float b, float c, float eps, void* workspace,
+                       size_t workspace_bytes, int dtype, veda_stream_t stream);
+/* One Muon step of `batch` contiguous [rows, cols] weight matrices that lie `stride` elements apart
+ * in each of master, momentum, grad (fp32) and lowp (bf16, or NULL for fp32 weights):
+ *   g = grad grad_scale, times max_norm / total if sumsq is not NULL and total = sqrt(*sumsq)
+ *       |grad_scale| is finite and above max_norm (veda_adamw_step's clip);
+ *   momentum <- beta momentum + g;  u = nesterov ? g + beta momentum : momentum;
+ *   master <- master - lr weight_decay master - lr update_scale orthogonalize(u);
+ *   lowp <- bf16(master).
+ * The products run as for bf16 matrices when lowp is given, else as for fp32 ones
+ * (veda_orthogonalize). flags: VEDA_ADAMW_SKIP_NONFINITE leaves everything untouched when the norm
+ * is not finite. grad is not written. The workspace's dtype is VEDA_BF16 when lowp is given, else
+ * VEDA_F32. */
+size_t veda_muon_step_workspace(int64_t batch, int64_t rows, int64_t cols, int dtype);
+int veda_muon_step(float* master, float* momentum, const float* grad, void* lowp, int64_t batch,
+                   int64_t rows, int64_t cols, int64_t stride, float lr, float beta, int nesterov,
+                   float weight_decay, float update_scale, int steps, float a, float b, float c,
+                   float eps, const double* sumsq, float max_norm, float grad_scale, int flags,
+                   void* workspace, size_t workspace_bytes, veda_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------- */
 /* Element-wise and per-lane ops of the fine-grained autograd API.                           */
 /* ---------------------------------------------------------------------------------------- */
 /* out = a (+|*) b with numpy broadcasting expressed by strides (0 = broadcast axis), rank <= 8.

@@ -85,6 +85,12 @@ SIGNATURES = {
     "veda_adamw_step": (_i, [_p, _p, _p, _p, _p, _i64, _f, _f, _f, _f, _f, _d, _d, _p, _f, _f,
                              _i, _p]),
     "veda_adamw_step_dev": (_i, [_p, _p, _p, _p, _p, _i64, _f, _f, _f, _f, _f, _p, _p, _f, _f, _i, _p]),
+    "veda_orthogonalize_workspace": (_sz, [_i64, _i64, _i64, _i]),
+    "veda_orthogonalize": (_i, [_p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i, _f, _f, _f, _f, _p,
+                                _sz, _i, _p]),
+    "veda_muon_step_workspace": (_sz, [_i64, _i64, _i64, _i]),
+    "veda_muon_step": (_i, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _f, _f, _i, _f, _f, _i, _f, _f, _f,
+                            _f, _p, _f, _f, _i, _p, _sz, _p]),
     "veda_launch_count_add": (_i, [_i64]),
     "veda_binary": (_i, [_i, _p, _p, _p, _p, _p, _p, _i, _i, _p]),
     "veda_scale": (_i, [_p, _f, _p, _i64, _i, _p]),

@@ -10,6 +10,7 @@
 //         fused multiply-adds, which keeps the result equal to the CPU's bit for bit on equal
 //         gradients. The clip scale is computed in the kernel from the device-side sumsq, so the
 //         clipped step needs no host round trip.
+#include "clip.cuh"
 #include "common.cuh"
 
 namespace veda::cuda
@@ -85,27 +86,6 @@ __global__ void sumsq_final_kernel(const double* __restrict__ partials, int coun
     }
 }
 
-// total = sqrt(sumsq) * grad_scale: the norm of the gradient after the grad_scale factor (the
-// 1/world average of data-parallel training) has been applied.
-__device__ __forceinline__ float clip_scale(const double* sumsq, float max_norm,
-                                            float grad_scale = 1.0f)
-{
-    if (sumsq == nullptr)
-    {
-        return 1.0f;
-    }
-    double total = sqrt(*sumsq);
-    if (grad_scale != 1.0f)
-    {
-        total *= fabs(static_cast<double>(grad_scale));
-    }
-    if (!isfinite(total) || total <= static_cast<double>(max_norm))
-    {
-        return 1.0f;
-    }
-    return static_cast<float>(static_cast<double>(max_norm) / total);
-}
-
 __global__ void clip_kernel(float* __restrict__ g, int64_t n, const double* __restrict__ sumsq,
                             float max_norm)
 {
@@ -155,8 +135,7 @@ adamw_kernel(float* __restrict__ master, float* __restrict__ m, float* __restric
         a.bias1 = bias[0];
         a.bias2 = bias[1];
     }
-    if ((a.write_grad & 2) && sumsq != nullptr &&
-        !isfinite(static_cast<float>(sqrt(*sumsq) * fabs(static_cast<double>(a.grad_scale)))))
+    if (skipped_step(a.write_grad, sumsq, a.grad_scale))
     {
         return;   // a non-finite norm: the whole step is skipped, nothing is written
     }
