@@ -20,7 +20,7 @@
 //
 // fp32 operands: each is split into two fp16 planes, value 2^e = hi + lo (22 bits, e chosen from
 // the tensor's largest finite value), and a product becomes hi hi + hi lo + lo hi on the same tiles
-// with three times the k-blocks; lo lo is below the 22nd bit. fp32 CUDA-core products run at a
+// with three times the k-blocks (pair_mma.cuh); lo lo is below the 22nd bit. fp32 CUDA-core products run at a
 // twentieth of the tensor cores' rate, so three tensor products are still far cheaper.
 #include "pair_mma.cuh"
 
@@ -65,7 +65,7 @@ struct Params
     CUtensorMap q_out;       // piece of q written (store boxes)
     CUtensorMap dx, dw;      // fp32 sums of dx; dW (store boxes)
     int rows, vocab, dim;
-    int segments;            // products per pair of operands: 1, or 3 (split)
+    int split;               // operands are pairs of fp16 planes
     int is_bf16;
     int num_m;               // row tiles
     // logits of this launch: vocabulary rows v0 .. v0 + 256 num_n
@@ -116,13 +116,6 @@ __device__ __forceinline__ int counted_target(const Params& p, int row)
     return t == p.ignore || t < 0 || t >= p.vocab ? -1 : static_cast<int>(t);
 }
 
-// The operand planes of segment s of a split product: hi hi, hi lo, lo hi.
-__device__ __forceinline__ void planes_of(int segment, int& za, int& zb)
-{
-    za = segment == 2 ? 1 : 0;
-    zb = segment == 1 ? 1 : 0;
-}
-
 // ---- forward: running (max, sum) per row over strips of logit tiles ---------------------------
 struct StatsWork
 {
@@ -156,26 +149,21 @@ struct StatsWork
         t.skip = t.nb >= p.num_n;
         t.first = sub == 0;
         t.last = sub == p.strip - 1 || t.nb == p.num_n - 1;
-        t.kbs = (p.dim + pair::kBK - 1) / pair::kBK * p.segments;
+        t.kbs = (p.dim + pair::kBK - 1) / pair::kBK;
         t.a_mn = t.b_mn = false;
         t.idesc = pair::idesc(p.is_bf16 != 0, false, false);
         return true;
     }
 
-    static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, int kb,
-                                                    pair::Piece& a, pair::Piece& b)
+    static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, int k, int za,
+                                                    int zb, pair::Piece& a, pair::Piece& b)
     {
-        const int per = (p.dim + pair::kBK - 1) / pair::kBK;
-        const int seg = kb / per;
-        const int k = (kb - seg * per) * pair::kBK;
-        int za, zb;
-        planes_of(seg, za, zb);
         a = {&p.x, k, t.mb * pair::kTile + rank * 128, za};
         b = {&p.w, k, p.v0 + t.nb * pair::kTile + rank * 128, zb};
     }
 
     static __device__ __forceinline__ void before(const Params& p, const Tile& t, State& s, int row0, int,
-                                                  int lane)
+                                                  pair::Staging&, int lane)
     {
         if (t.first)
         {
@@ -195,7 +183,7 @@ struct StatsWork
         }
         const int row = t.mb * pair::kTile + row0 + lane;
         const int first = p.v0 + t.nb * pair::kTile + col0;
-        const float zs = p.segments > 1 ? p.scalars->z : 1.0f;
+        const float zs = p.split ? p.scalars->z : 1.0f;
 #pragma unroll 1
         for (int c = 0; c < COLS; c += 32)
         {
@@ -212,7 +200,7 @@ struct StatsWork
             {
                 z[j] = __uint_as_float(r[j]);
             }
-            if (p.segments > 1)
+            if (p.split)
             {
 #pragma unroll
                 for (int j = 0; j < 32; ++j) z[j] *= zs;
@@ -281,7 +269,7 @@ struct GradWork
             t.kind = kDw;
             t.mb = u / p.num_d;
             t.nb = u - t.mb * p.num_d;
-            t.kbs = (p.rows + pair::kBK - 1) / pair::kBK * p.segments;
+            t.kbs = (p.rows + pair::kBK - 1) / pair::kBK;
             t.a_mn = t.b_mn = true;
             t.idesc = pair::idesc(bf, true, true);
             return true;
@@ -292,7 +280,7 @@ struct GradWork
             t.kind = kDx;
             t.mb = u / p.num_d;
             t.nb = u - t.mb * p.num_d;
-            t.kbs = (p.gcols + pair::kBK - 1) / pair::kBK * p.segments;
+            t.kbs = (p.gcols + pair::kBK - 1) / pair::kBK;
             t.a_mn = false;
             t.b_mn = true;
             t.idesc = pair::idesc(bf, false, true);
@@ -306,21 +294,16 @@ struct GradWork
         t.kind = kQ;
         t.nb = u / p.num_m;
         t.mb = u - t.nb * p.num_m;
-        t.kbs = (p.dim + pair::kBK - 1) / pair::kBK * p.segments;
+        t.kbs = (p.dim + pair::kBK - 1) / pair::kBK;
         t.a_mn = t.b_mn = false;
         t.idesc = pair::idesc(bf, false, false);
         return true;
     }
 
-    static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, int kb,
-                                                    pair::Piece& a, pair::Piece& b)
+    static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, int k, int za,
+                                                    int zb, pair::Piece& a, pair::Piece& b)
     {
-        const int per = p.segments > 1 ? t.kbs / p.segments : t.kbs;
-        const int seg = p.segments > 1 ? kb / per : 0;
-        const int k = (kb - seg * per) * pair::kBK;
         const int m = t.mb * pair::kTile + rank * 128, n = t.nb * pair::kTile + rank * 128;
-        int za, zb;
-        planes_of(seg, za, zb);
         if (t.kind == kDw)
         {
             a = {&p.q_in, m, k, za};
@@ -339,7 +322,7 @@ struct GradWork
     }
 
     static __device__ __forceinline__ void before(const Params& p, const Tile& t, State& s, int row0, int,
-                                                  int lane)
+                                                  pair::Staging&, int lane)
     {
         if (t.kind == kQ)
         {
@@ -374,8 +357,8 @@ struct GradWork
         {
             return;
         }
-        const float zs = p.segments > 1 ? p.scalars->z * kLog2e : kLog2e;
-        const float scale = p.segments > 1 ? kQScale : 1.0f;
+        const float zs = p.split ? p.scalars->z * kLog2e : kLog2e;
+        const float scale = p.split ? kQScale : 1.0f;
 #pragma unroll 1
         for (int c = 0; c < COLS; c += 64)
         {
@@ -401,7 +384,7 @@ struct GradWork
                         q[j] = s.target >= 0 && 32 * half + j < left ? v : 0.0f;
                     }
                 }
-                if (p.segments > 1)
+                if (p.split)
                 {
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
@@ -419,7 +402,7 @@ struct GradWork
                 }
             }
             send(p, hi, col, trow, 0, st, lane);
-            if (p.segments > 1)
+            if (p.split)
             {
                 send(p, lo, col, trow, 1, st, lane);
             }
@@ -963,7 +946,7 @@ int prepare(const Call& c, const int64_t* targets, int64_t ignore, const float* 
     p.rows = static_cast<int>(c.rows);
     p.vocab = static_cast<int>(c.vocab);
     p.dim = static_cast<int>(c.dim);
-    p.segments = bf ? 1 : 3;
+    p.split = !bf;
     p.is_bf16 = bf;
     p.num_m = static_cast<int>((c.rows + 255) / 256);
     p.num_d = static_cast<int>((c.dim + 255) / 256);
@@ -1034,7 +1017,9 @@ extern "C" int veda_linear_cross_entropy_fwd(const void* x, int64_t ldx, const v
     lce::Call c{x, w, ldx, ldw, rows, vocab, dim, dtype};
     int rc = lce::check(c, workspace, workspace_bytes, false, "veda_linear_cross_entropy_fwd");
     if (rc != VEDA_OK) return rc;
-    const int clusters = pair::clusters_available<lce::StatsWork, 4>();
+    const bool split = dtype == VEDA_F32;
+    const int clusters = split ? pair::clusters_available<lce::StatsWork, 4, true>()
+                               : pair::clusters_available<lce::StatsWork, 4, false>();
     if (clusters < 1)
     {
         return fail(VEDA_ERR_UNSUPPORTED, "veda_linear_cross_entropy_fwd: no CTA pair fits on this device");
@@ -1048,8 +1033,9 @@ extern "C" int veda_linear_cross_entropy_fwd(const void* x, int64_t ldx, const v
     p.target_logit = reinterpret_cast<float*>(c.ws + c.l.target_logit);
     const int64_t units = static_cast<int64_t>(c.l.slots) * p.num_m;
     VEDA_REQUIRE(units <= lce::kLimit, "too many tiles");
-    rc = pair::launch_pair<lce::StatsWork, 4>("veda_linear_cross_entropy_fwd", p,
-                                              static_cast<int>(std::min<int64_t>(units, clusters)), stream);
+    const int grid = static_cast<int>(std::min<int64_t>(units, clusters));
+    rc = split ? pair::launch_pair<lce::StatsWork, 4, true>("veda_linear_cross_entropy_fwd", p, grid, stream)
+               : pair::launch_pair<lce::StatsWork, 4, false>("veda_linear_cross_entropy_fwd", p, grid, stream);
     if (rc != VEDA_OK) return rc;
     rc = launch("veda_linear_cross_entropy_fwd (merge)", lce::merge_kernel, dim3(static_cast<unsigned>((rows + 31) / 32)),
                 dim3(256), 0, stream, static_cast<const float2*>(p.parts), c.l.slots, rows, vocab, targets, ignore_index,
@@ -1091,7 +1077,9 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
     lce::Call c{x, w, ldx, ldw, rows, vocab, dim, dtype};
     int rc = lce::check(c, workspace, workspace_bytes, true, "veda_linear_cross_entropy_bwd");
     if (rc != VEDA_OK) return rc;
-    const int clusters = pair::clusters_available<lce::GradWork, 4>();
+    const bool split = dtype == VEDA_F32;
+    const int clusters = split ? pair::clusters_available<lce::GradWork, 4, true>()
+                               : pair::clusters_available<lce::GradWork, 4, false>();
     if (clusters < 1)
     {
         return fail(VEDA_ERR_UNSUPPORTED, "veda_linear_cross_entropy_bwd: no CTA pair fits on this device");
@@ -1151,8 +1139,9 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
             p.dx_add = k > 1;
         }
         const int64_t units = static_cast<int64_t>(p.num_m) * p.num_n + p.dw_tiles + p.dx_tiles;
-        rc = pair::launch_pair<lce::GradWork, 4>("veda_linear_cross_entropy_bwd", p,
-                                                 static_cast<int>(std::min<int64_t>(units, clusters)), stream);
+        const int grid = static_cast<int>(std::min<int64_t>(units, clusters));
+        rc = split ? pair::launch_pair<lce::GradWork, 4, true>("veda_linear_cross_entropy_bwd", p, grid, stream)
+                   : pair::launch_pair<lce::GradWork, 4, false>("veda_linear_cross_entropy_bwd", p, grid, stream);
         if (rc != VEDA_OK) return rc;
     }
     if (dx == nullptr)

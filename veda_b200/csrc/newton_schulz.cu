@@ -12,7 +12,7 @@
 // of 3.4 at 0 amplifies what is rounded off X some 480 times over five steps: with X in 16 bits
 // alone, rounding noise grows into spurious directions (bf16: 1 % of the result on random matrices,
 // a third of it on low-rank ones; fp16 with the lo half in the a X term: 0.15 % and 0.03 %). The
-// products read hi (bf16 outputs), or hi hi + hi lo + lo hi (fp32 outputs, errors of order 2^-20)
+// products read hi (bf16 outputs), or hi lo + lo hi + hi hi (fp32 outputs, errors of order 2^-20)
 // with three times the k-blocks. fp16, not bf16: the values are bounded (singular values stay below
 // 1.3, entries of P below 8), so its 11 bits cost nothing in range; 1024 keeps entries of order
 // 1 / n and their lo halves away from fp16's smallest step.
@@ -38,9 +38,9 @@ struct Params
 {
     CUtensorMap x;           // [cols, rows, 2 batch]: planes hi, lo of each matrix (64 x 64 boxes)
     CUtensorMap a, b;        // [m, m, planes batch]: S and P
-    CUtensorMap out;         // store boxes (64 x 32) of what the launch writes
-    CUtensorMap out_t;       // transposed store boxes (32 x 64) of the same
-    int kind, tall, segments, planes;
+    CUtensorMap out;         // what the launch writes, in boxes of 32 x 32
+    CUtensorMap out_t;       // S, P: the same for transposed tiles; kMuon: the bf16 weights
+    int kind, tall, planes;
     int rows, cols, m;
     int batch, tm, tn, tiles;   // tiles of 256 per matrix: tm x tn, or tm (tm + 1) / 2 symmetric ones
     float ca, cb, cc;
@@ -51,6 +51,7 @@ struct Params
     void* dst;
     int64_t ldo, stride_o;
     int out_f32;
+    int vec;                 // kOut, kMuon: the destination is stored by TMA
     // kMuon
     float* master;
     bf16* lowp;
@@ -77,7 +78,7 @@ struct Work
     struct Tile
     {
         bool skip, a_mn, b_mn;
-        int kbs, per, b, mb, nb;
+        int kbs, b, mb, nb;
         uint32_t idesc;
     };
     struct State
@@ -111,20 +112,16 @@ struct Work
             t.nb = r - t.mb * p.tn;
         }
         const int k = p.kind == kGram ? (p.tall ? p.rows : p.cols) : p.m;
-        t.per = (k + pair::kBK - 1) / pair::kBK;
-        t.kbs = t.per * p.segments;
+        t.kbs = (k + pair::kBK - 1) / pair::kBK;
         t.a_mn = p.kind == kGram && p.tall;
         t.b_mn = p.kind == kGram ? p.tall != 0 : p.kind == kPoly ? false : p.tall == 0;
         t.idesc = pair::idesc(false, t.a_mn, t.b_mn);
         return true;
     }
 
-    static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, int kb,
-                                                    pair::Piece& a, pair::Piece& b)
+    static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, int k, int za,
+                                                    int zb, pair::Piece& a, pair::Piece& b)
     {
-        const int seg = p.segments > 1 ? kb / t.per : 0;
-        const int k = (kb - seg * t.per) * pair::kBK;
-        const int za = seg == 2 ? 1 : 0, zb = seg == 1 ? 1 : 0;
         const int m = t.mb * pair::kTile + rank * 128, n = t.nb * pair::kTile + rank * 128;
         const int x0 = 2 * t.b, s0 = p.planes * t.b;
         if (p.kind == kGram)
@@ -149,35 +146,131 @@ struct Work
         }
     }
 
-    static __device__ __forceinline__ void before(const Params&, const Tile&, State&, int, int, int) {}
-
-    // 64 columns of one plane's row as fp32 pairs, added to v (columns at or past `cols` left alone).
-    static __device__ __forceinline__ void add_row(const uint16_t* src, int left, float f, float (&v)[64])
+    // Epilogue staging. A warp takes 32 rows x 128 columns in four chunks of 32 columns through 8 KB
+    // of shared memory: what a chunk needs of X or S (and the weights) is copied in asynchronously,
+    // coalesced, before the tile's products are done; each lane then works on its row in place, and
+    // the chunk leaves by TMA. Read directly by each lane from its own row, the same epilogues made
+    // the products wait (a X + P X of 28 x 2048 x 1024: 195 us; the weights' update 1860 us).
+    //   offset 0    hi tile (32 rows x 64 bytes, 64-byte swizzle); out: hi, bf16 result, bf16 weights
+    //          2 K  lo tile; out: lo (for unsplit S and P: the transposed tile)
+    //          4 K  fp32 weights (32 rows x 128 bytes, 128-byte swizzle); split S and P: transposed
+    //               hi and lo; fp32 results take 0 .. 4 K
+    // Where a chunk needs 4 KB, two sets alternate.
+    static constexpr int kChunk = 32;
+    static constexpr int kHalfTile = 32 * 64;
+    static __device__ __forceinline__ int sets(const Params& p)
     {
-        if (left >= 64)
+        return p.kind == kMuon || (p.kind <= kPoly && p.planes > 1) ? 1 : 2;
+    }
+    static __device__ __forceinline__ uint32_t swz64(int r, int s)
+    {
+        return static_cast<uint32_t>(r * 64 + ((s ^ ((r >> 1) & 3)) << 4));
+    }
+    static __device__ __forceinline__ void copy16(void* dst, const void* src, bool in)
+    {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(dst)), "l"(src),
+                     "r"(in ? 16u : 0u)
+                     : "memory");
+    }
+    // 32 rows x 32 16-bit columns of a plane; zeros past the last row and column
+    static __device__ __forceinline__ void copy_plane(uint8_t* tile, const uint16_t* src, int64_t ld, int row, int col,
+                                                      int nrows, int ncols, int lane)
+    {
+        const int seg = lane & 3, c = col + seg * 8;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
         {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
+            const int r = 8 * k + (lane >> 2);
+            const bool in = row + r < nrows && c < ncols;
+            copy16(tile + swz64(r, seg), in ? src + (row + r) * ld + c : src, in);
+        }
+    }
+
+    // Starts the copies of chunk j into its set, one group per chunk (empty where nothing is read).
+    static __device__ __forceinline__ void load_chunk(const Params& p, const Tile& t, int j, int trow, int tcol,
+                                                      uint8_t* stage, int lane)
+    {
+        uint8_t* set = stage + (sets(p) == 2 ? (j & 1) * 2 * kHalfTile : 0);
+        const int col = tcol + j * kChunk;
+        if (p.kind == kPoly)
+        {
+            const uint16_t* src = p.s + p.plane_s * p.planes * t.b;
+            copy_plane(set, src, p.lds, trow, col, p.m, p.m, lane);
+            if (p.planes > 1) copy_plane(set + kHalfTile, src + p.plane_s, p.lds, trow, col, p.m, p.m, lane);
+        }
+        else if (p.kind != kGram)
+        {
+            const uint16_t* src = p.xh + p.plane_x * 2 * t.b;
+            copy_plane(set, src, p.ldx, trow, col, p.rows, p.cols, lane);
+            copy_plane(set + kHalfTile, src + p.plane_x, p.ldx, trow, col, p.rows, p.cols, lane);
+            if (p.kind == kMuon && p.vec)
             {
-                const uint4 q = reinterpret_cast<const uint4*>(src)[k];
-                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+                const float* w = p.master + p.stride_o * t.b;
+                const int seg = lane & 7, c = col + seg * 4;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int k = 0; k < 8; ++k)
                 {
-                    const float2 e = unpack_f16(w[j]);
-                    v[8 * k + 2 * j] = fmaf(f, e.x, v[8 * k + 2 * j]);
-                    v[8 * k + 2 * j + 1] = fmaf(f, e.y, v[8 * k + 2 * j + 1]);
+                    const int r = 4 * k + (lane >> 3);
+                    const bool in = trow + r < p.rows && c < p.cols;
+                    copy16(set + 2 * kHalfTile + tc::sw128_offset(r, seg), in ? w + (trow + r) * p.ldo + c : w, in);
                 }
             }
-            return;
         }
-#pragma unroll
-        for (int j = 0; j < 64; ++j)
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+
+    static __device__ __forceinline__ void before(const Params& p, const Tile& t, State&, int row0, int col0,
+                                                  pair::Staging& st, int lane)
+    {
+        // the last tile's copies have landed and its stores have read the staging
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (lane == 0)
         {
-            if (j < left)
+            tc::bulk_wait_group_read<0>();
+        }
+        __syncwarp();
+        const int n = sets(p);
+        for (int j = 0; j < n; ++j)
+        {
+            load_chunk(p, t, j, t.mb * pair::kTile + row0, t.nb * pair::kTile + col0, st.base, lane);
+        }
+    }
+
+    // v += f x the lane's row of a staged 16-bit tile
+    static __device__ __forceinline__ void add_tile(const uint8_t* tile, int lane, float f, float (&v)[kChunk])
+    {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+        {
+            const uint4 q = *reinterpret_cast<const uint4*>(tile + swz64(lane, k));
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
             {
-                v[j] = fmaf(f, __half2float(__ushort_as_half(src[j])), v[j]);
+                const float2 e = unpack_f16(w[i]);
+                v[8 * k + 2 * i] = fmaf(f, e.x, v[8 * k + 2 * i]);
+                v[8 * k + 2 * i + 1] = fmaf(f, e.y, v[8 * k + 2 * i + 1]);
             }
+        }
+    }
+    static __device__ __forceinline__ void put_tile(uint8_t* tile, int lane, const uint32_t (&w)[16])
+    {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+        {
+            *reinterpret_cast<uint4*>(tile + swz64(lane, k)) =
+                make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+        }
+    }
+    // the same transposed: tile row = column, tile column = lane, no swizzle (64 contiguous bytes a store)
+    static __device__ __forceinline__ void put_transposed(uint8_t* tile, int lane, const uint32_t (&w)[16])
+    {
+        uint16_t* out = reinterpret_cast<uint16_t*>(tile) + lane;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+        {
+            out[(2 * i) * 32] = static_cast<uint16_t>(w[i] & 0xFFFFu);
+            out[(2 * i + 1) * 32] = static_cast<uint16_t>(w[i] >> 16);
         }
     }
 
@@ -185,163 +278,205 @@ struct Work
     static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, State&, uint32_t taddr,
                                                     int row0, int col0, pair::Staging& st, int lane)
     {
-        const int trow = t.mb * pair::kTile + row0;
+        const int trow = t.mb * pair::kTile + row0, tcol = t.nb * pair::kTile + col0;
         const bool sym = p.kind <= kPoly;
         const int nrows = sym ? p.m : p.rows, ncols = sym ? p.m : p.cols;
-        if (trow >= nrows)
+        if (trow >= nrows || (p.kind == kMuon && skipped_step(p.flags, p.sumsq, p.grad_scale)))
         {
             return;
         }
         const int row = trow + lane;
-        const bool in = row < nrows;
-        if (p.kind == kMuon && skipped_step(p.flags, p.sumsq, p.grad_scale))
-        {
-            return;
-        }
+        const int nsets = sets(p);
+        const bool mirror = sym && t.mb != t.nb;
+        // the tile's sums carry kUnit^2; what is stored carries kUnit
+        const float f = (p.kind == kPoly ? p.cc : 1.0f) / kUnit;
+        const float g = p.kind == kPoly ? p.cb : p.ca;
 #pragma unroll 1
-        for (int c = 0; c < COLS; c += 64)
+        for (int j = 0; j < COLS / kChunk; ++j)
         {
-            const int col = t.nb * pair::kTile + col0 + c;
-            const int left = ncols - col;
-            if (left <= 0)
+            const int col = tcol + j * kChunk;
+            if (col >= ncols)
             {
                 break;
             }
-            uint32_t r0[32], r1[32];
-            tc::tmem_ld32_async(taddr + static_cast<uint32_t>(c), r0);
-            tc::tmem_ld32_async(taddr + static_cast<uint32_t>(c + 32), r1);
-            tc::tmem_wait_ld();
-            tc::reg_fence(r0);
-            tc::reg_fence(r1);
-            // the tile's sums carry kUnit^2; what is stored carries kUnit
-            const float f = (p.kind == kPoly ? p.cc : 1.0f) / kUnit;
-            float v[64];
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
+            uint8_t* set = st.base + (nsets == 2 ? (j & 1) * 2 * kHalfTile : 0);
+            if (p.kind == kGram)
             {
-                v[j] = __uint_as_float(r0[j]) * f;
-                v[32 + j] = __uint_as_float(r1[j]) * f;
+                // nothing is copied in: the stores of the chunk that last used the set have read it
+                if (lane == 0)
+                {
+                    nsets == 2 ? tc::bulk_wait_group_read<1>() : tc::bulk_wait_group_read<0>();
+                }
             }
-            if (p.kind != kGram && in)
+            else if (nsets == 2)
+            {
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            }
+            else
+            {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+            }
+            __syncwarp();
+            uint32_t r[kChunk];
+            tc::tmem_ld32(taddr + static_cast<uint32_t>(j * kChunk), r);
+            float v[kChunk];
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) v[i] = __uint_as_float(r[i]) * f;
+            if (p.kind != kGram)
             {
                 // lo first: the smaller addend
-                const uint16_t* src = p.kind == kPoly ? p.s + p.plane_s * p.planes * t.b + row * p.lds + col
-                                                      : p.xh + p.plane_x * 2 * t.b + row * p.ldx + col;
-                const int64_t plane = p.kind == kPoly ? p.plane_s : p.plane_x;
-                const float g = p.kind == kPoly ? p.cb : p.ca;
-                if (p.kind != kPoly || p.planes > 1)
-                {
-                    add_row(src + plane, left, g, v);
-                }
-                add_row(src, left, g, v);
+                if (!sym || p.planes > 1) add_tile(set + kHalfTile, lane, g, v);
+                add_tile(set, lane, g, v);
             }
             if (p.kind == kOut || p.kind == kMuon)
             {
-                if (in)
+                finish(p, t, row, col, ncols - col, row < nrows, set, lane, v);
+            }
+            else
+            {
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
                 {
-                    finish(p, t, row, col, left, v);
+                    hi[i] = pack_f16(v[2 * i], v[2 * i + 1]);
+                    const float2 h = unpack_f16(hi[i]);
+                    lo[i] = pack_f16(v[2 * i] - h.x, v[2 * i + 1] - h.y);
                 }
-                continue;
-            }
-            uint32_t hi[32], lo[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-            {
-                hi[j] = pack_f16(v[2 * j], v[2 * j + 1]);
-                const float2 h = unpack_f16(hi[j]);
-                lo[j] = pack_f16(v[2 * j] - h.x, v[2 * j + 1] - h.y);
-            }
-            const int planes = p.kind == kApply ? 2 : p.planes;
-            const int z = planes * t.b;
-            send(p, hi, col, trow, z, st, lane);
-            if (planes > 1)
-            {
-                send(p, lo, col, trow, z + 1, st, lane);
-            }
-            if (sym && t.mb != t.nb)
-            {
-                send_t(p, hi, col, trow, z, st, lane);
-                if (planes > 1)
+                const int planes = sym ? p.planes : 2, z = planes * t.b;
+                put_tile(set, lane, hi);
+                if (planes > 1) put_tile(set + kHalfTile, lane, lo);
+                if (mirror)
                 {
-                    send_t(p, lo, col, trow, z + 1, st, lane);
+                    put_transposed(set + planes * kHalfTile, lane, hi);
+                    if (planes > 1) put_transposed(set + 3 * kHalfTile, lane, lo);
                 }
-            }
-        }
-    }
-
-    static __device__ __forceinline__ void send(const Params& p, const uint32_t (&w)[32], int col, int row,
-                                                int plane, pair::Staging& st, int lane)
-    {
-        uint8_t* buf = st.buffer(lane);
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-        {
-            *reinterpret_cast<uint4*>(buf + tc::sw128_offset(lane, k)) =
-                make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-        }
-        tc::fence_proxy_async();
-        __syncwarp();
-        if (lane == 0)
-        {
-            tc::tma_store_3d(&p.out, buf, col, row, plane);
-            tc::bulk_commit_group();
-        }
-        st.sent();
-    }
-
-    // The same 32 rows x 64 columns at (col, row) transposed: a lane is a column of the 64 x 32 box.
-    static __device__ __forceinline__ void send_t(const Params& p, const uint32_t (&w)[32], int col, int row,
-                                                  int plane, pair::Staging& st, int lane)
-    {
-        uint16_t* buf = reinterpret_cast<uint16_t*>(st.buffer(lane));
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-        {
-            buf[(2 * j) * 32 + lane] = static_cast<uint16_t>(w[j] & 0xFFFFu);
-            buf[(2 * j + 1) * 32 + lane] = static_cast<uint16_t>(w[j] >> 16);
-        }
-        tc::fence_proxy_async();
-        __syncwarp();
-        if (lane == 0)
-        {
-            tc::tma_store_3d(&p.out_t, buf, row, col, plane);
-            tc::bulk_commit_group();
-        }
-        st.sent();
-    }
-
-    // The last product's result: written out, or applied to the weights.
-    static __device__ __forceinline__ void finish(const Params& p, const Tile& t, int row, int col, int left,
-                                                  const float (&v)[64])
-    {
-        const int64_t at = p.stride_o * t.b + static_cast<int64_t>(row) * p.ldo + col;
-#pragma unroll
-        for (int j = 0; j < 64; ++j)
-        {
-            if (j < left)
-            {
-                const float o = v[j] / kUnit;
-                if (p.kind == kMuon)
+                tc::fence_proxy_async();
+                __syncwarp();
+                if (lane == 0)
                 {
-                    float w = p.master[at + j];
-                    w = __fsub_rn(w, __fmul_rn(p.decay, w));
-                    w = __fsub_rn(w, __fmul_rn(p.step, o));
-                    p.master[at + j] = w;
-                    if (p.lowp != nullptr)
+                    tc::tma_store_3d(&p.out, set, col, trow, z);
+                    if (planes > 1) tc::tma_store_3d(&p.out, set + kHalfTile, col, trow, z + 1);
+                    if (mirror)
                     {
-                        p.lowp[at + j] = __float2bfloat16_rn(w);
+                        tc::tma_store_3d(&p.out_t, set + planes * kHalfTile, trow, col, z);
+                        if (planes > 1) tc::tma_store_3d(&p.out_t, set + 3 * kHalfTile, trow, col, z + 1);
                     }
+                    tc::bulk_commit_group();
                 }
-                else if (p.out_f32)
+            }
+            if (p.kind != kGram)
+            {
+                if (j + nsets < COLS / kChunk)
                 {
-                    static_cast<float*>(p.dst)[at + j] = o;
+                    if (lane == 0)
+                    {
+                        tc::bulk_wait_group_read<0>();   // the set's stores have read it
+                    }
+                    __syncwarp();
+                    load_chunk(p, t, j + nsets, trow, tcol, st.base, lane);
                 }
                 else
                 {
-                    static_cast<bf16*>(p.dst)[at + j] = __float2bfloat16_rn(o);
+                    asm volatile("cp.async.commit_group;" ::: "memory");   // keeps the group count
                 }
             }
         }
+    }
+
+    // The last product's result: written out, or applied to the weights, through the staged tiles
+    // where TMA can describe the destination (vec), else element by element.
+    static __device__ __forceinline__ void finish(const Params& p, const Tile& t, int row, int col, int left, bool in,
+                                                  uint8_t* set, int lane, float (&v)[kChunk])
+    {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) v[i] *= 1.0f / kUnit;
+        const int64_t at = p.stride_o * t.b + static_cast<int64_t>(row) * p.ldo + col;
+        if (p.kind == kMuon)
+        {
+            uint8_t* tile = set + 2 * kHalfTile;
+            if (p.vec)
+            {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                {
+                    float4* w4 = reinterpret_cast<float4*>(tile + tc::sw128_offset(lane, k));
+                    float4 w = *w4;
+                    v[4 * k] = update(p, w.x, v[4 * k]);
+                    v[4 * k + 1] = update(p, w.y, v[4 * k + 1]);
+                    v[4 * k + 2] = update(p, w.z, v[4 * k + 2]);
+                    v[4 * k + 3] = update(p, w.w, v[4 * k + 3]);
+                    *w4 = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                }
+            }
+            else if (in)
+            {
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i)
+                {
+                    if (i < left)
+                    {
+                        v[i] = update(p, p.master[at + i], v[i]);
+                        p.master[at + i] = v[i];
+                        if (p.lowp != nullptr) p.lowp[at + i] = __float2bfloat16_rn(v[i]);
+                    }
+                }
+            }
+        }
+        else if (p.out_f32 && p.vec)
+        {
+            __syncwarp();   // every lane has read its row of the tiles that the result overwrites
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+            {
+                *reinterpret_cast<float4*>(set + tc::sw128_offset(lane, k)) =
+                    make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+            }
+        }
+        if (!p.vec)
+        {
+            if (p.kind == kOut && in)
+            {
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i)
+                {
+                    if (i < left)
+                    {
+                        if (p.out_f32) static_cast<float*>(p.dst)[at + i] = v[i];
+                        else static_cast<bf16*>(p.dst)[at + i] = __float2bfloat16_rn(v[i]);
+                    }
+                }
+            }
+            __syncwarp();   // the tiles may be loaded again
+            return;
+        }
+        const bool half = p.kind == kMuon ? p.lowp != nullptr : !p.out_f32;
+        if (half)
+        {
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+            {
+                const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+            put_tile(set, lane, w);
+        }
+        tc::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0)
+        {
+            const int trow = row - lane;
+            if (p.kind == kMuon) tc::tma_store_3d(&p.out, set + 2 * kHalfTile, col, trow, t.b);
+            else tc::tma_store_3d(&p.out, set, col, trow, t.b);
+            if (p.kind == kMuon && half) tc::tma_store_3d(&p.out_t, set, col, trow, t.b);
+            tc::bulk_commit_group();
+        }
+    }
+
+    static __device__ __forceinline__ float update(const Params& p, float w, float o)
+    {
+        w = __fsub_rn(w, __fmul_rn(p.decay, w));
+        return __fsub_rn(w, __fmul_rn(p.step, o));
     }
 };
 
@@ -359,18 +494,36 @@ struct Source
 };
 
 // The gradient as the step sees it: scaled and clipped.
-template <typename T>
-__device__ __forceinline__ float gradient(const Source& s, int64_t at, float scale, float clip)
+__device__ __forceinline__ float seen(float g, float scale, float clip)
 {
-    float g = to_f32(static_cast<const T*>(s.g)[at]);
     if (scale != 1.0f) g = __fmul_rn(g, scale);
     if (clip != 1.0f) g = __fmul_rn(g, clip);
     return g;
 }
 
-// One block of a matrix's rows: updates the momentum (Muon) and leaves the block's sum of squares of
-// what is orthogonalised: G, the momentum m <- beta m + g, or g + beta m (Nesterov).
-template <typename T>
+// N elements at p: one vector load when N > 1
+template <typename T, int N>
+__device__ __forceinline__ void load_n(const T* p, float (&v)[N])
+{
+    if constexpr (N == 1) v[0] = to_f32(*p);
+    else if constexpr (sizeof(T) == 4)
+    {
+        const float4 q = *reinterpret_cast<const float4*>(p);
+        v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+    }
+    else
+    {
+        const uint2 q = *reinterpret_cast<const uint2*>(p);
+        v[0] = __uint_as_float(q.x << 16), v[1] = __uint_as_float(q.x & 0xFFFF0000u);
+        v[2] = __uint_as_float(q.y << 16), v[3] = __uint_as_float(q.y & 0xFFFF0000u);
+    }
+}
+
+// A block takes every gridDim.x-th group of eight rows of matrix blockIdx.y, a warp a row, N elements
+// a lane at a time (4 where rows and bases allow 16-byte accesses of fp32).
+// Updates the momentum (Muon) and leaves the block's sum of squares of what is orthogonalised: G, the
+// momentum m <- beta m + g, or g + beta m (Nesterov). Sums in double: fp32 squares overflow at 2^64.
+template <typename T, int N>
 __global__ void __launch_bounds__(256)
 norm_kernel(Source s, int rows, int cols, double* __restrict__ partials)
 {
@@ -382,20 +535,32 @@ norm_kernel(Source s, int rows, int cols, double* __restrict__ partials)
         return;
     }
     const float clip = clip_scale(s.sumsq, s.max_norm, s.grad_scale);
+    const T* g = static_cast<const T*>(s.g);
     double total = 0.0;
     for (int r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8)
     {
         const int64_t base = s.stride * blockIdx.y + r * s.ld;
-        for (int c = threadIdx.x & 31; c < cols; c += 32)
+#pragma unroll 4
+        for (int c = (threadIdx.x & 31) * N; c < cols; c += 32 * N)
         {
-            float u = gradient<T>(s, base + c, s.grad_scale, clip);
+            float u[N];
+            load_n<T, N>(g + base + c, u);
             if (s.momentum != nullptr)
             {
-                const float m = fmaf(s.beta, s.momentum[base + c], u);
-                s.momentum[base + c] = m;
-                u = s.nesterov ? fmaf(s.beta, m, u) : m;
+                float m[N];
+                load_n<float, N>(s.momentum + base + c, m);
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+                {
+                    u[k] = seen(u[k], s.grad_scale, clip);
+                    m[k] = fmaf(s.beta, m[k], u[k]);
+                    u[k] = s.nesterov ? fmaf(s.beta, m[k], u[k]) : m[k];
+                }
+                if constexpr (N == 4) *reinterpret_cast<float4*>(s.momentum + base + c) = make_float4(m[0], m[1], m[2], m[3]);
+                else s.momentum[base + c] = m[0];
             }
-            total += static_cast<double>(u) * u;
+#pragma unroll
+            for (int k = 0; k < N; ++k) total += static_cast<double>(u[k]) * u[k];
         }
     }
     total = warp_sum(total);
@@ -408,48 +573,69 @@ norm_kernel(Source s, int rows, int cols, double* __restrict__ partials)
     }
 }
 
-// X's two planes: 1024 u / (|u| + eps), the norm summed from the blocks' partials in order.
-template <typename T>
+// X's two planes: 1024 u / (|u| + eps), the norm summed from the blocks' partials in a fixed order.
+template <typename T, int N>
 __global__ void __launch_bounds__(256)
 init_kernel(Source s, int rows, int cols, const double* __restrict__ partials, float eps, uint16_t* __restrict__ x,
             int64_t ldx, int64_t plane)
 {
-    __shared__ float scale_shared;
+    __shared__ double part[8];
     dep_wait();
     dep_release();
     if (skipped_step(s.flags, s.sumsq, s.grad_scale))
     {
         return;
     }
-    if (threadIdx.x == 0)
-    {
-        double total = 0.0;
-        for (int k = 0; k < static_cast<int>(gridDim.x); ++k) total += partials[blockIdx.y * gridDim.x + k];
-        scale_shared = static_cast<float>(static_cast<double>(kUnit) / (sqrt(total) + static_cast<double>(eps)));
-    }
+    // at most 256 blocks a matrix
+    double total = threadIdx.x < gridDim.x ? partials[blockIdx.y * gridDim.x + threadIdx.x] : 0.0;
+    total = warp_sum(total);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = total;
     __syncthreads();
-    const float scale = scale_shared;
+    total = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
+    const float scale = static_cast<float>(static_cast<double>(kUnit) / (sqrt(total) + static_cast<double>(eps)));
     const float clip = clip_scale(s.sumsq, s.max_norm, s.grad_scale);
+    const T* g = static_cast<const T*>(s.g);
     for (int r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8)
     {
         const int64_t base = s.stride * blockIdx.y + r * s.ld;
         uint16_t* out = x + plane * 2 * blockIdx.y + r * ldx;
-        for (int c = threadIdx.x & 31; c < cols; c += 32)
+#pragma unroll 4
+        for (int c = (threadIdx.x & 31) * N; c < cols; c += 32 * N)
         {
-            float u;
+            float u[N];
+            if (s.momentum == nullptr || s.nesterov)
+            {
+                load_n<T, N>(g + base + c, u);
+            }
             if (s.momentum != nullptr)
             {
-                const float m = s.momentum[base + c];
-                u = s.nesterov ? fmaf(s.beta, m, gradient<T>(s, base + c, s.grad_scale, clip)) : m;
+                float m[N];
+                load_n<float, N>(s.momentum + base + c, m);
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+                {
+                    u[k] = s.nesterov ? fmaf(s.beta, m[k], seen(u[k], s.grad_scale, clip)) : m[k];
+                }
+            }
+            uint16_t hi[N], lo[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+            {
+                const float v = u[k] * scale;
+                const __half h = __float2half_rn(v);
+                hi[k] = __half_as_ushort(h);
+                lo[k] = __half_as_ushort(__float2half_rn(v - __half2float(h)));
+            }
+            if constexpr (N == 4)
+            {
+                *reinterpret_cast<uint2*>(out + c) = make_uint2(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16);
+                *reinterpret_cast<uint2*>(out + plane + c) = make_uint2(lo[0] | lo[1] << 16, lo[2] | lo[3] << 16);
             }
             else
             {
-                u = gradient<T>(s, base + c, 1.0f, 1.0f);
+                out[c] = hi[0];
+                out[plane + c] = lo[0];
             }
-            const float v = u * scale;
-            const __half h = __float2half_rn(v);
-            out[c] = __half_as_ushort(h);
-            out[plane + c] = __half_as_ushort(__float2half_rn(v - __half2float(h)));
         }
     }
 }
@@ -483,9 +669,8 @@ Layout layout(int64_t batch, int64_t rows, int64_t cols, bool split)
     l.plane_x = rows * l.ldx;
     l.lds = round_up(l.m, 8);
     l.plane_s = l.m * l.lds;
-    // 8 rows a pass; enough blocks to fill the GPU four times over the batch, at most 64 a matrix
-    const int64_t want = std::max<int64_t>(1, 4 * 148 / batch);
-    l.blocks = static_cast<unsigned>(std::min<int64_t>({(rows + 7) / 8, want, 64}));
+    // 8 rows a pass, at most 256 blocks a matrix; the same for every batch, so that a matrix's norm is
+    l.blocks = static_cast<unsigned>(std::min<int64_t>((rows + 7) / 8, 256));
     l.partials = take(batch * l.blocks * 8);
     l.x[0] = take(batch * 2 * l.plane_x * 2);
     l.x[1] = take(batch * 2 * l.plane_x * 2);
@@ -501,7 +686,8 @@ int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, in
             float b, float c, float eps, bool split, int last, char* ws, Params p, cudaStream_t stream)
 {
     const Layout l = layout(batch, rows, cols, split);
-    const int clusters = pair::clusters_available<Work, 4>();
+    const int clusters =
+        split ? pair::clusters_available<Work, 8, true>() : pair::clusters_available<Work, 8, false>();
     if (clusters < 1)
     {
         return fail(VEDA_ERR_UNSUPPORTED, std::string(what) + ": no CTA pair fits on this device");
@@ -511,30 +697,55 @@ int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, in
     uint16_t* s = reinterpret_cast<uint16_t*>(ws + l.s);
     uint16_t* q = reinterpret_cast<uint16_t*>(ws + l.p);
     // tensor maps: X of either buffer (load, store), S and P (load, store, transposed store)
-    CUtensorMap xl[2], xs[2], ml[2], ms[2], mt[2];
+    CUtensorMap xl[2], xs[2], ml[2], ms[2], mt[2], dst{}, dst_low{};
     bool ok = true;
     for (int k = 0; k < 2; ++k)
     {
         ok = ok && pair::make_map3(&xl[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 64, 64) &&
-             pair::make_map3(&xs[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 64, 32);
+             pair::make_map3(&xs[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 32, 32,
+                             pair::Swizzle::k64);
         const uint16_t* m = k == 0 ? s : q;
         ok = ok && pair::make_map3(&ml[k], m, 2, false, l.m, l.m, l.planes * batch, l.lds, l.plane_s, 64, 64) &&
-             pair::make_map3(&ms[k], m, 2, false, l.m, l.m, l.planes * batch, l.lds, l.plane_s, 64, 32) &&
-             pair::make_map3(&mt[k], m, 2, false, l.m, l.m, l.planes * batch, l.lds, l.plane_s, 32, 64, false);
+             pair::make_map3(&ms[k], m, 2, false, l.m, l.m, l.planes * batch, l.lds, l.plane_s, 32, 32,
+                             pair::Swizzle::k64) &&
+             pair::make_map3(&mt[k], m, 2, false, l.m, l.m, l.planes * batch, l.lds, l.plane_s, 32, 32,
+                             pair::Swizzle::kNone);
     }
     if (!ok)
     {
         return fail(VEDA_ERR_CUDA, std::string(what) + ": tensor map creation failed");
     }
+    // the destination by TMA where its base, pitch and stride are multiples of 16 bytes
+    const auto fits = [&](const void* base, int es) {
+        return aligned16(base) && p.ldo * es % 16 == 0 && (batch == 1 || p.stride_o * es % 16 == 0);
+    };
+    const int64_t stride = batch == 1 ? rows * p.ldo : p.stride_o;
+    if (last == kMuon)
+    {
+        p.vec = fits(p.master, 4) && (p.lowp == nullptr || fits(p.lowp, 2)) &&
+                pair::make_map3(&dst, p.master, 4, false, cols, rows, batch, p.ldo, stride, 32, 32) &&
+                (p.lowp == nullptr || pair::make_map3(&dst_low, p.lowp, 2, true, cols, rows, batch, p.ldo, stride, 32,
+                                                      32, pair::Swizzle::k64));
+    }
+    else
+    {
+        const int es = p.out_f32 ? 4 : 2;
+        p.vec = fits(p.dst, es) && pair::make_map3(&dst, p.dst, es, !p.out_f32, cols, rows, batch, p.ldo, stride, 32, 32,
+                                                   p.out_f32 ? pair::Swizzle::k128 : pair::Swizzle::k64);
+    }
     const dim3 grid(l.blocks, static_cast<unsigned>(batch));
-    int rc = launch(what, norm_kernel<T>, grid, dim3(256), 0, stream, src, static_cast<int>(rows),
-                    static_cast<int>(cols), partials);
+    // four elements at a time where every row of every matrix allows it
+    const uintptr_t bases = reinterpret_cast<uintptr_t>(src.g) | reinterpret_cast<uintptr_t>(src.momentum);
+    const bool four = (bases & (src.momentum != nullptr ? 15u : 4 * sizeof(T) - 1)) == 0 && cols % 4 == 0 &&
+                      src.ld % 4 == 0 && (batch == 1 || src.stride % 4 == 0);
+    int rc = launch(what, four ? norm_kernel<T, 4> : norm_kernel<T, 1>, grid, dim3(256), 0, stream, src,
+                    static_cast<int>(rows), static_cast<int>(cols), partials);
     if (rc != VEDA_OK) return rc;
-    rc = launch(what, init_kernel<T>, grid, dim3(256), 0, stream, src, static_cast<int>(rows),
-                static_cast<int>(cols), static_cast<const double*>(partials), eps, x[0], l.ldx, l.plane_x);
+    rc = launch(what, four ? init_kernel<T, 4> : init_kernel<T, 1>, grid, dim3(256), 0, stream, src,
+                static_cast<int>(rows), static_cast<int>(cols), static_cast<const double*>(partials), eps, x[0], l.ldx,
+                l.plane_x);
     if (rc != VEDA_OK) return rc;
     p.tall = rows > cols;
-    p.segments = split ? 3 : 1;
     p.planes = l.planes;
     p.rows = static_cast<int>(rows);
     p.cols = static_cast<int>(cols);
@@ -562,14 +773,16 @@ int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, in
             p.tm = step < 2 ? tm : static_cast<int>((rows + 255) / 256);
             p.tn = step < 2 ? tm : static_cast<int>((cols + 255) / 256);
             p.tiles = step < 2 ? tm * (tm + 1) / 2 : p.tm * p.tn;
-            p.out = step == 0 ? ms[0] : step == 1 ? ms[1] : xs[(k + 1) & 1];
-            p.out_t = step == 0 ? mt[0] : mt[1];
+            p.out = step == 0 ? ms[0] : step == 1 ? ms[1] : k < steps - 1 ? xs[(k + 1) & 1] : dst;
+            p.out_t = step == 0 ? mt[0] : step == 1 ? mt[1] : dst_low;
             const int64_t units = static_cast<int64_t>(p.tiles) * batch;
             if (units >= (1ll << 30))
             {
                 return fail(VEDA_ERR_INVALID_ARGUMENT, std::string(what) + ": too many tiles");
             }
-            rc = pair::launch_pair<Work, 4>(what, p, static_cast<int>(std::min<int64_t>(units, clusters)), stream);
+            const int grid = static_cast<int>(std::min<int64_t>(units, clusters));
+            rc = split ? pair::launch_pair<Work, 8, true>(what, p, grid, stream)
+                       : pair::launch_pair<Work, 8, false>(what, p, grid, stream);
             if (rc != VEDA_OK) return rc;
         }
     }

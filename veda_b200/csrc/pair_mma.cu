@@ -9,7 +9,8 @@ namespace veda::cuda::pair
 {
 
 bool make_map3(CUtensorMap* map, const void* base, int es, bool is_bf16, int64_t cols, int64_t rows,
-               int64_t planes, int64_t ld, int64_t plane, uint32_t bx, uint32_t by, bool swizzle)
+               int64_t planes, int64_t ld, int64_t plane, uint32_t bx, uint32_t by,
+               Swizzle swizzle)
 {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     static std::once_flag once;
@@ -36,7 +37,9 @@ bool make_map3(CUtensorMap* map, const void* base, int es, bool is_bf16, int64_t
     const cuuint32_t box[3] = {bx, by, 1};
     const cuuint32_t estr[3] = {1, 1, 1};
     return fn(map, type, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+              swizzle == Swizzle::k128  ? CU_TENSOR_MAP_SWIZZLE_128B
+              : swizzle == Swizzle::k64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                        : CU_TENSOR_MAP_SWIZZLE_NONE,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

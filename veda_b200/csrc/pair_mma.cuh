@@ -10,11 +10,19 @@
 // in both orders: K-major (two boxes down the rows) and MN-major (two boxes along the columns).
 // Loads carry no multicast. Every wait is bounded (tc::mbar_wait).
 //
+// SPLIT: operands are pairs of fp16 planes, value = hi + lo, and a product is hi lo + lo hi + hi hi.
+// The tensor core truncates as it adds into its accumulator, an error of some 2^-25 of the running
+// sum per 16 terms and always towards zero: sums of 10000 terms came out 3e-5 short. So the small
+// products go first, and every kChain k-blocks the accumulator is folded into a running sum kept in
+// the other half of TMEM, rounded to nearest (1e-6 and less). The fold is not overlapped with the
+// products: the accumulator has no second buffer then.
+//
 // Work provides
 //   struct Params                      the kernel's argument (tensor maps, pointers, sizes, status)
 //   struct Tile { bool skip; int kbs; uint32_t idesc; bool a_mn, b_mn; ... }
 //   bool tile(p, cid, clusters, i, t)  the i-th tile of cluster cid; false at the end of its list
-//   void operands(p, t, rank, kb, a, b)  where k-block kb's operand pieces of CTA `rank` lie
+//   void operands(p, t, rank, k, za, zb, a, b)  where the operand pieces of CTA `rank` lie for the
+//                                      k-block at k, from the planes za and zb
 //   void epilogue(p, t, state, ...)    one warp's 32 rows x COLS columns of the finished tile
 // All roles walk the same list, so tile() must depend on its arguments and on Params alone.
 #pragma once
@@ -26,6 +34,7 @@ namespace veda::cuda::pair
 
 constexpr int kTile = 256;   // tile rows and columns of a CTA pair
 constexpr int kBK = 64;      // k-block: 64 16-bit values, one 128-byte swizzle row
+constexpr int kChain = 4;    // SPLIT: k-blocks between folds
 
 template <int EPI_WARPS_>
 struct Cfg
@@ -127,7 +136,28 @@ struct Staging
     __device__ __forceinline__ void sent() { ++count; }
 };
 
-template <class Work, int EPI_WARPS>
+// SPLIT: adds the accumulator at `acc` (COLS columns) onto the running sum at `sum`, or starts it;
+// the last fold leaves the total at `acc`, where the epilogue reads it.
+template <int COLS>
+__device__ __forceinline__ void fold(uint32_t acc, uint32_t sum, bool first, bool last)
+{
+#pragma unroll 1
+    for (int c = 0; c < COLS; c += 32)
+    {
+        uint32_t a[32];
+        tc::tmem_ld32(acc + static_cast<uint32_t>(c), a);
+        if (!first)
+        {
+            uint32_t b[32];
+            tc::tmem_ld32(sum + static_cast<uint32_t>(c), b);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) + __uint_as_float(b[j]));
+        }
+        tc::tmem_st32((last ? acc : sum) + static_cast<uint32_t>(c), a);
+    }
+}
+
+template <class Work, int EPI_WARPS, bool SPLIT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI_WARPS>::THREADS, 1)
 pair_kernel(const __grid_constant__ typename Work::Params p)
 {
@@ -193,10 +223,9 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
             {
                 continue;
             }
-            for (int kb = 0; kb < t.kbs; ++kb)
-            {
+            auto load = [&](int kb, int za, int zb) {
                 Piece a, b;
-                Work::operands(p, t, static_cast<int>(rank), kb, a, b);
+                Work::operands(p, t, static_cast<int>(rank), kb * kBK, za, zb, a, b);
                 mbar_wait(&empty[stage], phase ^ 1, p.status, abort);
                 if (rank == 0)
                 {
@@ -214,6 +243,20 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
                     stage = 0;
                     phase ^= 1;
                 }
+            };
+            if constexpr (!SPLIT)
+            {
+                for (int kb = 0; kb < t.kbs; ++kb) load(kb, 0, 0);
+            }
+            else
+            {
+                for (int k0 = 0; k0 < t.kbs; k0 += kChain)
+                {
+                    const int k1 = min(t.kbs, k0 + kChain);
+                    for (int kb = k0; kb < k1; ++kb) load(kb, 0, 1);
+                    for (int kb = k0; kb < k1; ++kb) load(kb, 1, 0);
+                    for (int kb = k0; kb < k1; ++kb) load(kb, 0, 0);
+                }
             }
         }
     }
@@ -227,33 +270,37 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
             {
                 continue;
             }
-            const int buf = it & 1;
-            mbar_wait(&tempty[buf], ((it >> 1) & 1) ^ 1, p.status, abort);
-            fence_after();
-            const uint32_t d = tmem + static_cast<uint32_t>(buf * kTile);
             const uint32_t astep = t.a_mn ? 2048 : 32, bstep = t.b_mn ? 2048 : 32;
             const uint32_t albo = t.a_mn ? kBK * 128 : 16, blbo = t.b_mn ? kBK * 128 : 16;
-            for (int kb = 0; kb < t.kbs; ++kb)
+            for (int k0 = 0; k0 < t.kbs; k0 += SPLIT ? kChain : t.kbs)
             {
-                mbar_wait(&full[stage], phase, p.status, abort);
+                const int blocks = SPLIT ? 3 * (min(t.kbs, k0 + kChain) - k0) : t.kbs;
+                const int buf = SPLIT ? 0 : it & 1;
+                mbar_wait(&tempty[buf], ((SPLIT ? it : it >> 1) & 1) ^ 1, p.status, abort);
                 fence_after();
-                const uint32_t ab = smem_u32(sa + stage * C_::OPERAND);
-                const uint32_t bb = smem_u32(sb + stage * C_::OPERAND);
+                const uint32_t d = tmem + static_cast<uint32_t>(buf * kTile);
+                for (int kb = 0; kb < blocks; ++kb)
+                {
+                    mbar_wait(&full[stage], phase, p.status, abort);
+                    fence_after();
+                    const uint32_t ab = smem_u32(sa + stage * C_::OPERAND);
+                    const uint32_t bb = smem_u32(sb + stage * C_::OPERAND);
 #pragma unroll
-                for (int kk = 0; kk < kBK / 16; ++kk)
-                {
-                    mma2(d, smem_desc(ab + kk * astep, albo, 1024), smem_desc(bb + kk * bstep, blbo, 1024),
-                         t.idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+                    for (int kk = 0; kk < kBK / 16; ++kk)
+                    {
+                        mma2(d, smem_desc(ab + kk * astep, albo, 1024), smem_desc(bb + kk * bstep, blbo, 1024),
+                             t.idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+                    }
+                    commit2(&empty[stage]);
+                    if (++stage == C_::STAGES)
+                    {
+                        stage = 0;
+                        phase ^= 1;
+                    }
                 }
-                commit2(&empty[stage]);
-                if (++stage == C_::STAGES)
-                {
-                    stage = 0;
-                    phase ^= 1;
-                }
+                commit2(&tfull[buf]);
+                ++it;
             }
-            commit2(&tfull[buf]);
-            ++it;
         }
     }
     else if (warp >= 2)
@@ -271,24 +318,39 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
             {
                 continue;
             }
-            const int buf = it & 1;
             const int row0 = static_cast<int>(rank) * 128 + quarter * 32;   // within the tile
-            Work::before(p, t, state, row0, col0, lane);
-            mbar_wait(&tfull[buf], (it >> 1) & 1, p.status, abort);
-            fence_after();
-            const uint32_t base = tmem + static_cast<uint32_t>(buf * kTile + col0) +
-                                  (static_cast<uint32_t>(quarter * 32) << 16);
-            Work::template epilogue<COLS>(p, t, state, base, row0, col0, st, lane);
-            fence_before();
-            __syncwarp();
-            if (lane == 0)
+            Work::before(p, t, state, row0, col0, st, lane);
+            for (int k0 = 0; k0 < t.kbs; k0 += SPLIT ? kChain : t.kbs)
             {
-                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
-                                 release + static_cast<uint32_t>(buf * 8))
-                             : "memory");
+                const int buf = SPLIT ? 0 : it & 1;
+                mbar_wait(&tfull[buf], (SPLIT ? it : it >> 1) & 1, p.status, abort);
+                fence_after();
+                const uint32_t base = tmem + static_cast<uint32_t>(buf * kTile + col0) +
+                                      (static_cast<uint32_t>(quarter * 32) << 16);
+                const bool last = !SPLIT || k0 + kChain >= t.kbs;
+                if constexpr (SPLIT)
+                {
+                    if (t.kbs > kChain)
+                    {
+                        fold<COLS>(base, base + kTile, k0 == 0, last);
+                    }
+                }
+                if (last)
+                {
+                    Work::template epilogue<COLS>(p, t, state, base, row0, col0, st, lane);
+                }
+                fence_before();
+                __syncwarp();
+                if (lane == 0)
+                {
+                    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                                     release + static_cast<uint32_t>(buf * 8))
+                                 : "memory");
+                }
+                ++it;
             }
-            ++it;
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");   // copies an epilogue left in flight
         if (lane == 0)
         {
             bulk_wait_group<0>();   // staged output fully written before the CTA's memory goes
@@ -306,14 +368,16 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
 
 // ---- host ------------------------------------------------------------------------------------
 // A tensor map over `planes` row-major matrices of `rows` x `cols` (element size es: 2 for 16-bit,
-// 4 for fp32), rows ld elements and planes `plane` elements apart, with boxes of bx x by and the
-// 128-byte swizzle (or none). The base must be 16-byte aligned, ld and plane multiples of 16 bytes.
+// 4 for fp32), rows ld elements and planes `plane` elements apart, with boxes of bx x by (bx of at
+// most the swizzle's bytes). The base must be 16-byte aligned, ld and plane multiples of 16 bytes.
+enum class Swizzle { kNone, k64, k128 };
 bool make_map3(CUtensorMap* map, const void* base, int es, bool is_bf16, int64_t cols, int64_t rows,
-               int64_t planes, int64_t ld, int64_t plane, uint32_t bx, uint32_t by, bool swizzle = true);
+               int64_t planes, int64_t ld, int64_t plane, uint32_t bx, uint32_t by,
+               Swizzle swizzle = Swizzle::k128);
 
 // Clusters of the kernel that the current device can hold at once, capped by the SMs that
 // veda_set_reserved_sms leaves (0: none fit). Cached per device.
-template <class Work, int EPI_WARPS>
+template <class Work, int EPI_WARPS, bool SPLIT>
 int clusters_available()
 {
     constexpr int kDevices = 64;
@@ -327,7 +391,7 @@ int clusters_available()
     int have = cached[device].load(std::memory_order_acquire);
     if (have == 0)
     {
-        auto kernel = pair_kernel<Work, EPI_WARPS>;
+        auto kernel = pair_kernel<Work, EPI_WARPS, SPLIT>;
         int n = 0;
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<EPI_WARPS>::SMEM) ==
             cudaSuccess)
@@ -356,10 +420,10 @@ int clusters_available()
     return have - 1 < cap ? have - 1 : cap;
 }
 
-template <class Work, int EPI_WARPS>
+template <class Work, int EPI_WARPS, bool SPLIT>
 int launch_pair(const char* what, const typename Work::Params& p, int clusters, cudaStream_t s)
 {
-    return launch(what, pair_kernel<Work, EPI_WARPS>, dim3(2 * clusters), dim3(Cfg<EPI_WARPS>::THREADS),
+    return launch(what, pair_kernel<Work, EPI_WARPS, SPLIT>, dim3(2 * clusters), dim3(Cfg<EPI_WARPS>::THREADS),
                   Cfg<EPI_WARPS>::SMEM, s, p);
 }
 
