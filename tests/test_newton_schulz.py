@@ -54,10 +54,11 @@ def rounded(g, split, steps=5, coef=NS, eps=EPS):
     x = two(x / (x.square().sum((-2, -1), keepdim=True).sqrt() + eps))
     op = two if split else h
     a, b, c = coef
+    eye = t.eye(x.shape[-2], dtype=t.float64, device=x.device)
     for k in range(steps):
         s = op(op(x) @ op(x).mT)
-        p = op(b * s + c * (s @ s))
-        x = a * x + p @ op(x)
+        m = op(a * eye + b * s + c * (s @ s))
+        x = m @ op(x) + a * (x - op(x))
         if k < steps - 1:
             x = two(x)
     return x.mT if tall else x

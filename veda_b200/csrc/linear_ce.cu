@@ -60,8 +60,9 @@ struct Scalars
 
 struct Params
 {
-    CUtensorMap x, w;        // operands [rows, dim], [vocab, dim]; plane 1: the lo halves
-    CUtensorMap q_in;        // piece of q read by the gradient products
+    CUtensorMap x, w;        // operands [rows, dim], [vocab, dim] K-major; plane 1: the lo halves
+    CUtensorMap x_mn, w_mn;  // the same, MN-major
+    CUtensorMap q_in, q_mn;  // piece of q read by the gradient products
     CUtensorMap q_out;       // piece of q written (store boxes)
     CUtensorMap dx, dw;      // fp32 sums of dx; dW (store boxes)
     int rows, vocab, dim;
@@ -69,7 +70,8 @@ struct Params
     int is_bf16;
     int num_m;               // row tiles
     // logits of this launch: vocabulary rows v0 .. v0 + 256 num_n
-    int v0, num_n, strip;
+    int v0, num_n, strip_log2;
+    pair::Divisor by_m, by_d;   // num_m, num_d
     // gradient products of this launch: q_in holds vocabulary rows g0 .. g0 + gcols
     int g0, gcols, num_d, dw_tiles, dx_tiles;
     int dx_add;              // dx sums: 0 store, 1 add
@@ -136,30 +138,32 @@ struct StatsWork
     // the head, which therefore comes from HBM once, while the rows stay in L2.
     static __device__ __forceinline__ bool tile(const Params& p, int cid, int clusters, int i, Tile& t)
     {
-        const int strips = (p.num_n + p.strip - 1) / p.strip;
-        const int unit = cid + i / p.strip * clusters;
-        if (unit >= strips * p.num_m)
+        const int strip = 1 << p.strip_log2, sub = i & (strip - 1);
+        t.slot = p.by_m.div(cid + (i >> p.strip_log2) * clusters, t.mb);
+        t.nb = (t.slot << p.strip_log2) + sub;
+        if (t.nb - sub >= p.num_n)
         {
             return false;
         }
-        const int sub = i % p.strip;
-        t.slot = unit / p.num_m;
-        t.mb = unit - t.slot * p.num_m;
-        t.nb = t.slot * p.strip + sub;
         t.skip = t.nb >= p.num_n;
         t.first = sub == 0;
-        t.last = sub == p.strip - 1 || t.nb == p.num_n - 1;
+        t.last = sub == strip - 1 || t.nb == p.num_n - 1;
         t.kbs = (p.dim + pair::kBK - 1) / pair::kBK;
         t.a_mn = t.b_mn = false;
         t.idesc = pair::idesc(p.is_bf16 != 0, false, false);
         return true;
     }
 
-    static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, int k, int za,
-                                                    int zb, pair::Piece& a, pair::Piece& b)
+    static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, pair::Piece& a,
+                                                    pair::Piece& b)
     {
-        a = {&p.x, k, t.mb * pair::kTile + rank * 128, za};
-        b = {&p.w, k, p.v0 + t.nb * pair::kTile + rank * 128, zb};
+        a = {&p.x, 0, t.mb * pair::kTile + rank * 128, 0};
+        b = {&p.w, 0, p.v0 + t.nb * pair::kTile + rank * 128, 0};
+    }
+    static __device__ __forceinline__ void prefetch(const Params& p)
+    {
+        tc::tma_prefetch(&p.x);
+        tc::tma_prefetch(&p.w);
     }
 
     static __device__ __forceinline__ void before(const Params& p, const Tile& t, State& s, int row0, int,
@@ -267,8 +271,7 @@ struct GradWork
         if (u < p.dw_tiles)
         {
             t.kind = kDw;
-            t.mb = u / p.num_d;
-            t.nb = u - t.mb * p.num_d;
+            t.mb = p.by_d.div(u, t.nb);
             t.kbs = (p.rows + pair::kBK - 1) / pair::kBK;
             t.a_mn = t.b_mn = true;
             t.idesc = pair::idesc(bf, true, true);
@@ -278,8 +281,7 @@ struct GradWork
         if (u < p.dx_tiles)
         {
             t.kind = kDx;
-            t.mb = u / p.num_d;
-            t.nb = u - t.mb * p.num_d;
+            t.mb = p.by_d.div(u, t.nb);
             t.kbs = (p.gcols + pair::kBK - 1) / pair::kBK;
             t.a_mn = false;
             t.b_mn = true;
@@ -292,33 +294,41 @@ struct GradWork
             return false;
         }
         t.kind = kQ;
-        t.nb = u / p.num_m;
-        t.mb = u - t.nb * p.num_m;
+        t.nb = p.by_m.div(u, t.mb);
         t.kbs = (p.dim + pair::kBK - 1) / pair::kBK;
         t.a_mn = t.b_mn = false;
         t.idesc = pair::idesc(bf, false, false);
         return true;
     }
 
-    static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, int k, int za,
-                                                    int zb, pair::Piece& a, pair::Piece& b)
+    static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, pair::Piece& a,
+                                                    pair::Piece& b)
     {
         const int m = t.mb * pair::kTile + rank * 128, n = t.nb * pair::kTile + rank * 128;
         if (t.kind == kDw)
         {
-            a = {&p.q_in, m, k, za};
-            b = {&p.x, n, k, zb};
+            a = {&p.q_mn, m, 0, 0};
+            b = {&p.x_mn, n, 0, 0};
         }
         else if (t.kind == kDx)
         {
-            a = {&p.q_in, k, m, za};
-            b = {&p.w, n, p.g0 + k, zb};
+            a = {&p.q_in, 0, m, 0};
+            b = {&p.w_mn, n, p.g0, 0};
         }
         else
         {
-            a = {&p.x, k, m, za};
-            b = {&p.w, k, p.v0 + n, zb};
+            a = {&p.x, 0, m, 0};
+            b = {&p.w, 0, p.v0 + n, 0};
         }
+    }
+    static __device__ __forceinline__ void prefetch(const Params& p)
+    {
+        tc::tma_prefetch(&p.x);
+        tc::tma_prefetch(&p.w);
+        tc::tma_prefetch(&p.x_mn);
+        tc::tma_prefetch(&p.w_mn);
+        tc::tma_prefetch(&p.q_in);
+        tc::tma_prefetch(&p.q_mn);
     }
 
     static __device__ __forceinline__ void before(const Params& p, const Tile& t, State& s, int row0, int,
@@ -938,8 +948,11 @@ int prepare(const Call& c, const int64_t* targets, int64_t ignore, const float* 
         }
     }
     const bool bf = c.dtype == VEDA_BF16;
-    if (!pair::make_map3(&p.x, px, 2, bf, c.dim, c.rows, c.l.planes, ldx, c.rows * ldx, 64, 64) ||
-        !pair::make_map3(&p.w, pw, 2, bf, c.dim, c.vocab, c.l.planes, ldw, c.vocab * ldw, 64, 64))
+    if (!pair::make_map3(&p.x, px, 2, bf, c.dim, c.rows, c.l.planes, ldx, c.rows * ldx, 64, 128) ||
+        !pair::make_map3(&p.w, pw, 2, bf, c.dim, c.vocab, c.l.planes, ldw, c.vocab * ldw, 64, 128) ||
+        (c.backward &&
+         (!pair::make_map3(&p.x_mn, px, 2, bf, c.dim, c.rows, c.l.planes, ldx, c.rows * ldx, 64, 64) ||
+          !pair::make_map3(&p.w_mn, pw, 2, bf, c.dim, c.vocab, c.l.planes, ldw, c.vocab * ldw, 64, 64))))
     {
         return fail(VEDA_ERR_CUDA, "veda_linear_cross_entropy: tensor map creation failed");
     }
@@ -950,6 +963,8 @@ int prepare(const Call& c, const int64_t* targets, int64_t ignore, const float* 
     p.is_bf16 = bf;
     p.num_m = static_cast<int>((c.rows + 255) / 256);
     p.num_d = static_cast<int>((c.dim + 255) / 256);
+    p.by_m = pair::Divisor(static_cast<uint32_t>(p.num_m));
+    p.by_d = pair::Divisor(static_cast<uint32_t>(p.num_d));
     p.scalars = c.scalars();
     p.targets = targets;
     p.ignore = ignore;
@@ -1028,7 +1043,7 @@ extern "C" int veda_linear_cross_entropy_fwd(const void* x, int64_t ldx, const v
     rc = lce::prepare(c, targets, ignore_index, nullptr, nullptr, false, p, stream);
     if (rc != VEDA_OK) return rc;
     p.num_n = static_cast<int>((vocab + 255) / 256);
-    p.strip = c.l.strip;
+    while ((1 << p.strip_log2) < c.l.strip) ++p.strip_log2;
     p.parts = reinterpret_cast<float2*>(c.ws + c.l.parts);
     p.target_logit = reinterpret_cast<float*>(c.ws + c.l.target_logit);
     const int64_t units = static_cast<int64_t>(c.l.slots) * p.num_m;
@@ -1089,12 +1104,13 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
     if (rc != VEDA_OK) return rc;
     const int64_t piece = c.l.piece, plane = rows * piece;
     const bool bf = dtype == VEDA_BF16;
-    CUtensorMap q_load[2], q_store[2];
+    CUtensorMap q_load[2], q_mn[2], q_store[2];
     bool ok = true;
     for (int b = 0; b < 2; ++b)
     {
         char* q = c.ws + c.l.q + static_cast<size_t>(b) * c.l.planes * plane * 2;
-        ok = ok && pair::make_map3(&q_load[b], q, 2, bf, piece, rows, c.l.planes, piece, plane, 64, 64) &&
+        ok = ok && pair::make_map3(&q_load[b], q, 2, bf, piece, rows, c.l.planes, piece, plane, 64, 128) &&
+             pair::make_map3(&q_mn[b], q, 2, bf, piece, rows, c.l.planes, piece, plane, 64, 64) &&
              pair::make_map3(&q_store[b], q, 2, bf, piece, rows, c.l.planes, piece, plane, 64, 32);
     }
     float* acc = reinterpret_cast<float*>(c.ws + c.l.acc);
@@ -1117,6 +1133,8 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
         return fail(VEDA_ERR_CUDA, "veda_linear_cross_entropy_bwd: tensor map creation failed");
     }
     p.lse = lse;
+    p.q_in = q_load[0];
+    p.q_mn = q_mn[0];
     // launch c: q of piece c, and the products of piece c - 1
     const int64_t pieces = (vocab + piece - 1) / piece;
     for (int64_t k = 0; k <= pieces; ++k)
@@ -1134,6 +1152,7 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
             p.g0 = static_cast<int>((k - 1) * piece);
             p.gcols = static_cast<int>(std::min(piece, vocab - (k - 1) * piece));
             p.q_in = q_load[(k - 1) & 1];
+            p.q_mn = q_mn[(k - 1) & 1];
             p.dw_tiles = dw != nullptr ? (p.gcols + 255) / 256 * p.num_d : 0;
             p.dx_tiles = dx != nullptr ? p.num_m * p.num_d : 0;
             p.dx_add = k > 1;

@@ -1,21 +1,23 @@
 // Orthogonalisation of matrices by Newton-Schulz products, and the Muon step built on it.
 //
 // For each matrix of a batch, X = G / (|G|_F + eps), then `steps` times
-//   S = X X^T (of the smaller side),  P = b S + c S^2,  X <- a X + P X,
+//   S = X X^T (of the smaller side),  M = a I + b S + c S^2,  X <- M X,
 // the odd quintic a s + b s^3 + c s^5 applied to every singular value. Three products an iteration
 // on the CTA-pair tensor-core kernel (pair_mma.cuh), the whole batch in one launch each; a tall
-// matrix is multiplied from the other side (S = X^T X, X <- a X + X P) by operand order alone, so
-// nothing is transposed. S and P are symmetric: the tiles on and above the diagonal are computed,
-// and each one above it is written a second time, transposed.
+// matrix is multiplied from the other side (S = X^T X, X <- X M) by operand order alone, so nothing
+// is transposed. S and M are symmetric: the tiles on and above the diagonal are computed, and each
+// one above it is written a second time, transposed.
 //
 // Precision. X is held as two fp16 values, 1024 X = hi + lo (22 bits), because the quintic's slope
 // of 3.4 at 0 amplifies what is rounded off X some 480 times over five steps: with X in 16 bits
-// alone, rounding noise grows into spurious directions (bf16: 1 % of the result on random matrices,
-// a third of it on low-rank ones; fp16 with the lo half in the a X term: 0.15 % and 0.03 %). The
-// products read hi (bf16 outputs), or hi lo + lo hi + hi hi (fp32 outputs, errors of order 2^-20)
-// with three times the k-blocks. fp16, not bf16: the values are bounded (singular values stay below
-// 1.3, entries of P below 8), so its 11 bits cost nothing in range; 1024 keeps entries of order
-// 1 / n and their lo halves away from fp16's smallest step.
+// alone, rounding noise grows into spurious directions (errors, relative to the result, on random /
+// rank-8 matrices of 512 x 1024: bf16 1.0 % / 32 %; fp16 0.14 % / 4 %). For bf16 results the products
+// read hi, and a lo, exact to first order where the slope matters, is added to them: 0.15 % / 0.13 %,
+// less than the result's own rounding. Because M multiplies X as a whole, rounding M leaves the rank
+// of X as it is. For fp32 results S, M and X enter as hi lo + lo hi + hi hi (errors of order 2^-20).
+// fp16, not bf16: the values are bounded (singular values stay below 1.3, entries of M below 8), so
+// its 11 bits cost nothing in range; 1024 keeps entries of order 1 / n and their lo halves away from
+// fp16's smallest step.
 #include "clip.cuh"
 #include "pair_mma.cuh"
 
@@ -32,28 +34,28 @@ namespace ns
 
 constexpr float kUnit = 1024.0f;   // stored value = kUnit x value
 
+// What a launch computes: S, M, the next X, or the last X as a result or as the weights' update.
 enum Kind { kGram, kPoly, kApply, kOut, kMuon };
 
 struct Params
 {
-    CUtensorMap x;           // [cols, rows, 2 batch]: planes hi, lo of each matrix (64 x 64 boxes)
-    CUtensorMap a, b;        // [m, m, planes batch]: S and P
+    CUtensorMap a, b;        // operands: planes hi, lo of each matrix (X; S and M when split)
     CUtensorMap out;         // what the launch writes, in boxes of 32 x 32
-    CUtensorMap out_t;       // S, P: the same for transposed tiles; kMuon: the bf16 weights
-    int kind, tall, planes;
-    int rows, cols, m;
-    int batch, tm, tn, tiles;   // tiles of 256 per matrix: tm x tn, or tm (tm + 1) / 2 symmetric ones
+    CUtensorMap out_t;       // S, M: the same for transposed tiles; kMuon: the bf16 weights
+    int tall;
+    int rows, cols;          // of X
+    int nrows, ncols;        // of what is written
+    int k;                   // terms of a sum
+    int planes_a, planes_b;  // planes of a matrix in a and b
+    int total, tm;           // tiles in all; kGram, kPoly: tiles of a side
+    pair::Divisor per_matrix, by_n;
     float ca, cb, cc;
-    const uint16_t* xh;      // X as read by the epilogue: planes, pitch and plane stride
-    const uint16_t* s;       // S as read by the epilogue
-    int64_t ldx, plane_x, lds, plane_s;
-    // kOut
-    void* dst;
+    const uint16_t* src;     // kPoly: S; later kinds: X (read by the epilogue)
+    int64_t ld, plane;       // its pitch and plane stride
+    // kOut, kMuon: the destination, stored by TMA if vec
+    void* dst;               // kMuon: the fp32 weights
     int64_t ldo, stride_o;
-    int out_f32;
-    int vec;                 // kOut, kMuon: the destination is stored by TMA
-    // kMuon
-    float* master;
+    int out_f32, vec;
     bf16* lowp;
     float decay, step;       // lr weight_decay, lr scale
     const double* sumsq;
@@ -72,9 +74,11 @@ __device__ __forceinline__ float2 unpack_f16(uint32_t w)
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
+template <int KIND, bool SPLIT>
 struct Work
 {
     using Params = ns::Params;
+    static constexpr bool SYM = KIND <= kPoly;
     struct Tile
     {
         bool skip, a_mn, b_mn;
@@ -83,19 +87,19 @@ struct Work
     };
     struct State
     {
+        int sent = 0;   // chunks written out so far: the output sets take turns by it across tiles
     };
 
     static __device__ __forceinline__ bool tile(const Params& p, int cid, int clusters, int i, Tile& t)
     {
         const int u = cid + i * clusters;
-        if (u >= p.tiles * p.batch)
+        if (u >= p.total)
         {
             return false;
         }
-        t.skip = false;
-        t.b = u / p.tiles;
-        int r = u - t.b * p.tiles;
-        if (p.kind <= kPoly)
+        int r;
+        t.b = p.per_matrix.div(u, r);
+        if constexpr (SYM)
         {
             // row mb of the upper triangle holds tm - mb tiles
             t.mb = 0;
@@ -108,60 +112,72 @@ struct Work
         }
         else
         {
-            t.mb = r / p.tn;
-            t.nb = r - t.mb * p.tn;
+            t.mb = p.by_n.div(r, t.nb);
         }
-        const int k = p.kind == kGram ? (p.tall ? p.rows : p.cols) : p.m;
-        t.kbs = (k + pair::kBK - 1) / pair::kBK;
-        t.a_mn = p.kind == kGram && p.tall;
-        t.b_mn = p.kind == kGram ? p.tall != 0 : p.kind == kPoly ? false : p.tall == 0;
+        t.skip = false;
+        t.kbs = (p.k + pair::kBK - 1) / pair::kBK;
+        // tall: S = X^T X, X M; else S = X X^T, M X; S and M read as they are, being symmetric
+        t.a_mn = KIND == kGram && p.tall;
+        t.b_mn = KIND == kGram ? p.tall != 0 : KIND != kPoly && p.tall == 0;
         t.idesc = pair::idesc(false, t.a_mn, t.b_mn);
         return true;
     }
 
-    static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, int k, int za,
-                                                    int zb, pair::Piece& a, pair::Piece& b)
+    static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, pair::Piece& a,
+                                                    pair::Piece& b)
     {
         const int m = t.mb * pair::kTile + rank * 128, n = t.nb * pair::kTile + rank * 128;
-        const int x0 = 2 * t.b, s0 = p.planes * t.b;
-        if (p.kind == kGram)
-        {
-            a = p.tall ? pair::Piece{&p.x, m, k, x0 + za} : pair::Piece{&p.x, k, m, x0 + za};
-            b = p.tall ? pair::Piece{&p.x, n, k, x0 + zb} : pair::Piece{&p.x, k, n, x0 + zb};
-        }
-        else if (p.kind == kPoly)
-        {
-            a = {&p.a, k, m, s0 + za};
-            b = {&p.a, k, n, s0 + zb};
-        }
-        else if (p.tall)
-        {
-            a = {&p.x, k, m, x0 + za};
-            b = {&p.b, k, n, s0 + zb};
-        }
-        else
-        {
-            a = {&p.b, k, m, s0 + za};
-            b = {&p.x, n, k, x0 + zb};
-        }
+        a = {&p.a, t.a_mn ? m : 0, t.a_mn ? 0 : m, p.planes_a * t.b};
+        b = {&p.b, t.b_mn ? n : 0, t.b_mn ? 0 : n, p.planes_b * t.b};
+    }
+    static __device__ __forceinline__ void prefetch(const Params& p)
+    {
+        tc::tma_prefetch(&p.a);
+        tc::tma_prefetch(&p.b);
     }
 
     // Epilogue staging. A warp takes 32 rows x 128 columns in four chunks of 32 columns through 8 KB
-    // of shared memory: what a chunk needs of X or S (and the weights) is copied in asynchronously,
-    // coalesced, before the tile's products are done; each lane then works on its row in place, and
-    // the chunk leaves by TMA. Read directly by each lane from its own row, the same epilogues made
-    // the products wait (a X + P X of 28 x 2048 x 1024: 195 us; the weights' update 1860 us).
-    //   offset 0    hi tile (32 rows x 64 bytes, 64-byte swizzle); out: hi, bf16 result, bf16 weights
-    //          2 K  lo tile; out: lo (for unsplit S and P: the transposed tile)
-    //          4 K  fp32 weights (32 rows x 128 bytes, 128-byte swizzle); split S and P: transposed
-    //               hi and lo; fp32 results take 0 .. 4 K
-    // Where a chunk needs 4 KB, two sets alternate.
+    // of shared memory, four units of 2 KB (32 rows x 64 bytes, 64-byte swizzle) or two of 4 KB (32
+    // rows x 128 bytes, 128-byte swizzle): what a chunk needs is copied in asynchronously, coalesced,
+    // before the tile's products are done, each lane works on its row, and the chunk leaves by TMA.
+    // Read and written by each lane in its own row of global memory instead, the epilogue held the
+    // products up (M X of 28 x 2048 x 1024 195 us, the weights' update 1860 us).
+    //                 copied in                     written out
+    //   kGram         -                             hi, transposed hi, two sets
+    //         split   -                             hi, lo, transposed hi, lo
+    //   kPoly         S hi at 0 and 1 in turn       hi at 2, transposed at 3
+    //         split   S hi at 0, lo at 1            hi, lo in place, transposed at 2 and 3
+    //   kApply, kOut  X lo at 0 and 1 in turn       hi at 2, lo at 3; result at 2 and 3 in turn
+    //         split   -                             hi, lo in two sets; fp32 result in two sets
+    //   kMuon         X lo at 0, weights at 2 - 3   weights in place, bf16 weights at 1
+    //         split   weights at 0 - 1, 2 - 3       in place
     static constexpr int kChunk = 32;
-    static constexpr int kHalfTile = 32 * 64;
-    static __device__ __forceinline__ int sets(const Params& p)
+    static constexpr int kUnitBytes = 32 * 64;
+    static constexpr bool READS_X = !SPLIT && !SYM;        // the a lo term
+    static constexpr bool IN_PLACE = KIND == kMuon || (KIND == kPoly && SPLIT);
+    // chunks copied in ahead, and sets that a chunk's output takes turns in
+    static constexpr int AHEAD = KIND == kGram              ? 0
+                                 : KIND == kPoly            ? (SPLIT ? 1 : 2)
+                                 : KIND == kMuon            ? (SPLIT ? 2 : 1)
+                                 : READS_X                  ? 2
+                                                            : 0;
+    static constexpr int OUTS = KIND == kGram    ? (SPLIT ? 1 : 2)
+                                : KIND == kPoly  ? 1
+                                : KIND == kApply ? (SPLIT ? 2 : 1)
+                                                 : 2;
+    static __device__ __forceinline__ int in_unit(int j)
     {
-        return p.kind == kMuon || (p.kind <= kPoly && p.planes > 1) ? 1 : 2;
+        return AHEAD == 2 ? (j & 1) * (KIND == kMuon ? 2 : 1) : 0;
     }
+    static __device__ __forceinline__ int out_unit(int j)
+    {
+        if constexpr (KIND == kMuon) return 1;             // of the bf16 weights
+        else if constexpr (KIND == kPoly) return SPLIT ? 0 : 2;
+        else if constexpr (KIND == kGram) return SPLIT ? 0 : 2 * (j & 1);
+        else if constexpr (SPLIT) return 2 * (j & 1);
+        else return KIND == kOut ? 2 + (j & 1) : 2;
+    }
+
     static __device__ __forceinline__ uint32_t swz64(int r, int s)
     {
         return static_cast<uint32_t>(r * 64 + ((s ^ ((r >> 1) & 3)) << 4));
@@ -173,46 +189,48 @@ struct Work
                      : "memory");
     }
     // 32 rows x 32 16-bit columns of a plane; zeros past the last row and column
-    static __device__ __forceinline__ void copy_plane(uint8_t* tile, const uint16_t* src, int64_t ld, int row, int col,
-                                                      int nrows, int ncols, int lane)
+    static __device__ __forceinline__ void copy_plane(uint8_t* tile, const uint16_t* src, const Params& p, int row,
+                                                      int col, int lane)
     {
         const int seg = lane & 3, c = col + seg * 8;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
         {
             const int r = 8 * k + (lane >> 2);
-            const bool in = row + r < nrows && c < ncols;
-            copy16(tile + swz64(r, seg), in ? src + (row + r) * ld + c : src, in);
+            const bool in = row + r < p.nrows && c < p.ncols;
+            copy16(tile + swz64(r, seg), in ? src + (row + r) * p.ld + c : src, in);
         }
     }
 
-    // Starts the copies of chunk j into its set, one group per chunk (empty where nothing is read).
+    // Starts the copies of chunk j, one group (empty where nothing is read).
     static __device__ __forceinline__ void load_chunk(const Params& p, const Tile& t, int j, int trow, int tcol,
                                                       uint8_t* stage, int lane)
     {
-        uint8_t* set = stage + (sets(p) == 2 ? (j & 1) * 2 * kHalfTile : 0);
+        uint8_t* in = stage + in_unit(j) * kUnitBytes;
         const int col = tcol + j * kChunk;
-        if (p.kind == kPoly)
+        if constexpr (KIND == kPoly)
         {
-            const uint16_t* src = p.s + p.plane_s * p.planes * t.b;
-            copy_plane(set, src, p.lds, trow, col, p.m, p.m, lane);
-            if (p.planes > 1) copy_plane(set + kHalfTile, src + p.plane_s, p.lds, trow, col, p.m, p.m, lane);
+            const uint16_t* src = p.src + p.plane * p.planes_a * t.b;
+            copy_plane(in, src, p, trow, col, lane);
+            if constexpr (SPLIT) copy_plane(in + kUnitBytes, src + p.plane, p, trow, col, lane);
         }
-        else if (p.kind != kGram)
+        if constexpr (READS_X)
         {
-            const uint16_t* src = p.xh + p.plane_x * 2 * t.b;
-            copy_plane(set, src, p.ldx, trow, col, p.rows, p.cols, lane);
-            copy_plane(set + kHalfTile, src + p.plane_x, p.ldx, trow, col, p.rows, p.cols, lane);
-            if (p.kind == kMuon && p.vec)
+            copy_plane(in, p.src + p.plane * (2 * t.b + 1), p, trow, col, lane);
+        }
+        if constexpr (KIND == kMuon)
+        {
+            if (p.vec)
             {
-                const float* w = p.master + p.stride_o * t.b;
+                uint8_t* tile = SPLIT ? in : stage + 2 * kUnitBytes;
+                const float* w = static_cast<const float*>(p.dst) + p.stride_o * t.b;
                 const int seg = lane & 7, c = col + seg * 4;
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
                 {
                     const int r = 4 * k + (lane >> 3);
-                    const bool in = trow + r < p.rows && c < p.cols;
-                    copy16(set + 2 * kHalfTile + tc::sw128_offset(r, seg), in ? w + (trow + r) * p.ldo + c : w, in);
+                    const bool inside = trow + r < p.nrows && c < p.ncols;
+                    copy16(tile + tc::sw128_offset(r, seg), inside ? w + (trow + r) * p.ldo + c : w, inside);
                 }
             }
         }
@@ -222,17 +240,20 @@ struct Work
     static __device__ __forceinline__ void before(const Params& p, const Tile& t, State&, int row0, int col0,
                                                   pair::Staging& st, int lane)
     {
-        // the last tile's copies have landed and its stores have read the staging
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        if (lane == 0)
+        if constexpr (AHEAD > 0)
         {
-            tc::bulk_wait_group_read<0>();
-        }
-        __syncwarp();
-        const int n = sets(p);
-        for (int j = 0; j < n; ++j)
-        {
-            load_chunk(p, t, j, t.mb * pair::kTile + row0, t.nb * pair::kTile + col0, st.base, lane);
+            // the last tile's copies have landed, and in place, its stores have read the staging
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (IN_PLACE && lane == 0)
+            {
+                tc::bulk_wait_group_read<0>();
+            }
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j)
+            {
+                load_chunk(p, t, j, t.mb * pair::kTile + row0, t.nb * pair::kTile + col0, st.base, lane);
+            }
         }
     }
 
@@ -262,6 +283,15 @@ struct Work
                 make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
         }
     }
+    static __device__ __forceinline__ void put_f32(uint8_t* tile, int lane, const float (&v)[kChunk])
+    {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+        {
+            *reinterpret_cast<float4*>(tile + tc::sw128_offset(lane, k)) =
+                make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+        }
+    }
     // the same transposed: tile row = column, tile column = lane, no swizzle (64 contiguous bytes a store)
     static __device__ __forceinline__ void put_transposed(uint8_t* tile, int lane, const uint32_t (&w)[16])
     {
@@ -275,201 +305,127 @@ struct Work
     }
 
     template <int COLS>
-    static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, State&, uint32_t taddr,
+    static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, State& s, uint32_t taddr,
                                                     int row0, int col0, pair::Staging& st, int lane)
     {
         const int trow = t.mb * pair::kTile + row0, tcol = t.nb * pair::kTile + col0;
-        const bool sym = p.kind <= kPoly;
-        const int nrows = sym ? p.m : p.rows, ncols = sym ? p.m : p.cols;
-        if (trow >= nrows || (p.kind == kMuon && skipped_step(p.flags, p.sumsq, p.grad_scale)))
+        if (trow >= p.nrows || (KIND == kMuon && skipped_step(p.flags, p.sumsq, p.grad_scale)))
         {
             return;
         }
-        const int row = trow + lane;
-        const int nsets = sets(p);
-        const bool mirror = sym && t.mb != t.nb;
+        const bool mirror = SYM && t.mb != t.nb;
         // the tile's sums carry kUnit^2; what is stored carries kUnit
-        const float f = (p.kind == kPoly ? p.cc : 1.0f) / kUnit;
-        const float g = p.kind == kPoly ? p.cb : p.ca;
+        const float f = (KIND == kPoly ? p.cc : 1.0f) / kUnit;
 #pragma unroll 1
         for (int j = 0; j < COLS / kChunk; ++j)
         {
             const int col = tcol + j * kChunk;
-            if (col >= ncols)
+            if (col >= p.ncols)
             {
                 break;
             }
-            uint8_t* set = st.base + (nsets == 2 ? (j & 1) * 2 * kHalfTile : 0);
-            if (p.kind == kGram)
-            {
-                // nothing is copied in: the stores of the chunk that last used the set have read it
-                if (lane == 0)
-                {
-                    nsets == 2 ? tc::bulk_wait_group_read<1>() : tc::bulk_wait_group_read<0>();
-                }
-            }
-            else if (nsets == 2)
-            {
-                asm volatile("cp.async.wait_group 1;" ::: "memory");
-            }
-            else
-            {
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-            }
-            __syncwarp();
+            uint8_t* in = st.base + in_unit(j) * kUnitBytes;
+            uint8_t* out = st.base + out_unit(s.sent++) * kUnitBytes;
             uint32_t r[kChunk];
             tc::tmem_ld32(taddr + static_cast<uint32_t>(j * kChunk), r);
             float v[kChunk];
 #pragma unroll
             for (int i = 0; i < kChunk; ++i) v[i] = __uint_as_float(r[i]) * f;
-            if (p.kind != kGram)
+            if constexpr (AHEAD > 0)
             {
-                // lo first: the smaller addend
-                if (!sym || p.planes > 1) add_tile(set + kHalfTile, lane, g, v);
-                add_tile(set, lane, g, v);
+                asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD > 0 ? AHEAD - 1 : 0) : "memory");
+                __syncwarp();   // every lane's copies are visible to the warp
+                if constexpr (KIND == kPoly)
+                {
+                    // lo first: the smaller addend
+                    if constexpr (SPLIT) add_tile(in + kUnitBytes, lane, p.cb, v);
+                    add_tile(in, lane, p.cb, v);
+                }
+                if constexpr (READS_X) add_tile(in, lane, p.ca, v);
             }
-            if (p.kind == kOut || p.kind == kMuon)
+            if constexpr (KIND == kPoly)
             {
-                finish(p, t, row, col, ncols - col, row < nrows, set, lane, v);
+                const int d = trow + lane - col;   // the lane's diagonal element
+#pragma unroll
+                for (int i = 0; i < kChunk; ++i) v[i] = i == d ? v[i] + p.ca * kUnit : v[i];
+            }
+            if constexpr (!IN_PLACE)
+            {
+                if constexpr (AHEAD > 0)
+                {
+                    __syncwarp();   // the chunk is read: its unit is free
+                    next_chunk<COLS>(p, t, j, trow, tcol, st.base, lane);
+                }
+                if (lane == 0)
+                {
+                    tc::bulk_wait_group_read<OUTS - 1>();   // the stores that last used `out` have read it
+                }
+                __syncwarp();
+            }
+            if constexpr (KIND == kOut || KIND == kMuon)
+            {
+                finish(p, t, trow, col, in, out, st.base, lane, v);
             }
             else
             {
+                constexpr int PLANES = KIND == kApply || SPLIT ? 2 : 1;
+                const int z = PLANES * t.b;
                 uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                 {
                     hi[i] = pack_f16(v[2 * i], v[2 * i + 1]);
-                    const float2 h = unpack_f16(hi[i]);
-                    lo[i] = pack_f16(v[2 * i] - h.x, v[2 * i + 1] - h.y);
+                    if constexpr (PLANES == 2)
+                    {
+                        const float2 h = unpack_f16(hi[i]);
+                        lo[i] = pack_f16(v[2 * i] - h.x, v[2 * i + 1] - h.y);
+                    }
                 }
-                const int planes = sym ? p.planes : 2, z = planes * t.b;
-                put_tile(set, lane, hi);
-                if (planes > 1) put_tile(set + kHalfTile, lane, lo);
+                put_tile(out, lane, hi);
+                if constexpr (PLANES == 2) put_tile(out + kUnitBytes, lane, lo);
                 if (mirror)
                 {
-                    put_transposed(set + planes * kHalfTile, lane, hi);
-                    if (planes > 1) put_transposed(set + 3 * kHalfTile, lane, lo);
+                    put_transposed(out + PLANES * kUnitBytes, lane, hi);
+                    if constexpr (PLANES == 2) put_transposed(out + 3 * kUnitBytes, lane, lo);
                 }
                 tc::fence_proxy_async();
                 __syncwarp();
                 if (lane == 0)
                 {
-                    tc::tma_store_3d(&p.out, set, col, trow, z);
-                    if (planes > 1) tc::tma_store_3d(&p.out, set + kHalfTile, col, trow, z + 1);
+                    tc::tma_store_3d(&p.out, out, col, trow, z);
+                    if constexpr (PLANES == 2) tc::tma_store_3d(&p.out, out + kUnitBytes, col, trow, z + 1);
                     if (mirror)
                     {
-                        tc::tma_store_3d(&p.out_t, set + planes * kHalfTile, trow, col, z);
-                        if (planes > 1) tc::tma_store_3d(&p.out_t, set + 3 * kHalfTile, trow, col, z + 1);
+                        tc::tma_store_3d(&p.out_t, out + PLANES * kUnitBytes, trow, col, z);
+                        if constexpr (PLANES == 2) tc::tma_store_3d(&p.out_t, out + 3 * kUnitBytes, trow, col, z + 1);
                     }
                     tc::bulk_commit_group();
                 }
             }
-            if (p.kind != kGram)
+            if constexpr (IN_PLACE)
             {
-                if (j + nsets < COLS / kChunk)
+                if (lane == 0)
                 {
-                    if (lane == 0)
-                    {
-                        tc::bulk_wait_group_read<0>();   // the set's stores have read it
-                    }
-                    __syncwarp();
-                    load_chunk(p, t, j + nsets, trow, tcol, st.base, lane);
+                    tc::bulk_wait_group_read<0>();   // the stores have read the units
                 }
-                else
-                {
-                    asm volatile("cp.async.commit_group;" ::: "memory");   // keeps the group count
-                }
+                __syncwarp();
+                next_chunk<COLS>(p, t, j, trow, tcol, st.base, lane);
             }
         }
     }
 
-    // The last product's result: written out, or applied to the weights, through the staged tiles
-    // where TMA can describe the destination (vec), else element by element.
-    static __device__ __forceinline__ void finish(const Params& p, const Tile& t, int row, int col, int left, bool in,
-                                                  uint8_t* set, int lane, float (&v)[kChunk])
+    // The copies of chunk j + AHEAD, or an empty group past the last, which keeps the groups counted.
+    template <int COLS>
+    static __device__ __forceinline__ void next_chunk(const Params& p, const Tile& t, int j, int trow, int tcol,
+                                                      uint8_t* stage, int lane)
     {
-#pragma unroll
-        for (int i = 0; i < kChunk; ++i) v[i] *= 1.0f / kUnit;
-        const int64_t at = p.stride_o * t.b + static_cast<int64_t>(row) * p.ldo + col;
-        if (p.kind == kMuon)
+        if (j + AHEAD < COLS / kChunk)
         {
-            uint8_t* tile = set + 2 * kHalfTile;
-            if (p.vec)
-            {
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                {
-                    float4* w4 = reinterpret_cast<float4*>(tile + tc::sw128_offset(lane, k));
-                    float4 w = *w4;
-                    v[4 * k] = update(p, w.x, v[4 * k]);
-                    v[4 * k + 1] = update(p, w.y, v[4 * k + 1]);
-                    v[4 * k + 2] = update(p, w.z, v[4 * k + 2]);
-                    v[4 * k + 3] = update(p, w.w, v[4 * k + 3]);
-                    *w4 = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-                }
-            }
-            else if (in)
-            {
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i)
-                {
-                    if (i < left)
-                    {
-                        v[i] = update(p, p.master[at + i], v[i]);
-                        p.master[at + i] = v[i];
-                        if (p.lowp != nullptr) p.lowp[at + i] = __float2bfloat16_rn(v[i]);
-                    }
-                }
-            }
+            load_chunk(p, t, j + AHEAD, trow, tcol, stage, lane);
         }
-        else if (p.out_f32 && p.vec)
+        else
         {
-            __syncwarp();   // every lane has read its row of the tiles that the result overwrites
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-            {
-                *reinterpret_cast<float4*>(set + tc::sw128_offset(lane, k)) =
-                    make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-            }
-        }
-        if (!p.vec)
-        {
-            if (p.kind == kOut && in)
-            {
-#pragma unroll
-                for (int i = 0; i < kChunk; ++i)
-                {
-                    if (i < left)
-                    {
-                        if (p.out_f32) static_cast<float*>(p.dst)[at + i] = v[i];
-                        else static_cast<bf16*>(p.dst)[at + i] = __float2bfloat16_rn(v[i]);
-                    }
-                }
-            }
-            __syncwarp();   // the tiles may be loaded again
-            return;
-        }
-        const bool half = p.kind == kMuon ? p.lowp != nullptr : !p.out_f32;
-        if (half)
-        {
-            uint32_t w[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-            {
-                const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-                w[i] = *reinterpret_cast<const uint32_t*>(&b);
-            }
-            put_tile(set, lane, w);
-        }
-        tc::fence_proxy_async();
-        __syncwarp();
-        if (lane == 0)
-        {
-            const int trow = row - lane;
-            if (p.kind == kMuon) tc::tma_store_3d(&p.out, set + 2 * kHalfTile, col, trow, t.b);
-            else tc::tma_store_3d(&p.out, set, col, trow, t.b);
-            if (p.kind == kMuon && half) tc::tma_store_3d(&p.out_t, set, col, trow, t.b);
-            tc::bulk_commit_group();
+            asm volatile("cp.async.commit_group;" ::: "memory");
         }
     }
 
@@ -477,6 +433,107 @@ struct Work
     {
         w = __fsub_rn(w, __fmul_rn(p.decay, w));
         return __fsub_rn(w, __fmul_rn(p.step, o));
+    }
+    static __device__ __forceinline__ void pack_bf16(const float (&v)[kChunk], uint32_t (&w)[16])
+    {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+        {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+    }
+
+    // The last product's result: written out, or applied to the weights, through the staging where TMA
+    // can describe the destination, else element by element.
+    static __device__ __forceinline__ void finish(const Params& p, const Tile& t, int trow, int col, uint8_t* in,
+                                                  uint8_t* out, uint8_t* stage, int lane, float (&v)[kChunk])
+    {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) v[i] *= 1.0f / kUnit;
+        if (!p.vec)
+        {
+            finish_direct(p, t, trow + lane, col, v);
+            return;
+        }
+        uint32_t w16[16];
+        if constexpr (KIND == kMuon)
+        {
+            uint8_t* tile = SPLIT ? in : stage + 2 * kUnitBytes;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+            {
+                const float4 w = *reinterpret_cast<const float4*>(tile + tc::sw128_offset(lane, k));
+                v[4 * k] = update(p, w.x, v[4 * k]);
+                v[4 * k + 1] = update(p, w.y, v[4 * k + 1]);
+                v[4 * k + 2] = update(p, w.z, v[4 * k + 2]);
+                v[4 * k + 3] = update(p, w.w, v[4 * k + 3]);
+            }
+            put_f32(tile, lane, v);
+            if constexpr (!SPLIT)
+            {
+                pack_bf16(v, w16);
+                put_tile(out, lane, w16);
+            }
+            tc::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0)
+            {
+                tc::tma_store_3d(&p.out, tile, col, trow, t.b);
+                if constexpr (!SPLIT) tc::tma_store_3d(&p.out_t, out, col, trow, t.b);
+                tc::bulk_commit_group();
+            }
+        }
+        else
+        {
+            if constexpr (SPLIT)
+            {
+                put_f32(out, lane, v);
+            }
+            else
+            {
+                pack_bf16(v, w16);
+                put_tile(out, lane, w16);
+            }
+            tc::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0)
+            {
+                tc::tma_store_3d(&p.out, out, col, trow, t.b);
+                tc::bulk_commit_group();
+            }
+        }
+    }
+
+    static __device__ __forceinline__ void finish_direct(const Params& p, const Tile& t, int row, int col,
+                                                         float (&v)[kChunk])
+    {
+        if (row >= p.nrows)
+        {
+            return;
+        }
+        const int64_t at = p.stride_o * t.b + static_cast<int64_t>(row) * p.ldo + col;
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i)
+        {
+            if (col + i < p.ncols)
+            {
+                if constexpr (KIND == kMuon)
+                {
+                    float* w = static_cast<float*>(p.dst) + at + i;
+                    *w = update(p, *w, v[i]);
+                    if (p.lowp != nullptr) p.lowp[at + i] = __float2bfloat16_rn(*w);
+                }
+                else if (p.out_f32)
+                {
+                    static_cast<float*>(p.dst)[at + i] = v[i];
+                }
+                else
+                {
+                    static_cast<bf16*>(p.dst)[at + i] = __float2bfloat16_rn(v[i]);
+                }
+            }
+        }
     }
 };
 
@@ -680,36 +737,42 @@ Layout layout(int64_t batch, int64_t rows, int64_t cols, bool split)
     return l;
 }
 
-// norm, X, then the products of every step; p's output fields say what the last one writes.
-template <typename T>
-int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, int64_t cols, int steps, float a,
-            float b, float c, float eps, bool split, int last, char* ws, Params p, cudaStream_t stream)
+template <int KIND, bool SPLIT>
+int product(const char* what, const Params& p, cudaStream_t stream)
 {
-    const Layout l = layout(batch, rows, cols, split);
-    const int clusters =
-        split ? pair::clusters_available<Work, 8, true>() : pair::clusters_available<Work, 8, false>();
+    const int clusters = pair::clusters_available<Work<KIND, SPLIT>, 8, SPLIT>();
     if (clusters < 1)
     {
         return fail(VEDA_ERR_UNSUPPORTED, std::string(what) + ": no CTA pair fits on this device");
     }
+    return pair::launch_pair<Work<KIND, SPLIT>, 8, SPLIT>(what, p, std::min(p.total, clusters), stream);
+}
+
+// norm, X, then the products of every step; p's destination says what the last one (LAST) writes.
+template <typename T, bool SPLIT, int LAST>
+int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, int64_t cols, int steps, float a,
+            float b, float c, float eps, char* ws, Params p, cudaStream_t stream)
+{
+    const Layout l = layout(batch, rows, cols, SPLIT);
     double* partials = reinterpret_cast<double*>(ws + l.partials);
     uint16_t* x[2] = {reinterpret_cast<uint16_t*>(ws + l.x[0]), reinterpret_cast<uint16_t*>(ws + l.x[1])};
-    uint16_t* s = reinterpret_cast<uint16_t*>(ws + l.s);
-    uint16_t* q = reinterpret_cast<uint16_t*>(ws + l.p);
-    // tensor maps: X of either buffer (load, store), S and P (load, store, transposed store)
-    CUtensorMap xl[2], xs[2], ml[2], ms[2], mt[2], dst{}, dst_low{};
+    uint16_t* sm[2] = {reinterpret_cast<uint16_t*>(ws + l.s), reinterpret_cast<uint16_t*>(ws + l.p)};
+    const bool tall = rows > cols;
+    const int64_t m = l.m, sp = l.planes * batch;
+    // X of either buffer as S's operands, as M's partner (K-major boxes are 128 high) and written; S and
+    // M read (they are symmetric: K-major always), written, and written transposed
+    CUtensorMap xg[2], xa[2], xs[2], ml[2], ms[2], mt[2], dst{}, dst_low{};
     bool ok = true;
     for (int k = 0; k < 2; ++k)
     {
-        ok = ok && pair::make_map3(&xl[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 64, 64) &&
+        ok = ok &&
+             pair::make_map3(&xg[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 64, tall ? 64 : 128) &&
+             pair::make_map3(&xa[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 64, tall ? 128 : 64) &&
              pair::make_map3(&xs[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 32, 32,
-                             pair::Swizzle::k64);
-        const uint16_t* m = k == 0 ? s : q;
-        ok = ok && pair::make_map3(&ml[k], m, 2, false, l.m, l.m, l.planes * batch, l.lds, l.plane_s, 64, 64) &&
-             pair::make_map3(&ms[k], m, 2, false, l.m, l.m, l.planes * batch, l.lds, l.plane_s, 32, 32,
                              pair::Swizzle::k64) &&
-             pair::make_map3(&mt[k], m, 2, false, l.m, l.m, l.planes * batch, l.lds, l.plane_s, 32, 32,
-                             pair::Swizzle::kNone);
+             pair::make_map3(&ml[k], sm[k], 2, false, m, m, sp, l.lds, l.plane_s, 64, 128) &&
+             pair::make_map3(&ms[k], sm[k], 2, false, m, m, sp, l.lds, l.plane_s, 32, 32, pair::Swizzle::k64) &&
+             pair::make_map3(&mt[k], sm[k], 2, false, m, m, sp, l.lds, l.plane_s, 32, 32, pair::Swizzle::kNone);
     }
     if (!ok)
     {
@@ -720,19 +783,13 @@ int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, in
         return aligned16(base) && p.ldo * es % 16 == 0 && (batch == 1 || p.stride_o * es % 16 == 0);
     };
     const int64_t stride = batch == 1 ? rows * p.ldo : p.stride_o;
-    if (last == kMuon)
-    {
-        p.vec = fits(p.master, 4) && (p.lowp == nullptr || fits(p.lowp, 2)) &&
-                pair::make_map3(&dst, p.master, 4, false, cols, rows, batch, p.ldo, stride, 32, 32) &&
-                (p.lowp == nullptr || pair::make_map3(&dst_low, p.lowp, 2, true, cols, rows, batch, p.ldo, stride, 32,
-                                                      32, pair::Swizzle::k64));
-    }
-    else
-    {
-        const int es = p.out_f32 ? 4 : 2;
-        p.vec = fits(p.dst, es) && pair::make_map3(&dst, p.dst, es, !p.out_f32, cols, rows, batch, p.ldo, stride, 32, 32,
-                                                   p.out_f32 ? pair::Swizzle::k128 : pair::Swizzle::k64);
-    }
+    const bool f32 = LAST == kMuon || SPLIT;
+    p.out_f32 = f32;
+    p.vec = fits(p.dst, f32 ? 4 : 2) && (p.lowp == nullptr || fits(p.lowp, 2)) &&
+            pair::make_map3(&dst, p.dst, f32 ? 4 : 2, !f32, cols, rows, batch, p.ldo, stride, 32, 32,
+                            f32 ? pair::Swizzle::k128 : pair::Swizzle::k64) &&
+            (p.lowp == nullptr || pair::make_map3(&dst_low, p.lowp, 2, true, cols, rows, batch, p.ldo, stride, 32, 32,
+                                                  pair::Swizzle::k64));
     const dim3 grid(l.blocks, static_cast<unsigned>(batch));
     // four elements at a time where every row of every matrix allows it
     const uintptr_t bases = reinterpret_cast<uintptr_t>(src.g) | reinterpret_cast<uintptr_t>(src.momentum);
@@ -745,46 +802,62 @@ int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, in
                 static_cast<int>(rows), static_cast<int>(cols), static_cast<const double*>(partials), eps, x[0], l.ldx,
                 l.plane_x);
     if (rc != VEDA_OK) return rc;
-    p.tall = rows > cols;
-    p.planes = l.planes;
+    const int64_t tm = (m + 255) / 256, tr = (rows + 255) / 256, tc = (cols + 255) / 256;
+    const int64_t half = tm * (tm + 1) / 2 * batch, whole = tr * tc * batch;
+    if (half >= (1ll << 30) || whole >= (1ll << 30))
+    {
+        return fail(VEDA_ERR_INVALID_ARGUMENT, std::string(what) + ": too many tiles");
+    }
+    p.tall = tall;
     p.rows = static_cast<int>(rows);
     p.cols = static_cast<int>(cols);
-    p.m = static_cast<int>(l.m);
-    p.batch = static_cast<int>(batch);
     p.ca = a;
     p.cb = b;
     p.cc = c;
-    p.s = s;
-    p.ldx = l.ldx;
-    p.plane_x = l.plane_x;
-    p.lds = l.lds;
-    p.plane_s = l.plane_s;
-    p.a = ml[0];
-    p.b = ml[1];
+    p.tm = static_cast<int>(tm);
+    p.by_n = pair::Divisor(static_cast<uint32_t>(tc));
     p.status = device_status_ptr();
-    const int tm = static_cast<int>((l.m + 255) / 256);
+    const pair::Divisor per_half(static_cast<uint32_t>(tm * (tm + 1) / 2)), per_whole(static_cast<uint32_t>(tr * tc));
     for (int k = 0; k < steps; ++k)
     {
-        p.x = xl[k & 1];
-        p.xh = x[k & 1];
-        for (int step = 0; step < 3; ++step)
-        {
-            p.kind = step < 2 ? step : k == steps - 1 ? last : kApply;
-            p.tm = step < 2 ? tm : static_cast<int>((rows + 255) / 256);
-            p.tn = step < 2 ? tm : static_cast<int>((cols + 255) / 256);
-            p.tiles = step < 2 ? tm * (tm + 1) / 2 : p.tm * p.tn;
-            p.out = step == 0 ? ms[0] : step == 1 ? ms[1] : k < steps - 1 ? xs[(k + 1) & 1] : dst;
-            p.out_t = step == 0 ? mt[0] : step == 1 ? mt[1] : dst_low;
-            const int64_t units = static_cast<int64_t>(p.tiles) * batch;
-            if (units >= (1ll << 30))
-            {
-                return fail(VEDA_ERR_INVALID_ARGUMENT, std::string(what) + ": too many tiles");
-            }
-            const int grid = static_cast<int>(std::min<int64_t>(units, clusters));
-            rc = split ? pair::launch_pair<Work, 8, true>(what, p, grid, stream)
-                       : pair::launch_pair<Work, 8, false>(what, p, grid, stream);
-            if (rc != VEDA_OK) return rc;
-        }
+        p.total = static_cast<int>(half);
+        p.per_matrix = per_half;
+        p.nrows = p.ncols = static_cast<int>(m);
+        // S
+        p.a = p.b = xg[k & 1];
+        p.planes_a = p.planes_b = 2;
+        p.k = static_cast<int>(std::max(rows, cols));
+        p.out = ms[0];
+        p.out_t = mt[0];
+        rc = product<kGram, SPLIT>(what, p, stream);
+        if (rc != VEDA_OK) return rc;
+        // M
+        p.a = p.b = ml[0];
+        p.planes_a = p.planes_b = l.planes;
+        p.k = static_cast<int>(m);
+        p.src = sm[0];
+        p.ld = l.lds;
+        p.plane = l.plane_s;
+        p.out = ms[1];
+        p.out_t = mt[1];
+        rc = product<kPoly, SPLIT>(what, p, stream);
+        if (rc != VEDA_OK) return rc;
+        // M X, or X M
+        p.total = static_cast<int>(whole);
+        p.per_matrix = per_whole;
+        p.nrows = p.rows;
+        p.ncols = p.cols;
+        p.a = tall ? xa[k & 1] : ml[1];
+        p.b = tall ? ml[1] : xa[k & 1];
+        p.planes_a = tall ? 2 : l.planes;
+        p.planes_b = tall ? l.planes : 2;
+        p.src = x[k & 1];
+        p.ld = l.ldx;
+        p.plane = l.plane_x;
+        p.out = k < steps - 1 ? xs[(k + 1) & 1] : dst;
+        p.out_t = dst_low;
+        rc = k < steps - 1 ? product<kApply, SPLIT>(what, p, stream) : product<LAST, SPLIT>(what, p, stream);
+        if (rc != VEDA_OK) return rc;
     }
     return VEDA_OK;
 }
@@ -848,13 +921,12 @@ extern "C" int veda_orthogonalize(const void* g, int64_t ldg, int64_t stride_g, 
     p.dst = out;
     p.ldo = ldo;
     p.stride_o = stride_o;
-    p.out_f32 = split;
     const ns::Source src{g, ldg, stride_g, nullptr, 0.0f, 0, nullptr, 1.0f, 1.0f, 0};
     char* ws = static_cast<char*>(workspace);
-    return split ? ns::iterate<float>("veda_orthogonalize", src, batch, rows, cols, steps, a, b, c, eps, true, ns::kOut,
-                                      ws, p, stream)
-                 : ns::iterate<bf16>("veda_orthogonalize", src, batch, rows, cols, steps, a, b, c, eps, false, ns::kOut,
-                                     ws, p, stream);
+    return split ? ns::iterate<float, true, ns::kOut>("veda_orthogonalize", src, batch, rows, cols, steps, a, b, c, eps,
+                                                      ws, p, stream)
+                 : ns::iterate<bf16, false, ns::kOut>("veda_orthogonalize", src, batch, rows, cols, steps, a, b, c, eps,
+                                                      ws, p, stream);
 }
 
 extern "C" int veda_muon_step(float* master, float* momentum, const float* grad, void* lowp, int64_t batch,
@@ -880,7 +952,7 @@ extern "C" int veda_muon_step(float* master, float* momentum, const float* grad,
                                  ns::layout(batch, rows, cols, split).total);
     if (rc != VEDA_OK) return rc;
     ns::Params p{};
-    p.master = master;
+    p.dst = master;
     p.lowp = static_cast<bf16*>(lowp);
     p.ldo = cols;
     p.stride_o = stride;
@@ -890,6 +962,9 @@ extern "C" int veda_muon_step(float* master, float* momentum, const float* grad,
     p.grad_scale = grad_scale;
     p.flags = flags;
     const ns::Source src{grad, cols, stride, momentum, beta, nesterov, sumsq, max_norm, grad_scale, flags};
-    return ns::iterate<float>("veda_muon_step", src, batch, rows, cols, steps, a, b, c, eps, split, ns::kMuon,
-                              static_cast<char*>(workspace), p, stream);
+    char* ws = static_cast<char*>(workspace);
+    return split ? ns::iterate<float, true, ns::kMuon>("veda_muon_step", src, batch, rows, cols, steps, a, b, c, eps, ws,
+                                                       p, stream)
+                 : ns::iterate<float, false, ns::kMuon>("veda_muon_step", src, batch, rows, cols, steps, a, b, c, eps, ws,
+                                                        p, stream);
 }

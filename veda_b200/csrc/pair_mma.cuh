@@ -4,11 +4,13 @@
 //
 // A cluster of two CTAs computes a tile with tcgen05.mma.cta_group::2 (M 256, N 256, K 16; 16-bit
 // operands, fp32 accumulators in TMEM). Each CTA stages its own 128 rows of A and 128 columns of B
-// (32 KB per 64-deep k-block, six stages), the even CTA issues the products, two 256-column
+// (32 KB per 64-deep k-block, five or six stages), the even CTA issues the products, two 256-column
 // accumulators alternate so that a tile's epilogue runs under the next tile's products. Operands are
-// read through 3-D tensor maps (column, row, plane) with 64 x 64 boxes, so one map serves an operand
-// in both orders: K-major (two boxes down the rows) and MN-major (two boxes along the columns).
-// Loads carry no multicast. Every wait is bounded (tc::mbar_wait).
+// read through 3-D tensor maps (column, row, plane): K-major pieces as one 64 x 128 box, MN-major
+// ones as two 64 x 64 boxes. Loads carry no multicast. Every wait is bounded (tc::mbar_wait).
+// Timestamps of the roles set the rest: a tile's coordinates are worked out while the tile before it
+// is in flight (its divisions held the product thread up by 600 to 2000 cycles a tile, against 8192
+// of products for k = 1024), and a k-block costs the loading thread additions only.
 //
 // SPLIT: operands are pairs of fp16 planes, value = hi + lo, and a product is hi lo + lo hi + hi hi.
 // The tensor core truncates as it adds into its accumulator, an error of some 2^-25 of the running
@@ -21,8 +23,9 @@
 //   struct Params                      the kernel's argument (tensor maps, pointers, sizes, status)
 //   struct Tile { bool skip; int kbs; uint32_t idesc; bool a_mn, b_mn; ... }
 //   bool tile(p, cid, clusters, i, t)  the i-th tile of cluster cid; false at the end of its list
-//   void operands(p, t, rank, k, za, zb, a, b)  where the operand pieces of CTA `rank` lie for the
-//                                      k-block at k, from the planes za and zb
+//   void operands(p, t, rank, a, b)    where the operand pieces of CTA `rank` lie at k = 0
+//   void prefetch(p)                   fetches the tensor maps of the operands
+//   void before(p, t, state, ...)      per epilogue warp, while the tile's products run
 //   void epilogue(p, t, state, ...)    one warp's 32 rows x COLS columns of the finished tile
 // All roles walk the same list, so tile() must depend on its arguments and on Params alone.
 #pragma once
@@ -49,8 +52,8 @@ struct Cfg
     static constexpr int SMEM = STAGES * STAGE + STAGING + 1024 + 256;
 };
 
-// A 128 x 64 operand piece: the tensor map and the coordinates of its first 64 x 64 box; the second
-// lies 64 rows further down (K-major) or 64 columns further right (MN-major).
+// A 128 x 64 operand piece at k = 0: k runs along x (K-major, box 64 x 128) or along y (MN-major, two
+// boxes 64 x 64 side by side). z is the hi plane, z + 1 the lo plane of split operands.
 struct Piece
 {
     const CUtensorMap* map;
@@ -64,6 +67,24 @@ __host__ __device__ constexpr uint32_t idesc(bool is_bf16, bool a_mn, bool b_mn)
     return (1u << 4) | (type << 7) | (type << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
            (static_cast<uint32_t>(kTile >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
 }
+
+// n / d for 0 <= n < 2^31 by a multiplication: m = ceil(2^(31 + s) / d) with 2^s >= d.
+struct Divisor
+{
+    uint32_t m = 0, s = 0, d = 1;
+    __host__ __device__ Divisor() = default;
+    __host__ explicit Divisor(uint32_t n) : d(n)
+    {
+        while ((1ull << s) < n) ++s;
+        m = static_cast<uint32_t>(((1ull << (31 + s)) + n - 1) / n);
+    }
+    __device__ __forceinline__ int div(int n, int& rest) const
+    {
+        const int q = d == 1 ? n : static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * m) >> (31 + s));
+        rest = n - q * static_cast<int>(d);
+        return q;
+    }
+};
 
 __device__ __forceinline__ uint32_t cluster_rank()
 {
@@ -209,70 +230,81 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
     cluster_sync();   // both CTAs' barriers exist before any signal crosses
     fence_after();
     const uint32_t tmem = *tmem_slot;
+    if (threadIdx.x == 0)
+    {
+        Work::prefetch(p);   // the maps are arguments: no need to wait for the kernels before
+    }
     dep_wait();
     dep_release();
 
-    typename Work::Tile t;
+    typename Work::Tile t, next;
+    bool more = Work::tile(p, cid, clusters, 0, t);
+    int i = 0;
     if (warp == 0 && lane == 0)
     {
         int stage = 0;
         uint32_t phase = 0;
-        for (int i = 0; Work::tile(p, cid, clusters, i, t); ++i)
+        while (more)
         {
-            if (t.skip)
+            if (!t.skip)
             {
-                continue;
-            }
-            auto load = [&](int kb, int za, int zb) {
                 Piece a, b;
-                Work::operands(p, t, static_cast<int>(rank), kb * kBK, za, zb, a, b);
-                mbar_wait(&empty[stage], phase ^ 1, p.status, abort);
-                if (rank == 0)
+                Work::operands(p, t, static_cast<int>(rank), a, b);
+                const int adx = t.a_mn ? 0 : kBK, ady = t.a_mn ? kBK : 0;
+                const int bdx = t.b_mn ? 0 : kBK, bdy = t.b_mn ? kBK : 0;
+                auto load = [&](int kb, int za, int zb) {
+                    mbar_wait(&empty[stage], phase ^ 1, p.status, abort);
+                    if (rank == 0)
+                    {
+                        mbar_expect_tx(&full[stage], 2 * C_::STAGE);   // both CTAs' halves
+                    }
+                    const uint32_t bar = peer_addr(&full[stage], 0);
+                    uint8_t* ad = sa + stage * C_::OPERAND;
+                    uint8_t* bd = sb + stage * C_::OPERAND;
+                    const int ax = a.x + kb * adx, ay = a.y + kb * ady;
+                    const int bx = b.x + kb * bdx, by = b.y + kb * bdy;
+                    load_box(ad, a.map, bar, ax, ay, a.z + za);
+                    if (t.a_mn) load_box(ad + C_::OPERAND / 2, a.map, bar, ax + 64, ay, a.z + za);
+                    load_box(bd, b.map, bar, bx, by, b.z + zb);
+                    if (t.b_mn) load_box(bd + C_::OPERAND / 2, b.map, bar, bx + 64, by, b.z + zb);
+                    if (++stage == C_::STAGES)
+                    {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                };
+                if constexpr (!SPLIT)
                 {
-                    mbar_expect_tx(&full[stage], 2 * C_::STAGE);   // both CTAs' halves
+                    for (int kb = 0; kb < t.kbs; ++kb) load(kb, 0, 0);
                 }
-                const uint32_t bar = peer_addr(&full[stage], 0);
-                uint8_t* ad = sa + stage * C_::OPERAND;
-                uint8_t* bd = sb + stage * C_::OPERAND;
-                load_box(ad, a.map, bar, a.x, a.y, a.z);
-                load_box(ad + C_::OPERAND / 2, a.map, bar, a.x + (t.a_mn ? 64 : 0), a.y + (t.a_mn ? 0 : 64), a.z);
-                load_box(bd, b.map, bar, b.x, b.y, b.z);
-                load_box(bd + C_::OPERAND / 2, b.map, bar, b.x + (t.b_mn ? 64 : 0), b.y + (t.b_mn ? 0 : 64), b.z);
-                if (++stage == C_::STAGES)
+                else
                 {
-                    stage = 0;
-                    phase ^= 1;
+                    for (int k0 = 0; k0 < t.kbs; k0 += kChain)
+                    {
+                        const int k1 = min(t.kbs, k0 + kChain);
+                        for (int kb = k0; kb < k1; ++kb) load(kb, 0, 1);
+                        for (int kb = k0; kb < k1; ++kb) load(kb, 1, 0);
+                        for (int kb = k0; kb < k1; ++kb) load(kb, 0, 0);
+                    }
                 }
-            };
-            if constexpr (!SPLIT)
-            {
-                for (int kb = 0; kb < t.kbs; ++kb) load(kb, 0, 0);
             }
-            else
-            {
-                for (int k0 = 0; k0 < t.kbs; k0 += kChain)
-                {
-                    const int k1 = min(t.kbs, k0 + kChain);
-                    for (int kb = k0; kb < k1; ++kb) load(kb, 0, 1);
-                    for (int kb = k0; kb < k1; ++kb) load(kb, 1, 0);
-                    for (int kb = k0; kb < k1; ++kb) load(kb, 0, 0);
-                }
-            }
+            more = Work::tile(p, cid, clusters, ++i, t);   // the ring is full of this tile's blocks
         }
     }
     else if (warp == 1 && lane == 0 && rank == 0)
     {
         int stage = 0, it = 0;
         uint32_t phase = 0;
-        for (int i = 0; Work::tile(p, cid, clusters, i, t); ++i)
+        while (more)
         {
+            bool more_next = false;
             if (t.skip)
             {
-                continue;
+                more_next = Work::tile(p, cid, clusters, ++i, next);
             }
             const uint32_t astep = t.a_mn ? 2048 : 32, bstep = t.b_mn ? 2048 : 32;
             const uint32_t albo = t.a_mn ? kBK * 128 : 16, blbo = t.b_mn ? kBK * 128 : 16;
-            for (int k0 = 0; k0 < t.kbs; k0 += SPLIT ? kChain : t.kbs)
+            for (int k0 = 0; !t.skip && k0 < t.kbs; k0 += SPLIT ? kChain : t.kbs)
             {
                 const int blocks = SPLIT ? 3 * (min(t.kbs, k0 + kChain) - k0) : t.kbs;
                 const int buf = SPLIT ? 0 : it & 1;
@@ -297,10 +329,16 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
                         stage = 0;
                         phase ^= 1;
                     }
+                    if (kb == 0 && k0 == 0)
+                    {
+                        more_next = Work::tile(p, cid, clusters, ++i, next);   // under the products
+                    }
                 }
                 commit2(&tfull[buf]);
                 ++it;
             }
+            t = next;
+            more = more_next;
         }
     }
     else if (warp >= 2)
@@ -308,19 +346,19 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
         const int quarter = warp & 3;   // the TMEM lanes this warp may read
         constexpr int COLS = kTile / (EPI_WARPS / 4);
         const int col0 = ((warp - 2) >> 2) * COLS;
+        const int row0 = static_cast<int>(rank) * 128 + quarter * 32;   // within the tile
         const uint32_t release = peer_addr(&tempty[0], 0);
         Staging st{staging + (warp - 2) * 2 * C_::STAGE_TILE};
         typename Work::State state;
         int it = 0;
-        for (int i = 0; Work::tile(p, cid, clusters, i, t); ++i)
+        while (more)
         {
-            if (t.skip)
+            if (!t.skip)
             {
-                continue;
+                Work::before(p, t, state, row0, col0, st, lane);
             }
-            const int row0 = static_cast<int>(rank) * 128 + quarter * 32;   // within the tile
-            Work::before(p, t, state, row0, col0, st, lane);
-            for (int k0 = 0; k0 < t.kbs; k0 += SPLIT ? kChain : t.kbs)
+            const bool more_next = Work::tile(p, cid, clusters, ++i, next);
+            for (int k0 = 0; !t.skip && k0 < t.kbs; k0 += SPLIT ? kChain : t.kbs)
             {
                 const int buf = SPLIT ? 0 : it & 1;
                 mbar_wait(&tfull[buf], (SPLIT ? it : it >> 1) & 1, p.status, abort);
@@ -349,6 +387,8 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
                 }
                 ++it;
             }
+            t = next;
+            more = more_next;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");   // copies an epilogue left in flight
         if (lane == 0)
