@@ -58,6 +58,14 @@ struct Scalars
     float x, w;             // 2^ex, 2^ew of split operands
 };
 
+// Which tiles each cluster of a backward launch computes: its tiles of kind k are first[k][cid] up to
+// first[k][cid + 1].
+constexpr int kMaxClusters = 80;
+struct Shares
+{
+    int first[3][kMaxClusters + 1];
+};
+
 struct Params
 {
     CUtensorMap x, w;        // operands [rows, dim], [vocab, dim] K-major; plane 1: the lo halves
@@ -73,7 +81,8 @@ struct Params
     int v0, num_n, strip_log2;
     pair::Divisor by_m, by_d;   // num_m, num_d
     // gradient products of this launch: q_in holds vocabulary rows g0 .. g0 + gcols
-    int g0, gcols, num_d, dw_tiles, dx_tiles;
+    int g0, gcols, num_d;
+    Shares shares;
     int dx_add;              // dx sums: 0 store, 1 add
     int dw_mode;             // 0: from registers; 1: TMA store; 2: TMA add (fp32)
     int dw_f32, dw_beta;
@@ -262,13 +271,16 @@ struct GradWork
         int target;
     };
 
-    // Longest tiles first: dW (k runs over the rows), dx (over the piece), then q (over dim).
+    // dW tiles first (k runs over the rows), then dx (over the piece), then q (over dim): Shares gives
+    // every cluster the same number of k-blocks as nearly as whole tiles allow.
     static __device__ __forceinline__ bool tile(const Params& p, int cid, int clusters, int i, Tile& t)
     {
-        int u = cid + i * clusters;
-        t.skip = false;
+        (void)clusters;
         const bool bf = p.is_bf16 != 0;
-        if (u < p.dw_tiles)
+        t.skip = false;
+        int u = p.shares.first[kDw][cid] + i;
+        int end = p.shares.first[kDw][cid + 1];
+        if (u < end)
         {
             t.kind = kDw;
             t.mb = p.by_d.div(u, t.nb);
@@ -277,8 +289,9 @@ struct GradWork
             t.idesc = pair::idesc(bf, true, true);
             return true;
         }
-        u -= p.dw_tiles;
-        if (u < p.dx_tiles)
+        u = p.shares.first[kDx][cid] + (u - end);
+        end = p.shares.first[kDx][cid + 1];
+        if (u < end)
         {
             t.kind = kDx;
             t.mb = p.by_d.div(u, t.nb);
@@ -288,8 +301,9 @@ struct GradWork
             t.idesc = pair::idesc(bf, false, true);
             return true;
         }
-        u -= p.dx_tiles;
-        if (u >= p.num_m * p.num_n)
+        u = p.shares.first[kQ][cid] + (u - end);
+        end = p.shares.first[kQ][cid + 1];
+        if (u >= end)
         {
             return false;
         }
@@ -878,6 +892,56 @@ Layout layout(int64_t rows, int64_t vocab, int64_t dim, bool pack_x, bool pack_w
     return l;
 }
 
+// Shares of `tiles[k]` tiles of `cost[k]` k-blocks each among the clusters: the costlier kinds first,
+// each filled up to a common level, then one more tile each to the least loaded. Dealt out in turn
+// instead, the clusters with a dW tile (128 k-blocks at 8192 rows) had 240 k-blocks of a launch's 166
+// on average.
+void share(const int64_t (&tiles)[3], const int64_t (&cost)[3], int clusters, Shares& out)
+{
+    int64_t load[kMaxClusters] = {}, count[3][kMaxClusters] = {};
+    int order[3] = {0, 1, 2};
+    std::sort(order, order + 3, [&](int a, int b) { return cost[a] > cost[b]; });
+    for (const int k : order)
+    {
+        int64_t lo = 0, hi = 0;   // the highest level that all of kind k's tiles still cover
+        for (int c = 0; c < clusters; ++c) hi = std::max(hi, load[c]);
+        hi += tiles[k] * cost[k] + 1;
+        const auto fits = [&](int64_t level) {
+            int64_t n = 0;
+            for (int c = 0; c < clusters; ++c) n += level > load[c] ? (level - load[c]) / cost[k] : 0;
+            return n <= tiles[k];
+        };
+        while (hi - lo > 1)
+        {
+            const int64_t mid = (lo + hi) / 2;
+            (fits(mid) ? lo : hi) = mid;
+        }
+        int64_t left = tiles[k];
+        for (int c = 0; c < clusters; ++c)
+        {
+            const int64_t n = lo > load[c] ? (lo - load[c]) / cost[k] : 0;
+            count[k][c] = n;
+            load[c] += n * cost[k];
+            left -= n;
+        }
+        for (; left > 0; --left)
+        {
+            const int c = static_cast<int>(std::min_element(load, load + clusters) - load);
+            ++count[k][c];
+            load[c] += cost[k];
+        }
+    }
+    for (int k = 0; k < 3; ++k)
+    {
+        int64_t at = 0;
+        for (int c = 0; c <= kMaxClusters; ++c)
+        {
+            out.first[k][c] = static_cast<int>(at);
+            at += c < clusters ? count[k][c] : 0;
+        }
+    }
+}
+
 struct Call
 {
     const void *x, *w;
@@ -1093,8 +1157,8 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
     int rc = lce::check(c, workspace, workspace_bytes, true, "veda_linear_cross_entropy_bwd");
     if (rc != VEDA_OK) return rc;
     const bool split = dtype == VEDA_F32;
-    const int clusters = split ? pair::clusters_available<lce::GradWork, 4, true>()
-                               : pair::clusters_available<lce::GradWork, 4, false>();
+    const int clusters = std::min(lce::kMaxClusters, split ? pair::clusters_available<lce::GradWork, 4, true>()
+                                                           : pair::clusters_available<lce::GradWork, 4, false>());
     if (clusters < 1)
     {
         return fail(VEDA_ERR_UNSUPPORTED, "veda_linear_cross_entropy_bwd: no CTA pair fits on this device");
@@ -1139,12 +1203,11 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
     const int64_t pieces = (vocab + piece - 1) / piece;
     for (int64_t k = 0; k <= pieces; ++k)
     {
-        p.num_n = 0;
-        p.dw_tiles = p.dx_tiles = 0;
+        int64_t tiles[3] = {};
         if (k < pieces)
         {
             p.v0 = static_cast<int>(k * piece);
-            p.num_n = static_cast<int>((std::min(piece, vocab - k * piece) + 255) / 256);
+            tiles[lce::GradWork::kQ] = (std::min(piece, vocab - k * piece) + 255) / 256 * p.num_m;
             p.q_out = q_store[k & 1];
         }
         if (k > 0)
@@ -1153,12 +1216,16 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
             p.gcols = static_cast<int>(std::min(piece, vocab - (k - 1) * piece));
             p.q_in = q_load[(k - 1) & 1];
             p.q_mn = q_mn[(k - 1) & 1];
-            p.dw_tiles = dw != nullptr ? (p.gcols + 255) / 256 * p.num_d : 0;
-            p.dx_tiles = dx != nullptr ? p.num_m * p.num_d : 0;
+            tiles[lce::GradWork::kDw] = dw != nullptr ? static_cast<int64_t>((p.gcols + 255) / 256) * p.num_d : 0;
+            tiles[lce::GradWork::kDx] = dx != nullptr ? static_cast<int64_t>(p.num_m) * p.num_d : 0;
             p.dx_add = k > 1;
         }
-        const int64_t units = static_cast<int64_t>(p.num_m) * p.num_n + p.dw_tiles + p.dx_tiles;
+        const int64_t units = tiles[0] + tiles[1] + tiles[2];
+        VEDA_REQUIRE(units <= lce::kLimit, "too many tiles");
         const int grid = static_cast<int>(std::min<int64_t>(units, clusters));
+        // k-blocks a tile, and what its epilogue adds
+        const int64_t cost[3] = {(rows + 63) / 64 + 2, (p.gcols + 63) / 64 + 2, (dim + 63) / 64 + 2};
+        lce::share(tiles, cost, grid, p.shares);
         rc = split ? pair::launch_pair<lce::GradWork, 4, true>("veda_linear_cross_entropy_bwd", p, grid, stream)
                    : pair::launch_pair<lce::GradWork, 4, false>("veda_linear_cross_entropy_bwd", p, grid, stream);
         if (rc != VEDA_OK) return rc;

@@ -72,7 +72,7 @@ __host__ __device__ constexpr uint32_t idesc(bool is_bf16, bool a_mn, bool b_mn)
 struct Divisor
 {
     uint32_t m = 0, s = 0, d = 1;
-    __host__ __device__ Divisor() = default;
+    Divisor() = default;
     __host__ explicit Divisor(uint32_t n) : d(n)
     {
         while ((1ull << s) < n) ++s;
