@@ -881,8 +881,10 @@ Layout layout(int64_t rows, int64_t vocab, int64_t dim, bool pack_x, bool pack_w
     }
     else
     {
-        // two pieces of q of about 32 MB each, so that both, the dx sums and x stay in L2
-        const int64_t fit = (int64_t{32} << 20) / (rows * 2 * l.planes) / 256 * 256;
+        // Two pieces of q of about 64 MB: one is written while the other is read, mostly from L2, and
+        // the launches are long enough for their tails not to count. Backward of 8192 x 151936 x 1024
+        // with pieces of 8 / 16 / 32 / 64 / 128 MB: 13.4 / 7.71 / 6.42 / 6.06 / 6.27 ms.
+        const int64_t fit = (int64_t{64} << 20) / (rows * 2 * l.planes) / 256 * 256;
         l.piece = std::min(round_up(vocab, 256), std::max<int64_t>(256, fit));
         l.q = take(2 * l.planes * rows * l.piece * 2);
         l.ld_acc = round_up(dim, 4);
