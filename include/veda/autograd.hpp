@@ -17,7 +17,7 @@
 // Fused modules (one node each, B200 kernels): rms_norm (norm + gain), linear (x W^T over
 // flattened tokens), attention (QK-norm + RoPE + causal GQA attention on a fused q|k|v buffer),
 // swiglu (on a fused gate|up buffer), cross_entropy (streaming softmax-CE with the gradient
-// formed in the same pass).
+// formed in the same pass), linear_cross_entropy (the LM head and its loss without the logits).
 #pragma once
 
 #include "veda/tensor.hpp"
@@ -138,6 +138,19 @@ using RowsSink = std::function<void(const core::Tensor& ids, size_t count, const
 Variable embedding_device_rows(const Variable& table, const core::Tensor& ids, RowsSink sink);
 // Mean cross-entropy with device targets (int64 [lanes]).
 Variable cross_entropy_device(const Variable& logits, const core::Tensor& targets);
+
+// cross_entropy(linear(x, w), targets) as one node that stores no logits: x [.., in] flattened to
+// rows, w [out, in], a target per row; the loss is a scalar. The forward keeps one log-sum-exp per
+// row, the backward forms the logits again piece by piece of the vocabulary, so neither the
+// [rows, out] logits nor their gradient is ever in memory (in bf16 both, 5 GB at 8192 x 151936).
+// Rows whose target is ignore_index are not counted in the mean; with none counted the loss is 0.
+inline constexpr int64_t kIgnoreTarget = -100;
+Variable linear_cross_entropy(const Variable& x, const Variable& w, const std::vector<int64_t>& targets,
+                              int64_t ignore_index = kIgnoreTarget);
+// The same with device targets (int64 [rows]); a target outside [0, out) that is not ignore_index
+// raises std::out_of_range at the next synchronisation point.
+Variable linear_cross_entropy_device(const Variable& x, const Variable& w, const core::Tensor& targets,
+                                     int64_t ignore_index = kIgnoreTarget);
 
 // Central finite differences against the tape's gradient (src/libs/autograd/GradientCheck.h):
 // dL/dx_i ~ (L(x + h e_i) - L(x - h e_i)) / 2h for every element of `at`, compared relatively per

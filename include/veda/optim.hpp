@@ -65,7 +65,9 @@ public:
     // fp32 master weights of parameter i (the value itself for fp32 parameters).
     core::Tensor master(size_t i) const { return masters_[i]; }
     // Number of kernel launches one step issues (one per contiguous run).
-    size_t runs() const noexcept { return runs_.size(); }
+    size_t runs() const noexcept { return updates_.size(); }
+    // The device sum of squares that the last launch_clipped left (before grad_scale).
+    const double* sumsq() const { return static_cast<const double*>(sumsq_.data_ptr()); }
 
 private:
     bool skip_nonfinite_ = false;
@@ -79,13 +81,19 @@ private:
         float* v;
         void* lowp;   // bf16 value copy, or null for fp32 parameters
     };
+    friend class Muon;
     void build_runs();
+    std::vector<Run> runs_of(bool all) const;
+    // Leaves parameters to another optimizer, or takes them back.
+    void set_taken(const std::vector<size_t>& indices, bool taken);
     void launch(const double* sumsq, float max_norm, float grad_scale);
 
     std::vector<autograd::Variable> parameters_;
     std::vector<core::Tensor> masters_;
     core::Tensor m_arena_, v_arena_, master_arena_;
-    std::vector<Run> runs_;
+    std::vector<Run> runs_;      // every parameter: what the global norm covers
+    std::vector<Run> updates_;   // those that step() updates
+    std::vector<bool> taken_;
     AdamWConfig config_;
     size_t steps_ = 0;
     core::Tensor sumsq_;     // device double
@@ -93,6 +101,78 @@ private:
     double bias_host_[2] = {1.0, 1.0};
     core::Tensor workspace_;
     float last_scale_ = 1.0f;
+};
+
+struct MuonConfig
+{
+    float learning_rate = 3e-4f;
+    float momentum = 0.95f;
+    bool nesterov = true;
+    float weight_decay = 0.1f;
+    size_t steps = 5;              // Newton-Schulz iterations
+    float a = 3.4445f, b = -4.7750f, c = 2.0315f;
+    float eps = 1e-7f;
+    // The orthogonalised update is scaled by 0.2 sqrt(max(rows, cols)), which gives its entries the
+    // size of AdamW's, so learning rates carry over (false: by sqrt(max(1, rows / cols))).
+    bool match_adamw = true;
+};
+
+// Momentum orthogonalised by Newton-Schulz products (veda_muon_step) for rank-2 parameters:
+//   m <- momentum m + g;  u = nesterov ? g + momentum m : m;
+//   w <- w - lr weight_decay w - lr scale orthogonalize(u).
+// Momentum and, for bf16 parameters, master weights are fp32. Parameters of one shape that lie a
+// constant distance apart (the same matrix of every layer of train::TinyTransformer) are updated as
+// one batch. Not part of the reference, whose optimizer is AdamW.
+class Muon
+{
+public:
+    // Keeps momentum and master weights of its own.
+    explicit Muon(std::vector<autograd::Variable> parameters, MuonConfig config = {});
+    // Takes over the parameters `indices` of an AdamW: its steps no longer update them (its global
+    // norm still counts them), their momentum is their first moment there and their master weights
+    // are its. `base` must outlive this object; what it holds for them is given back then.
+    Muon(AdamW& base, const std::vector<size_t>& indices, MuonConfig config = {});
+    ~Muon();
+    Muon(const Muon&) = delete;
+    Muon& operator=(const Muon&) = delete;
+
+    // One step on the gradients as they are; does not clear them.
+    void step();
+    // The global-norm clip over these parameters fused into the step, as AdamW::step_clipped.
+    void step_clipped(float max_norm, float grad_scale = 1.0f);
+    // Only launches kernels (capturable): the step with the clip of a sum of squares in device memory
+    // (null: none).
+    void launch(const double* sumsq, float max_norm, float grad_scale);
+    void zero_grad();
+    const MuonConfig& config() const noexcept { return config_; }
+    const std::vector<autograd::Variable>& parameters() const noexcept { return parameters_; }
+    // fp32 momentum and master weights of parameter i (the value itself for fp32 parameters).
+    core::Tensor momentum(size_t i) const { return momenta_[i]; }
+    core::Tensor master(size_t i) const { return masters_[i]; }
+    // Batches a step launches.
+    size_t batches() const noexcept { return batches_.size(); }
+
+private:
+    struct Batch
+    {
+        size_t first;
+        int64_t count, rows, cols, stride;
+        float* master;
+        float* momentum;
+        float* grad;
+        void* lowp;
+    };
+    void check_config() const;
+    void build_batches();
+
+    AdamW* base_ = nullptr;
+    std::vector<size_t> taken_;
+    std::vector<autograd::Variable> parameters_;
+    std::vector<core::Tensor> momenta_, masters_;
+    std::vector<Batch> batches_;
+    MuonConfig config_;
+    core::Tensor workspace_, sumsq_, norm_workspace_;
+    size_t workspace_bytes_ = 0;
 };
 
 // Global-norm clip in place; returns the pre-clip norm (Clip.cpp semantics; synchronises).

@@ -71,6 +71,10 @@ public:
     autograd::Variable forward(const std::vector<int64_t>& ids, size_t batch, size_t length);
     // ids already on the device (int64 [B*T]).
     autograd::Variable forward_device(const core::Tensor& ids, size_t batch, size_t length);
+    // What the LM head reads, the final norm's rows [B*T, D], and the head itself (the tied embedding
+    // [V, D]): forward_device(ids) is linear(hidden_device(ids), head()).
+    autograd::Variable hidden_device(const core::Tensor& ids, size_t batch, size_t length);
+    const autograd::Variable& head() const noexcept { return embed_; }
 
     // Every trainable leaf, once each, in the reference's order (views into the arenas).
     const std::vector<autograd::Variable>& parameters() const noexcept { return parameters_; }
@@ -115,7 +119,7 @@ public:
     bool recompute_attention() const noexcept { return recompute_attention_; }
 
 private:
-    autograd::Variable forward_from(const autograd::Variable& x, size_t batch, size_t length);
+    autograd::Variable hidden_from(const autograd::Variable& x, size_t batch, size_t length);
 
     friend class generate::Generator;   // reads the weights for inference
     ModelConfig config_;
@@ -211,6 +215,16 @@ public:
     // a captured step graph is dropped and captured again with the new path.
     void set_recompute_attention(bool on);
 
+    // The loss as autograd::linear_cross_entropy_device (on) instead of the LM head's logits and
+    // their cross-entropy (off, the default): the step never holds the [B*T, V] logits and their
+    // gradient, in exchange for forming the logits twice. Targets of autograd::kIgnoreTarget are then
+    // not counted. A captured step graph is dropped and captured again.
+    void set_linear_loss(bool on);
+    // Muon for the hidden matrices (q/k/v/o, gate/up/down of every layer), AdamW for the rest. Their
+    // momentum is the optimizer's first moment, so checkpoints keep it. Not with a sharded optimizer.
+    // A captured step graph is dropped and captured again.
+    void use_muon(const optim::MuonConfig& config);
+
     TinyTransformer& model() noexcept { return *model_; }
     optim::AdamW& optimizer() noexcept { return *opt_; }
     size_t batch() const noexcept { return batch_; }
@@ -225,6 +239,9 @@ private:
     core::Tensor ids_, targets_, loss_;
     core::Tensor pinned_;   // host-side staging is done by the caller; kept for symmetry
     bool graph_eligible() const;
+    void drop_step_graph();
+    bool linear_loss_ = false;
+    std::unique_ptr<optim::Muon> muon_;
     void step_impl(const core::Tensor& ids, const core::Tensor& targets);
     ::CUgraphExec_st* graph_exec_ = nullptr;
     int64_t graph_launches_ = 0;

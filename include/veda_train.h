@@ -145,6 +145,17 @@ int veda_trainer_step_skipped(veda_trainer* t, int* skipped);
  * output again before the output projection's and the attention's backward. */
 int veda_trainer_set_recompute_attention(veda_trainer* t, int on);
 
+/* on = 1: the LM head and its cross-entropy as one operator that never stores the [batch*seq_len,
+ * vocab] logits or their gradient (veda_linear_cross_entropy_*); targets of -100 are then not counted
+ * in the mean. Default off. */
+int veda_trainer_set_linear_loss(veda_trainer* t, int on);
+/* Muon (veda_muon_step) for every layer's q/k/v/o and gate/up/down matrices from the next step on,
+ * AdamW for the rest; the clip covers all of them. The update is scaled by 0.2 sqrt(max(rows, cols)),
+ * so AdamW's learning rates carry over. Momentum is kept in the first moments, checkpoints included. Not
+ * with a sharded optimizer. */
+int veda_trainer_use_muon(veda_trainer* t, float lr, float momentum, int nesterov, float weight_decay,
+                          int steps);
+
 /* Device-time profile of kernel classes (gemm_fwd, gemm_dx, gemm_dw, attn_fwd, attn_bwd,
  * cross_entropy, rmsnorm_bwd, swiglu_bwd, adamw), recorded with CUDA events while enabled. */
 int veda_profile_enable(int on);

@@ -1570,6 +1570,105 @@ Variable linear(const Variable& x, const Variable& w)
     return make({x, w}, std::move(value), [l](const Tensor& g) { linear_backward(l, g); });
 }
 
+namespace
+{
+Variable linear_cross_entropy_impl(const LinearSaved& l, const Variable& x, const Variable& w,
+                                   const Tensor& targets, int64_t ignore, bool device_check)
+{
+    const DType d = l.xs.dtype();
+    const size_t V = l.out, D = l.in, rows = l.rows;
+    const double es = static_cast<double>(core::dtype_size(d));
+    Tensor row_loss = Tensor::empty(Shape({rows}), DType::F32);
+    Tensor lse = Tensor::empty(Shape({rows}), DType::F32);
+    Tensor loss = Tensor::empty(Shape({}), DType::F32);
+    int* flag = device_check ? detail::device_flag() : nullptr;
+    {
+        const size_t bytes = veda_linear_cross_entropy_workspace(rows, V, D, l.ldx, D, dt(d), 0);
+        Tensor ws = Tensor::empty(Shape({(bytes + 3) / 4}), DType::F32);
+        profile::Scope scope("linear_ce_fwd", 2.0 * rows * V * D,
+                             es * (static_cast<double>(rows) * D + static_cast<double>(V) * D));
+        check(veda_linear_cross_entropy_fwd(l.xs.data_ptr(), l.ldx, l.wc.data_ptr(), D,
+                                            static_cast<const int64_t*>(targets.data_ptr()), ignore,
+                                            static_cast<float*>(row_loss.data_ptr()),
+                                            static_cast<float*>(lse.data_ptr()),
+                                            static_cast<float*>(loss.data_ptr()), rows, V, D, ws.data_ptr(),
+                                            bytes, flag, dt(d), S()),
+              "linear_cross_entropy");
+    }
+    return make({x, w}, std::move(loss), [l, lse, targets, ignore, flag, d, V, D, rows, es](const Tensor& g) {
+        Tensor dx;
+        if (l.xin->requires_grad)
+        {
+            dx = Tensor::empty(l.xin->value.shape(), d);
+        }
+        float* dw = nullptr;
+        bool fresh = false;
+        if (l.win->requires_grad)
+        {
+            dw = static_cast<float*>(grad_target(*l.win, &fresh, DType::F32).data_ptr());
+        }
+        const Tensor up = as_dtype(g, DType::F32);
+        const size_t bytes = veda_linear_cross_entropy_workspace(rows, V, D, l.ldx, D, dt(d), 1);
+        Tensor ws = Tensor::empty(Shape({(bytes + 3) / 4}), DType::F32);
+        {
+            profile::Scope scope("linear_ce_bwd", 6.0 * rows * V * D,
+                                 es * (2.0 * rows * D + static_cast<double>(V) * D) + 4.0 * V * D);
+            check(veda_linear_cross_entropy_bwd(l.xs.data_ptr(), l.ldx, l.wc.data_ptr(), D,
+                                                static_cast<const int64_t*>(targets.data_ptr()), ignore,
+                                                static_cast<const float*>(lse.data_ptr()),
+                                                static_cast<const float*>(up.data_ptr()),
+                                                dx.defined() ? dx.data_ptr() : nullptr, D, dw, D, VEDA_F32,
+                                                fresh ? 0.0f : 1.0f, rows, V, D, ws.data_ptr(), bytes, flag,
+                                                dt(d), S()),
+                  "linear_cross_entropy backward");
+        }
+        if (dx.defined())
+        {
+            accumulate(*l.xin, dx);
+        }
+    });
+}
+} // namespace
+
+Variable linear_cross_entropy(const Variable& x, const Variable& w, const std::vector<int64_t>& targets,
+                              int64_t ignore_index)
+{
+    const LinearSaved l = linear_setup(x.value(), x.node(), w);
+    if (targets.size() != l.rows)
+    {
+        throw std::invalid_argument("linear_cross_entropy: " + std::to_string(targets.size()) +
+                                    " targets for " + std::to_string(l.rows) + " rows");
+    }
+    if (l.rows == 0 || l.out == 0)
+    {
+        throw std::invalid_argument("linear_cross_entropy: nothing to average over");
+    }
+    for (size_t row = 0; row < targets.size(); ++row)
+    {
+        if (targets[row] != ignore_index &&
+            (targets[row] < 0 || static_cast<size_t>(targets[row]) >= l.out))
+        {
+            throw std::invalid_argument("linear_cross_entropy: target " + std::to_string(targets[row]) +
+                                        " at row " + std::to_string(row) + " is outside [0, " +
+                                        std::to_string(l.out) + ")");
+        }
+    }
+    return linear_cross_entropy_impl(l, x, w, upload_ids(targets), ignore_index, false);
+}
+
+Variable linear_cross_entropy_device(const Variable& x, const Variable& w, const Tensor& targets,
+                                     int64_t ignore_index)
+{
+    const LinearSaved l = linear_setup(x.value(), x.node(), w);
+    const size_t count = targets.numel() * core::dtype_size(targets.dtype()) / sizeof(int64_t);
+    if (count != l.rows || l.rows == 0 || l.out == 0)
+    {
+        throw std::invalid_argument("linear_cross_entropy_device: " + std::to_string(count) +
+                                    " targets for " + std::to_string(l.rows) + " rows");
+    }
+    return linear_cross_entropy_impl(l, x, w, targets, ignore_index, true);
+}
+
 Variable attention(const Variable& qkv, const Variable& q_norm, const Variable& k_norm,
                    const Tensor& cosines, const Tensor& sines, size_t B, size_t T, size_t H,
                    size_t Hkv, size_t Dh, float eps)

@@ -298,11 +298,17 @@ Variable TinyTransformer::forward(const std::vector<int64_t>& ids, size_t batch,
     }
     if (gate_) gate_(embed_range_.first, embed_range_.second);
     Variable x = autograd::embedding(embed_, ids, Shape({batch * length}));
-    return autograd::reshape(forward_from(x, batch, length),
+    // tied LM head: the embedding matrix read the other way round (Model.cpp:253-254)
+    return autograd::reshape(autograd::linear(hidden_from(x, batch, length), embed_),
                              Shape({batch, length, config_.vocab_size}));
 }
 
 Variable TinyTransformer::forward_device(const Tensor& ids, size_t batch, size_t length)
+{
+    return autograd::linear(hidden_device(ids, batch, length), embed_);
+}
+
+Variable TinyTransformer::hidden_device(const Tensor& ids, size_t batch, size_t length)
 {
     if (config_.max_position_embeddings != 0 && length > config_.max_position_embeddings)
     {
@@ -311,10 +317,10 @@ Variable TinyTransformer::forward_device(const Tensor& ids, size_t batch, size_t
     if (gate_) gate_(embed_range_.first, embed_range_.second);
     Variable x = rows_sink_ ? autograd::embedding_device_rows(embed_, ids, rows_sink_)
                             : autograd::embedding_device(embed_, ids);
-    return forward_from(x, batch, length);
+    return hidden_from(x, batch, length);
 }
 
-Variable TinyTransformer::forward_from(const Variable& x0, size_t B, size_t T)
+Variable TinyTransformer::hidden_from(const Variable& x0, size_t B, size_t T)
 {
     const size_t H = config_.num_heads, Hk = config_.num_kv_heads, Dh = config_.head_dim;
     const float eps = config_.rms_norm_eps;
@@ -348,8 +354,7 @@ Variable TinyTransformer::forward_from(const Variable& x0, size_t B, size_t T)
         const Variable& next = l + 1 < layers_.size() ? layers_[l + 1].in_norm : final_norm_;
         a = autograd::add_rms_norm(x, autograd::mlp(b, L.gate_up, L.down), next, eps, &x);
     }
-    // tied LM head: the embedding matrix read the other way round (Model.cpp:253-254)
-    return autograd::linear(a, embed_);
+    return a;
 }
 
 } // namespace veda::train

@@ -5,8 +5,11 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
+#include <cstdint>
 #include <stdexcept>
+#include <string>
 
 namespace veda::optim
 {
@@ -93,15 +96,15 @@ AdamW::AdamW(std::vector<autograd::Variable> parameters, AdamWConfig config)
 
 AdamW::~AdamW() = default;
 
-void AdamW::build_runs()
+std::vector<AdamW::Run> AdamW::runs_of(bool all) const
 {
-    runs_.clear();
+    std::vector<Run> runs;
     size_t offset = 0;
     for (size_t i = 0; i < parameters_.size(); ++i)
     {
         const auto& p = parameters_[i];
         const size_t n = p.value().numel();
-        if (!p.requires_grad() || n == 0)
+        if (!p.requires_grad() || n == 0 || (!all && taken_[i]))
         {
             offset += n;
             continue;
@@ -114,9 +117,9 @@ void AdamW::build_runs()
         Run r{i, 1, static_cast<int64_t>(n), fptr(g), fptr(masters_[i]), fptr(m_arena_) + offset,
               fptr(v_arena_) + offset,
               p.value().dtype() == DType::BF16 ? p.value().data_ptr() : nullptr};
-        if (!runs_.empty())
+        if (!runs.empty())
         {
-            Run& last = runs_.back();
+            Run& last = runs.back();
             const bool adjacent = last.first + last.count == i &&
                                   last.grad + last.n == r.grad && last.master + last.n == r.master &&
                                   last.m + last.n == r.m &&
@@ -132,9 +135,17 @@ void AdamW::build_runs()
                 continue;
             }
         }
-        runs_.push_back(r);
+        runs.push_back(r);
         offset += n;
     }
+    return runs;
+}
+
+void AdamW::build_runs()
+{
+    taken_.resize(parameters_.size(), false);
+    runs_ = runs_of(true);
+    updates_ = runs_of(false);
     int64_t largest = 1;
     for (const Run& r : runs_)
     {
@@ -142,6 +153,15 @@ void AdamW::build_runs()
     }
     const size_t ws = veda_sumsq_workspace(largest);
     workspace_ = Tensor::empty(Shape({(ws + 3) / 4 + 1}), DType::F32);
+}
+
+void AdamW::set_taken(const std::vector<size_t>& indices, bool taken)
+{
+    for (const size_t i : indices)
+    {
+        taken_[i] = taken;
+    }
+    updates_ = runs_of(false);
 }
 
 void AdamW::advance()
@@ -160,7 +180,7 @@ void AdamW::launch(const double* sumsq, float max_norm, float grad_scale)
 {
     flush_host_writes(parameters_);
     const double* bias = static_cast<const double*>(bias_.data_ptr());
-    for (const Run& r : runs_)
+    for (const Run& r : updates_)
     {
         check(veda_adamw_step_dev(r.master, r.m, r.v, r.grad, r.lowp, r.n, config_.learning_rate,
                                   config_.beta1, config_.beta2, config_.eps, config_.weight_decay,
@@ -233,6 +253,255 @@ void AdamW::zero_grad()
         }
     }
 }
+
+namespace
+{
+// Clears the gradients of the parameters that have one.
+void clear_grads(const std::vector<autograd::Variable>& parameters, const char* what)
+{
+    for (const auto& p : parameters)
+    {
+        auto& node = *p.node();
+        if (p.requires_grad() && node.grad.defined())
+        {
+            if (cudaMemsetAsync(node.grad.data_ptr(), 0, node.grad.numel() * 4, cs()) != cudaSuccess)
+            {
+                throw std::runtime_error(std::string(what) + ": memset failed");
+            }
+            node.grad_zero = true;
+            node.grad_owned = true;
+        }
+    }
+}
+
+// A batch's scratch is about 8 bytes per weight; larger batches are cut so that it stays below this.
+constexpr size_t kMuonWorkspace = size_t{1} << 30;
+} // namespace
+
+void Muon::check_config() const
+{
+    const MuonConfig& c = config_;
+    if (!(c.learning_rate >= 0.0f) || !(c.weight_decay >= 0.0f) || !(c.eps >= 0.0f))
+    {
+        throw std::invalid_argument("Muon: learning rate, eps and weight decay must not be negative");
+    }
+    if (!(c.momentum >= 0.0f) || c.momentum >= 1.0f)
+    {
+        throw std::invalid_argument("Muon: momentum must lie in [0, 1)");
+    }
+    if (c.steps == 0)
+    {
+        throw std::invalid_argument("Muon: at least one Newton-Schulz step");
+    }
+    for (const auto& p : parameters_)
+    {
+        if (p.value().rank() != 2)
+        {
+            throw std::invalid_argument("Muon: a parameter of shape " + p.value().shape().to_string() +
+                                        " is not a matrix");
+        }
+    }
+}
+
+Muon::Muon(std::vector<autograd::Variable> parameters, MuonConfig config)
+    : parameters_(std::move(parameters)), config_(config)
+{
+    check_config();
+    // Momentum and masters lie as the gradients do where those are views of one arena, so that equal
+    // matrices at a constant distance stay so; back to back where the gradients are scattered.
+    size_t total = 0;
+    uintptr_t low = UINTPTR_MAX, high = 0;
+    for (const auto& p : parameters_)
+    {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(fptr(p.grad()));
+        low = std::min(low, at);
+        high = std::max(high, at + p.value().numel() * sizeof(float));
+        total += p.value().numel();
+    }
+    const size_t span = total > 0 ? (high - low) / sizeof(float) : 0;
+    const bool together = span <= total + total / 2 + 4096;
+    const bool bf16 = !parameters_.empty() && parameters_[0].value().dtype() == DType::BF16;
+    Tensor momentum(Shape({std::max<size_t>(1, together ? span : total)}), DType::F32);
+    Tensor master;
+    for (const auto& p : parameters_)
+    {
+        if ((p.value().dtype() == DType::BF16) != bf16)
+        {
+            throw std::invalid_argument("Muon: parameters of one dtype");
+        }
+    }
+    if (bf16)
+    {
+        master = Tensor(Shape({std::max<size_t>(1, together ? span : total)}), DType::F32);
+    }
+    size_t at = 0;
+    for (const auto& p : parameters_)
+    {
+        const size_t offset =
+            together ? (reinterpret_cast<uintptr_t>(fptr(p.grad())) - low) / sizeof(float) : at;
+        at += p.value().numel();
+        momenta_.push_back(Tensor::view(momentum.storage(), offset, p.value().shape(), DType::F32));
+        if (!bf16)
+        {
+            masters_.push_back(p.value());
+            continue;
+        }
+        Tensor w = Tensor::view(master.storage(), offset, p.value().shape(), DType::F32);
+        const int64_t shape[2] = {static_cast<int64_t>(p.value().shape()[0]),
+                                  static_cast<int64_t>(p.value().shape()[1])};
+        const int64_t strides[2] = {static_cast<int64_t>(p.value().strides()[0]),
+                                    static_cast<int64_t>(p.value().strides()[1])};
+        check(veda_copy_strided(p.value().storage()->data(), VEDA_BF16, strides,
+                                static_cast<int64_t>(p.value().offset()), w.data_ptr(), VEDA_F32, shape, 2,
+                                current_stream()),
+              "Muon: master copy");
+        masters_.push_back(w);
+    }
+    build_batches();
+}
+
+Muon::Muon(AdamW& base, const std::vector<size_t>& indices, MuonConfig config) : config_(config)
+{
+    size_t at = 0;
+    std::vector<size_t> offsets;
+    for (const auto& p : base.parameters())
+    {
+        offsets.push_back(at);
+        at += p.value().numel();
+    }
+    for (const size_t i : indices)
+    {
+        if (i >= base.parameters().size())
+        {
+            throw std::invalid_argument("Muon: no parameter " + std::to_string(i));
+        }
+        if (base.taken_[i])
+        {
+            throw std::invalid_argument("Muon: parameter " + std::to_string(i) + " is taken already");
+        }
+        const auto& p = base.parameters()[i];
+        parameters_.push_back(p);
+        momenta_.push_back(Tensor::view(base.first_moments().storage(), offsets[i], p.value().shape(), DType::F32));
+        masters_.push_back(base.master(i));
+    }
+    check_config();
+    build_batches();
+    base.set_taken(indices, true);
+    base_ = &base;
+    taken_ = indices;
+}
+
+Muon::~Muon()
+{
+    if (base_ != nullptr)
+    {
+        base_->set_taken(taken_, false);
+    }
+}
+
+void Muon::build_batches()
+{
+    // Elements from a to b if their values, masters, momenta and gradients lie equally far apart.
+    const auto distance = [&](size_t a, size_t b, int64_t* out) {
+        const auto step = [&](const Tensor& x, const Tensor& y) {
+            return (static_cast<const char*>(y.data_ptr()) - static_cast<const char*>(x.data_ptr())) /
+                   static_cast<int64_t>(core::dtype_size(x.dtype()));
+        };
+        const int64_t d = step(parameters_[a].grad(), parameters_[b].grad());
+        *out = d;
+        return d >= static_cast<int64_t>(parameters_[a].value().numel()) &&
+               step(parameters_[a].value(), parameters_[b].value()) == d &&
+               step(masters_[a], masters_[b]) == d && step(momenta_[a], momenta_[b]) == d;
+    };
+    batches_.clear();
+    std::vector<bool> done(parameters_.size(), false);
+    size_t largest = 1;
+    for (size_t i = 0; i < parameters_.size(); ++i)
+    {
+        const auto& p = parameters_[i];
+        if (done[i] || !p.requires_grad() || p.value().numel() == 0)
+        {
+            continue;
+        }
+        const Tensor& g = p.grad();
+        if (g.dtype() != DType::F32 || !g.is_contiguous() || !p.value().is_contiguous())
+        {
+            throw std::invalid_argument("Muon: parameters need contiguous values and fp32 gradients");
+        }
+        const Shape& shape = p.value().shape();
+        const int64_t rows = static_cast<int64_t>(shape[0]), cols = static_cast<int64_t>(shape[1]);
+        const bool lowp = p.value().dtype() == DType::BF16;
+        const int d = lowp ? VEDA_BF16 : VEDA_F32;
+        Batch b{i, 1, rows, cols, 0, fptr(masters_[i]), fptr(momenta_[i]), fptr(g),
+                lowp ? p.value().data_ptr() : nullptr};
+        size_t last = i;
+        for (size_t j = i + 1; j < parameters_.size(); ++j)
+        {
+            int64_t step = 0;
+            if (done[j] || !parameters_[j].requires_grad() || parameters_[j].value().shape() != shape ||
+                parameters_[j].value().dtype() != p.value().dtype() || !distance(last, j, &step) ||
+                (b.count > 1 && step != b.stride) ||
+                veda_muon_step_workspace(b.count + 1, rows, cols, d) > kMuonWorkspace)
+            {
+                continue;
+            }
+            b.stride = step;
+            b.count += 1;
+            done[j] = true;
+            last = j;
+        }
+        workspace_bytes_ = std::max(workspace_bytes_, veda_muon_step_workspace(b.count, rows, cols, d));
+        largest = std::max(largest, p.value().numel());
+        batches_.push_back(b);
+    }
+    workspace_ = Tensor::empty(Shape({workspace_bytes_ / 4 + 1}), DType::F32);
+    sumsq_ = Tensor(Shape({2}), DType::F32);   // 8 bytes: one double
+    norm_workspace_ = Tensor::empty(Shape({veda_sumsq_workspace(static_cast<int64_t>(largest)) / 4 + 1}), DType::F32);
+}
+
+void Muon::launch(const double* sumsq, float max_norm, float grad_scale)
+{
+    flush_host_writes(parameters_);
+    const MuonConfig& c = config_;
+    const int flags = base_ != nullptr && base_->skip_nonfinite() ? VEDA_ADAMW_SKIP_NONFINITE : 0;
+    for (const Batch& b : batches_)
+    {
+        const float rows = static_cast<float>(b.rows), cols = static_cast<float>(b.cols);
+        const float scale = c.match_adamw ? 0.2f * std::sqrt(std::max(rows, cols))
+                                          : std::sqrt(std::max(1.0f, rows / cols));
+        check(veda_muon_step(b.master, b.momentum, b.grad, b.lowp, b.count, b.rows, b.cols, b.stride,
+                             c.learning_rate, c.momentum, c.nesterov ? 1 : 0, c.weight_decay, scale,
+                             static_cast<int>(c.steps), c.a, c.b, c.c, c.eps, sumsq, max_norm, grad_scale, flags,
+                             workspace_.data_ptr(), workspace_bytes_, current_stream()),
+              "Muon::step");
+    }
+}
+
+void Muon::step() { launch(nullptr, 1.0f, 1.0f); }
+
+void Muon::step_clipped(float max_norm, float grad_scale)
+{
+    if (!(max_norm > 0.0f))
+    {
+        throw std::invalid_argument("clip_gradient_norm: max_norm must be positive");
+    }
+    flush_host_writes(parameters_);
+    double* ss = static_cast<double*>(sumsq_.data_ptr());
+    bool first = true;
+    for (const auto& p : parameters_)
+    {
+        if (p.requires_grad())
+        {
+            check(veda_sumsq(fptr(p.grad()), static_cast<int64_t>(p.value().numel()), ss, first ? 0 : 1,
+                             norm_workspace_.data_ptr(), norm_workspace_.numel() * 4, current_stream()),
+                  "Muon::step_clipped (norm)");
+            first = false;
+        }
+    }
+    launch(ss, max_norm, grad_scale);
+}
+
+void Muon::zero_grad() { clear_grads(parameters_, "Muon::zero_grad"); }
 
 float clip_gradient_norm(const std::vector<autograd::Variable>& parameters, float max_norm)
 {

@@ -398,6 +398,28 @@ int veda_trainer_set_recompute_attention(veda_trainer* t, int on)
     return guarded([&] { t->impl->set_recompute_attention(on != 0); });
 }
 
+int veda_trainer_set_linear_loss(veda_trainer* t, int on)
+{
+    return guarded([&] { t->impl->set_linear_loss(on != 0); });
+}
+
+int veda_trainer_use_muon(veda_trainer* t, float lr, float momentum, int nesterov, float weight_decay, int steps)
+{
+    return guarded([&] {
+        if (steps < 1)
+        {
+            throw std::invalid_argument("Muon: at least one Newton-Schulz step");
+        }
+        veda::optim::MuonConfig config;
+        config.learning_rate = lr;
+        config.momentum = momentum;
+        config.nesterov = nesterov != 0;
+        config.weight_decay = weight_decay;
+        config.steps = static_cast<size_t>(steps);
+        t->impl->use_muon(config);
+    });
+}
+
 int veda_trainer_step_skipped(veda_trainer* t, int* skipped)
 {
     return guarded([&] {

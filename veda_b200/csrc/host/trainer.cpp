@@ -755,6 +755,10 @@ void Trainer::init_data_parallel(const void* nccl_unique_id, int rank, int world
         dp_.reset();
         return;
     }
+    if (sharded && muon_)
+    {
+        throw std::invalid_argument("Trainer: a sharded optimizer does not run Muon");
+    }
     dp_ = std::make_unique<DataParallel>(nccl_unique_id, rank, world, sharded);
     dp_->attach(*model_, bucket_bytes, master_weights(), opt_->steps(), batch_ * length_);
     dp_->set_skip_nonfinite(skip_nonfinite_);
@@ -823,13 +827,59 @@ void Trainer::set_recompute_attention(bool on)
         return;
     }
     model_->set_recompute_attention(on);
+    drop_step_graph();
+}
+
+void Trainer::drop_step_graph()
+{
     if (graph_exec_ != nullptr)
     {
-        cuda_check(cudaStreamSynchronize(cs()), "recompute switch");
+        cuda_check(cudaStreamSynchronize(cs()), "step graph switch");
         cudaGraphExecDestroy(graph_exec_);
         graph_exec_ = nullptr;
     }
     eager_steps_ = 0;   // the next step runs eagerly before a capture of the new path
+}
+
+void Trainer::set_linear_loss(bool on)
+{
+    if (on != linear_loss_)
+    {
+        linear_loss_ = on;
+        drop_step_graph();
+    }
+}
+
+void Trainer::use_muon(const optim::MuonConfig& config)
+{
+    if (sharded())
+    {
+        throw std::invalid_argument("Trainer::use_muon: not with a sharded optimizer");
+    }
+    // every rank-2 parameter but the embedding, which comes first
+    std::vector<size_t> hidden;
+    const auto& parameters = model_->parameters();
+    for (size_t i = 1; i < parameters.size(); ++i)
+    {
+        if (parameters[i].value().rank() == 2)
+        {
+            hidden.push_back(i);
+        }
+    }
+    drop_step_graph();
+    // an earlier Muon hands its parameters back first, and takes them again if this one is refused
+    const bool had = muon_ != nullptr;
+    const optim::MuonConfig before = had ? muon_->config() : config;
+    muon_.reset();
+    try
+    {
+        muon_ = std::make_unique<optim::Muon>(*opt_, hidden, config);
+    }
+    catch (...)
+    {
+        if (had) muon_ = std::make_unique<optim::Muon>(*opt_, hidden, before);
+        throw;
+    }
 }
 
 int Trainer::world() const noexcept { return dp_ ? dp_->world() : 1; }
@@ -1004,16 +1054,19 @@ void Trainer::step_impl(const Tensor& ids, const Tensor& targets)
     {
         dp_->begin_forward();
     }
-    Variable logits = [&] {
+    // the logits, or with set_linear_loss the rows that the LM head's loss reads
+    Variable out = [&] {
         profile::HostScope scope("host:forward");
-        return model_->forward_device(ids, batch_, length_);
+        return linear_loss_ ? model_->hidden_device(ids, batch_, length_)
+                            : model_->forward_device(ids, batch_, length_);
     }();
     capture_checkpoint("the forward");
     if (dp_)
     {
         dp_->end_forward();
     }
-    Variable loss = autograd::cross_entropy_device(logits, targets);
+    Variable loss = linear_loss_ ? autograd::linear_cross_entropy_device(out, model_->head(), targets)
+                                 : autograd::cross_entropy_device(out, targets);
     capture_checkpoint("the cross-entropy");
     autograd::BackwardOptions options;
     options.retain_intermediate_grads = false;
@@ -1043,7 +1096,12 @@ void Trainer::step_impl(const Tensor& ids, const Tensor& targets)
         }
         else
         {
-            opt_->launch_clipped(max_norm_, 1.0f / static_cast<float>(world()));
+            const float scale = 1.0f / static_cast<float>(world());
+            opt_->launch_clipped(max_norm_, scale);
+            if (muon_)
+            {
+                muon_->launch(opt_->sumsq(), max_norm_, scale);
+            }
         }
     }
     cuda_check(cudaMemcpyAsync(loss_.data_ptr(), loss.value().data_ptr(), sizeof(float),

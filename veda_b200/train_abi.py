@@ -51,6 +51,8 @@ SIGNATURES = {
     "veda_trainer_abort_comm": (_i, [_p]),
     "veda_trainer_set_skip_nonfinite": (_i, [_p, _i]),
     "veda_trainer_set_recompute_attention": (_i, [_p, _i]),
+    "veda_trainer_set_linear_loss": (_i, [_p, _i]),
+    "veda_trainer_use_muon": (_i, [_p, _f, _f, _i, _f, _i]),
     "veda_trainer_step_skipped": (_i, [_p, _p]),
     "veda_profile_enable": (_i, [_i]),
     "veda_profile_collect": (_i, [_p, _p, _p, _p, _p, _i]),
@@ -194,6 +196,13 @@ class Trainer:
 
     def set_recompute_attention(self, on: bool):
         _check(self.L, self.L.veda_trainer_set_recompute_attention(self.h, 1 if on else 0))
+
+    def set_linear_loss(self, on: bool):
+        _check(self.L, self.L.veda_trainer_set_linear_loss(self.h, 1 if on else 0))
+
+    def use_muon(self, lr, momentum=0.95, nesterov=True, weight_decay=0.1, steps=5):
+        _check(self.L, self.L.veda_trainer_use_muon(self.h, lr, momentum, 1 if nesterov else 0,
+                                                    weight_decay, steps))
 
     def step_skipped(self) -> bool:
         out = C.c_int(0)
