@@ -96,7 +96,10 @@ def make(b, r, c, dtype, seed=0, kind="noise"):
 
 
 SHAPES = [(1, 1, 1), (2, 1, 7), (1, 9, 1), (3, 16, 16), (2, 64, 64), (2, 192, 64), (1, 65, 300), (2, 300, 65),
-          (1, 256, 256), (3, 257, 100), (1, 100, 520), (2, 520, 600), (1, 1001, 523)]
+          (1, 256, 256), (3, 257, 100), (1, 100, 520), (2, 520, 600), (1, 1001, 523),
+          # the small form's borders: sides of 128 and 256, one past them, sides that are no multiple of 16
+          (2, 128, 256), (2, 256, 128), (1, 129, 256), (1, 128, 257), (2, 128, 128), (3, 97, 111), (2, 33, 250),
+          (2, 241, 17), (200, 24, 40)]
 
 
 @pytest.mark.gpu

@@ -24,6 +24,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace veda::cuda
 {
@@ -697,6 +698,367 @@ init_kernel(Source s, int rows, int cols, const double* __restrict__ partials, f
     }
 }
 
+// ---- small matrices: the whole iteration in one block ------------------------------------------
+// A matrix whose smaller side is at most 128 and whose larger side is at most 256 stays in one SM from
+// its norm to the result: X, then S and M in turn, as hi and lo planes in shared memory (128-byte
+// swizzle, blocks of 128 rows x 64 columns), S, S^2 and M X in tensor memory, 16 warps between them.
+// X is held with its smaller side as rows, a tall matrix transposed on the way in and out. The block
+// of columns that is K-major for S = X X^T is MN-major for M X without moving a byte. Products are split
+// (hi lo + lo hi + hi hi) for either dtype: what such a matrix costs is the latency of its 15 products
+// one after the other, not their size. As 17 launches of the tiled kernels the two 192 x 64 matrices
+// took 81 us on the GPU; in one block each, 27 us.
+struct Small
+{
+    Source src;
+    int rows, cols, steps;
+    float ca, cb, cc, eps;
+    void* dst;               // result, or the fp32 weights
+    int64_t ldo, stride_o;
+    bf16* lowp;
+    float decay, step;
+    int vec;                 // source rows can be read four elements at a time
+    int* status;
+};
+
+constexpr int kSmallSide = 128, kSmallLong = 256;
+constexpr int kSmallThreads = 512;
+constexpr int kBlockBytes = 128 * 128;   // 128 rows of 64 fp16
+
+inline int small_smem(int m, int n)
+{
+    const int nb = (n + 63) / 64, sb = (m + 63) / 64;
+    return (2 * nb + 2 * sb) * kBlockBytes + 1024 + 256;
+}
+
+// Byte offset of element (row, col) of a plane.
+__device__ __forceinline__ uint32_t plane_at(int row, int col)
+{
+    return static_cast<uint32_t>((col >> 6) * kBlockBytes) + tc::sw128_offset(row, (col & 63) >> 3) + (col & 7) * 2;
+}
+
+// 32 columns from `col` of the lane's row as hi and lo: 1024 x value = v.
+__device__ __forceinline__ void put_planes(uint8_t* hi, uint8_t* lo, int row, int col, const float (&v)[32])
+{
+    const uint32_t block = static_cast<uint32_t>((col >> 6) * kBlockBytes);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+    {
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+        {
+            const float x = v[8 * k + 2 * i], y = v[8 * k + 2 * i + 1];
+            h[i] = pack_f16(x, y);
+            const float2 back = unpack_f16(h[i]);
+            l[i] = pack_f16(x - back.x, y - back.y);
+        }
+        const uint32_t at = block + tc::sw128_offset(row, ((col & 63) >> 3) + k);
+        *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+}
+
+template <typename T, bool MUON>
+__global__ void __launch_bounds__(kSmallThreads, 1)
+small_kernel(const Small p)
+{
+    using namespace tc;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    const bool tall = p.rows > p.cols;
+    const int m = tall ? p.cols : p.rows, n = tall ? p.rows : p.cols;
+    const int m16 = (m + 15) & ~15, n16 = (n + 15) & ~15;
+    const int nb = (n + 63) >> 6, sb = (m + 63) >> 6;
+    uint8_t* const xh = smem;
+    uint8_t* const xl = xh + nb * kBlockBytes;
+    uint8_t* const sh = xl + nb * kBlockBytes;
+    uint8_t* const sl = sh + sb * kBlockBytes;
+    uint64_t* const done = reinterpret_cast<uint64_t*>(sl + sb * kBlockBytes);
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    volatile int* const abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    __shared__ double part[kSmallThreads / 32];
+    __shared__ float shared_scale;
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0)
+    {
+        *abort = 0;
+        mbar_init(done, 1);
+        mbar_fence_init();
+    }
+    if (warp == 1) tmem_alloc(tmem_slot, 512);
+    if ((m | n) & 15)
+    {
+        // what pads the products' 16-term steps is zero
+        for (int i = threadIdx.x; i < 2 * nb * kBlockBytes / 16; i += kSmallThreads)
+        {
+            reinterpret_cast<uint4*>(xh)[i] = make_uint4(0, 0, 0, 0);
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+    dep_wait();
+    dep_release();
+
+    const bool skip = skipped_step(p.src.flags, p.src.sumsq, p.src.grad_scale);
+    if (!skip)
+    {
+        // the norm (and the momentum), then X
+        const Source& s = p.src;
+        const float clip = clip_scale(s.sumsq, s.max_norm, s.grad_scale);
+        const T* g = static_cast<const T*>(s.g) + s.stride * blockIdx.x;
+        float* mom = MUON ? s.momentum + s.stride * blockIdx.x : nullptr;
+        const int step = p.vec ? 4 : 1, per_row = p.cols / step, total = p.rows * per_row;
+        const auto value = [&](int64_t at, float (&u)[4], bool first) {
+            if (p.vec) load_n<T, 4>(g + at, u);
+            else u[0] = to_f32(g[at]);
+            if constexpr (MUON)
+            {
+                float o[4];
+                if (p.vec) load_n<float, 4>(mom + at, o);
+                else o[0] = mom[at];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                {
+                    if (k < step)
+                    {
+                        u[k] = seen(u[k], s.grad_scale, clip);
+                        if (first) o[k] = fmaf(s.beta, o[k], u[k]);
+                        u[k] = s.nesterov ? fmaf(s.beta, o[k], u[k]) : o[k];
+                    }
+                }
+                if (first)
+                {
+                    if (p.vec) *reinterpret_cast<float4*>(mom + at) = make_float4(o[0], o[1], o[2], o[3]);
+                    else mom[at] = o[0];
+                }
+            }
+        };
+        const auto store = [&](int e, const float (&u)[4], float scale) {
+            const int r = e / per_row, c = (e - r * per_row) * step;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+            {
+                if (k < step)
+                {
+                    const float v = u[k] * scale;
+                    const __half h = __float2half_rn(v);
+                    const uint32_t at = tall ? plane_at(c + k, r) : plane_at(r, c + k);
+                    *reinterpret_cast<__half*>(xh + at) = h;
+                    *reinterpret_cast<__half*>(xl + at) = __float2half_rn(v - __half2float(h));
+                }
+            }
+        };
+        // the first kKept values of a thread stay in registers from one pass to the other; the rest are
+        // read again (by the thread that wrote them, for Muon)
+        constexpr int kKept = 8;
+        float kept[kKept][4];
+        double sum = 0.0;
+#pragma unroll
+        for (int q = 0; q < kKept; ++q)
+        {
+            const int e = threadIdx.x + q * kSmallThreads;
+            if (e < total)
+            {
+                const int r = e / per_row, c = (e - r * per_row) * step;
+                value(r * s.ld + c, kept[q], true);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < kKept; ++q)
+        {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+            {
+                if (static_cast<int>(threadIdx.x) + q * kSmallThreads < total && k < step)
+                {
+                    sum += static_cast<double>(kept[q][k]) * kept[q][k];
+                }
+            }
+        }
+#pragma unroll 4
+        for (int e = threadIdx.x + kKept * kSmallThreads; e < total; e += kSmallThreads)
+        {
+            const int r = e / per_row, c = (e - r * per_row) * step;
+            float u[4];
+            value(r * s.ld + c, u, true);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+            {
+                if (k < step) sum += static_cast<double>(u[k]) * u[k];
+            }
+        }
+        sum = warp_sum(sum);
+        if (lane == 0) part[warp] = sum;
+        __syncthreads();
+        if (warp == 0)
+        {
+            sum = warp_sum(lane < kSmallThreads / 32 ? part[lane] : 0.0);
+            if (lane == 0)
+            {
+                shared_scale = static_cast<float>(static_cast<double>(kUnit) / (sqrt(sum) + static_cast<double>(p.eps)));
+            }
+        }
+        __syncthreads();
+        const float scale = shared_scale;
+#pragma unroll
+        for (int q = 0; q < kKept; ++q)
+        {
+            const int e = threadIdx.x + q * kSmallThreads;
+            if (e < total) store(e, kept[q], scale);
+        }
+#pragma unroll 4
+        for (int e = threadIdx.x + kKept * kSmallThreads; e < total; e += kSmallThreads)
+        {
+            const int r = e / per_row, c = (e - r * per_row) * step;
+            float u[4];
+            value(r * s.ld + c, u, false);
+            store(e, u, scale);
+        }
+    }
+
+    const uint32_t ts = tmem, tx = tmem + 128;   // S or S^2; M X
+    const int quarter = warp & 3, half = warp >> 2;   // TMEM lanes, and which quarter of the columns
+    const int row = quarter * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    uint32_t phase = 0;
+    // D = A B over `terms` (a multiple of 16) from the planes of a and b; thread 0 issues
+    const auto product = [&](uint32_t d, const uint8_t* ah, const uint8_t* al, const uint8_t* bh, const uint8_t* bl,
+                             auto b_mn, int cols_, int terms) {
+        fence_proxy_async();
+        fence_before();
+        __syncthreads();
+        if (warp == 0)
+        {
+            fence_after();
+            // The whole warp works out the descriptors, in registers that it shares, and one lane issues:
+            // under a branch for one thread each product took 100 to 130 cycles to issue.
+            const bool leader = pair::elect_one();
+            const uint32_t idesc = (1u << 4) | ((decltype(b_mn)::value ? 1u : 0u) << 16) |
+                                   (static_cast<uint32_t>(cols_ >> 3) << 17) | (8u << 24);
+            constexpr uint64_t bstep = decltype(b_mn)::value ? 16 * 128 / 16 : 2;
+            constexpr uint64_t bblock = decltype(b_mn)::value ? 64 * 128 / 16 : kBlockBytes / 16;
+            uint32_t accumulate = 0;
+#pragma unroll
+            for (int seg = 0; seg < 3; ++seg)
+            {
+                uint64_t a = smem_desc(smem_u32(seg == 1 ? al : ah), 16, 1024);
+                uint64_t b = smem_desc(smem_u32(seg == 0 ? bl : bh), decltype(b_mn)::value ? kBlockBytes : 16, 1024);
+#pragma unroll 1
+                for (int k = 0; k < terms; k += 64)
+                {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                    {
+                        if (k + 16 * q < terms)
+                        {
+                            if (leader) mma(d, a + 2 * q, b + bstep * q, idesc, accumulate);
+                            accumulate = 1;
+                        }
+                    }
+                    a += kBlockBytes / 16;
+                    b += bblock;
+                }
+            }
+            if (leader) commit(done);
+            __syncwarp();
+        }
+        mbar_wait(done, phase, p.status, abort);
+        phase ^= 1;
+        fence_after();
+    };
+
+    for (int k = 0; k < p.steps; ++k)
+    {
+        product(ts, xh, xl, xh, xl, std::false_type{}, m16, n16);
+        const int c0 = half * 32;
+        float v[32];
+        uint32_t r[32];
+        const auto fetch = [&](uint32_t at, float f) {
+            __syncwarp();
+            tmem_ld32(at, r);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) * f;
+        };
+        if (c0 < m16)
+        {
+            fetch(ts + lanes + c0, 1.0f / kUnit);
+            if (row < m16) put_planes(sh, sl, row, c0, v);
+        }
+        product(ts, sh, sl, sh, sl, std::false_type{}, m16, m16);
+        if (c0 < m16)
+        {
+            fetch(ts + lanes + c0, p.cc / kUnit);
+            if (row < m16)
+            {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                {
+                    const uint32_t at = (c0 >> 6) * kBlockBytes + sw128_offset(row, ((c0 & 63) >> 3) + q);
+                    const uint4 l4 = *reinterpret_cast<const uint4*>(sl + at), h4 = *reinterpret_cast<const uint4*>(sh + at);
+                    const uint32_t l[4] = {l4.x, l4.y, l4.z, l4.w}, h[4] = {h4.x, h4.y, h4.z, h4.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                    {
+                        const float2 le = unpack_f16(l[i]), he = unpack_f16(h[i]);
+                        v[8 * q + 2 * i] = fmaf(p.cb, he.x, fmaf(p.cb, le.x, v[8 * q + 2 * i]));
+                        v[8 * q + 2 * i + 1] = fmaf(p.cb, he.y, fmaf(p.cb, le.y, v[8 * q + 2 * i + 1]));
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = c0 + i == row ? v[i] + p.ca * kUnit : v[i];
+                put_planes(sh, sl, row, c0, v);
+            }
+        }
+        product(tx, sh, sl, xh, xl, std::true_type{}, n16, m16);
+#pragma unroll 1
+        for (int c = c0; c < n16; c += 128)
+        {
+            fetch(tx + lanes + c, 1.0f / kUnit);
+            if (k < p.steps - 1)
+            {
+                if (row < m16) put_planes(xh, xl, row, c, v);
+            }
+            else if (row < m && !skip)
+            {
+                const int64_t base = p.stride_o * blockIdx.x + (tall ? row : row * p.ldo);
+                const int64_t by = tall ? p.ldo : 1;
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                {
+                    if (c + i < n)
+                    {
+                        const int64_t at = base + (c + i) * by;
+                        const float o = v[i] * (1.0f / kUnit);
+                        if constexpr (MUON)
+                        {
+                            float* w = static_cast<float*>(p.dst) + at;
+                            float x = __fsub_rn(*w, __fmul_rn(p.decay, *w));
+                            x = __fsub_rn(x, __fmul_rn(p.step, o));
+                            *w = x;
+                            if (p.lowp != nullptr) p.lowp[at] = __float2bfloat16_rn(x);
+                        }
+                        else
+                        {
+                            static_cast<T*>(p.dst)[at] = from_f32<T>(o);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 1)
+    {
+        fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
 // ---- host ------------------------------------------------------------------------------------
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
@@ -737,6 +1099,46 @@ Layout layout(int64_t batch, int64_t rows, int64_t cols, bool split)
     return l;
 }
 
+bool is_small(int64_t rows, int64_t cols)
+{
+    return std::min(rows, cols) <= kSmallSide && std::max(rows, cols) <= kSmallLong;
+}
+
+template <typename T, bool MUON>
+int launch_small(const char* what, const Small& p, int64_t batch, cudaStream_t stream)
+{
+    auto kernel = small_kernel<T, MUON>;
+    constexpr int kDevices = 64;
+    static std::atomic<bool> configured[kDevices];
+    int device = 0;
+    cudaGetDevice(&device);
+    if (device < 0 || device >= kDevices)
+    {
+        return fail(VEDA_ERR_UNSUPPORTED, std::string(what) + ": no such device");
+    }
+    if (!configured[device].load(std::memory_order_acquire))
+    {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 small_smem(kSmallSide, kSmallLong)) != cudaSuccess)
+        {
+            cudaGetLastError();
+            return fail(VEDA_ERR_CUDA, std::string(what) + ": shared memory for small matrices");
+        }
+        configured[device].store(true, std::memory_order_release);
+    }
+    return launch(what, kernel, dim3(static_cast<unsigned>(batch)), dim3(kSmallThreads),
+                  small_smem(std::min(p.rows, p.cols), std::max(p.rows, p.cols)), stream, p);
+}
+
+// Whether four elements at a time can be read of every row of every matrix.
+template <typename T>
+bool reads_four(const Source& src, int64_t batch, int64_t cols)
+{
+    const uintptr_t bases = reinterpret_cast<uintptr_t>(src.g) | reinterpret_cast<uintptr_t>(src.momentum);
+    return (bases & (src.momentum != nullptr ? 15u : 4 * sizeof(T) - 1)) == 0 && cols % 4 == 0 && src.ld % 4 == 0 &&
+           (batch == 1 || src.stride % 4 == 0);
+}
+
 template <int KIND, bool SPLIT>
 int product(const char* what, const Params& p, cudaStream_t stream)
 {
@@ -753,6 +1155,13 @@ template <typename T, bool SPLIT, int LAST>
 int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, int64_t cols, int steps, float a,
             float b, float c, float eps, char* ws, Params p, cudaStream_t stream)
 {
+    if (is_small(rows, cols))
+    {
+        const Small q{src,   static_cast<int>(rows), static_cast<int>(cols), steps,   a,      b,
+                      c,     eps,                    p.dst,                  p.ldo,   p.stride_o, p.lowp,
+                      p.decay, p.step,               reads_four<T>(src, batch, cols), device_status_ptr()};
+        return launch_small<T, LAST == kMuon>(what, q, batch, stream);
+    }
     const Layout l = layout(batch, rows, cols, SPLIT);
     double* partials = reinterpret_cast<double*>(ws + l.partials);
     uint16_t* x[2] = {reinterpret_cast<uint16_t*>(ws + l.x[0]), reinterpret_cast<uint16_t*>(ws + l.x[1])};
@@ -791,10 +1200,7 @@ int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, in
             (p.lowp == nullptr || pair::make_map3(&dst_low, p.lowp, 2, true, cols, rows, batch, p.ldo, stride, 32, 32,
                                                   pair::Swizzle::k64));
     const dim3 grid(l.blocks, static_cast<unsigned>(batch));
-    // four elements at a time where every row of every matrix allows it
-    const uintptr_t bases = reinterpret_cast<uintptr_t>(src.g) | reinterpret_cast<uintptr_t>(src.momentum);
-    const bool four = (bases & (src.momentum != nullptr ? 15u : 4 * sizeof(T) - 1)) == 0 && cols % 4 == 0 &&
-                      src.ld % 4 == 0 && (batch == 1 || src.stride % 4 == 0);
+    const bool four = reads_four<T>(src, batch, cols);
     int rc = launch(what, four ? norm_kernel<T, 4> : norm_kernel<T, 1>, grid, dim3(256), 0, stream, src,
                     static_cast<int>(rows), static_cast<int>(cols), partials);
     if (rc != VEDA_OK) return rc;

@@ -86,6 +86,14 @@ struct Divisor
     }
 };
 
+// One lane of the converged warp.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 __device__ __forceinline__ uint32_t cluster_rank()
 {
     uint32_t r;
@@ -197,7 +205,7 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0);   // known to be the same in all lanes
     const int lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const int cid = static_cast<int>(blockIdx.x >> 1);
@@ -240,8 +248,9 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
     typename Work::Tile t, next;
     bool more = Work::tile(p, cid, clusters, 0, t);
     int i = 0;
-    if (warp == 0 && lane == 0)
+    if (warp == 0)
     {
+        const bool leader = elect_one();
         int stage = 0;
         uint32_t phase = 0;
         while (more)
@@ -254,19 +263,24 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
                 const int bdx = t.b_mn ? 0 : kBK, bdy = t.b_mn ? kBK : 0;
                 auto load = [&](int kb, int za, int zb) {
                     mbar_wait(&empty[stage], phase ^ 1, p.status, abort);
-                    if (rank == 0)
-                    {
-                        mbar_expect_tx(&full[stage], 2 * C_::STAGE);   // both CTAs' halves
-                    }
+                    __syncwarp();
                     const uint32_t bar = peer_addr(&full[stage], 0);
                     uint8_t* ad = sa + stage * C_::OPERAND;
                     uint8_t* bd = sb + stage * C_::OPERAND;
                     const int ax = a.x + kb * adx, ay = a.y + kb * ady;
                     const int bx = b.x + kb * bdx, by = b.y + kb * bdy;
-                    load_box(ad, a.map, bar, ax, ay, a.z + za);
-                    if (t.a_mn) load_box(ad + C_::OPERAND / 2, a.map, bar, ax + 64, ay, a.z + za);
-                    load_box(bd, b.map, bar, bx, by, b.z + zb);
-                    if (t.b_mn) load_box(bd + C_::OPERAND / 2, b.map, bar, bx + 64, by, b.z + zb);
+                    if (leader)
+                    {
+                        if (rank == 0)
+                        {
+                            mbar_expect_tx(&full[stage], 2 * C_::STAGE);   // both CTAs' halves
+                        }
+                        load_box(ad, a.map, bar, ax, ay, a.z + za);
+                        if (t.a_mn) load_box(ad + C_::OPERAND / 2, a.map, bar, ax + 64, ay, a.z + za);
+                        load_box(bd, b.map, bar, bx, by, b.z + zb);
+                        if (t.b_mn) load_box(bd + C_::OPERAND / 2, b.map, bar, bx + 64, by, b.z + zb);
+                    }
+                    __syncwarp();
                     if (++stage == C_::STAGES)
                     {
                         stage = 0;
@@ -291,8 +305,12 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
             more = Work::tile(p, cid, clusters, ++i, t);   // the ring is full of this tile's blocks
         }
     }
-    else if (warp == 1 && lane == 0 && rank == 0)
+    else if (warp == 1 && rank == 0)
     {
+        // The whole warp walks the tiles and works out the descriptors, in registers that it shares, and
+        // one lane issues: under a branch for one thread a product took some 110 cycles to issue, and four
+        // of them with their barriers more than the 512 that a k-block takes to multiply.
+        const bool leader = elect_one();
         int stage = 0, it = 0;
         uint32_t phase = 0;
         while (more)
@@ -302,28 +320,33 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
             {
                 more_next = Work::tile(p, cid, clusters, ++i, next);
             }
-            const uint32_t astep = t.a_mn ? 2048 : 32, bstep = t.b_mn ? 2048 : 32;
+            const uint32_t astep = (t.a_mn ? 2048 : 32) / 16, bstep = (t.b_mn ? 2048 : 32) / 16;   // 16 terms on
             const uint32_t albo = t.a_mn ? kBK * 128 : 16, blbo = t.b_mn ? kBK * 128 : 16;
             for (int k0 = 0; !t.skip && k0 < t.kbs; k0 += SPLIT ? kChain : t.kbs)
             {
                 const int blocks = SPLIT ? 3 * (min(t.kbs, k0 + kChain) - k0) : t.kbs;
                 const int buf = SPLIT ? 0 : it & 1;
                 mbar_wait(&tempty[buf], ((SPLIT ? it : it >> 1) & 1) ^ 1, p.status, abort);
+                __syncwarp();
                 fence_after();
                 const uint32_t d = tmem + static_cast<uint32_t>(buf * kTile);
                 for (int kb = 0; kb < blocks; ++kb)
                 {
                     mbar_wait(&full[stage], phase, p.status, abort);
+                    __syncwarp();
                     fence_after();
-                    const uint32_t ab = smem_u32(sa + stage * C_::OPERAND);
-                    const uint32_t bb = smem_u32(sb + stage * C_::OPERAND);
-#pragma unroll
-                    for (int kk = 0; kk < kBK / 16; ++kk)
+                    const uint64_t ad = smem_desc(smem_u32(sa + stage * C_::OPERAND), albo, 1024);
+                    const uint64_t bd = smem_desc(smem_u32(sb + stage * C_::OPERAND), blbo, 1024);
+                    if (leader)
                     {
-                        mma2(d, smem_desc(ab + kk * astep, albo, 1024), smem_desc(bb + kk * bstep, blbo, 1024),
-                             t.idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+#pragma unroll
+                        for (int kk = 0; kk < kBK / 16; ++kk)
+                        {
+                            mma2(d, ad + kk * astep, bd + kk * bstep, t.idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+                        }
+                        commit2(&empty[stage]);
                     }
-                    commit2(&empty[stage]);
+                    __syncwarp();
                     if (++stage == C_::STAGES)
                     {
                         stage = 0;
@@ -334,7 +357,8 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
                         more_next = Work::tile(p, cid, clusters, ++i, next);   // under the products
                     }
                 }
-                commit2(&tfull[buf]);
+                if (leader) commit2(&tfull[buf]);
+                __syncwarp();
                 ++it;
             }
             t = next;
