@@ -169,6 +169,8 @@ struct StatsWork
         a = {&p.x, 0, t.mb * pair::kTile + rank * 128, 0};
         b = {&p.w, 0, p.v0 + t.nb * pair::kTile + rank * 128, 0};
     }
+    static __device__ __forceinline__ void ready(const Params&, const Tile&, volatile int*) {}
+    static __device__ __forceinline__ void after(const Params&, const Tile&, int) {}
     static __device__ __forceinline__ void prefetch(const Params& p)
     {
         tc::tma_prefetch(&p.x);
@@ -176,7 +178,7 @@ struct StatsWork
     }
 
     static __device__ __forceinline__ void before(const Params& p, const Tile& t, State& s, int row0, int,
-                                                  pair::Staging&, int lane)
+                                                  pair::Staging&, int lane, volatile int*)
     {
         if (t.first)
         {
@@ -335,6 +337,8 @@ struct GradWork
             b = {&p.w, 0, p.v0 + n, 0};
         }
     }
+    static __device__ __forceinline__ void ready(const Params&, const Tile&, volatile int*) {}
+    static __device__ __forceinline__ void after(const Params&, const Tile&, int) {}
     static __device__ __forceinline__ void prefetch(const Params& p)
     {
         tc::tma_prefetch(&p.x);
@@ -346,7 +350,7 @@ struct GradWork
     }
 
     static __device__ __forceinline__ void before(const Params& p, const Tile& t, State& s, int row0, int,
-                                                  pair::Staging&, int lane)
+                                                  pair::Staging&, int lane, volatile int*)
     {
         if (t.kind == kQ)
         {

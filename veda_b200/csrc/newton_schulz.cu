@@ -2,11 +2,15 @@
 //
 // For each matrix of a batch, X = G / (|G|_F + eps), then `steps` times
 //   S = X X^T (of the smaller side),  M = a I + b S + c S^2,  X <- M X,
-// the odd quintic a s + b s^3 + c s^5 applied to every singular value. Three products an iteration
-// on the CTA-pair tensor-core kernel (pair_mma.cuh), the whole batch in one launch each; a tall
-// matrix is multiplied from the other side (S = X^T X, X <- X M) by operand order alone, so nothing
-// is transposed. S and M are symmetric: the tiles on and above the diagonal are computed, and each
-// one above it is written a second time, transposed.
+// the odd quintic a s + b s^3 + c s^5 applied to every singular value. All 3 x steps products of all
+// matrices are one launch of the persistent CTA-pair tensor-core kernel (pair_mma.cuh): the tiles are
+// listed step by step, matrix by matrix, and a tile of a step starts once every tile of the same
+// matrix's step before it is stored, which a counter per matrix and step tells. With a few matrices the
+// next step of one runs beside the last tiles of another, so neither the last, partly filled wave of a
+// product nor its epilogue leaves SMs idle. As one launch per product, 28 x 1024 x 1024 took 870 us
+// against @CHAIN28@. A tall matrix is multiplied from the other side (S = X^T X, X <- X M) by operand
+// order alone, so nothing is transposed. S and M are symmetric: the tiles on and above the diagonal are
+// computed, and each one above it is written a second time, transposed.
 //
 // Precision. X is held as two fp16 values, 1024 X = hi + lo (22 bits), because the quintic's slope
 // of 3.4 at 0 amplifies what is rounded off X some 480 times over five steps: with X in 16 bits
@@ -35,26 +39,31 @@ namespace ns
 
 constexpr float kUnit = 1024.0f;   // stored value = kUnit x value
 
-// What a launch computes: S, M, the next X, or the last X as a result or as the weights' update.
+// What a tile computes: S, M, the next X, or the last X as a result or as the weights' update.
 enum Kind { kGram, kPoly, kApply, kOut, kMuon };
 
 struct Params
 {
-    CUtensorMap a, b;        // operands: planes hi, lo of each matrix (X; S and M when split)
-    CUtensorMap out;         // what the launch writes, in boxes of 32 x 32
-    CUtensorMap out_t;       // S, M: the same for transposed tiles; kMuon: the bf16 weights
+    // X of either buffer as S's operands and as M's partner, S and M: planes hi, lo of each matrix
+    // (K-major boxes of 64 x 128, MN-major ones of 64 x 64)
+    CUtensorMap xg[2], xa[2], s, m;
+    // what is written, in boxes of 32 x 32: X of either buffer, S and M as they are and transposed, the
+    // destination (kMuon: fp32 weights) and the bf16 weights
+    CUtensorMap x_out[2], s_out, s_out_t, m_out, m_out_t, dst_out, lowp_out;
     int tall;
     int rows, cols;          // of X
-    int nrows, ncols;        // of what is written
-    int k;                   // terms of a sum
-    int planes_a, planes_b;  // planes of a matrix in a and b
-    int total, tm;           // tiles in all; kGram, kPoly: tiles of a side
-    pair::Divisor per_matrix, by_n;
+    int side;                // of S and M: the smaller of them
+    int planes;              // of S and M
+    int batch, steps;
+    int tm, half, whole;     // tiles of S's side; tiles of S or M of one matrix, of X of one matrix
+    int sym_tiles, iteration;   // tiles of S of all matrices; of an iteration
+    pair::Divisor by_iteration, by_sym, by_half, by_whole, by_n;
     float ca, cb, cc;
-    const uint16_t* src;     // kPoly: S; later kinds: X (read by the epilogue)
-    int64_t ld, plane;       // its pitch and plane stride
+    const uint16_t *x[2], *s_ptr;   // read by the epilogues
+    int64_t ldx, plane_x, lds, plane_s;
+    unsigned* counters;      // [batch][3 steps] finished epilogue warps
     // kOut, kMuon: the destination, stored by TMA if vec
-    void* dst;               // kMuon: the fp32 weights
+    void* dst;
     int64_t ldo, stride_o;
     int out_f32, vec;
     bf16* lowp;
@@ -63,6 +72,22 @@ struct Params
     float grad_scale;
     int flags;
     int* status;
+};
+
+struct Tile
+{
+    bool skip, a_mn, b_mn;
+    int kbs, b, mb, nb, kind, k;
+    uint32_t idesc;
+};
+
+// What a kind of tile reads and writes in its epilogue.
+struct View
+{
+    const CUtensorMap *out, *out_t;
+    int nrows, ncols;
+    const uint16_t* src;     // kPoly: S; later kinds: X
+    int64_t ld, plane;
 };
 
 __device__ __forceinline__ uint32_t pack_f16(float a, float b)
@@ -76,66 +101,9 @@ __device__ __forceinline__ float2 unpack_f16(uint32_t w)
 }
 
 template <int KIND, bool SPLIT>
-struct Work
+struct Part
 {
-    using Params = ns::Params;
     static constexpr bool SYM = KIND <= kPoly;
-    struct Tile
-    {
-        bool skip, a_mn, b_mn;
-        int kbs, b, mb, nb;
-        uint32_t idesc;
-    };
-    struct State
-    {
-        int sent = 0;   // chunks written out so far: the output sets take turns by it across tiles
-    };
-
-    static __device__ __forceinline__ bool tile(const Params& p, int cid, int clusters, int i, Tile& t)
-    {
-        const int u = cid + i * clusters;
-        if (u >= p.total)
-        {
-            return false;
-        }
-        int r;
-        t.b = p.per_matrix.div(u, r);
-        if constexpr (SYM)
-        {
-            // row mb of the upper triangle holds tm - mb tiles
-            t.mb = 0;
-            while (r >= p.tm - t.mb)
-            {
-                r -= p.tm - t.mb;
-                ++t.mb;
-            }
-            t.nb = t.mb + r;
-        }
-        else
-        {
-            t.mb = p.by_n.div(r, t.nb);
-        }
-        t.skip = false;
-        t.kbs = (p.k + pair::kBK - 1) / pair::kBK;
-        // tall: S = X^T X, X M; else S = X X^T, M X; S and M read as they are, being symmetric
-        t.a_mn = KIND == kGram && p.tall;
-        t.b_mn = KIND == kGram ? p.tall != 0 : KIND != kPoly && p.tall == 0;
-        t.idesc = pair::idesc(false, t.a_mn, t.b_mn);
-        return true;
-    }
-
-    static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, pair::Piece& a,
-                                                    pair::Piece& b)
-    {
-        const int m = t.mb * pair::kTile + rank * 128, n = t.nb * pair::kTile + rank * 128;
-        a = {&p.a, t.a_mn ? m : 0, t.a_mn ? 0 : m, p.planes_a * t.b};
-        b = {&p.b, t.b_mn ? n : 0, t.b_mn ? 0 : n, p.planes_b * t.b};
-    }
-    static __device__ __forceinline__ void prefetch(const Params& p)
-    {
-        tc::tma_prefetch(&p.a);
-        tc::tma_prefetch(&p.b);
-    }
 
     // Epilogue staging. A warp takes 32 rows x 128 columns in four chunks of 32 columns through 8 KB
     // of shared memory, four units of 2 KB (32 rows x 64 bytes, 64-byte swizzle) or two of 4 KB (32
@@ -190,7 +158,7 @@ struct Work
                      : "memory");
     }
     // 32 rows x 32 16-bit columns of a plane; zeros past the last row and column
-    static __device__ __forceinline__ void copy_plane(uint8_t* tile, const uint16_t* src, const Params& p, int row,
+    static __device__ __forceinline__ void copy_plane(uint8_t* tile, const uint16_t* src, const View& w, int row,
                                                       int col, int lane)
     {
         const int seg = lane & 3, c = col + seg * 8;
@@ -198,62 +166,58 @@ struct Work
         for (int k = 0; k < 4; ++k)
         {
             const int r = 8 * k + (lane >> 2);
-            const bool in = row + r < p.nrows && c < p.ncols;
-            copy16(tile + swz64(r, seg), in ? src + (row + r) * p.ld + c : src, in);
+            const bool in = row + r < w.nrows && c < w.ncols;
+            copy16(tile + swz64(r, seg), in ? src + (row + r) * w.ld + c : src, in);
         }
     }
 
     // Starts the copies of chunk j, one group (empty where nothing is read).
-    static __device__ __forceinline__ void load_chunk(const Params& p, const Tile& t, int j, int trow, int tcol,
+    static __device__ __forceinline__ void load_chunk(const Params& p, const View& w, const Tile& t, int j, int trow, int tcol,
                                                       uint8_t* stage, int lane)
     {
         uint8_t* in = stage + in_unit(j) * kUnitBytes;
         const int col = tcol + j * kChunk;
         if constexpr (KIND == kPoly)
         {
-            const uint16_t* src = p.src + p.plane * p.planes_a * t.b;
-            copy_plane(in, src, p, trow, col, lane);
-            if constexpr (SPLIT) copy_plane(in + kUnitBytes, src + p.plane, p, trow, col, lane);
+            const uint16_t* src = w.src + w.plane * p.planes * t.b;
+            copy_plane(in, src, w, trow, col, lane);
+            if constexpr (SPLIT) copy_plane(in + kUnitBytes, src + w.plane, w, trow, col, lane);
         }
         if constexpr (READS_X)
         {
-            copy_plane(in, p.src + p.plane * (2 * t.b + 1), p, trow, col, lane);
+            copy_plane(in, w.src + w.plane * (2 * t.b + 1), w, trow, col, lane);
         }
         if constexpr (KIND == kMuon)
         {
             if (p.vec)
             {
                 uint8_t* tile = SPLIT ? in : stage + 2 * kUnitBytes;
-                const float* w = static_cast<const float*>(p.dst) + p.stride_o * t.b;
+                const float* weights = static_cast<const float*>(p.dst) + p.stride_o * t.b;
                 const int seg = lane & 7, c = col + seg * 4;
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
                 {
                     const int r = 4 * k + (lane >> 3);
-                    const bool inside = trow + r < p.nrows && c < p.ncols;
-                    copy16(tile + tc::sw128_offset(r, seg), inside ? w + (trow + r) * p.ldo + c : w, inside);
+                    const bool inside = trow + r < w.nrows && c < w.ncols;
+                    copy16(tile + tc::sw128_offset(r, seg), inside ? weights + (trow + r) * p.ldo + c : weights, inside);
                 }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
 
-    static __device__ __forceinline__ void before(const Params& p, const Tile& t, State&, int row0, int col0,
-                                                  pair::Staging& st, int lane)
+    static __device__ __forceinline__ void before(const Params& p, const View& w, const Tile& t, int row0, int col0,
+                                                  uint8_t* stage, int lane)
     {
         if constexpr (AHEAD > 0)
         {
-            // the last tile's copies have landed, and in place, its stores have read the staging
+            // the last tile's copies have landed (its stores are complete)
             asm volatile("cp.async.wait_all;" ::: "memory");
-            if (IN_PLACE && lane == 0)
-            {
-                tc::bulk_wait_group_read<0>();
-            }
             __syncwarp();
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j)
             {
-                load_chunk(p, t, j, t.mb * pair::kTile + row0, t.nb * pair::kTile + col0, st.base, lane);
+                load_chunk(p, w, t, j, t.mb * pair::kTile + row0, t.nb * pair::kTile + col0, stage, lane);
             }
         }
     }
@@ -306,11 +270,11 @@ struct Work
     }
 
     template <int COLS>
-    static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, State& s, uint32_t taddr,
-                                                    int row0, int col0, pair::Staging& st, int lane)
+    static __device__ __forceinline__ void epilogue(const Params& p, const View& w, const Tile& t, uint32_t taddr,
+                                                    int row0, int col0, uint8_t* stage, int lane)
     {
         const int trow = t.mb * pair::kTile + row0, tcol = t.nb * pair::kTile + col0;
-        if (trow >= p.nrows || (KIND == kMuon && skipped_step(p.flags, p.sumsq, p.grad_scale)))
+        if (trow >= w.nrows || (KIND == kMuon && skipped_step(p.flags, p.sumsq, p.grad_scale)))
         {
             return;
         }
@@ -321,12 +285,12 @@ struct Work
         for (int j = 0; j < COLS / kChunk; ++j)
         {
             const int col = tcol + j * kChunk;
-            if (col >= p.ncols)
+            if (col >= w.ncols)
             {
                 break;
             }
-            uint8_t* in = st.base + in_unit(j) * kUnitBytes;
-            uint8_t* out = st.base + out_unit(s.sent++) * kUnitBytes;
+            uint8_t* in = stage + in_unit(j) * kUnitBytes;
+            uint8_t* out = stage + out_unit(j) * kUnitBytes;
             uint32_t r[kChunk];
             tc::tmem_ld32(taddr + static_cast<uint32_t>(j * kChunk), r);
             float v[kChunk];
@@ -355,7 +319,7 @@ struct Work
                 if constexpr (AHEAD > 0)
                 {
                     __syncwarp();   // the chunk is read: its unit is free
-                    next_chunk<COLS>(p, t, j, trow, tcol, st.base, lane);
+                    next_chunk<COLS>(p, w, t, j, trow, tcol, stage, lane);
                 }
                 if (lane == 0)
                 {
@@ -365,7 +329,7 @@ struct Work
             }
             if constexpr (KIND == kOut || KIND == kMuon)
             {
-                finish(p, t, trow, col, in, out, st.base, lane, v);
+                finish(p, w, t, trow, col, in, out, stage, lane, v);
             }
             else
             {
@@ -393,12 +357,12 @@ struct Work
                 __syncwarp();
                 if (lane == 0)
                 {
-                    tc::tma_store_3d(&p.out, out, col, trow, z);
-                    if constexpr (PLANES == 2) tc::tma_store_3d(&p.out, out + kUnitBytes, col, trow, z + 1);
+                    tc::tma_store_3d(w.out, out, col, trow, z);
+                    if constexpr (PLANES == 2) tc::tma_store_3d(w.out, out + kUnitBytes, col, trow, z + 1);
                     if (mirror)
                     {
-                        tc::tma_store_3d(&p.out_t, out + PLANES * kUnitBytes, trow, col, z);
-                        if constexpr (PLANES == 2) tc::tma_store_3d(&p.out_t, out + 3 * kUnitBytes, trow, col, z + 1);
+                        tc::tma_store_3d(w.out_t, out + PLANES * kUnitBytes, trow, col, z);
+                        if constexpr (PLANES == 2) tc::tma_store_3d(w.out_t, out + 3 * kUnitBytes, trow, col, z + 1);
                     }
                     tc::bulk_commit_group();
                 }
@@ -410,19 +374,19 @@ struct Work
                     tc::bulk_wait_group_read<0>();   // the stores have read the units
                 }
                 __syncwarp();
-                next_chunk<COLS>(p, t, j, trow, tcol, st.base, lane);
+                next_chunk<COLS>(p, w, t, j, trow, tcol, stage, lane);
             }
         }
     }
 
     // The copies of chunk j + AHEAD, or an empty group past the last, which keeps the groups counted.
     template <int COLS>
-    static __device__ __forceinline__ void next_chunk(const Params& p, const Tile& t, int j, int trow, int tcol,
+    static __device__ __forceinline__ void next_chunk(const Params& p, const View& w, const Tile& t, int j, int trow, int tcol,
                                                       uint8_t* stage, int lane)
     {
         if (j + AHEAD < COLS / kChunk)
         {
-            load_chunk(p, t, j + AHEAD, trow, tcol, stage, lane);
+            load_chunk(p, w, t, j + AHEAD, trow, tcol, stage, lane);
         }
         else
         {
@@ -447,14 +411,14 @@ struct Work
 
     // The last product's result: written out, or applied to the weights, through the staging where TMA
     // can describe the destination, else element by element.
-    static __device__ __forceinline__ void finish(const Params& p, const Tile& t, int trow, int col, uint8_t* in,
+    static __device__ __forceinline__ void finish(const Params& p, const View& w, const Tile& t, int trow, int col, uint8_t* in,
                                                   uint8_t* out, uint8_t* stage, int lane, float (&v)[kChunk])
     {
 #pragma unroll
         for (int i = 0; i < kChunk; ++i) v[i] *= 1.0f / kUnit;
         if (!p.vec)
         {
-            finish_direct(p, t, trow + lane, col, v);
+            finish_direct(p, w, t, trow + lane, col, v);
             return;
         }
         uint32_t w16[16];
@@ -464,11 +428,11 @@ struct Work
 #pragma unroll
             for (int k = 0; k < 8; ++k)
             {
-                const float4 w = *reinterpret_cast<const float4*>(tile + tc::sw128_offset(lane, k));
-                v[4 * k] = update(p, w.x, v[4 * k]);
-                v[4 * k + 1] = update(p, w.y, v[4 * k + 1]);
-                v[4 * k + 2] = update(p, w.z, v[4 * k + 2]);
-                v[4 * k + 3] = update(p, w.w, v[4 * k + 3]);
+                const float4 old = *reinterpret_cast<const float4*>(tile + tc::sw128_offset(lane, k));
+                v[4 * k] = update(p, old.x, v[4 * k]);
+                v[4 * k + 1] = update(p, old.y, v[4 * k + 1]);
+                v[4 * k + 2] = update(p, old.z, v[4 * k + 2]);
+                v[4 * k + 3] = update(p, old.w, v[4 * k + 3]);
             }
             put_f32(tile, lane, v);
             if constexpr (!SPLIT)
@@ -480,8 +444,8 @@ struct Work
             __syncwarp();
             if (lane == 0)
             {
-                tc::tma_store_3d(&p.out, tile, col, trow, t.b);
-                if constexpr (!SPLIT) tc::tma_store_3d(&p.out_t, out, col, trow, t.b);
+                tc::tma_store_3d(w.out, tile, col, trow, t.b);
+                if constexpr (!SPLIT) tc::tma_store_3d(w.out_t, out, col, trow, t.b);
                 tc::bulk_commit_group();
             }
         }
@@ -500,16 +464,16 @@ struct Work
             __syncwarp();
             if (lane == 0)
             {
-                tc::tma_store_3d(&p.out, out, col, trow, t.b);
+                tc::tma_store_3d(w.out, out, col, trow, t.b);
                 tc::bulk_commit_group();
             }
         }
     }
 
-    static __device__ __forceinline__ void finish_direct(const Params& p, const Tile& t, int row, int col,
+    static __device__ __forceinline__ void finish_direct(const Params& p, const View& w, const Tile& t, int row, int col,
                                                          float (&v)[kChunk])
     {
-        if (row >= p.nrows)
+        if (row >= w.nrows)
         {
             return;
         }
@@ -517,13 +481,13 @@ struct Work
 #pragma unroll
         for (int i = 0; i < kChunk; ++i)
         {
-            if (col + i < p.ncols)
+            if (col + i < w.ncols)
             {
                 if constexpr (KIND == kMuon)
                 {
-                    float* w = static_cast<float*>(p.dst) + at + i;
-                    *w = update(p, *w, v[i]);
-                    if (p.lowp != nullptr) p.lowp[at + i] = __float2bfloat16_rn(*w);
+                    float* weight = static_cast<float*>(p.dst) + at + i;
+                    *weight = update(p, *weight, v[i]);
+                    if (p.lowp != nullptr) p.lowp[at + i] = __float2bfloat16_rn(*weight);
                 }
                 else if (p.out_f32)
                 {
@@ -535,6 +499,176 @@ struct Work
                 }
             }
         }
+    }
+};
+
+// The tiles of all products, step by step and matrix by matrix. LAST: kOut or kMuon.
+template <int LAST, bool SPLIT>
+struct Work
+{
+    using Params = ns::Params;
+    using Tile = ns::Tile;
+    struct State
+    {
+    };
+    static constexpr unsigned kArrivals = 16;   // epilogue warps of a CTA pair
+
+    static __device__ __forceinline__ bool tile(const Params& p, int cid, int clusters, int i, Tile& t)
+    {
+        int r;
+        t.k = p.by_iteration.div(cid + i * clusters, r);
+        if (t.k >= p.steps)
+        {
+            return false;
+        }
+        if (r < 2 * p.sym_tiles)
+        {
+            t.kind = p.by_sym.div(r, r);   // kGram, kPoly
+            t.b = p.by_half.div(r, r);
+            // row mb of the upper triangle holds tm - mb tiles
+            t.mb = 0;
+            while (r >= p.tm - t.mb)
+            {
+                r -= p.tm - t.mb;
+                ++t.mb;
+            }
+            t.nb = t.mb + r;
+        }
+        else
+        {
+            t.kind = kApply;
+            t.b = p.by_whole.div(r - 2 * p.sym_tiles, r);
+            t.mb = p.by_n.div(r, t.nb);
+        }
+        t.skip = false;
+        const int terms = t.kind == kGram ? (p.tall ? p.rows : p.cols) : p.side;
+        t.kbs = (terms + pair::kBK - 1) / pair::kBK;
+        // tall: S = X^T X, X M; else S = X X^T, M X; S and M read as they are, being symmetric
+        t.a_mn = t.kind == kGram && p.tall;
+        t.b_mn = t.kind == kGram ? p.tall != 0 : t.kind != kPoly && p.tall == 0;
+        t.idesc = pair::idesc(false, t.a_mn, t.b_mn);
+        return true;
+    }
+
+    static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, pair::Piece& a,
+                                                    pair::Piece& b)
+    {
+        const int m = t.mb * pair::kTile + rank * 128, n = t.nb * pair::kTile + rank * 128;
+        const CUtensorMap* x = t.kind == kGram ? &p.xg[t.k & 1] : &p.xa[t.k & 1];
+        const bool x_first = t.kind == kGram || (t.kind == kApply && p.tall);
+        const bool x_second = t.kind == kGram || (t.kind == kApply && !p.tall);
+        const CUtensorMap* sym = t.kind == kPoly ? &p.s : &p.m;
+        a = {x_first ? x : sym, t.a_mn ? m : 0, t.a_mn ? 0 : m, (x_first ? 2 : p.planes) * t.b};
+        b = {x_second ? x : sym, t.b_mn ? n : 0, t.b_mn ? 0 : n, (x_second ? 2 : p.planes) * t.b};
+    }
+    static __device__ __forceinline__ void prefetch(const Params& p)
+    {
+        tc::tma_prefetch(&p.xg[0]);
+        tc::tma_prefetch(&p.s);
+        tc::tma_prefetch(&p.m);
+        tc::tma_prefetch(&p.xa[0]);
+    }
+
+    // Waits (bounded) until the matrix's step before is stored: its counter is full.
+    static __device__ __forceinline__ void ready(const Params& p, const Tile& t, volatile int* abort)
+    {
+        const int step = 3 * t.k + t.kind;
+        if (step == 0)
+        {
+            return;
+        }
+        const unsigned want = kArrivals * static_cast<unsigned>(t.kind == kGram ? p.whole : p.half);
+        const unsigned* c = p.counters + static_cast<int64_t>(t.b) * 3 * p.steps + step - 1;
+        const auto full = [&] {
+            unsigned have;
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(have) : "l"(c) : "memory");
+            return have >= want;
+        };
+        if (!full())
+        {
+            const long long start = clock64();
+            while (!full())
+            {
+                if (*abort != 0)
+                {
+                    break;
+                }
+                if (clock64() - start > tc::kWaitBudget)
+                {
+                    *abort = 1;
+                    if (p.status != nullptr) atomicExch(p.status, VEDA_ERR_TIMEOUT);
+                    break;
+                }
+            }
+        }
+        // what other SMs stored is read by TMA next
+        asm volatile("fence.proxy.async.global;" ::: "memory");
+    }
+
+    static __device__ __forceinline__ View view(const Params& p, const Tile& t)
+    {
+        View w;
+        if (t.kind == kGram)
+        {
+            w = {&p.s_out, &p.s_out_t, p.side, p.side, nullptr, 0, 0};
+        }
+        else if (t.kind == kPoly)
+        {
+            w = {&p.m_out, &p.m_out_t, p.side, p.side, p.s_ptr, p.lds, p.plane_s};
+        }
+        else
+        {
+            const bool last = t.k == p.steps - 1;
+            w = {last ? &p.dst_out : &p.x_out[(t.k + 1) & 1], &p.lowp_out, p.rows, p.cols, p.x[t.k & 1], p.ldx, p.plane_x};
+        }
+        return w;
+    }
+
+    // A function of the Part that the tile's kind names.
+    template <typename F>
+    static __device__ __forceinline__ void with_part(const Params& p, const Tile& t, F&& f)
+    {
+        if (t.kind == kGram) f(Part<kGram, SPLIT>{});
+        else if (t.kind == kPoly) f(Part<kPoly, SPLIT>{});
+        else if (t.k < p.steps - 1) f(Part<kApply, SPLIT>{});
+        else f(Part<LAST, SPLIT>{});
+    }
+
+    static __device__ __forceinline__ void before(const Params& p, const Tile& t, State&, int row0, int col0,
+                                                  pair::Staging& st, int lane, volatile int* abort)
+    {
+        if (t.kind == kGram)
+        {
+            return;   // its epilogue reads nothing
+        }
+        if (lane == 0)
+        {
+            ready(p, t, abort);
+        }
+        __syncwarp();
+        const View w = view(p, t);
+        with_part(p, t, [&](auto part) { part.before(p, w, t, row0, col0, st.base, lane); });
+    }
+
+    template <int COLS>
+    static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, State&, uint32_t taddr,
+                                                    int row0, int col0, pair::Staging& st, int lane)
+    {
+        const View w = view(p, t);
+        with_part(p, t, [&](auto part) { part.template epilogue<COLS>(p, w, t, taddr, row0, col0, st.base, lane); });
+    }
+
+    // The warp's share of the tile is stored: counts it.
+    static __device__ __forceinline__ void after(const Params& p, const Tile& t, int lane)
+    {
+        if (lane == 0)
+        {
+            tc::bulk_wait_group<0>();
+            asm volatile("fence.proxy.async.global;" ::: "memory");
+            unsigned* c = p.counters + static_cast<int64_t>(t.b) * 3 * p.steps + 3 * t.k + t.kind;
+            asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(c) : "memory");
+        }
+        __syncwarp();
     }
 };
 
@@ -631,15 +765,20 @@ norm_kernel(Source s, int rows, int cols, double* __restrict__ partials)
     }
 }
 
-// X's two planes: 1024 u / (|u| + eps), the norm summed from the blocks' partials in a fixed order.
+// X's two planes: 1024 u / (|u| + eps), the norm summed from the blocks' partials in a fixed order; and
+// the matrix's counters, cleared.
 template <typename T, int N>
 __global__ void __launch_bounds__(256)
 init_kernel(Source s, int rows, int cols, const double* __restrict__ partials, float eps, uint16_t* __restrict__ x,
-            int64_t ldx, int64_t plane)
+            int64_t ldx, int64_t plane, unsigned* __restrict__ counters, int steps)
 {
     __shared__ double part[8];
     dep_wait();
     dep_release();
+    if (blockIdx.x == 0)
+    {
+        for (int i = threadIdx.x; i < 3 * steps; i += 256) counters[static_cast<int64_t>(blockIdx.y) * 3 * steps + i] = 0;
+    }
     if (skipped_step(s.flags, s.sumsq, s.grad_scale))
     {
         return;
@@ -1064,16 +1203,17 @@ int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 constexpr int64_t kMaxExtent = 1 << 20;
 constexpr int64_t kMaxBatch = 1 << 15;
+constexpr int kMaxSteps = 64;   // the workspace holds counters for as many
 
 struct Layout
 {
     int planes;              // of S and P: 1, or 2 for split products
     int64_t m, ldx, plane_x, lds, plane_s;
     unsigned blocks;         // per matrix, of the elementwise launches
-    size_t partials, x[2], s, p, total;
+    size_t partials, counters, x[2], s, p, total;
 };
 
-Layout layout(int64_t batch, int64_t rows, int64_t cols, bool split)
+Layout layout(int64_t batch, int64_t rows, int64_t cols, bool split, int steps)
 {
     Layout l{};
     size_t at = 0;
@@ -1091,6 +1231,7 @@ Layout layout(int64_t batch, int64_t rows, int64_t cols, bool split)
     // 8 rows a pass, at most 256 blocks a matrix; the same for every batch, so that a matrix's norm is
     l.blocks = static_cast<unsigned>(std::min<int64_t>((rows + 7) / 8, 256));
     l.partials = take(batch * l.blocks * 8);
+    l.counters = take(batch * 3 * steps * 4);
     l.x[0] = take(batch * 2 * l.plane_x * 2);
     l.x[1] = take(batch * 2 * l.plane_x * 2);
     l.s = take(batch * l.planes * l.plane_s * 2);
@@ -1139,17 +1280,6 @@ bool reads_four(const Source& src, int64_t batch, int64_t cols)
            (batch == 1 || src.stride % 4 == 0);
 }
 
-template <int KIND, bool SPLIT>
-int product(const char* what, const Params& p, cudaStream_t stream)
-{
-    const int clusters = pair::clusters_available<Work<KIND, SPLIT>, 8, SPLIT>();
-    if (clusters < 1)
-    {
-        return fail(VEDA_ERR_UNSUPPORTED, std::string(what) + ": no CTA pair fits on this device");
-    }
-    return pair::launch_pair<Work<KIND, SPLIT>, 8, SPLIT>(what, p, std::min(p.total, clusters), stream);
-}
-
 // norm, X, then the products of every step; p's destination says what the last one (LAST) writes.
 template <typename T, bool SPLIT, int LAST>
 int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, int64_t cols, int steps, float a,
@@ -1162,26 +1292,26 @@ int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, in
                       p.decay, p.step,               reads_four<T>(src, batch, cols), device_status_ptr()};
         return launch_small<T, LAST == kMuon>(what, q, batch, stream);
     }
-    const Layout l = layout(batch, rows, cols, SPLIT);
+    const Layout l = layout(batch, rows, cols, SPLIT, kMaxSteps);
     double* partials = reinterpret_cast<double*>(ws + l.partials);
     uint16_t* x[2] = {reinterpret_cast<uint16_t*>(ws + l.x[0]), reinterpret_cast<uint16_t*>(ws + l.x[1])};
     uint16_t* sm[2] = {reinterpret_cast<uint16_t*>(ws + l.s), reinterpret_cast<uint16_t*>(ws + l.p)};
     const bool tall = rows > cols;
     const int64_t m = l.m, sp = l.planes * batch;
-    // X of either buffer as S's operands, as M's partner (K-major boxes are 128 high) and written; S and
-    // M read (they are symmetric: K-major always), written, and written transposed
-    CUtensorMap xg[2], xa[2], xs[2], ml[2], ms[2], mt[2], dst{}, dst_low{};
-    bool ok = true;
+    bool ok = pair::make_map3(&p.s, sm[0], 2, false, m, m, sp, l.lds, l.plane_s, 64, 128) &&
+              pair::make_map3(&p.m, sm[1], 2, false, m, m, sp, l.lds, l.plane_s, 64, 128) &&
+              pair::make_map3(&p.s_out, sm[0], 2, false, m, m, sp, l.lds, l.plane_s, 32, 32, pair::Swizzle::k64) &&
+              pair::make_map3(&p.m_out, sm[1], 2, false, m, m, sp, l.lds, l.plane_s, 32, 32, pair::Swizzle::k64) &&
+              pair::make_map3(&p.s_out_t, sm[0], 2, false, m, m, sp, l.lds, l.plane_s, 32, 32, pair::Swizzle::kNone) &&
+              pair::make_map3(&p.m_out_t, sm[1], 2, false, m, m, sp, l.lds, l.plane_s, 32, 32, pair::Swizzle::kNone);
     for (int k = 0; k < 2; ++k)
     {
         ok = ok &&
-             pair::make_map3(&xg[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 64, tall ? 64 : 128) &&
-             pair::make_map3(&xa[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 64, tall ? 128 : 64) &&
-             pair::make_map3(&xs[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 32, 32,
-                             pair::Swizzle::k64) &&
-             pair::make_map3(&ml[k], sm[k], 2, false, m, m, sp, l.lds, l.plane_s, 64, 128) &&
-             pair::make_map3(&ms[k], sm[k], 2, false, m, m, sp, l.lds, l.plane_s, 32, 32, pair::Swizzle::k64) &&
-             pair::make_map3(&mt[k], sm[k], 2, false, m, m, sp, l.lds, l.plane_s, 32, 32, pair::Swizzle::kNone);
+             pair::make_map3(&p.xg[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 64, tall ? 64 : 128) &&
+             pair::make_map3(&p.xa[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 64, tall ? 128 : 64) &&
+             pair::make_map3(&p.x_out[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 32, 32,
+                             pair::Swizzle::k64);
+        p.x[k] = x[k];
     }
     if (!ok)
     {
@@ -1195,9 +1325,9 @@ int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, in
     const bool f32 = LAST == kMuon || SPLIT;
     p.out_f32 = f32;
     p.vec = fits(p.dst, f32 ? 4 : 2) && (p.lowp == nullptr || fits(p.lowp, 2)) &&
-            pair::make_map3(&dst, p.dst, f32 ? 4 : 2, !f32, cols, rows, batch, p.ldo, stride, 32, 32,
+            pair::make_map3(&p.dst_out, p.dst, f32 ? 4 : 2, !f32, cols, rows, batch, p.ldo, stride, 32, 32,
                             f32 ? pair::Swizzle::k128 : pair::Swizzle::k64) &&
-            (p.lowp == nullptr || pair::make_map3(&dst_low, p.lowp, 2, true, cols, rows, batch, p.ldo, stride, 32, 32,
+            (p.lowp == nullptr || pair::make_map3(&p.lowp_out, p.lowp, 2, true, cols, rows, batch, p.ldo, stride, 32, 32,
                                                   pair::Swizzle::k64));
     const dim3 grid(l.blocks, static_cast<unsigned>(batch));
     const bool four = reads_four<T>(src, batch, cols);
@@ -1206,66 +1336,50 @@ int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, in
     if (rc != VEDA_OK) return rc;
     rc = launch(what, four ? init_kernel<T, 4> : init_kernel<T, 1>, grid, dim3(256), 0, stream, src,
                 static_cast<int>(rows), static_cast<int>(cols), static_cast<const double*>(partials), eps, x[0], l.ldx,
-                l.plane_x);
+                l.plane_x, reinterpret_cast<unsigned*>(ws + l.counters), steps);
     if (rc != VEDA_OK) return rc;
     const int64_t tm = (m + 255) / 256, tr = (rows + 255) / 256, tc = (cols + 255) / 256;
-    const int64_t half = tm * (tm + 1) / 2 * batch, whole = tr * tc * batch;
-    if (half >= (1ll << 30) || whole >= (1ll << 30))
+    const int64_t half = tm * (tm + 1) / 2, whole = tr * tc, iteration = (2 * half + whole) * batch;
+    if (iteration >= (1ll << 30) / steps)
     {
         return fail(VEDA_ERR_INVALID_ARGUMENT, std::string(what) + ": too many tiles");
     }
     p.tall = tall;
     p.rows = static_cast<int>(rows);
     p.cols = static_cast<int>(cols);
+    p.side = static_cast<int>(m);
+    p.planes = l.planes;
+    p.batch = static_cast<int>(batch);
+    p.steps = steps;
+    p.tm = static_cast<int>(tm);
+    p.half = static_cast<int>(half);
+    p.whole = static_cast<int>(whole);
+    p.sym_tiles = static_cast<int>(half * batch);
+    p.iteration = static_cast<int>(iteration);
+    p.by_iteration = pair::Divisor(static_cast<uint32_t>(iteration));
+    p.by_sym = pair::Divisor(static_cast<uint32_t>(half * batch));
+    p.by_half = pair::Divisor(static_cast<uint32_t>(half));
+    p.by_whole = pair::Divisor(static_cast<uint32_t>(whole));
+    p.by_n = pair::Divisor(static_cast<uint32_t>(tc));
     p.ca = a;
     p.cb = b;
     p.cc = c;
-    p.tm = static_cast<int>(tm);
-    p.by_n = pair::Divisor(static_cast<uint32_t>(tc));
+    p.s_ptr = sm[0];
+    p.ldx = l.ldx;
+    p.plane_x = l.plane_x;
+    p.lds = l.lds;
+    p.plane_s = l.plane_s;
+    p.counters = reinterpret_cast<unsigned*>(ws + l.counters);
     p.status = device_status_ptr();
-    const pair::Divisor per_half(static_cast<uint32_t>(tm * (tm + 1) / 2)), per_whole(static_cast<uint32_t>(tr * tc));
-    for (int k = 0; k < steps; ++k)
+    using W = Work<LAST, SPLIT>;
+    const int clusters = pair::clusters_available<W, 8, SPLIT>();
+    if (clusters < 1)
     {
-        p.total = static_cast<int>(half);
-        p.per_matrix = per_half;
-        p.nrows = p.ncols = static_cast<int>(m);
-        // S
-        p.a = p.b = xg[k & 1];
-        p.planes_a = p.planes_b = 2;
-        p.k = static_cast<int>(std::max(rows, cols));
-        p.out = ms[0];
-        p.out_t = mt[0];
-        rc = product<kGram, SPLIT>(what, p, stream);
-        if (rc != VEDA_OK) return rc;
-        // M
-        p.a = p.b = ml[0];
-        p.planes_a = p.planes_b = l.planes;
-        p.k = static_cast<int>(m);
-        p.src = sm[0];
-        p.ld = l.lds;
-        p.plane = l.plane_s;
-        p.out = ms[1];
-        p.out_t = mt[1];
-        rc = product<kPoly, SPLIT>(what, p, stream);
-        if (rc != VEDA_OK) return rc;
-        // M X, or X M
-        p.total = static_cast<int>(whole);
-        p.per_matrix = per_whole;
-        p.nrows = p.rows;
-        p.ncols = p.cols;
-        p.a = tall ? xa[k & 1] : ml[1];
-        p.b = tall ? ml[1] : xa[k & 1];
-        p.planes_a = tall ? 2 : l.planes;
-        p.planes_b = tall ? l.planes : 2;
-        p.src = x[k & 1];
-        p.ld = l.ldx;
-        p.plane = l.plane_x;
-        p.out = k < steps - 1 ? xs[(k + 1) & 1] : dst;
-        p.out_t = dst_low;
-        rc = k < steps - 1 ? product<kApply, SPLIT>(what, p, stream) : product<LAST, SPLIT>(what, p, stream);
-        if (rc != VEDA_OK) return rc;
+        return fail(VEDA_ERR_UNSUPPORTED, std::string(what) + ": no CTA pair fits on this device");
     }
-    return VEDA_OK;
+    // more clusters than a step of the batch has tiles would only wait
+    const int64_t most = std::max(half, whole) * batch;
+    return pair::launch_together<W, 8, SPLIT>(what, p, static_cast<int>(std::min<int64_t>(most, clusters)), stream);
 }
 
 bool bad_extent(int64_t batch, int64_t rows, int64_t cols)
@@ -1294,7 +1408,7 @@ extern "C" size_t veda_orthogonalize_workspace(int64_t batch, int64_t rows, int6
     {
         return 0;
     }
-    return ns::layout(batch, rows, cols, dtype == VEDA_F32).total;
+    return ns::layout(batch, rows, cols, dtype == VEDA_F32, ns::kMaxSteps).total;
 }
 
 extern "C" size_t veda_muon_step_workspace(int64_t batch, int64_t rows, int64_t cols, int dtype)
@@ -1312,7 +1426,7 @@ extern "C" int veda_orthogonalize(const void* g, int64_t ldg, int64_t stride_g, 
     VEDA_REQUIRE(ldg >= cols && ldo >= cols, "leading dimension smaller than cols");
     VEDA_REQUIRE(batch <= 1 || (stride_g >= 0 && stride_o >= (rows - 1) * ldo + cols),
                  "the matrices of the output overlap");
-    VEDA_REQUIRE(steps >= 1, "at least one step");
+    VEDA_REQUIRE(steps >= 1 && steps <= ns::kMaxSteps, "steps must lie in 1 .. 64");
     VEDA_REQUIRE(eps >= 0.0f, "eps must not be negative");
     if (batch == 0 || rows == 0 || cols == 0)
     {
@@ -1321,7 +1435,7 @@ extern "C" int veda_orthogonalize(const void* g, int64_t ldg, int64_t stride_g, 
     VEDA_REQUIRE(g != nullptr && out != nullptr, "null pointer");
     const bool split = dtype == VEDA_F32;
     int rc = ns::check_workspace("veda_orthogonalize", workspace, workspace_bytes,
-                                 ns::layout(batch, rows, cols, split).total);
+                                 ns::layout(batch, rows, cols, split, ns::kMaxSteps).total);
     if (rc != VEDA_OK) return rc;
     ns::Params p{};
     p.dst = out;
@@ -1347,7 +1461,7 @@ extern "C" int veda_muon_step(float* master, float* momentum, const float* grad,
                  "learning rate, eps and weight decay must not be negative");
     VEDA_REQUIRE(beta >= 0.0f && beta < 1.0f, "beta must lie in [0, 1)");
     VEDA_REQUIRE(sumsq == nullptr || max_norm > 0.0f, "max_norm must be positive");
-    VEDA_REQUIRE(steps >= 1, "at least one step");
+    VEDA_REQUIRE(steps >= 1 && steps <= ns::kMaxSteps, "steps must lie in 1 .. 64");
     if (batch == 0 || rows == 0 || cols == 0)
     {
         return VEDA_OK;
@@ -1355,7 +1469,7 @@ extern "C" int veda_muon_step(float* master, float* momentum, const float* grad,
     VEDA_REQUIRE(master != nullptr && momentum != nullptr && grad != nullptr, "null pointer");
     const bool split = lowp == nullptr;
     int rc = ns::check_workspace("veda_muon_step", workspace, workspace_bytes,
-                                 ns::layout(batch, rows, cols, split).total);
+                                 ns::layout(batch, rows, cols, split, ns::kMaxSteps).total);
     if (rc != VEDA_OK) return rc;
     ns::Params p{};
     p.dst = master;

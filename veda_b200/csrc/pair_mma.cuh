@@ -25,8 +25,10 @@
 //   bool tile(p, cid, clusters, i, t)  the i-th tile of cluster cid; false at the end of its list
 //   void operands(p, t, rank, a, b)    where the operand pieces of CTA `rank` lie at k = 0
 //   void prefetch(p)                   fetches the tensor maps of the operands
+//   void ready(p, t, abort)            by one thread, before the tile's operands are loaded
 //   void before(p, t, state, ...)      per epilogue warp, while the tile's products run
 //   void epilogue(p, t, state, ...)    one warp's 32 rows x COLS columns of the finished tile
+//   void after(p, t, lane)             per epilogue warp, the accumulator handed back
 // All roles walk the same list, so tile() must depend on its arguments and on Params alone.
 #pragma once
 
@@ -257,6 +259,11 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
         {
             if (!t.skip)
             {
+                if (leader)
+                {
+                    Work::ready(p, t, abort);
+                }
+                __syncwarp();
                 Piece a, b;
                 Work::operands(p, t, static_cast<int>(rank), a, b);
                 const int adx = t.a_mn ? 0 : kBK, ady = t.a_mn ? kBK : 0;
@@ -379,7 +386,7 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
         {
             if (!t.skip)
             {
-                Work::before(p, t, state, row0, col0, st, lane);
+                Work::before(p, t, state, row0, col0, st, lane, abort);
             }
             const bool more_next = Work::tile(p, cid, clusters, ++i, next);
             for (int k0 = 0; !t.skip && k0 < t.kbs; k0 += SPLIT ? kChain : t.kbs)
@@ -408,6 +415,10 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
                     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
                                      release + static_cast<uint32_t>(buf * 8))
                                  : "memory");
+                }
+                if (last)
+                {
+                    Work::after(p, t, lane);
                 }
                 ++it;
             }
@@ -489,6 +500,31 @@ int launch_pair(const char* what, const typename Work::Params& p, int clusters, 
 {
     return launch(what, pair_kernel<Work, EPI_WARPS, SPLIT>, dim3(2 * clusters), dim3(Cfg<EPI_WARPS>::THREADS),
                   Cfg<EPI_WARPS>::SMEM, s, p);
+}
+
+// The same with all clusters on the device at once (a cooperative launch), for a Work whose tiles wait
+// for one another. Such a launch does not start before its predecessor has ended.
+template <class Work, int EPI_WARPS, bool SPLIT>
+int launch_together(const char* what, const typename Work::Params& p, int clusters, cudaStream_t s)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(2 * clusters);
+    cfg.blockDim = dim3(Cfg<EPI_WARPS>::THREADS);
+    cfg.dynamicSmemBytes = Cfg<EPI_WARPS>::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeCooperative;
+    attr.val.cooperative = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    count_launch();
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, pair_kernel<Work, EPI_WARPS, SPLIT>, p);
+    if (err != cudaSuccess)
+    {
+        cudaGetLastError();
+        return fail(VEDA_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(err));
+    }
+    return check_launch(what);
 }
 
 } // namespace veda::cuda::pair
