@@ -131,6 +131,7 @@ __device__ __forceinline__ int counted_target(const Params& p, int row)
 struct StatsWork
 {
     using Params = lce::Params;
+    static constexpr int TN = pair::kTile;
     struct Tile
     {
         bool skip, first, last, a_mn, b_mn;
@@ -260,6 +261,7 @@ struct StatsWork
 struct GradWork
 {
     using Params = lce::Params;
+    static constexpr int TN = pair::kTile;
     enum Kind { kDw, kDx, kQ };
     struct Tile
     {

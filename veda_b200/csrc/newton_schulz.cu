@@ -55,7 +55,7 @@ struct Params
     int side;                // of S and M: the smaller of them
     int planes;              // of S and M
     int batch, steps;
-    int tm, half, whole;     // tiles of S's side; tiles of S or M of one matrix, of X of one matrix
+    int tn, half, whole;     // column tiles of S; tiles of S or M of one matrix, of X of one matrix
     int sym_tiles, iteration;   // tiles of S of all matrices; of an iteration
     pair::Divisor by_iteration, by_sym, by_half, by_whole, by_n;
     float ca, cb, cc;
@@ -100,7 +100,7 @@ __device__ __forceinline__ float2 unpack_f16(uint32_t w)
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
-template <int KIND, bool SPLIT>
+template <int KIND, bool SPLIT, int TN>
 struct Part
 {
     static constexpr bool SYM = KIND <= kPoly;
@@ -217,7 +217,7 @@ struct Part
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j)
             {
-                load_chunk(p, w, t, j, t.mb * pair::kTile + row0, t.nb * pair::kTile + col0, stage, lane);
+                load_chunk(p, w, t, j, t.mb * pair::kTile + row0, t.nb * TN + col0, stage, lane);
             }
         }
     }
@@ -273,12 +273,12 @@ struct Part
     static __device__ __forceinline__ void epilogue(const Params& p, const View& w, const Tile& t, uint32_t taddr,
                                                     int row0, int col0, uint8_t* stage, int lane)
     {
-        const int trow = t.mb * pair::kTile + row0, tcol = t.nb * pair::kTile + col0;
+        const int trow = t.mb * pair::kTile + row0, tcol = t.nb * TN + col0;
         if (trow >= w.nrows || (KIND == kMuon && skipped_step(p.flags, p.sumsq, p.grad_scale)))
         {
             return;
         }
-        const bool mirror = SYM && t.mb != t.nb;
+        const bool mirror = SYM && t.nb >= (pair::kTile / TN) * (t.mb + 1);   // right of the diagonal tiles
         // the tile's sums carry kUnit^2; what is stored carries kUnit
         const float f = (KIND == kPoly ? p.cc : 1.0f) / kUnit;
 #pragma unroll 1
@@ -503,9 +503,10 @@ struct Part
 };
 
 // The tiles of all products, step by step and matrix by matrix. LAST: kOut or kMuon.
-template <int LAST, bool SPLIT>
+template <int LAST, bool SPLIT, int TN_>
 struct Work
 {
+    static constexpr int TN = TN_;
     using Params = ns::Params;
     using Tile = ns::Tile;
     struct State
@@ -525,14 +526,16 @@ struct Work
         {
             t.kind = p.by_sym.div(r, r);   // kGram, kPoly
             t.b = p.by_half.div(r, r);
-            // row mb of the upper triangle holds tm - mb tiles
+            // row mb of the upper triangle holds the tiles from column tile mb kTile / TN on
             t.mb = 0;
-            while (r >= p.tm - t.mb)
+            t.nb = 0;
+            while (r >= p.tn - t.nb)
             {
-                r -= p.tm - t.mb;
+                r -= p.tn - t.nb;
                 ++t.mb;
+                t.nb += pair::kTile / TN;
             }
-            t.nb = t.mb + r;
+            t.nb += r;
         }
         else
         {
@@ -546,14 +549,14 @@ struct Work
         // tall: S = X^T X, X M; else S = X X^T, M X; S and M read as they are, being symmetric
         t.a_mn = t.kind == kGram && p.tall;
         t.b_mn = t.kind == kGram ? p.tall != 0 : t.kind != kPoly && p.tall == 0;
-        t.idesc = pair::idesc(false, t.a_mn, t.b_mn);
+        t.idesc = pair::idesc<TN>(false, t.a_mn, t.b_mn);
         return true;
     }
 
     static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, pair::Piece& a,
                                                     pair::Piece& b)
     {
-        const int m = t.mb * pair::kTile + rank * 128, n = t.nb * pair::kTile + rank * 128;
+        const int m = t.mb * pair::kTile + rank * 128, n = t.nb * TN + rank * (TN / 2);
         const CUtensorMap* x = t.kind == kGram ? &p.xg[t.k & 1] : &p.xa[t.k & 1];
         const bool x_first = t.kind == kGram || (t.kind == kApply && p.tall);
         const bool x_second = t.kind == kGram || (t.kind == kApply && !p.tall);
@@ -628,10 +631,10 @@ struct Work
     template <typename F>
     static __device__ __forceinline__ void with_part(const Params& p, const Tile& t, F&& f)
     {
-        if (t.kind == kGram) f(Part<kGram, SPLIT>{});
-        else if (t.kind == kPoly) f(Part<kPoly, SPLIT>{});
-        else if (t.k < p.steps - 1) f(Part<kApply, SPLIT>{});
-        else f(Part<LAST, SPLIT>{});
+        if (t.kind == kGram) f(Part<kGram, SPLIT, TN>{});
+        else if (t.kind == kPoly) f(Part<kPoly, SPLIT, TN>{});
+        else if (t.k < p.steps - 1) f(Part<kApply, SPLIT, TN>{});
+        else f(Part<LAST, SPLIT, TN>{});
     }
 
     static __device__ __forceinline__ void before(const Params& p, const Tile& t, State&, int row0, int col0,
@@ -1280,6 +1283,94 @@ bool reads_four(const Source& src, int64_t batch, int64_t cols)
            (batch == 1 || src.stride % 4 == 0);
 }
 
+// Tiles of one matrix: of S or M (on and right of the diagonal), and of X.
+struct Tiling
+{
+    int64_t half, whole;
+};
+
+Tiling tiling(int64_t rows, int64_t cols, int tn)
+{
+    const int64_t m = std::min(rows, cols), cols_of_s = (m + tn - 1) / tn;
+    Tiling t{0, (rows + 255) / 256 * ((cols + tn - 1) / tn)};
+    for (int64_t mb = 0; mb < (m + 255) / 256; ++mb) t.half += cols_of_s - mb * (256 / tn);
+    return t;
+}
+
+// The products of every step, on 256 x TN tiles; p's destination says what the last one (LAST) writes.
+template <bool SPLIT, int LAST, int TN>
+int products(const char* what, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c,
+             const Layout& l, char* ws, Params p, cudaStream_t stream)
+{
+    uint16_t* x[2] = {reinterpret_cast<uint16_t*>(ws + l.x[0]), reinterpret_cast<uint16_t*>(ws + l.x[1])};
+    uint16_t* sm[2] = {reinterpret_cast<uint16_t*>(ws + l.s), reinterpret_cast<uint16_t*>(ws + l.p)};
+    const bool tall = rows > cols;
+    const int64_t m = l.m, sp = l.planes * batch;
+    bool ok = pair::make_map3(&p.s, sm[0], 2, false, m, m, sp, l.lds, l.plane_s, 64, TN == pair::kTile ? 128 : 64) &&
+              pair::make_map3(&p.m, sm[1], 2, false, m, m, sp, l.lds, l.plane_s, 64, TN == pair::kTile ? 128 : 64) &&
+              pair::make_map3(&p.s_out, sm[0], 2, false, m, m, sp, l.lds, l.plane_s, 32, 32, pair::Swizzle::k64) &&
+              pair::make_map3(&p.m_out, sm[1], 2, false, m, m, sp, l.lds, l.plane_s, 32, 32, pair::Swizzle::k64) &&
+              pair::make_map3(&p.s_out_t, sm[0], 2, false, m, m, sp, l.lds, l.plane_s, 32, 32, pair::Swizzle::kNone) &&
+              pair::make_map3(&p.m_out_t, sm[1], 2, false, m, m, sp, l.lds, l.plane_s, 32, 32, pair::Swizzle::kNone);
+    for (int k = 0; k < 2; ++k)
+    {
+        ok = ok &&
+             pair::make_map3(&p.xg[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 64,
+                             tall || TN < pair::kTile ? 64 : 128) &&
+             pair::make_map3(&p.xa[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 64,
+                             tall && TN == pair::kTile ? 128 : 64) &&
+             pair::make_map3(&p.x_out[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 32, 32,
+                             pair::Swizzle::k64);
+        p.x[k] = x[k];
+    }
+    if (!ok)
+    {
+        return fail(VEDA_ERR_CUDA, std::string(what) + ": tensor map creation failed");
+    }
+    const Tiling tl = tiling(rows, cols, TN);
+    const int64_t half = tl.half, whole = tl.whole, iteration = (2 * half + whole) * batch;
+    if (iteration >= (1ll << 30) / steps)
+    {
+        return fail(VEDA_ERR_INVALID_ARGUMENT, std::string(what) + ": too many tiles");
+    }
+    p.tall = tall;
+    p.rows = static_cast<int>(rows);
+    p.cols = static_cast<int>(cols);
+    p.side = static_cast<int>(m);
+    p.planes = l.planes;
+    p.batch = static_cast<int>(batch);
+    p.steps = steps;
+    p.tn = static_cast<int>((m + TN - 1) / TN);
+    p.half = static_cast<int>(half);
+    p.whole = static_cast<int>(whole);
+    p.sym_tiles = static_cast<int>(half * batch);
+    p.iteration = static_cast<int>(iteration);
+    p.by_iteration = pair::Divisor(static_cast<uint32_t>(iteration));
+    p.by_sym = pair::Divisor(static_cast<uint32_t>(half * batch));
+    p.by_half = pair::Divisor(static_cast<uint32_t>(half));
+    p.by_whole = pair::Divisor(static_cast<uint32_t>(whole));
+    p.by_n = pair::Divisor(static_cast<uint32_t>((cols + TN - 1) / TN));
+    p.ca = a;
+    p.cb = b;
+    p.cc = c;
+    p.s_ptr = sm[0];
+    p.ldx = l.ldx;
+    p.plane_x = l.plane_x;
+    p.lds = l.lds;
+    p.plane_s = l.plane_s;
+    p.counters = reinterpret_cast<unsigned*>(ws + l.counters);
+    p.status = device_status_ptr();
+    using W = Work<LAST, SPLIT, TN>;
+    const int clusters = pair::clusters_available<W, 8, SPLIT>();
+    if (clusters < 1)
+    {
+        return fail(VEDA_ERR_UNSUPPORTED, std::string(what) + ": no CTA pair fits on this device");
+    }
+    // more clusters than a step of the batch has tiles would only wait
+    const int64_t most = std::max(half, whole) * batch;
+    return pair::launch_together<W, 8, SPLIT>(what, p, static_cast<int>(std::min<int64_t>(most, clusters)), stream);
+}
+
 // norm, X, then the products of every step; p's destination says what the last one (LAST) writes.
 template <typename T, bool SPLIT, int LAST>
 int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, int64_t cols, int steps, float a,
@@ -1294,29 +1385,7 @@ int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, in
     }
     const Layout l = layout(batch, rows, cols, SPLIT, kMaxSteps);
     double* partials = reinterpret_cast<double*>(ws + l.partials);
-    uint16_t* x[2] = {reinterpret_cast<uint16_t*>(ws + l.x[0]), reinterpret_cast<uint16_t*>(ws + l.x[1])};
-    uint16_t* sm[2] = {reinterpret_cast<uint16_t*>(ws + l.s), reinterpret_cast<uint16_t*>(ws + l.p)};
-    const bool tall = rows > cols;
-    const int64_t m = l.m, sp = l.planes * batch;
-    bool ok = pair::make_map3(&p.s, sm[0], 2, false, m, m, sp, l.lds, l.plane_s, 64, 128) &&
-              pair::make_map3(&p.m, sm[1], 2, false, m, m, sp, l.lds, l.plane_s, 64, 128) &&
-              pair::make_map3(&p.s_out, sm[0], 2, false, m, m, sp, l.lds, l.plane_s, 32, 32, pair::Swizzle::k64) &&
-              pair::make_map3(&p.m_out, sm[1], 2, false, m, m, sp, l.lds, l.plane_s, 32, 32, pair::Swizzle::k64) &&
-              pair::make_map3(&p.s_out_t, sm[0], 2, false, m, m, sp, l.lds, l.plane_s, 32, 32, pair::Swizzle::kNone) &&
-              pair::make_map3(&p.m_out_t, sm[1], 2, false, m, m, sp, l.lds, l.plane_s, 32, 32, pair::Swizzle::kNone);
-    for (int k = 0; k < 2; ++k)
-    {
-        ok = ok &&
-             pair::make_map3(&p.xg[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 64, tall ? 64 : 128) &&
-             pair::make_map3(&p.xa[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 64, tall ? 128 : 64) &&
-             pair::make_map3(&p.x_out[k], x[k], 2, false, cols, rows, 2 * batch, l.ldx, l.plane_x, 32, 32,
-                             pair::Swizzle::k64);
-        p.x[k] = x[k];
-    }
-    if (!ok)
-    {
-        return fail(VEDA_ERR_CUDA, std::string(what) + ": tensor map creation failed");
-    }
+    uint16_t* x0 = reinterpret_cast<uint16_t*>(ws + l.x[0]);
     // the destination by TMA where its base, pitch and stride are multiples of 16 bytes
     const auto fits = [&](const void* base, int es) {
         return aligned16(base) && p.ldo * es % 16 == 0 && (batch == 1 || p.stride_o * es % 16 == 0);
@@ -1335,51 +1404,22 @@ int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, in
                     static_cast<int>(rows), static_cast<int>(cols), partials);
     if (rc != VEDA_OK) return rc;
     rc = launch(what, four ? init_kernel<T, 4> : init_kernel<T, 1>, grid, dim3(256), 0, stream, src,
-                static_cast<int>(rows), static_cast<int>(cols), static_cast<const double*>(partials), eps, x[0], l.ldx,
+                static_cast<int>(rows), static_cast<int>(cols), static_cast<const double*>(partials), eps, x0, l.ldx,
                 l.plane_x, reinterpret_cast<unsigned*>(ws + l.counters), steps);
     if (rc != VEDA_OK) return rc;
-    const int64_t tm = (m + 255) / 256, tr = (rows + 255) / 256, tc = (cols + 255) / 256;
-    const int64_t half = tm * (tm + 1) / 2, whole = tr * tc, iteration = (2 * half + whole) * batch;
-    if (iteration >= (1ll << 30) / steps)
+    // Narrow tiles (256 x 128) have half the latency and one and a half times the operand traffic a flop:
+    // they win while the wide ones of X leave the 74 CTA pairs at most about one and a half each (1024 x
+    // 1024: 136 against 176 us; 8 x 500 x 1500, 96 wide tiles: 362 against 457; 2048 x 4096, 128: 420
+    // against 414; 28 x 1024 x 1024, 448: 992 against 843). Split products take them always: with wide
+    // tiles their folds are not overlapped.
+    if constexpr (!SPLIT)
     {
-        return fail(VEDA_ERR_INVALID_ARGUMENT, std::string(what) + ": too many tiles");
+        if (tiling(rows, cols, 256).whole * batch > 110)
+        {
+            return products<SPLIT, LAST, 256>(what, batch, rows, cols, steps, a, b, c, l, ws, p, stream);
+        }
     }
-    p.tall = tall;
-    p.rows = static_cast<int>(rows);
-    p.cols = static_cast<int>(cols);
-    p.side = static_cast<int>(m);
-    p.planes = l.planes;
-    p.batch = static_cast<int>(batch);
-    p.steps = steps;
-    p.tm = static_cast<int>(tm);
-    p.half = static_cast<int>(half);
-    p.whole = static_cast<int>(whole);
-    p.sym_tiles = static_cast<int>(half * batch);
-    p.iteration = static_cast<int>(iteration);
-    p.by_iteration = pair::Divisor(static_cast<uint32_t>(iteration));
-    p.by_sym = pair::Divisor(static_cast<uint32_t>(half * batch));
-    p.by_half = pair::Divisor(static_cast<uint32_t>(half));
-    p.by_whole = pair::Divisor(static_cast<uint32_t>(whole));
-    p.by_n = pair::Divisor(static_cast<uint32_t>(tc));
-    p.ca = a;
-    p.cb = b;
-    p.cc = c;
-    p.s_ptr = sm[0];
-    p.ldx = l.ldx;
-    p.plane_x = l.plane_x;
-    p.lds = l.lds;
-    p.plane_s = l.plane_s;
-    p.counters = reinterpret_cast<unsigned*>(ws + l.counters);
-    p.status = device_status_ptr();
-    using W = Work<LAST, SPLIT>;
-    const int clusters = pair::clusters_available<W, 8, SPLIT>();
-    if (clusters < 1)
-    {
-        return fail(VEDA_ERR_UNSUPPORTED, std::string(what) + ": no CTA pair fits on this device");
-    }
-    // more clusters than a step of the batch has tiles would only wait
-    const int64_t most = std::max(half, whole) * batch;
-    return pair::launch_together<W, 8, SPLIT>(what, p, static_cast<int>(std::min<int64_t>(most, clusters)), stream);
+    return products<SPLIT, LAST, 128>(what, batch, rows, cols, steps, a, b, c, l, ws, p, stream);
 }
 
 bool bad_extent(int64_t batch, int64_t rows, int64_t cols)

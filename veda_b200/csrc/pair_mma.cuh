@@ -1,5 +1,6 @@
-// A persistent CTA-pair tensor-core kernel over a list of 256 x 256 output tiles, with the list and
-// the epilogue supplied by a Work type: the mainloop of the loss head (linear_ce.cu) and of the
+// A persistent CTA-pair tensor-core kernel over a list of 256 x 256 output tiles (or 256 x 128, where
+// there are too few tiles for all SMs and a tile's latency counts), with the list and the epilogue
+// supplied by a Work type: the mainloop of the loss head (linear_ce.cu) and of the
 // Newton-Schulz products (newton_schulz.cu).
 //
 // A cluster of two CTAs computes a tile with tcgen05.mma.cta_group::2 (M 256, N 256, K 16; 16-bit
@@ -16,8 +17,9 @@
 // The tensor core truncates as it adds into its accumulator, an error of some 2^-25 of the running
 // sum per 16 terms and always towards zero: sums of 10000 terms came out 3e-5 short. So the small
 // products go first, and every kChain k-blocks the accumulator is folded into a running sum kept in
-// the other half of TMEM, rounded to nearest (1e-6 and less). The fold is not overlapped with the
-// products: the accumulator has no second buffer then.
+// another part of TMEM, rounded to nearest (1e-6 and less). With TN = 128 two accumulators and the sum
+// fit, and a fold runs under the next chain's products; with TN = 256 the accumulator has no second
+// buffer then, and the products wait for it.
 //
 // Work provides
 //   struct Params                      the kernel's argument (tensor maps, pointers, sizes, status)
@@ -37,25 +39,27 @@
 namespace veda::cuda::pair
 {
 
-constexpr int kTile = 256;   // tile rows and columns of a CTA pair
+constexpr int kTile = 256;   // tile rows of a CTA pair, and columns unless the Work has TN = 128
 constexpr int kBK = 64;      // k-block: 64 16-bit values, one 128-byte swizzle row
 constexpr int kChain = 4;    // SPLIT: k-blocks between folds
 
-template <int EPI_WARPS_>
+template <int EPI_WARPS_, int TN = kTile>
 struct Cfg
 {
     static constexpr int EPI_WARPS = EPI_WARPS_;   // 4, or 8 with half the columns each
     static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-    static constexpr int STAGES = EPI_WARPS == 8 ? 5 : 6;
-    static constexpr int OPERAND = 128 * kBK * 2;   // one CTA's half of an operand's k-block
-    static constexpr int STAGE = 2 * OPERAND;
+    static constexpr int STAGES = EPI_WARPS == 8 && TN == kTile ? 5 : 6;
+    static constexpr int A_BYTES = 128 * kBK * 2;      // one CTA's half of the operands' k-block
+    static constexpr int B_BYTES = TN / 2 * kBK * 2;
+    static constexpr int STAGE = A_BYTES + B_BYTES;
     static constexpr int STAGE_TILE = 32 * 128;     // epilogue staging: 32 rows x 128 bytes
     static constexpr int STAGING = EPI_WARPS * 2 * STAGE_TILE;
     static constexpr int SMEM = STAGES * STAGE + STAGING + 1024 + 256;
 };
 
-// A 128 x 64 operand piece at k = 0: k runs along x (K-major, box 64 x 128) or along y (MN-major, two
-// boxes 64 x 64 side by side). z is the hi plane, z + 1 the lo plane of split operands.
+// An operand piece at k = 0, 128 rows of A or TN / 2 of B by 64 terms: k runs along x (K-major, one box
+// 64 x 128; with TN = 128 one or two of 64 x 64, one below the other) or along y (MN-major, boxes
+// 64 x 64 side by side). z is the hi plane, z + 1 the lo plane of split operands.
 struct Piece
 {
     const CUtensorMap* map;
@@ -63,11 +67,12 @@ struct Piece
 };
 
 // kind::f16 instruction descriptor: fp32 accumulators, A and B both bf16 or both fp16.
+template <int TN = kTile>
 __host__ __device__ constexpr uint32_t idesc(bool is_bf16, bool a_mn, bool b_mn)
 {
     const uint32_t type = is_bf16 ? 1u : 0u;
     return (1u << 4) | (type << 7) | (type << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
-           (static_cast<uint32_t>(kTile >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
+           (static_cast<uint32_t>(TN >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
 }
 
 // n / d for 0 <= n < 2^31 by a multiplication: m = ceil(2^(31 + s) / d) with 2^s >= d.
@@ -189,17 +194,19 @@ __device__ __forceinline__ void fold(uint32_t acc, uint32_t sum, bool first, boo
 }
 
 template <class Work, int EPI_WARPS, bool SPLIT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI_WARPS>::THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<EPI_WARPS, Work::TN>::THREADS, 1)
 pair_kernel(const __grid_constant__ typename Work::Params p)
 {
     using namespace tc;
-    using C_ = Cfg<EPI_WARPS>;
+    using C_ = Cfg<EPI_WARPS, Work::TN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* sa = smem;
-    uint8_t* sb = smem + C_::STAGES * C_::OPERAND;
-    uint8_t* staging = sb + C_::STAGES * C_::OPERAND;
+    constexpr int TN = Work::TN;
+    constexpr bool TWO = !SPLIT || TN < kTile;   // two accumulators
+    uint8_t* sb = smem + C_::STAGES * C_::A_BYTES;
+    uint8_t* staging = sb + C_::STAGES * C_::B_BYTES;
     uint64_t* full = reinterpret_cast<uint64_t*>(staging + C_::STAGING);
     uint64_t* empty = full + C_::STAGES;
     uint64_t* tfull = empty + C_::STAGES;
@@ -272,8 +279,8 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
                     mbar_wait(&empty[stage], phase ^ 1, p.status, abort);
                     __syncwarp();
                     const uint32_t bar = peer_addr(&full[stage], 0);
-                    uint8_t* ad = sa + stage * C_::OPERAND;
-                    uint8_t* bd = sb + stage * C_::OPERAND;
+                    uint8_t* ad = sa + stage * C_::A_BYTES;
+                    uint8_t* bd = sb + stage * C_::B_BYTES;
                     const int ax = a.x + kb * adx, ay = a.y + kb * ady;
                     const int bx = b.x + kb * bdx, by = b.y + kb * bdy;
                     if (leader)
@@ -283,9 +290,10 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
                             mbar_expect_tx(&full[stage], 2 * C_::STAGE);   // both CTAs' halves
                         }
                         load_box(ad, a.map, bar, ax, ay, a.z + za);
-                        if (t.a_mn) load_box(ad + C_::OPERAND / 2, a.map, bar, ax + 64, ay, a.z + za);
+                        if (t.a_mn) load_box(ad + C_::A_BYTES / 2, a.map, bar, ax + 64, ay, a.z + za);
+                        else if (TN < kTile) load_box(ad + C_::A_BYTES / 2, a.map, bar, ax, ay + 64, a.z + za);
                         load_box(bd, b.map, bar, bx, by, b.z + zb);
-                        if (t.b_mn) load_box(bd + C_::OPERAND / 2, b.map, bar, bx + 64, by, b.z + zb);
+                        if (TN == kTile && t.b_mn) load_box(bd + C_::B_BYTES / 2, b.map, bar, bx + 64, by, b.z + zb);
                     }
                     __syncwarp();
                     if (++stage == C_::STAGES)
@@ -332,18 +340,18 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
             for (int k0 = 0; !t.skip && k0 < t.kbs; k0 += SPLIT ? kChain : t.kbs)
             {
                 const int blocks = SPLIT ? 3 * (min(t.kbs, k0 + kChain) - k0) : t.kbs;
-                const int buf = SPLIT ? 0 : it & 1;
-                mbar_wait(&tempty[buf], ((SPLIT ? it : it >> 1) & 1) ^ 1, p.status, abort);
+                const int buf = TWO ? it & 1 : 0;
+                mbar_wait(&tempty[buf], ((TWO ? it >> 1 : it) & 1) ^ 1, p.status, abort);
                 __syncwarp();
                 fence_after();
-                const uint32_t d = tmem + static_cast<uint32_t>(buf * kTile);
+                const uint32_t d = tmem + static_cast<uint32_t>(buf * TN);
                 for (int kb = 0; kb < blocks; ++kb)
                 {
                     mbar_wait(&full[stage], phase, p.status, abort);
                     __syncwarp();
                     fence_after();
-                    const uint64_t ad = smem_desc(smem_u32(sa + stage * C_::OPERAND), albo, 1024);
-                    const uint64_t bd = smem_desc(smem_u32(sb + stage * C_::OPERAND), blbo, 1024);
+                    const uint64_t ad = smem_desc(smem_u32(sa + stage * C_::A_BYTES), albo, 1024);
+                    const uint64_t bd = smem_desc(smem_u32(sb + stage * C_::B_BYTES), blbo, 1024);
                     if (leader)
                     {
 #pragma unroll
@@ -375,7 +383,7 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
     else if (warp >= 2)
     {
         const int quarter = warp & 3;   // the TMEM lanes this warp may read
-        constexpr int COLS = kTile / (EPI_WARPS / 4);
+        constexpr int COLS = TN / (EPI_WARPS / 4);
         const int col0 = ((warp - 2) >> 2) * COLS;
         const int row0 = static_cast<int>(rank) * 128 + quarter * 32;   // within the tile
         const uint32_t release = peer_addr(&tempty[0], 0);
@@ -391,17 +399,17 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
             const bool more_next = Work::tile(p, cid, clusters, ++i, next);
             for (int k0 = 0; !t.skip && k0 < t.kbs; k0 += SPLIT ? kChain : t.kbs)
             {
-                const int buf = SPLIT ? 0 : it & 1;
-                mbar_wait(&tfull[buf], (SPLIT ? it : it >> 1) & 1, p.status, abort);
+                const int buf = TWO ? it & 1 : 0;
+                mbar_wait(&tfull[buf], (TWO ? it >> 1 : it) & 1, p.status, abort);
                 fence_after();
-                const uint32_t base = tmem + static_cast<uint32_t>(buf * kTile + col0) +
+                const uint32_t base = tmem + static_cast<uint32_t>(buf * TN + col0) +
                                       (static_cast<uint32_t>(quarter * 32) << 16);
                 const bool last = !SPLIT || k0 + kChain >= t.kbs;
                 if constexpr (SPLIT)
                 {
                     if (t.kbs > kChain)
                     {
-                        fold<COLS>(base, base + kTile, k0 == 0, last);
+                        fold<COLS>(base, base - buf * TN + (TWO ? 2 : 1) * TN, k0 == 0, last);
                     }
                 }
                 if (last)
@@ -468,13 +476,13 @@ int clusters_available()
     {
         auto kernel = pair_kernel<Work, EPI_WARPS, SPLIT>;
         int n = 0;
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<EPI_WARPS>::SMEM) ==
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<EPI_WARPS, Work::TN>::SMEM) ==
             cudaSuccess)
         {
             cudaLaunchConfig_t cfg{};
             cfg.gridDim = dim3(2 * (sm_count() / 2));
-            cfg.blockDim = dim3(Cfg<EPI_WARPS>::THREADS);
-            cfg.dynamicSmemBytes = Cfg<EPI_WARPS>::SMEM;
+            cfg.blockDim = dim3(Cfg<EPI_WARPS, Work::TN>::THREADS);
+            cfg.dynamicSmemBytes = Cfg<EPI_WARPS, Work::TN>::SMEM;
             cudaLaunchAttribute attr{};
             attr.id = cudaLaunchAttributeClusterDimension;
             attr.val.clusterDim.x = 2;
@@ -498,8 +506,8 @@ int clusters_available()
 template <class Work, int EPI_WARPS, bool SPLIT>
 int launch_pair(const char* what, const typename Work::Params& p, int clusters, cudaStream_t s)
 {
-    return launch(what, pair_kernel<Work, EPI_WARPS, SPLIT>, dim3(2 * clusters), dim3(Cfg<EPI_WARPS>::THREADS),
-                  Cfg<EPI_WARPS>::SMEM, s, p);
+    return launch(what, pair_kernel<Work, EPI_WARPS, SPLIT>, dim3(2 * clusters), dim3(Cfg<EPI_WARPS, Work::TN>::THREADS),
+                  Cfg<EPI_WARPS, Work::TN>::SMEM, s, p);
 }
 
 // The same with all clusters on the device at once (a cooperative launch), for a Work whose tiles wait
@@ -509,8 +517,8 @@ int launch_together(const char* what, const typename Work::Params& p, int cluste
 {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(2 * clusters);
-    cfg.blockDim = dim3(Cfg<EPI_WARPS>::THREADS);
-    cfg.dynamicSmemBytes = Cfg<EPI_WARPS>::SMEM;
+    cfg.blockDim = dim3(Cfg<EPI_WARPS, Work::TN>::THREADS);
+    cfg.dynamicSmemBytes = Cfg<EPI_WARPS, Work::TN>::SMEM;
     cfg.stream = s;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeCooperative;
