@@ -72,7 +72,7 @@ struct Params
     CUtensorMap x_mn, w_mn;  // the same, MN-major
     CUtensorMap q_in, q_mn;  // piece of q read by the gradient products
     CUtensorMap q_out;       // piece of q written (store boxes)
-    CUtensorMap dx, dw;      // fp32 sums of dx; dW (store boxes)
+    CUtensorMap dx, dw;      // fp32 sums of dx, a plane per split; dW (store boxes)
     int rows, vocab, dim;
     int split;               // operands are pairs of fp16 planes
     int is_bf16;
@@ -82,6 +82,8 @@ struct Params
     pair::Divisor by_m, by_d;   // num_m, num_d
     // gradient products of this launch: q_in holds vocabulary rows g0 .. g0 + gcols
     int g0, gcols, num_d;
+    int dx_tiles, dx_kbs;    // tiles of dx, k-blocks of a split
+    pair::Divisor by_dx;     // dx_tiles
     Shares shares;
     int dx_add;              // dx sums: 0 store, 1 add
     int dw_mode;             // 0: from registers; 1: TMA store; 2: TMA add (fp32)
@@ -266,7 +268,7 @@ struct GradWork
     struct Tile
     {
         bool skip, a_mn, b_mn;
-        int kind, kbs, mb, nb;
+        int kind, kbs, mb, nb, split;
         uint32_t idesc;
     };
     struct State
@@ -298,8 +300,9 @@ struct GradWork
         if (u < end)
         {
             t.kind = kDx;
+            t.split = p.by_dx.div(u, u);
             t.mb = p.by_d.div(u, t.nb);
-            t.kbs = (p.gcols + pair::kBK - 1) / pair::kBK;
+            t.kbs = min(p.dx_kbs, (p.gcols + pair::kBK - 1) / pair::kBK - t.split * p.dx_kbs);
             t.a_mn = false;
             t.b_mn = true;
             t.idesc = pair::idesc(bf, false, true);
@@ -330,8 +333,9 @@ struct GradWork
         }
         else if (t.kind == kDx)
         {
-            a = {&p.q_in, 0, m, 0};
-            b = {&p.w_mn, n, p.g0, 0};
+            const int k = t.split * p.dx_kbs * pair::kBK;
+            a = {&p.q_in, k, m, 0};
+            b = {&p.w_mn, n, p.g0 + k, 0};
         }
         else
         {
@@ -534,13 +538,14 @@ struct GradWork
             if (lane == 0)
             {
                 const CUtensorMap* map = dw ? &p.dw : &p.dx;
+                const int z = dw ? 0 : t.split;
                 if (mode == 2)
                 {
-                    pair::reduce_add_3d(map, buf, col, orow, 0);
+                    pair::reduce_add_3d(map, buf, col, orow, z);
                 }
                 else
                 {
-                    tc::tma_store_3d(map, buf, col, orow, 0);
+                    tc::tma_store_3d(map, buf, col, orow, z);
                 }
                 tc::bulk_commit_group();
             }
@@ -809,10 +814,10 @@ mean_kernel(const float* __restrict__ row_loss, const int64_t* __restrict__ targ
     }
 }
 
-// dx = coef x the fp32 sums.
+// dx = coef x the fp32 sums, those of the splits added in their order.
 template <typename T>
 __global__ void __launch_bounds__(256)
-finish_dx_kernel(const float* __restrict__ acc, int64_t lda, T* __restrict__ dx, int64_t lddx, int64_t rows,
+finish_dx_kernel(const float* __restrict__ acc, int64_t lda, int splits, T* __restrict__ dx, int64_t lddx, int64_t rows,
                  int64_t dim, const Scalars* __restrict__ scalars)
 {
     dep_wait();
@@ -822,7 +827,9 @@ finish_dx_kernel(const float* __restrict__ acc, int64_t lda, T* __restrict__ dx,
     {
         for (int64_t c = threadIdx.x & 31; c < dim; c += 32)
         {
-            dx[r * lddx + c] = from_f32<T>(acc[r * lda + c] * unit * coef);
+            float sum = acc[r * lda + c];
+            for (int k = 1; k < splits; ++k) sum += acc[(k * rows + r) * lda + c];
+            dx[r * lddx + c] = from_f32<T>(sum * unit * coef);
         }
     }
 }
@@ -837,6 +844,7 @@ struct Layout
     int64_t ldp;          // pitch of the operand planes (elements)
     int64_t piece;        // columns of a piece of q (a multiple of 256)
     int64_t ld_acc;       // pitch of the fp32 dx sums
+    int splits;           // of dx's sum over a piece
     int strip, slots;     // forward: tiles a strip, strips
     size_t scalars, part, px, pw, parts, target_logit, q, acc, total;
 };
@@ -893,8 +901,14 @@ Layout layout(int64_t rows, int64_t vocab, int64_t dim, bool pack_x, bool pack_w
         const int64_t fit = (int64_t{64} << 20) / (rows * 2 * l.planes) / 256 * 256;
         l.piece = std::min(round_up(vocab, 256), std::max<int64_t>(256, fit));
         l.q = take(2 * l.planes * rows * l.piece * 2);
+        // Where dx has fewer tiles than the GPU has CTA pairs, its sums over a piece are cut into splits of
+        // at least 8 k-blocks, each kept apart: one cluster summing 100000 columns for 16 rows of 768 took
+        // 430 us by itself.
+        const int64_t tiles = num_m * ((dim + 255) / 256), kbs = (std::min(l.piece, vocab) + 63) / 64;
+        const int64_t want = std::min((74 + tiles - 1) / tiles, (kbs + 7) / 8);
+        l.splits = static_cast<int>((kbs + (kbs + want - 1) / want - 1) / ((kbs + want - 1) / want));
         l.ld_acc = round_up(dim, 4);
-        l.acc = take(rows * l.ld_acc * 4);
+        l.acc = take(l.splits * rows * l.ld_acc * 4);
     }
     l.total = at;
     return l;
@@ -1186,7 +1200,7 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
              pair::make_map3(&q_store[b], q, 2, bf, piece, rows, c.l.planes, piece, plane, 64, 32);
     }
     float* acc = reinterpret_cast<float*>(c.ws + c.l.acc);
-    ok = ok && pair::make_map3(&p.dx, acc, 4, false, dim, rows, 1, c.l.ld_acc, rows * c.l.ld_acc, 32, 32);
+    ok = ok && pair::make_map3(&p.dx, acc, 4, false, dim, rows, c.l.splits, c.l.ld_acc, rows * c.l.ld_acc, 32, 32);
     p.dw_f32 = dtype_dw == VEDA_F32;
     p.dw_beta = beta_dw != 0.0f;
     p.dw_ptr = dw;
@@ -1225,14 +1239,20 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
             p.q_in = q_load[(k - 1) & 1];
             p.q_mn = q_mn[(k - 1) & 1];
             tiles[lce::GradWork::kDw] = dw != nullptr ? static_cast<int64_t>((p.gcols + 255) / 256) * p.num_d : 0;
-            tiles[lce::GradWork::kDx] = dx != nullptr ? static_cast<int64_t>(p.num_m) * p.num_d : 0;
+            // a short last piece may fill fewer splits; all were stored with the first
+            const int kbs = (p.gcols + pair::kBK - 1) / pair::kBK;
+            p.dx_tiles = p.num_m * p.num_d;
+            p.by_dx = pair::Divisor(static_cast<uint32_t>(p.dx_tiles));
+            p.dx_kbs = (kbs + c.l.splits - 1) / c.l.splits;
+            tiles[lce::GradWork::kDx] =
+                dx != nullptr ? static_cast<int64_t>((kbs + p.dx_kbs - 1) / p.dx_kbs) * p.dx_tiles : 0;
             p.dx_add = k > 1;
         }
         const int64_t units = tiles[0] + tiles[1] + tiles[2];
         VEDA_REQUIRE(units <= lce::kLimit, "too many tiles");
         const int grid = static_cast<int>(std::min<int64_t>(units, clusters));
         // k-blocks a tile, and what its epilogue adds
-        const int64_t cost[3] = {(rows + 63) / 64 + 2, (p.gcols + 63) / 64 + 2, (dim + 63) / 64 + 2};
+        const int64_t cost[3] = {(rows + 63) / 64 + 4, p.dx_kbs + 2, (dim + 63) / 64 + 2};
         lce::share(tiles, cost, grid, p.shares);
         rc = split ? pair::launch_pair<lce::GradWork, 4, true>("veda_linear_cross_entropy_bwd", p, grid, stream)
                    : pair::launch_pair<lce::GradWork, 4, false>("veda_linear_cross_entropy_bwd", p, grid, stream);
@@ -1244,9 +1264,9 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
     }
     const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((rows + 7) / 8, 8ll * sm_count()));
     return bf ? launch("veda_linear_cross_entropy_bwd (dx)", lce::finish_dx_kernel<bf16>, dim3(blocks), dim3(256), 0,
-                       stream, static_cast<const float*>(acc), c.l.ld_acc, static_cast<bf16*>(dx), lddx, rows, dim,
+                       stream, static_cast<const float*>(acc), c.l.ld_acc, c.l.splits, static_cast<bf16*>(dx), lddx, rows, dim,
                        static_cast<const lce::Scalars*>(c.scalars()))
               : launch("veda_linear_cross_entropy_bwd (dx)", lce::finish_dx_kernel<float>, dim3(blocks), dim3(256), 0,
-                       stream, static_cast<const float*>(acc), c.l.ld_acc, static_cast<float*>(dx), lddx, rows, dim,
+                       stream, static_cast<const float*>(acc), c.l.ld_acc, c.l.splits, static_cast<float*>(dx), lddx, rows, dim,
                        static_cast<const lce::Scalars*>(c.scalars()));
 }
