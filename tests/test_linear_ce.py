@@ -125,7 +125,10 @@ def run_and_check(x, w, tg, dtype, dtype_dw=None):
 
 
 SHAPES = [(1, 1, 8), (1, 300, 64), (3, 2, 16), (31, 255, 24), (128, 512, 64), (257, 256, 40), (200, 1000, 256),
-          (300, 257, 72), (512, 2049, 128), (77, 5001, 520), (1030, 770, 136)]
+          (300, 257, 72), (512, 2049, 128), (77, 5001, 520), (1030, 770, 136),
+          # up to four rows of up to 2048 columns are streamed past; one past each border
+          (2, 700, 2048), (3, 601, 1000), (4, 9001, 776), (5, 4100, 64), (4, 50, 2056), (1, 20000, 40), (4, 33, 1),
+          (8, 9001, 776)]
 
 
 @pytest.mark.gpu
@@ -144,7 +147,7 @@ def test_many_pieces_of_the_vocabulary(cuda, dtype, rows, vocab, dim):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [V.BF16, V.F32])
-@pytest.mark.parametrize("rows,vocab,dim", [(65, 130, 7), (40, 300, 100), (129, 257, 33)])
+@pytest.mark.parametrize("rows,vocab,dim", [(65, 130, 7), (40, 300, 100), (129, 257, 33), (4, 300, 100), (2, 1001, 33)])
 def test_odd_widths_pitches_and_bases(cuda, dtype, rows, vocab, dim):
     t = torch()
     x, w, tg = make(rows, vocab, dim, dtype, seed=2)
@@ -182,9 +185,10 @@ def test_aligned_slices_are_read_in_place_and_padding_stays(cuda, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,dtype_dw", [(V.BF16, V.BF16), (V.BF16, V.F32), (V.F32, V.F32)])
 @pytest.mark.parametrize("pitch", [64, 67])
-def test_accumulated_weight_gradient_and_upstream(cuda, dtype, dtype_dw, pitch):
+@pytest.mark.parametrize("rows", [150, 3])
+def test_accumulated_weight_gradient_and_upstream(cuda, dtype, dtype_dw, pitch, rows):
     t = torch()
-    rows, vocab, dim = 150, 700, 64
+    vocab, dim = 700, 64
     x, w, tg = make(rows, vocab, dim, dtype, seed=4, ignored=0.3)
     up = t.tensor([-2.5], device="cuda")
     r = reference(x, w, tg, dtype, upstream=-2.5)
@@ -202,8 +206,9 @@ def test_accumulated_weight_gradient_and_upstream(cuda, dtype, dtype_dw, pitch):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [V.BF16, V.F32])
-def test_one_gradient_alone_has_the_bits_of_both(cuda, dtype):
-    x, w, tg = make(300, 1500, 96, dtype, seed=6)
+@pytest.mark.parametrize("rows", [300, 4])
+def test_one_gradient_alone_has_the_bits_of_both(cuda, dtype, rows):
+    x, w, tg = make(rows, 1500, 96, dtype, seed=6)
     _, lse, _ = fwd(x, w, tg, dtype)
     dx, dw, dx1, dw1 = empty(x.shape, dtype), empty(w.shape, dtype), empty(x.shape, dtype), empty(w.shape, dtype)
     bwd(x, w, tg, lse, dtype, dx=dx, dw=dw)
@@ -216,13 +221,14 @@ def test_one_gradient_alone_has_the_bits_of_both(cuda, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [V.BF16, V.F32])
-def test_padding_that_holds_nan_reaches_nothing(cuda, dtype):
+@pytest.mark.parametrize("rows", [200, 4])
+def test_padding_that_holds_nan_reaches_nothing(cuda, dtype, rows):
     t = torch()
-    x, w, tg = make(200, 600, 64, dtype, seed=7)
-    tg[::3] = IGN
+    x, w, tg = make(rows, 600, 64, dtype, seed=7)
+    tg[::2] = IGN
     clean = x.clone()
     for k, v in enumerate((float("nan"), float("inf"), -float("inf"), 3e38)):
-        x[3 * k] = v
+        x[2 * k % rows] = v
     _, lse, loss = fwd(x, w, tg, dtype)
     row, lse0, loss0 = fwd(clean, w, tg, dtype)
     got = [empty(x.shape, dtype), empty(w.shape, dtype)]
@@ -237,8 +243,9 @@ def test_padding_that_holds_nan_reaches_nothing(cuda, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [V.BF16, V.F32])
-def test_no_counted_row(cuda, dtype):
-    x, w, tg = make(50, 300, 32, dtype, seed=8)
+@pytest.mark.parametrize("rows", [50, 3])
+def test_no_counted_row(cuda, dtype, rows):
+    x, w, tg = make(rows, 300, 32, dtype, seed=8)
     tg[:] = IGN
     row, lse, loss = fwd(x, w, tg, dtype)
     dx, dw = empty(x.shape, dtype), empty(w.shape, dtype)
@@ -249,12 +256,13 @@ def test_no_counted_row(cuda, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("bad", [-1, 300, 1 << 40])
-def test_target_outside_the_vocabulary_sets_the_status_and_is_not_counted(cuda, bad):
+@pytest.mark.parametrize("rows", [60, 4])
+def test_target_outside_the_vocabulary_sets_the_status_and_is_not_counted(cuda, bad, rows):
     t = torch()
-    x, w, tg = make(60, 300, 32, V.BF16, seed=9)
+    x, w, tg = make(rows, 300, 32, V.BF16, seed=9)
     want = tg.clone()
-    want[11] = IGN
-    tg[11] = bad
+    want[3] = IGN
+    tg[3] = bad
     status = t.zeros(1, dtype=t.int32, device="cuda")
     row, lse, loss = fwd(x, w, tg, V.BF16, status=status)
     sync()

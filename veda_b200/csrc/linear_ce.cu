@@ -28,6 +28,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <cstring>
 
 namespace veda::cuda
 {
@@ -834,6 +835,531 @@ finish_dx_kernel(const float* __restrict__ acc, int64_t lda, int splits, T* __re
     }
 }
 
+// ---- up to four rows: the head streamed past the rows on the CUDA cores -------------------------
+// A few rows against the whole head are bound by reading it (and writing dW), not by the products: the
+// 256-row tensor tiles would read it at half of HBM's rate and compute mostly padding. Here the rows
+// stay in shared memory in fp32, a warp takes four vocabulary rows at a time, 16 bytes a lane and row,
+// and keeps 4 x R dot products; sums are fp32 for either dtype and nothing is laid out anew. Backward
+// reads the head once: a chunk of vocabulary rows waits in shared memory while its q are formed and
+// while dx and dW, each thread its own eight columns, are made of them.
+constexpr int kFewRows = 4;
+constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32;
+constexpr int kFewBlocks = 4 * 148;   // partial results are kept per block
+// Blocks an SM holds, by the registers that R rows take.
+constexpr int few_fwd_per_sm(int r) { return r == 1 ? 4 : r == 2 ? 3 : 2; }
+constexpr int kFewBwdPerSm = 2;
+
+struct Few
+{
+    const void *x, *w;
+    int64_t ldx, ldw;
+    int rows, dim, padded;   // padded: dim rounded up to 256
+    int64_t vocab;
+    const int64_t* targets;
+    int64_t ignore;
+    int vec;                 // head rows can be read 16 bytes at a time
+    // forward
+    float2* parts;           // [block][rows]
+    float* target_logit;
+    // backward
+    const float* lse;
+    const float* upstream;
+    int chunk;               // vocabulary rows held at a time
+    void* dw;
+    int64_t lddw;
+    int dw_f32, dw_beta, dw_vec;
+    float* acc;              // [block][rows][ld_acc] sums of dx, or null
+    int64_t ld_acc;
+    int* status;
+};
+
+// Eight elements of a head row, as they lie: 16 bytes of bf16, 32 of fp32. From global memory they are
+// read once and not kept in L1.
+template <typename T>
+struct Eight
+{
+    uint4 q[sizeof(T) / 2];
+    __device__ __forceinline__ void stream(const T* p)
+    {
+#pragma unroll
+        for (int k = 0; k < static_cast<int>(sizeof(T) / 2); ++k)
+        {
+            asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(q[k].x), "=r"(q[k].y), "=r"(q[k].z), "=r"(q[k].w)
+                         : "l"(reinterpret_cast<const uint4*>(p) + k));
+        }
+    }
+    __device__ __forceinline__ void read(const T* p)
+    {
+#pragma unroll
+        for (int k = 0; k < static_cast<int>(sizeof(T) / 2); ++k) q[k] = reinterpret_cast<const uint4*>(p)[k];
+    }
+    __device__ __forceinline__ void gather(const T* p, int left)
+    {
+        T v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = k < left ? p[k] : from_f32<T>(0.0f);
+        memcpy(q, v, sizeof(v));
+    }
+    __device__ __forceinline__ void zero()
+    {
+#pragma unroll
+        for (int k = 0; k < static_cast<int>(sizeof(T) / 2); ++k) q[k] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const
+    {
+        if constexpr (sizeof(T) == 2)
+        {
+            const uint32_t w[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+            }
+        }
+        else
+        {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+            {
+                v[4 * k] = __uint_as_float(q[k].x);
+                v[4 * k + 1] = __uint_as_float(q[k].y);
+                v[4 * k + 2] = __uint_as_float(q[k].z);
+                v[4 * k + 3] = __uint_as_float(q[k].w);
+            }
+        }
+    }
+};
+
+// The rows in fp32, zero past dim, past the rows and (clear) where a row is not counted; two planes of
+// four columns out of eight, so that a warp's 16-byte reads meet no bank twice.
+template <typename T, int R>
+__device__ __forceinline__ void stage_rows(const Few& p, float* xs, bool clear)
+{
+    const T* x = static_cast<const T*>(p.x);
+    for (int i = threadIdx.x; i < R * p.padded; i += kFewThreads)
+    {
+        const int r = i / p.padded, c = i - r * p.padded;
+        const bool in = r < p.rows && c < p.dim && !(clear && !counted(p.targets[r < p.rows ? r : 0], p.ignore, p.vocab));
+        xs[r * p.padded + (c & 4 ? p.padded / 2 : 0) + (c >> 3) * 4 + (c & 3)] = in ? to_f32(x[r * p.ldx + c]) : 0.0f;
+    }
+}
+
+// acc[j][r] += the dot product of the lane's columns c .. c + 7 of four head rows and of row r.
+template <typename T, int R>
+__device__ __forceinline__ void dot8(const Eight<T> (&raw)[4], const float* xs, int padded, int c, float (&acc)[4][R])
+{
+    float w[4][8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) raw[j].values(w[j]);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+    {
+        const float4 a = *reinterpret_cast<const float4*>(xs + r * padded + (c >> 3) * 4);
+        const float4 b = *reinterpret_cast<const float4*>(xs + r * padded + padded / 2 + (c >> 3) * 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+        {
+            float s = acc[j][r];
+            s = fmaf(w[j][0], a.x, s), s = fmaf(w[j][1], a.y, s), s = fmaf(w[j][2], a.z, s), s = fmaf(w[j][3], a.w, s);
+            s = fmaf(w[j][4], b.x, s), s = fmaf(w[j][5], b.y, s), s = fmaf(w[j][6], b.z, s), s = fmaf(w[j][7], b.w, s);
+            acc[j][r] = s;
+        }
+    }
+}
+
+// The lane's row (lane < R) of four summed dot products.
+template <int R>
+__device__ __forceinline__ void own_row(float (&acc)[4][R], int lane, float (&z)[4])
+{
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+    {
+        z[j] = 0.0f;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+        {
+            const float s = warp_sum(acc[j][r]);
+            z[j] = lane == r ? s : z[j];
+        }
+    }
+}
+
+template <typename T, int R, bool VEC>
+__global__ void __launch_bounds__(kFewThreads, few_fwd_per_sm(R))
+few_fwd_kernel(const Few p)
+{
+    extern __shared__ float few_smem[];
+    __shared__ float2 part[kFewWarps][R];
+    float* xs = few_smem;
+    dep_wait();
+    dep_release();
+    stage_rows<T, R>(p, xs, false);
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t target = lane < p.rows ? p.targets[lane] : -1;
+    const bool valid = lane < p.rows && counted(target, p.ignore, p.vocab);
+    float m = -INFINITY, s = 0.0f;
+    for (int64_t v = (static_cast<int64_t>(blockIdx.x) * kFewWarps + warp) * 4; v < p.vocab;
+         v += static_cast<int64_t>(gridDim.x) * kFewWarps * 4)
+    {
+        const T* row[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) row[j] = static_cast<const T*>(p.w) + (v + j < p.vocab ? v + j : v) * p.ldw;
+        float acc[4][R] = {};
+        // two chunks of columns at a time, all their loads first
+        for (int c = lane * 8; c < p.padded; c += 512)
+        {
+            Eight<T> w[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+            {
+                const int at = c + 256 * h;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                {
+                    if constexpr (VEC)
+                    {
+                        w[h][j].zero();
+                        if (at < p.dim) w[h][j].stream(row[j] + at);
+                    }
+                    else
+                    {
+                        w[h][j].gather(row[j] + at, p.dim - at);
+                    }
+                }
+            }
+            dot8<T, R>(w[0], xs, p.padded, c, acc);
+            if (c + 256 < p.padded) dot8<T, R>(w[1], xs, p.padded, c + 256, acc);
+        }
+        float z[4];
+        own_row<R>(acc, lane, z);
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+        {
+            if (v + j >= p.vocab) z[j] = -INFINITY;
+            else if (valid && target == v + j) p.target_logit[lane] = z[j];
+            top = fmaxf(top, z[j] * kLog2e);
+        }
+        const float ref = top == -INFINITY ? 0.0f : top;
+        s *= ex2(m - ref);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s += ex2(fmaf(z[j], kLog2e, -ref));
+        m = top;
+    }
+    if (lane < R) part[warp][lane] = make_float2(m, s);
+    __syncthreads();
+    if (threadIdx.x < p.rows)
+    {
+        for (int k = 1; k < kFewWarps; ++k)
+        {
+            const float2 o = part[k][threadIdx.x];
+            const float top = fmaxf(m, o.x);
+            const float ref = top == -INFINITY ? 0.0f : top;
+            s = s * ex2(m - ref) + o.y * ex2(o.x - ref);
+            m = top;
+        }
+        p.parts[static_cast<int64_t>(blockIdx.x) * p.rows + threadIdx.x] = make_float2(m, s);
+    }
+}
+
+// Merges the blocks' pairs of each row (a warp a row, in a fixed order) and takes the mean.
+__global__ void __launch_bounds__(kFewThreads)
+few_merge_kernel(const Few p, int blocks, float* __restrict__ row_loss, float* __restrict__ lse, float* loss)
+{
+    __shared__ float losses[kFewRows];
+    dep_wait();
+    dep_release();
+    const int row = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (row < p.rows)
+    {
+        float m = -INFINITY, s = 0.0f;
+        const auto add = [&](float om, float os) {
+            const float top = fmaxf(m, om);
+            const float ref = top == -INFINITY ? 0.0f : top;
+            s = s * ex2(m - ref) + os * ex2(om - ref);
+            m = top;
+        };
+        for (int b = lane; b < blocks; b += 32)
+        {
+            const float2 o = p.parts[static_cast<int64_t>(b) * p.rows + row];
+            add(o.x, o.y);
+        }
+        for (int d = 16; d > 0; d >>= 1)
+        {
+            const float om = __shfl_down_sync(0xFFFFFFFFu, m, d), os = __shfl_down_sync(0xFFFFFFFFu, s, d);
+            add(om, os);
+        }
+        if (lane == 0)
+        {
+            const float l = (m + log2f(s)) * kLn2;
+            const int64_t t = p.targets[row];
+            if (lse != nullptr) lse[row] = l;
+            losses[row] = counted(t, p.ignore, p.vocab) ? l - p.target_logit[row] : 0.0f;
+            row_loss[row] = losses[row];
+            if (t != p.ignore && !counted(t, p.ignore, p.vocab) && p.status != nullptr) *p.status = VEDA_ERR_OUT_OF_RANGE;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && loss != nullptr)
+    {
+        double sum = 0.0;
+        int n = 0;
+        for (int r = 0; r < p.rows; ++r)
+        {
+            if (counted(p.targets[r], p.ignore, p.vocab))
+            {
+                sum += static_cast<double>(losses[r]);
+                ++n;
+            }
+        }
+        *loss = n > 0 ? static_cast<float>(sum / n) : 0.0f;
+    }
+}
+
+// Copies vocabulary rows v .. v + chunk - 1 into `stage` (rows of `padded` elements), 16 bytes at a time
+// and asynchronously where the head allows it. What lies past dim or the vocabulary is zero.
+template <typename T>
+__device__ __forceinline__ void stage_head(const Few& p, T* stage, int64_t v)
+{
+    constexpr int V = 16 / sizeof(T);
+    const T* w = static_cast<const T*>(p.w);
+    if (p.vec)
+    {
+        const int per = p.padded / V;
+        for (int i = threadIdx.x; i < p.chunk * per; i += kFewThreads)
+        {
+            const int r = i / per, c = (i - r * per) * V;
+            const bool in = v + r < p.vocab && c < p.dim;   // dim is a multiple of V here
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(stage + r * p.padded + c)),
+                         "l"(in ? w + (v + r) * p.ldw + c : w), "r"(in ? 16u : 0u)
+                         : "memory");
+        }
+    }
+    else
+    {
+        for (int i = threadIdx.x; i < p.chunk * p.padded; i += kFewThreads)
+        {
+            const int r = i / p.padded, c = i - r * p.padded;
+            stage[i] = v + r < p.vocab && c < p.dim ? w[(v + r) * p.ldw + c] : from_f32<T>(0.0f);
+        }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+// Eight columns of a dW row (the first `left` of them), accumulated with beta.
+template <typename U>
+__device__ __forceinline__ void store_dw(U* at, float (&o)[8], int vec, int beta, int left)
+{
+    constexpr int V = 16 / sizeof(U);
+    if (vec && left >= 8)
+    {
+#pragma unroll
+        for (int k = 0; k < 8; k += V)
+        {
+            float part[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) part[i] = o[k + i];
+            if (beta)
+            {
+                float old[V];
+                load16(at + k, old);
+#pragma unroll
+                for (int i = 0; i < V; ++i) part[i] += old[i];
+            }
+            store16(at + k, part);
+        }
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+    {
+        if (k < left) at[k] = from_f32<U>(beta ? to_f32(at[k]) + o[k] : o[k]);
+    }
+}
+
+template <typename T, int R>
+__global__ void __launch_bounds__(kFewThreads, kFewBwdPerSm)
+few_bwd_kernel(const Few p)
+{
+    extern __shared__ float few_smem[];
+    __shared__ float coef_shared;
+    float* xs = few_smem;
+    float* qs = xs + R * p.padded;                                  // [chunk][R]
+    T* stage = reinterpret_cast<T*>(qs + 32 * R);                   // two chunks of head rows
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    dep_wait();
+    dep_release();
+    const int64_t step = static_cast<int64_t>(gridDim.x) * p.chunk;
+    int64_t v = static_cast<int64_t>(blockIdx.x) * p.chunk;
+    if (v < p.vocab) stage_head<T>(p, stage, v);
+    stage_rows<T, R>(p, xs, true);
+    if (threadIdx.x == 0)
+    {
+        int n = 0;
+        for (int r = 0; r < p.rows; ++r)
+        {
+            const int64_t t = p.targets[r];
+            if (counted(t, p.ignore, p.vocab)) ++n;
+            else if (t != p.ignore && p.status != nullptr) *p.status = VEDA_ERR_OUT_OF_RANGE;
+        }
+        coef_shared = n > 0 ? (p.upstream != nullptr ? *p.upstream : 1.0f) / static_cast<float>(n) : 0.0f;
+    }
+    const int64_t target = lane < p.rows ? p.targets[lane] : -1;
+    const bool valid = lane < p.rows && counted(target, p.ignore, p.vocab);
+    const float lse2 = valid ? p.lse[lane] * kLog2e : 0.0f;
+    __syncthreads();
+    const float coef = coef_shared;
+    // eight columns a thread; the threads that are left over take other rows of the chunk
+    const int groups = (p.dim + 7) / 8;
+    const int share = groups < kFewThreads ? kFewThreads / groups : 1;   // threads per eight columns
+    const int mine = threadIdx.x / groups;                               // which of them (>= share: none)
+    const int col0 = (threadIdx.x - mine * groups) * 8;
+    float dx[R][8] = {};
+    for (int buf = 0; v < p.vocab; v += step, buf ^= 1)
+    {
+        T* const here = stage + buf * p.chunk * p.padded;
+        if (v + step < p.vocab) stage_head<T>(p, stage + (buf ^ 1) * p.chunk * p.padded, v + step);
+        else asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncthreads();
+        // q of four head rows a warp at a time
+        for (int r0 = warp * 4; r0 < p.chunk; r0 += kFewWarps * 4)
+        {
+            float acc[4][R] = {};
+            for (int c = lane * 8; c < p.padded; c += 256)
+            {
+                Eight<T> w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j].read(here + (r0 + j) * p.padded + c);
+                dot8<T, R>(w, xs, p.padded, c, acc);
+            }
+            float z[4];
+            own_row<R>(acc, lane, z);
+            if (lane < R)
+            {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                {
+                    const float q = ex2(fmaf(z[j], kLog2e, -lse2)) - (target == v + r0 + j ? 1.0f : 0.0f);
+                    qs[(r0 + j) * R + lane] = valid && v + r0 + j < p.vocab ? q : 0.0f;
+                }
+            }
+        }
+        __syncthreads();
+        for (int col = col0; mine < share && col < p.dim; col += kFewThreads * 8)
+        {
+            float x8[R][8];
+            if (p.dw != nullptr)
+            {
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                {
+                    const float4 a = *reinterpret_cast<const float4*>(xs + r * p.padded + (col >> 3) * 4);
+                    const float4 b = *reinterpret_cast<const float4*>(xs + r * p.padded + p.padded / 2 + (col >> 3) * 4);
+                    x8[r][0] = a.x, x8[r][1] = a.y, x8[r][2] = a.z, x8[r][3] = a.w;
+                    x8[r][4] = b.x, x8[r][5] = b.y, x8[r][6] = b.z, x8[r][7] = b.w;
+                }
+            }
+            for (int k = mine; k < p.chunk && v + k < p.vocab; k += share)
+            {
+                float q[R];
+#pragma unroll
+                for (int r = 0; r < R; ++r) q[r] = qs[k * R + r];
+                if (p.acc != nullptr)
+                {
+                    Eight<T> raw;
+                    raw.read(here + k * p.padded + col);
+                    float w[8];
+                    raw.values(w);
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+                    {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) dx[r][i] = fmaf(q[r], w[i], dx[r][i]);
+                    }
+                }
+                if (p.dw != nullptr)
+                {
+                    float o[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                    {
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int r = 0; r < R; ++r) sum = fmaf(q[r], x8[r][i], sum);
+                        o[i] = sum * coef;
+                    }
+                    const int64_t at = (v + k) * p.lddw + col;
+                    if (p.dw_f32) store_dw(static_cast<float*>(p.dw) + at, o, p.dw_vec, p.dw_beta, p.dim - col);
+                    else store_dw(static_cast<bf16*>(p.dw) + at, o, p.dw_vec, p.dw_beta, p.dim - col);
+                }
+            }
+        }
+        __syncthreads();   // the chunk and its q are free
+    }
+    if (p.acc == nullptr)
+    {
+        return;
+    }
+    // The sums of the threads that share columns meet in shared memory, in order. A block holds one set
+    // of columns per thread, so dim <= 2048 (checked on the host).
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    for (int k = 0; k < share; ++k)
+    {
+        __syncthreads();
+        if (mine == k && col0 < p.dim)
+        {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+            {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                {
+                    float* at = xs + r * p.padded + col0 + i;   // x is no longer needed
+                    *at = k == 0 ? dx[r][i] : *at + dx[r][i];
+                }
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.rows * p.dim; i += kFewThreads)
+    {
+        const int r = i / p.dim, c = i - r * p.dim;
+        p.acc[(static_cast<int64_t>(blockIdx.x) * p.rows + r) * p.ld_acc + c] = xs[r * p.padded + c];
+    }
+}
+
+// dx = coef x the sum of the blocks' parts: 32 columns of a row per block, eight warps a share each.
+template <typename T>
+__global__ void __launch_bounds__(256)
+few_dx_kernel(const Few p, int blocks, T* __restrict__ dx, int64_t lddx)
+{
+    __shared__ float part[8][32];
+    dep_wait();
+    dep_release();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int c = blockIdx.x * 32 + lane, r = blockIdx.y;
+    float sum = 0.0f;
+    if (c < p.dim)
+    {
+#pragma unroll 8
+        for (int b = warp; b < blocks; b += 8) sum += p.acc[(static_cast<int64_t>(b) * p.rows + r) * p.ld_acc + c];
+    }
+    part[warp][lane] = sum;
+    __syncthreads();
+    if (warp == 0 && c < p.dim)
+    {
+        for (int k = 1; k < 8; ++k) sum += part[k][lane];
+        int n = 0;
+        for (int k = 0; k < p.rows; ++k) n += counted(p.targets[k], p.ignore, p.vocab) ? 1 : 0;
+        const float coef = n > 0 ? (p.upstream != nullptr ? *p.upstream : 1.0f) / static_cast<float>(n) : 0.0f;
+        dx[r * lddx + c] = from_f32<T>(sum * coef);
+    }
+}
+
 // ---- host ------------------------------------------------------------------------------------
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
@@ -869,6 +1395,11 @@ int choose_strip(int num_m, int num_n, int clusters)
     return best;
 }
 
+// Up to four rows of at most 2048 columns (a thread holds eight) go past the tensor cores. Against
+// 151936 x 1024, forward / backward: 1 row 51 / 143 us, 2 rows 52 / 167, 4 rows 66 / 231, 8 rows 101 / 359;
+// the tensor tiles take 98 / 288 for 9.
+bool is_few(int64_t rows, int64_t dim) { return rows <= kFewRows && dim <= 2048; }
+
 Layout layout(int64_t rows, int64_t vocab, int64_t dim, bool pack_x, bool pack_w, int dtype, bool backward)
 {
     Layout l{};
@@ -878,6 +1409,15 @@ Layout layout(int64_t rows, int64_t vocab, int64_t dim, bool pack_x, bool pack_w
         at += static_cast<size_t>(round_up(bytes, 256));
         return here;
     };
+    if (is_few(rows, dim))
+    {
+        l.parts = take(kFewBlocks * rows * 8);
+        l.target_logit = take(rows * 4);
+        l.ld_acc = round_up(dim, 4);
+        l.acc = take(backward ? kFewBlocks * rows * l.ld_acc * 4 : 0);
+        l.total = at;
+        return l;
+    }
     l.planes = dtype == VEDA_F32 ? 2 : 1;
     l.ldp = round_up(dim, 8);
     l.scalars = take(sizeof(Scalars));
@@ -1076,6 +1616,114 @@ int check(Call& c, void* workspace, size_t bytes, bool backward, const char* nam
     return VEDA_OK;
 }
 
+// ---- few rows, host -----------------------------------------------------------------------------
+Few few_params(const Call& c, const int64_t* targets, int64_t ignore, int* status)
+{
+    Few p{};
+    p.x = c.x;
+    p.w = c.w;
+    p.ldx = c.ldx;
+    p.ldw = c.ldw;
+    p.rows = static_cast<int>(c.rows);
+    p.dim = static_cast<int>(c.dim);
+    p.padded = static_cast<int>(round_up(c.dim, 256));
+    p.vocab = c.vocab;
+    p.targets = targets;
+    p.ignore = ignore;
+    const int64_t v = c.dtype == VEDA_BF16 ? 8 : 4;
+    p.vec = aligned16(c.w) && c.ldw % v == 0 && c.dim % 8 == 0;
+    p.parts = reinterpret_cast<float2*>(c.ws + c.l.parts);
+    p.target_logit = reinterpret_cast<float*>(c.ws + c.l.target_logit);
+    p.acc = reinterpret_cast<float*>(c.ws + c.l.acc);
+    p.ld_acc = c.l.ld_acc;
+    p.status = status;
+    return p;
+}
+
+// Opts a kernel into `bytes` of dynamic shared memory on the current device.
+template <typename K>
+bool allow_smem(K kernel, int bytes)
+{
+    if (bytes <= 48 * 1024)
+    {
+        return true;
+    }
+    const bool ok = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+    cudaGetLastError();
+    return ok;
+}
+
+// Blocks: what an SM holds of them on every SM, or fewer where there are fewer pieces of the vocabulary.
+int few_blocks(int64_t vocab, int piece, int per_sm)
+{
+    return static_cast<int>(std::min<int64_t>({(vocab + piece - 1) / piece, int64_t{per_sm} * sm_count(), kFewBlocks}));
+}
+
+template <typename T, int R>
+int launch_few_fwd(const Few& p, int* blocks, cudaStream_t s)
+{
+    *blocks = few_blocks(p.vocab, 4 * kFewWarps, few_fwd_per_sm(R));
+    const int smem = R * p.padded * 4;
+    const auto kernel = p.vec ? few_fwd_kernel<T, R, true> : few_fwd_kernel<T, R, false>;
+    if (!allow_smem(kernel, smem))
+    {
+        return fail(VEDA_ERR_CUDA, "veda_linear_cross_entropy_fwd: shared memory");
+    }
+    return launch("veda_linear_cross_entropy_fwd", kernel, dim3(*blocks), dim3(kFewThreads), smem, s, p);
+}
+
+template <typename T, int R>
+int launch_few_bwd(Few p, int* blocks, cudaStream_t s)
+{
+    // 32 vocabulary rows at a time, fewer where two sets of them would pass an SM's shared memory
+    const int room = 220 * 1024 / kFewBwdPerSm - 2048 - (R * p.padded + 32 * R) * 4;
+    p.chunk = 32;
+    while (p.chunk > 4 && 2 * p.chunk * p.padded * static_cast<int>(sizeof(T)) > room) p.chunk /= 2;
+    *blocks = few_blocks(p.vocab, p.chunk, kFewBwdPerSm);
+    const int smem = (R * p.padded + 32 * R) * 4 + 2 * p.chunk * p.padded * static_cast<int>(sizeof(T));
+    if (!allow_smem(few_bwd_kernel<T, R>, smem))
+    {
+        return fail(VEDA_ERR_CUDA, "veda_linear_cross_entropy_bwd: shared memory");
+    }
+    return launch("veda_linear_cross_entropy_bwd", few_bwd_kernel<T, R>, dim3(*blocks), dim3(kFewThreads), smem, s, p);
+}
+
+template <typename T>
+int few_fwd(const Call& c, const int64_t* targets, int64_t ignore, float* row_loss, float* lse, float* loss, int* status,
+            cudaStream_t s)
+{
+    const Few p = few_params(c, targets, ignore, status);
+    int blocks = 0;
+    int rc = p.rows == 1   ? launch_few_fwd<T, 1>(p, &blocks, s)
+             : p.rows == 2 ? launch_few_fwd<T, 2>(p, &blocks, s)
+                           : launch_few_fwd<T, 4>(p, &blocks, s);
+    if (rc != VEDA_OK) return rc;
+    return launch("veda_linear_cross_entropy_fwd (merge)", few_merge_kernel, dim3(1), dim3(kFewThreads), 0, s, p, blocks,
+                  row_loss, lse, loss);
+}
+
+template <typename T>
+int few_bwd(const Call& c, const int64_t* targets, int64_t ignore, const float* lse, const float* upstream, void* dx,
+            int64_t lddx, void* dw, int64_t lddw, int dtype_dw, bool beta, int* status, cudaStream_t s)
+{
+    Few p = few_params(c, targets, ignore, status);
+    p.lse = lse;
+    p.upstream = upstream;
+    p.dw = dw;
+    p.lddw = lddw;
+    p.dw_f32 = dtype_dw == VEDA_F32;
+    p.dw_beta = beta;
+    p.dw_vec = aligned16(dw) && lddw % (p.dw_f32 ? 4 : 8) == 0;
+    if (dx == nullptr) p.acc = nullptr;
+    int blocks = 0;
+    int rc = p.rows == 1   ? launch_few_bwd<T, 1>(p, &blocks, s)
+             : p.rows == 2 ? launch_few_bwd<T, 2>(p, &blocks, s)
+                           : launch_few_bwd<T, 4>(p, &blocks, s);
+    if (rc != VEDA_OK || dx == nullptr) return rc;
+    return launch("veda_linear_cross_entropy_bwd (dx)", few_dx_kernel<T>, dim3((p.dim + 31) / 32, p.rows), dim3(256), 0, s,
+                  p, blocks, static_cast<T*>(dx), lddx);
+}
+
 constexpr int64_t kLimit = (1ll << 31) - 512;   // tile coordinates are 32-bit
 
 } // namespace lce
@@ -1118,6 +1766,12 @@ extern "C" int veda_linear_cross_entropy_fwd(const void* x, int64_t ldx, const v
     lce::Call c{x, w, ldx, ldw, rows, vocab, dim, dtype};
     int rc = lce::check(c, workspace, workspace_bytes, false, "veda_linear_cross_entropy_fwd");
     if (rc != VEDA_OK) return rc;
+    if (lce::is_few(rows, dim))
+    {
+        return dtype == VEDA_BF16
+                   ? lce::few_fwd<bf16>(c, targets, ignore_index, row_loss, lse, loss, status, stream)
+                   : lce::few_fwd<float>(c, targets, ignore_index, row_loss, lse, loss, status, stream);
+    }
     const bool split = dtype == VEDA_F32;
     const int clusters = split ? pair::clusters_available<lce::StatsWork, 4, true>()
                                : pair::clusters_available<lce::StatsWork, 4, false>();
@@ -1178,9 +1832,16 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
     lce::Call c{x, w, ldx, ldw, rows, vocab, dim, dtype};
     int rc = lce::check(c, workspace, workspace_bytes, true, "veda_linear_cross_entropy_bwd");
     if (rc != VEDA_OK) return rc;
+    if (lce::is_few(rows, dim))
+    {
+        return dtype == VEDA_BF16 ? lce::few_bwd<bf16>(c, targets, ignore_index, lse, upstream, dx, lddx, dw, lddw,
+                                                       dtype_dw, beta_dw != 0.0f, status, stream)
+                                  : lce::few_bwd<float>(c, targets, ignore_index, lse, upstream, dx, lddx, dw, lddw,
+                                                        dtype_dw, beta_dw != 0.0f, status, stream);
+    }
     const bool split = dtype == VEDA_F32;
-    const int clusters = std::min(lce::kMaxClusters, split ? pair::clusters_available<lce::GradWork, 4, true>()
-                                                           : pair::clusters_available<lce::GradWork, 4, false>());
+    const int clusters = std::min(lce::kMaxClusters, split ? pair::clusters_available<lce::GradWork, 8, true>()
+                                                           : pair::clusters_available<lce::GradWork, 8, false>());
     if (clusters < 1)
     {
         return fail(VEDA_ERR_UNSUPPORTED, "veda_linear_cross_entropy_bwd: no CTA pair fits on this device");
@@ -1254,8 +1915,8 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
         // k-blocks a tile, and what its epilogue adds
         const int64_t cost[3] = {(rows + 63) / 64 + 4, p.dx_kbs + 2, (dim + 63) / 64 + 2};
         lce::share(tiles, cost, grid, p.shares);
-        rc = split ? pair::launch_pair<lce::GradWork, 4, true>("veda_linear_cross_entropy_bwd", p, grid, stream)
-                   : pair::launch_pair<lce::GradWork, 4, false>("veda_linear_cross_entropy_bwd", p, grid, stream);
+        rc = split ? pair::launch_pair<lce::GradWork, 8, true>("veda_linear_cross_entropy_bwd", p, grid, stream)
+                   : pair::launch_pair<lce::GradWork, 8, false>("veda_linear_cross_entropy_bwd", p, grid, stream);
         if (rc != VEDA_OK) return rc;
     }
     if (dx == nullptr)
