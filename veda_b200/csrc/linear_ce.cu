@@ -97,6 +97,7 @@ struct Params
     const float* lse;
     float2* parts;           // [strip slots][rows] running (max, sum)
     float* target_logit;     // [rows]
+    unsigned* done;          // cleared for the merge's blocks to count themselves
     int* status;
 };
 
@@ -186,6 +187,10 @@ struct StatsWork
     {
         if (t.first)
         {
+            if (t.slot == 0 && t.mb == 0 && row0 + lane == 0)
+            {
+                *p.done = 0;
+            }
             s.m = -INFINITY;
             s.s = 0.0f;
             s.target = counted_target(p, t.mb * pair::kTile + row0 + lane);
@@ -643,108 +648,157 @@ __device__ __forceinline__ float split_scale(float top)
     return ldexpf(1.0f, e < -120 ? -120 : e > 120 ? 120 : e);
 }
 
-// The call's scalars: split scales from the partial maxima, and upstream / counted rows.
-__global__ void __launch_bounds__(1024)
-scalars_kernel(const int64_t* __restrict__ targets, int64_t ignore, int64_t rows, int64_t vocab,
-               const float* __restrict__ upstream, const float* __restrict__ part, int gx, int gw,
-               Scalars* out, int* status)
+// What comes before the tensor-core launches, in one: the call's scalars (the last block: split scales
+// from the partial maxima, upstream / counted rows) and the operand planes of x (blocks below gx) and w
+// (the next gw) with a pitch of a multiple of 8 elements: a bf16 copy, or the two fp16 halves of an fp32
+// operand. clear: rows of x that are not counted become zeros, so that what padding holds (NaN
+// included) meets q = 0 in dW's product as 0. vx, vw: eight elements of a row can be read at a time.
+template <typename T>
+__global__ void __launch_bounds__(256)
+pack_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, const T* __restrict__ w, int64_t ldw, int64_t vocab,
+            int64_t dim, const int64_t* __restrict__ targets, int64_t ignore, bool clear, bool vx, bool vw, int gx, int gw,
+            uint16_t* __restrict__ px, uint16_t* __restrict__ pw, int64_t ldp, const float* __restrict__ part, int parts_x,
+            int parts_w, const float* __restrict__ upstream, Scalars* __restrict__ scalars, int* status)
 {
-    __shared__ int counts[32];
-    __shared__ float tops[2];
+    __shared__ int counts[8];
+    __shared__ float tops[2][8];
+    __shared__ float scale_shared[2];
     dep_wait();
     dep_release();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int n = 0, bad = 0;
-    for (int64_t i = threadIdx.x; i < rows; i += blockDim.x)
+    const int block = static_cast<int>(blockIdx.x);
+    if (part != nullptr)
     {
-        const int64_t t = targets[i];
-        if (t != ignore)
+        float tx = 0.0f, tw = 0.0f;
+        for (int i = threadIdx.x; i < parts_x; i += 256) tx = fmaxf(tx, part[i]);
+        for (int i = threadIdx.x; i < parts_w; i += 256) tw = fmaxf(tw, part[parts_x + i]);
+        tx = warp_max(tx);
+        tw = warp_max(tw);
+        if (lane == 0) tops[0][warp] = tx, tops[1][warp] = tw;
+        __syncthreads();
+        if (threadIdx.x < 2)
         {
-            t >= 0 && t < vocab ? ++n : ++bad;
+            float top = 0.0f;
+            for (int k = 0; k < 8; ++k) top = fmaxf(top, tops[threadIdx.x][k]);
+            scale_shared[threadIdx.x] = split_scale(top);
         }
+        __syncthreads();
     }
-    n = __reduce_add_sync(0xFFFFFFFFu, n);
-    if (__any_sync(0xFFFFFFFFu, bad != 0) && lane == 0 && status != nullptr)
+    if (block == gx + gw)
     {
-        *status = VEDA_ERR_OUT_OF_RANGE;
-    }
-    if (lane == 0) counts[warp] = n;
-    if (part != nullptr && warp < 2)
-    {
-        float top = 0.0f;
-        for (int i = lane; i < (warp == 0 ? gx : gw); i += 32) top = fmaxf(top, part[(warp == 0 ? 0 : gx) + i]);
-        top = warp_max(top);
-        if (lane == 0) tops[warp] = top;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0)
-    {
-        int total = 0;
-        for (int k = 0; k < 32; ++k) total += counts[k];
-        // no counted row: the loss and every gradient are zero
-        const float coef = total > 0 ? (upstream != nullptr ? *upstream : 1.0f) / static_cast<float>(total) : 0.0f;
-        Scalars s{1.0f, coef, 1.0f, 1.0f, 1.0f, 1.0f};
-        if (part != nullptr)
+        int n = 0, bad = 0;
+        for (int64_t i = threadIdx.x; i < rows; i += 256)
         {
-            s.x = split_scale(tops[0]);
-            s.w = split_scale(tops[1]);
-            s.z = 1.0f / s.x / s.w;
-            s.unit_dx = 1.0f / kQScale / s.w;
-            s.unit_dw = 1.0f / kQScale / s.x;
+            const int64_t t = targets[i];
+            if (t != ignore)
+            {
+                t >= 0 && t < vocab ? ++n : ++bad;
+            }
         }
-        *out = s;
+        n = __reduce_add_sync(0xFFFFFFFFu, n);
+        if (__any_sync(0xFFFFFFFFu, bad != 0) && lane == 0 && status != nullptr)
+        {
+            *status = VEDA_ERR_OUT_OF_RANGE;
+        }
+        if (lane == 0) counts[warp] = n;
+        __syncthreads();
+        if (threadIdx.x == 0)
+        {
+            int total = 0;
+            for (int k = 0; k < 8; ++k) total += counts[k];
+            // no counted row: the loss and every gradient are zero
+            const float coef = total > 0 ? (upstream != nullptr ? *upstream : 1.0f) / static_cast<float>(total) : 0.0f;
+            Scalars s{1.0f, coef, 1.0f, 1.0f, 1.0f, 1.0f};
+            if (part != nullptr)
+            {
+                s.x = scale_shared[0];
+                s.w = scale_shared[1];
+                s.z = 1.0f / s.x / s.w;
+                s.unit_dx = 1.0f / kQScale / s.w;
+                s.unit_dw = 1.0f / kQScale / s.x;
+            }
+            *scalars = s;
+        }
+        return;
     }
-}
-
-// Operand planes of x (blocks below gx) and w with a pitch of a multiple of 8 elements: a bf16 copy,
-// or the two fp16 halves of an fp32 operand. clear: rows of x that are not counted become zeros, so
-// that what padding holds (NaN included) meets q = 0 in dW's product as 0.
-template <typename T>
-__global__ void __launch_bounds__(256)
-pack_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, const T* __restrict__ w, int64_t ldw,
-            int64_t vocab, int64_t dim, const int64_t* __restrict__ targets, int64_t ignore, bool clear, int gx,
-            uint16_t* __restrict__ px, uint16_t* __restrict__ pw, int64_t ldp, const Scalars* __restrict__ scalars)
-{
-    dep_wait();
-    dep_release();
-    const bool is_w = static_cast<int>(blockIdx.x) >= gx;
+    const bool is_w = block >= gx;
     const T* m = is_w ? w : x;
     uint16_t* out = is_w ? pw : px;
     const int64_t ld = is_w ? ldw : ldx, n = is_w ? vocab : rows;
-    const int64_t b = is_w ? blockIdx.x - gx : blockIdx.x, blocks = is_w ? gridDim.x - gx : gx;
-    const float scale = sizeof(T) == 4 ? (is_w ? scalars->w : scalars->x) : 1.0f;
-    for (int64_t r = b * 8 + threadIdx.x / 32; r < n; r += blocks * 8)
+    const int64_t b = is_w ? block - gx : block, blocks = is_w ? gw : gx;
+    const float scale = part != nullptr ? scale_shared[is_w ? 1 : 0] : 1.0f;
+    const bool vec = is_w ? vw : vx;
+    const int64_t per_row = ldp / 8, groups = n * per_row;   // of eight columns
+#pragma unroll 2
+    for (int64_t g = b * 256 + threadIdx.x; g < groups; g += blocks * 256)
     {
-        const bool keep = is_w || !clear || counted(targets[r], ignore, vocab);
-        for (int64_t c = threadIdx.x & 31; c < dim; c += 32)
+        const int64_t r = g / per_row, c = (g - r * per_row) * 8;
+        const int left = static_cast<int>(dim - c < 8 ? dim - c : 8);
+        float v[8];
+        if (!is_w && clear && !counted(targets[r], ignore, vocab))
+        {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+        }
+        else if (vec && left == 8)
         {
             if constexpr (sizeof(T) == 2)
             {
-                out[r * ldp + c] = keep ? __bfloat16_as_ushort(m[r * ld + c]) : uint16_t{0};
+                load16(m + r * ld + c, v);
             }
             else
             {
-                const float v = keep ? m[r * ld + c] * scale : 0.0f;
-                const __half h = __float2half_rn(v);
-                out[r * ldp + c] = __half_as_ushort(h);
-                out[(n + r) * ldp + c] = __half_as_ushort(__float2half_rn(v - __half2float(h)));
+                float a[4], d[4];
+                load16(m + r * ld + c, a);
+                load16(m + r * ld + c + 4, d);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = a[k], v[4 + k] = d[k];
             }
+        }
+        else
+        {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = k < left ? to_f32(m[r * ld + c + k]) : 0.0f;
+        }
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+        {
+            if constexpr (sizeof(T) == 2)
+            {
+                hi[k] = pack_bf16(v[2 * k], v[2 * k + 1]);   // bf16 values: exact
+            }
+            else
+            {
+                const float a = v[2 * k] * scale, d = v[2 * k + 1] * scale;
+                hi[k] = pack_f16(a, d);
+                lo[k] = pack_f16(a - f16_lo(hi[k]), d - f16_hi(hi[k]));
+            }
+        }
+        *reinterpret_cast<uint4*>(out + r * ldp + c) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if constexpr (sizeof(T) == 4)
+        {
+            *reinterpret_cast<uint4*>(out + (n + r) * ldp + c) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
     }
 }
 
-// Merges a row's (max, sum) pairs in slot order: lse = ln 2 (max + log2 sum), loss = lse - z[target].
+// Merges each row's (max, sum) pairs, lse = ln 2 (max + log2 sum), loss = lse - z[target]; the block
+// that finishes last takes the mean over the counted rows, in double and in a fixed order (0 when none
+// is counted). A block has `width` rows (a power of two) and 256 / width threads a row.
 __global__ void __launch_bounds__(256)
-merge_kernel(const float2* __restrict__ parts, int slots, int64_t rows, int64_t vocab,
+merge_kernel(const float2* __restrict__ parts, int slots, int64_t rows, int64_t vocab, int width,
              const int64_t* __restrict__ targets, int64_t ignore, const float* __restrict__ target_logit,
-             float* __restrict__ row_loss, float* __restrict__ lse, int* status)
+             float* row_loss, float* __restrict__ lse, float* loss, unsigned* done, int* status)
 {
-    // 32 rows a block, eight slices of the slots
-    __shared__ float2 part[8][32];
+    __shared__ float2 part[256];
+    __shared__ double sums[8];
+    __shared__ int counts[8];
+    __shared__ bool last;
     dep_wait();
     dep_release();
-    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+    const int tid = static_cast<int>(threadIdx.x), mine = tid & (width - 1), slice = tid / width, slices = 256 / width;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * width + mine;
     float m = -INFINITY, s = 0.0f;
     auto add = [&](float2 o) {
         const float top = fmaxf(m, o.x);
@@ -754,84 +808,129 @@ merge_kernel(const float2* __restrict__ parts, int slots, int64_t rows, int64_t 
     };
     if (row < rows)
     {
-        for (int k = slice; k < slots; k += 8) add(parts[static_cast<int64_t>(k) * rows + row]);
+#pragma unroll 4
+        for (int k = slice; k < slots; k += slices) add(parts[static_cast<int64_t>(k) * rows + row]);
     }
-    part[slice][lane] = make_float2(m, s);
-    __syncthreads();
-    if (slice != 0 || row >= rows)
+    for (int d = slices / 2; d > 0; d /= 2)
+    {
+        part[tid] = make_float2(m, s);
+        __syncthreads();
+        if (slice < d) add(part[tid + d * width]);
+        __syncthreads();
+    }
+    if (slice == 0 && row < rows)
+    {
+        const float l = (m + log2f(s)) * kLn2;
+        if (lse != nullptr) lse[row] = l;
+        const int64_t t = targets[row];
+        const bool inside = t >= 0 && t < vocab;
+        if (t != ignore && !inside && status != nullptr)
+        {
+            *status = VEDA_ERR_OUT_OF_RANGE;
+        }
+        row_loss[row] = t != ignore && inside ? l - target_logit[row] : 0.0f;
+    }
+    if (loss == nullptr)
     {
         return;
     }
-    for (int k = 1; k < 8; ++k) add(part[k][lane]);
-    const float l = (m + log2f(s)) * kLn2;
-    if (lse != nullptr) lse[row] = l;
-    const int64_t t = targets[row];
-    const bool inside = t >= 0 && t < vocab;
-    if (t != ignore && !inside && status != nullptr)
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) last = atomicAdd(done, 1u) == gridDim.x - 1;
+    __syncthreads();
+    if (!last)
     {
-        *status = VEDA_ERR_OUT_OF_RANGE;
+        return;
     }
-    row_loss[row] = t != ignore && inside ? l - target_logit[row] : 0.0f;
-}
-
-// Mean of the counted rows' losses, summed in double in a fixed order; 0 when none is counted.
-__global__ void __launch_bounds__(1024)
-mean_kernel(const float* __restrict__ row_loss, const int64_t* __restrict__ targets, int64_t ignore, int64_t rows,
-            int64_t vocab, float* loss)
-{
-    __shared__ double sums[32];
-    __shared__ int counts[32];
-    dep_wait();
-    dep_release();
-    double s = 0.0;
+    __threadfence();
+    double sum = 0.0;
     int n = 0;
-    for (int64_t i = threadIdx.x; i < rows; i += blockDim.x)
+#pragma unroll 4
+    for (int64_t i = tid; i < rows; i += 256)
     {
-        const int64_t t = targets[i];
-        if (t != ignore && t >= 0 && t < vocab)
+        if (counted(targets[i], ignore, vocab))
         {
-            s += static_cast<double>(row_loss[i]);
+            sum += static_cast<double>(__ldcg(row_loss + i));
             ++n;
         }
     }
-    s = warp_sum(s);
+    sum = warp_sum(sum);
     n = __reduce_add_sync(0xFFFFFFFFu, n);
-    if ((threadIdx.x & 31) == 0)
-    {
-        sums[threadIdx.x >> 5] = s;
-        counts[threadIdx.x >> 5] = n;
-    }
+    if ((tid & 31) == 0) sums[tid >> 5] = sum, counts[tid >> 5] = n;
     __syncthreads();
-    if (threadIdx.x == 0)
+    if (tid == 0)
     {
-        int total = counts[0];
-        s = sums[0];
-        for (int k = 1; k < 32; ++k)
-        {
-            s += sums[k];
-            total += counts[k];
-        }
-        *loss = total > 0 ? static_cast<float>(s / total) : 0.0f;
+        for (int k = 1; k < 8; ++k) sum += sums[k], n += counts[k];
+        *loss = n > 0 ? static_cast<float>(sum / n) : 0.0f;
     }
 }
 
-// dx = coef x the fp32 sums, those of the splits added in their order.
+// dx = coef x the fp32 sums. One set of them: eight columns a thread, where rows allow it.
 template <typename T>
 __global__ void __launch_bounds__(256)
-finish_dx_kernel(const float* __restrict__ acc, int64_t lda, int splits, T* __restrict__ dx, int64_t lddx, int64_t rows,
-                 int64_t dim, const Scalars* __restrict__ scalars)
+finish_dx_kernel(const float* __restrict__ acc, int64_t lda, T* __restrict__ dx, int64_t lddx, int64_t rows,
+                 int64_t dim, bool vec, const Scalars* __restrict__ scalars)
 {
     dep_wait();
     dep_release();
     const float coef = scalars->coef, unit = scalars->unit_dx;
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32; r < rows; r += static_cast<int64_t>(gridDim.x) * 8)
+    const int64_t per_row = (dim + 7) / 8, groups = rows * per_row;
+    for (int64_t g = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; g < groups; g += static_cast<int64_t>(gridDim.x) * 256)
     {
-        for (int64_t c = threadIdx.x & 31; c < dim; c += 32)
+        const int64_t r = g / per_row, c = (g - r * per_row) * 8;
+        const float* from = acc + r * lda + c;
+        T* to = dx + r * lddx + c;
+        if (vec && c + 8 <= dim)
         {
-            float sum = acc[r * lda + c];
-            for (int k = 1; k < splits; ++k) sum += acc[(k * rows + r) * lda + c];
-            dx[r * lddx + c] = from_f32<T>(sum * unit * coef);
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; k += 4)
+            {
+                float a[4];
+                load16(from + k, a);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[k + i] = a[i] * unit * coef;
+            }
+            constexpr int V = 16 / sizeof(T);
+#pragma unroll
+            for (int k = 0; k < 8; k += V)
+            {
+                float o[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[i] = v[k + i];
+                store16(to + k, o);
+            }
         }
+        else
+        {
+            for (int k = 0; k < 8 && c + k < dim; ++k) to[k] = from_f32<T>(from[k] * unit * coef);
+        }
+    }
+}
+
+// The same of several sets, added in a fixed order: 32 columns of a row per block, a warp an eighth.
+template <typename T>
+__global__ void __launch_bounds__(256)
+finish_splits_kernel(const float* __restrict__ acc, int64_t lda, int splits, T* __restrict__ dx, int64_t lddx, int64_t rows,
+                     int64_t dim, const Scalars* __restrict__ scalars)
+{
+    __shared__ float part[8][32];
+    dep_wait();
+    dep_release();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane, r = blockIdx.y;
+    float sum = 0.0f;
+    if (c < dim)
+    {
+#pragma unroll 4
+        for (int k = warp; k < splits; k += 8) sum += acc[(k * rows + r) * lda + c];
+    }
+    part[warp][lane] = sum;
+    __syncthreads();
+    if (warp == 0 && c < dim)
+    {
+        for (int k = 1; k < 8; ++k) sum += part[k][lane];
+        dx[r * lddx + c] = from_f32<T>(sum * scalars->unit_dx * scalars->coef);
     }
 }
 
@@ -1372,7 +1471,7 @@ struct Layout
     int64_t ld_acc;       // pitch of the fp32 dx sums
     int splits;           // of dx's sum over a piece
     int strip, slots;     // forward: tiles a strip, strips
-    size_t scalars, part, px, pw, parts, target_logit, q, acc, total;
+    size_t scalars, done, part, px, pw, parts, target_logit, q, acc, total;
 };
 
 // Tiles per strip: up to 8, by the number of tile times the busiest of `clusters` clusters runs;
@@ -1421,6 +1520,7 @@ Layout layout(int64_t rows, int64_t vocab, int64_t dim, bool pack_x, bool pack_w
     l.planes = dtype == VEDA_F32 ? 2 : 1;
     l.ldp = round_up(dim, 8);
     l.scalars = take(sizeof(Scalars));
+    l.done = take(4);
     l.part = take(2 * kMaxBlocks * 4);
     l.px = take(pack_x ? l.planes * rows * l.ldp * 2 : 0);
     l.pw = take(pack_w ? l.planes * vocab * l.ldp * 2 : 0);
@@ -1537,30 +1637,27 @@ int prepare(const Call& c, const int64_t* targets, int64_t ignore, const float* 
                               c.vocab, c.dim, targets, ignore, static_cast<int>(gx), part);
         if (rc != VEDA_OK) return rc;
     }
-    if (scalars || part != nullptr)
-    {
-        const int rc = launch("veda_linear_cross_entropy", scalars_kernel, dim3(1), dim3(1024), 0, s, targets, ignore,
-                              c.rows, c.vocab, upstream, static_cast<const float*>(part), static_cast<int>(gx),
-                              static_cast<int>(gw), c.scalars(), status);
-        if (rc != VEDA_OK) return rc;
-    }
     const void *px = c.x, *pw = c.w;
     int64_t ldx = c.ldx, ldw = c.ldw;
-    if (c.pack_x || c.pack_w)
+    if (scalars || part != nullptr || c.pack_x || c.pack_w)
     {
         auto* ox = reinterpret_cast<uint16_t*>(c.ws + c.l.px);
         auto* ow = reinterpret_cast<uint16_t*>(c.ws + c.l.pw);
-        const unsigned bx = c.pack_x ? gx : 0, bw = c.pack_w ? gw : 0;
-        const int rc =
-            c.dtype == VEDA_F32
-                ? launch("veda_linear_cross_entropy", pack_kernel<float>, dim3(bx + bw), dim3(256), 0, s,
-                         static_cast<const float*>(c.x), c.ldx, c.rows, static_cast<const float*>(c.w), c.ldw,
-                         c.vocab, c.dim, targets, ignore, c.backward, static_cast<int>(bx), ox, ow, c.l.ldp,
-                         static_cast<const Scalars*>(c.scalars()))
-                : launch("veda_linear_cross_entropy", pack_kernel<bf16>, dim3(bx + bw), dim3(256), 0, s,
-                         static_cast<const bf16*>(c.x), c.ldx, c.rows, static_cast<const bf16*>(c.w), c.ldw,
-                         c.vocab, c.dim, targets, ignore, c.backward, static_cast<int>(bx), ox, ow, c.l.ldp,
-                         static_cast<const Scalars*>(c.scalars()));
+        const int64_t es = static_cast<int64_t>(dtype_size(c.dtype));
+        const auto blocks = [&](int64_t n) {
+            return static_cast<int>(std::min<int64_t>((n * (c.l.ldp / 8) + 255) / 256, 8ll * sm_count()));
+        };
+        const auto vec = [&](const void* m, int64_t ld) { return aligned16(m) && ld * es % 16 == 0; };
+        const int bx = c.pack_x ? blocks(c.rows) : 0, bw = c.pack_w ? blocks(c.vocab) : 0;
+        const auto go = [&](auto* x, auto* w, auto kernel) {
+            return launch("veda_linear_cross_entropy (operands)", kernel, dim3(bx + bw + 1), dim3(256), 0, s, x, c.ldx,
+                          c.rows, w, c.ldw, c.vocab, c.dim, targets, ignore, c.backward, vec(c.x, c.ldx), vec(c.w, c.ldw),
+                          bx, bw, ox, ow, c.l.ldp, static_cast<const float*>(part), static_cast<int>(gx),
+                          static_cast<int>(gw), upstream, c.scalars(), status);
+        };
+        const int rc = c.dtype == VEDA_F32
+                           ? go(static_cast<const float*>(c.x), static_cast<const float*>(c.w), pack_kernel<float>)
+                           : go(static_cast<const bf16*>(c.x), static_cast<const bf16*>(c.w), pack_kernel<bf16>);
         if (rc != VEDA_OK) return rc;
         if (c.pack_x)
         {
@@ -1786,18 +1883,20 @@ extern "C" int veda_linear_cross_entropy_fwd(const void* x, int64_t ldx, const v
     while ((1 << p.strip_log2) < c.l.strip) ++p.strip_log2;
     p.parts = reinterpret_cast<float2*>(c.ws + c.l.parts);
     p.target_logit = reinterpret_cast<float*>(c.ws + c.l.target_logit);
+    p.done = reinterpret_cast<unsigned*>(c.ws + c.l.done);
     const int64_t units = static_cast<int64_t>(c.l.slots) * p.num_m;
     VEDA_REQUIRE(units <= lce::kLimit, "too many tiles");
     const int grid = static_cast<int>(std::min<int64_t>(units, clusters));
     rc = split ? pair::launch_pair<lce::StatsWork, 4, true>("veda_linear_cross_entropy_fwd", p, grid, stream)
                : pair::launch_pair<lce::StatsWork, 4, false>("veda_linear_cross_entropy_fwd", p, grid, stream);
     if (rc != VEDA_OK) return rc;
-    rc = launch("veda_linear_cross_entropy_fwd (merge)", lce::merge_kernel, dim3(static_cast<unsigned>((rows + 31) / 32)),
-                dim3(256), 0, stream, static_cast<const float2*>(p.parts), c.l.slots, rows, vocab, targets, ignore_index,
-                static_cast<const float*>(p.target_logit), row_loss, lse, status);
-    if (rc != VEDA_OK || loss == nullptr) return rc;
-    return launch("veda_linear_cross_entropy_fwd (mean)", lce::mean_kernel, dim3(1), dim3(1024), 0, stream,
-                  static_cast<const float*>(row_loss), targets, ignore_index, rows, vocab, loss);
+    // 32 rows a block reads whole lines of pairs; fewer where the rows would not fill the GPU's SMs
+    int width = 32;
+    while (width > 1 && (rows + width - 1) / width < sm_count()) width /= 2;
+    return launch("veda_linear_cross_entropy_fwd (merge)", lce::merge_kernel,
+                  dim3(static_cast<unsigned>((rows + width - 1) / width)), dim3(256), 0, stream,
+                  static_cast<const float2*>(p.parts), c.l.slots, rows, vocab, width, targets, ignore_index,
+                  static_cast<const float*>(p.target_logit), row_loss, lse, loss, p.done, status);
 }
 
 extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
@@ -1923,11 +2022,20 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
     {
         return VEDA_OK;
     }
-    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((rows + 7) / 8, 8ll * sm_count()));
-    return bf ? launch("veda_linear_cross_entropy_bwd (dx)", lce::finish_dx_kernel<bf16>, dim3(blocks), dim3(256), 0,
-                       stream, static_cast<const float*>(acc), c.l.ld_acc, c.l.splits, static_cast<bf16*>(dx), lddx, rows, dim,
-                       static_cast<const lce::Scalars*>(c.scalars()))
-              : launch("veda_linear_cross_entropy_bwd (dx)", lce::finish_dx_kernel<float>, dim3(blocks), dim3(256), 0,
-                       stream, static_cast<const float*>(acc), c.l.ld_acc, c.l.splits, static_cast<float*>(dx), lddx, rows, dim,
-                       static_cast<const lce::Scalars*>(c.scalars()));
+    const lce::Scalars* scalars = c.scalars();
+    const auto finish = [&](auto* out, auto one, auto several) {
+        if (c.l.splits > 1)
+        {
+            return launch("veda_linear_cross_entropy_bwd (dx)", several,
+                          dim3(static_cast<unsigned>((dim + 31) / 32), static_cast<unsigned>(rows)), dim3(256), 0, stream,
+                          static_cast<const float*>(acc), c.l.ld_acc, c.l.splits, out, lddx, rows, dim, scalars);
+        }
+        const int64_t es = static_cast<int64_t>(dtype_size(dtype));
+        const bool vec = aligned16(dx) && lddx * es % 16 == 0;
+        const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((rows * ((dim + 7) / 8) + 255) / 256, 8ll * sm_count()));
+        return launch("veda_linear_cross_entropy_bwd (dx)", one, dim3(blocks), dim3(256), 0, stream,
+                      static_cast<const float*>(acc), c.l.ld_acc, out, lddx, rows, dim, vec, scalars);
+    };
+    return bf ? finish(static_cast<bf16*>(dx), lce::finish_dx_kernel<bf16>, lce::finish_splits_kernel<bf16>)
+              : finish(static_cast<float*>(dx), lce::finish_dx_kernel<float>, lce::finish_splits_kernel<float>);
 }
