@@ -128,7 +128,10 @@ SHAPES = [(1, 1, 8), (1, 300, 64), (3, 2, 16), (31, 255, 24), (128, 512, 64), (2
           (300, 257, 72), (512, 2049, 128), (77, 5001, 520), (1030, 770, 136),
           # up to four rows of up to 2048 columns are streamed past; one past each border
           (2, 700, 2048), (3, 601, 1000), (4, 9001, 776), (5, 4100, 64), (4, 50, 2056), (1, 20000, 40), (4, 33, 1),
-          (8, 9001, 776)]
+          (8, 9001, 776),
+          # the tensor-core form: over 1024 rows, 4096 words or 2^25 products
+          (31, 4355, 24), (128, 5000, 64), (257, 4353, 40), (300, 4097, 72), (512, 6145, 128), (1025, 255, 16),
+          (9, 4111, 8), (700, 4000, 100), (1024, 4096, 8)]
 
 
 @pytest.mark.gpu
@@ -147,7 +150,8 @@ def test_many_pieces_of_the_vocabulary(cuda, dtype, rows, vocab, dim):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [V.BF16, V.F32])
-@pytest.mark.parametrize("rows,vocab,dim", [(65, 130, 7), (40, 300, 100), (129, 257, 33), (4, 300, 100), (2, 1001, 33)])
+@pytest.mark.parametrize("rows,vocab,dim", [(65, 130, 7), (40, 300, 100), (129, 257, 33), (4, 300, 100), (2, 1001, 33), (65, 4130, 7),
+                                             (300, 4300, 100), (1029, 257, 33)])
 def test_odd_widths_pitches_and_bases(cuda, dtype, rows, vocab, dim):
     t = torch()
     x, w, tg = make(rows, vocab, dim, dtype, seed=2)
@@ -164,9 +168,10 @@ def test_odd_widths_pitches_and_bases(cuda, dtype, rows, vocab, dim):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [V.BF16, V.F32])
-def test_aligned_slices_are_read_in_place_and_padding_stays(cuda, dtype):
+@pytest.mark.parametrize("vocab", [500, 4500])
+def test_aligned_slices_are_read_in_place_and_padding_stays(cuda, dtype, vocab):
     t = torch()
-    rows, vocab, dim = 100, 500, 64
+    rows, dim = 100, 64
     x, w, tg = make(rows, vocab, dim, dtype, seed=3)
     wide = t.full((rows, 192), float("nan"), device="cuda", dtype=x.dtype)
     wide[:, 64:128] = x
@@ -185,10 +190,10 @@ def test_aligned_slices_are_read_in_place_and_padding_stays(cuda, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,dtype_dw", [(V.BF16, V.BF16), (V.BF16, V.F32), (V.F32, V.F32)])
 @pytest.mark.parametrize("pitch", [64, 67])
-@pytest.mark.parametrize("rows", [150, 3])
-def test_accumulated_weight_gradient_and_upstream(cuda, dtype, dtype_dw, pitch, rows):
+@pytest.mark.parametrize("rows,vocab", [(150, 700), (3, 700), (150, 4700)])
+def test_accumulated_weight_gradient_and_upstream(cuda, dtype, dtype_dw, pitch, rows, vocab):
     t = torch()
-    vocab, dim = 700, 64
+    dim = 64
     x, w, tg = make(rows, vocab, dim, dtype, seed=4, ignored=0.3)
     up = t.tensor([-2.5], device="cuda")
     r = reference(x, w, tg, dtype, upstream=-2.5)
@@ -206,9 +211,9 @@ def test_accumulated_weight_gradient_and_upstream(cuda, dtype, dtype_dw, pitch, 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [V.BF16, V.F32])
-@pytest.mark.parametrize("rows", [300, 4])
-def test_one_gradient_alone_has_the_bits_of_both(cuda, dtype, rows):
-    x, w, tg = make(rows, 1500, 96, dtype, seed=6)
+@pytest.mark.parametrize("rows,vocab", [(200, 1500), (4, 1500), (300, 5500)])
+def test_one_gradient_alone_has_the_bits_of_both(cuda, dtype, rows, vocab):
+    x, w, tg = make(rows, vocab, 96, dtype, seed=6)
     _, lse, _ = fwd(x, w, tg, dtype)
     dx, dw, dx1, dw1 = empty(x.shape, dtype), empty(w.shape, dtype), empty(x.shape, dtype), empty(w.shape, dtype)
     bwd(x, w, tg, lse, dtype, dx=dx, dw=dw)
@@ -221,10 +226,10 @@ def test_one_gradient_alone_has_the_bits_of_both(cuda, dtype, rows):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [V.BF16, V.F32])
-@pytest.mark.parametrize("rows", [200, 4])
-def test_padding_that_holds_nan_reaches_nothing(cuda, dtype, rows):
+@pytest.mark.parametrize("rows,vocab", [(200, 600), (4, 600), (200, 4600)])
+def test_padding_that_holds_nan_reaches_nothing(cuda, dtype, rows, vocab):
     t = torch()
-    x, w, tg = make(rows, 600, 64, dtype, seed=7)
+    x, w, tg = make(rows, vocab, 64, dtype, seed=7)
     tg[::2] = IGN
     clean = x.clone()
     for k, v in enumerate((float("nan"), float("inf"), -float("inf"), 3e38)):
@@ -243,9 +248,9 @@ def test_padding_that_holds_nan_reaches_nothing(cuda, dtype, rows):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [V.BF16, V.F32])
-@pytest.mark.parametrize("rows", [50, 3])
-def test_no_counted_row(cuda, dtype, rows):
-    x, w, tg = make(rows, 300, 32, dtype, seed=8)
+@pytest.mark.parametrize("rows,vocab", [(50, 300), (3, 300), (50, 4300)])
+def test_no_counted_row(cuda, dtype, rows, vocab):
+    x, w, tg = make(rows, vocab, 32, dtype, seed=8)
     tg[:] = IGN
     row, lse, loss = fwd(x, w, tg, dtype)
     dx, dw = empty(x.shape, dtype), empty(w.shape, dtype)
@@ -256,10 +261,11 @@ def test_no_counted_row(cuda, dtype, rows):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("bad", [-1, 300, 1 << 40])
-@pytest.mark.parametrize("rows", [60, 4])
-def test_target_outside_the_vocabulary_sets_the_status_and_is_not_counted(cuda, bad, rows):
+@pytest.mark.parametrize("rows,vocab", [(60, 300), (4, 300), (60, 4300)])
+def test_target_outside_the_vocabulary_sets_the_status_and_is_not_counted(cuda, bad, rows, vocab):
     t = torch()
-    x, w, tg = make(rows, 300, 32, V.BF16, seed=9)
+    x, w, tg = make(rows, vocab, 32, V.BF16, seed=9)
+    bad = vocab if bad == 300 else bad
     want = tg.clone()
     want[3] = IGN
     tg[3] = bad
@@ -283,13 +289,14 @@ def test_target_outside_the_vocabulary_sets_the_status_and_is_not_counted(cuda, 
 def test_large_logits(cuda, dtype):
     # logits of several hundred: exp of them overflows, of their differences does not
     run_and_check(*make(90, 700, 64, dtype, seed=10, scale=150.0), dtype)
+    run_and_check(*make(90, 4700, 64, dtype, seed=10, scale=150.0), dtype)
 
 
 @pytest.mark.gpu
 def test_fp32_operands_of_any_magnitude(cuda):
     # 2^100 on one side and 2^-100 on the other leave the logits as they are; the gradients scale
     t = torch()
-    x, w, tg = make(60, 300, 48, V.F32, seed=11)
+    x, w, tg = make(60, 4300, 48, V.F32, seed=11)
     base = run_and_check(x, w, tg, V.F32)
     big = (x * 2.0 ** 100, w * 2.0 ** -100)
     row, lse, loss = fwd(*big, tg, V.F32)
@@ -301,9 +308,10 @@ def test_fp32_operands_of_any_magnitude(cuda):
 
 
 @pytest.mark.gpu
-def test_gradients_against_differences(cuda):
+@pytest.mark.parametrize("rows,vocab", [(40, 200), (4, 200), (40, 4200)])
+def test_gradients_against_differences(cuda, rows, vocab):
     t = torch()
-    x, w, tg = make(40, 200, 32, V.F32, seed=12, ignored=0.2)
+    x, w, tg = make(rows, vocab, 32, V.F32, seed=12, ignored=0.2)
     _, lse, _ = fwd(x, w, tg, V.F32)
     dx, dw = empty(x.shape), empty(w.shape)
     bwd(x, w, tg, lse, V.F32, dx=dx, dw=dw)

@@ -811,7 +811,9 @@ merge_kernel(const float2* __restrict__ parts, int slots, int64_t rows, int64_t 
 #pragma unroll 4
         for (int k = slice; k < slots; k += slices) add(parts[static_cast<int64_t>(k) * rows + row]);
     }
-    for (int d = slices / 2; d > 0; d /= 2)
+    int top = slices;
+    while (top / 2 >= slots) top /= 2;   // the slices beyond the slots have nothing
+    for (int d = top / 2; d > 0; d /= 2)
     {
         part[tid] = make_float2(m, s);
         __syncthreads();
@@ -969,6 +971,11 @@ struct Few
     int dw_f32, dw_beta, dw_vec;
     float* acc;              // [block][rows][ld_acc] sums of dx, or null
     int64_t ld_acc;
+    // small problems
+    float* q;                // [rows][vocab]
+    void* dx;
+    int64_t lddx;
+    unsigned* done;
     int* status;
 };
 
@@ -1034,14 +1041,25 @@ struct Eight
 // The rows in fp32, zero past dim, past the rows and (clear) where a row is not counted; two planes of
 // four columns out of eight, so that a warp's 16-byte reads meet no bank twice.
 template <typename T, int R>
-__device__ __forceinline__ void stage_rows(const Few& p, float* xs, bool clear)
+__device__ __forceinline__ void stage_rows(const Few& p, int r0, float* xs, bool clear)
 {
     const T* x = static_cast<const T*>(p.x);
-    for (int i = threadIdx.x; i < R * p.padded; i += kFewThreads)
+    bool keep[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
     {
-        const int r = i / p.padded, c = i - r * p.padded;
-        const bool in = r < p.rows && c < p.dim && !(clear && !counted(p.targets[r < p.rows ? r : 0], p.ignore, p.vocab));
-        xs[r * p.padded + (c & 4 ? p.padded / 2 : 0) + (c >> 3) * 4 + (c & 3)] = in ? to_f32(x[r * p.ldx + c]) : 0.0f;
+        const int row = r0 + r;
+        keep[r] = row < p.rows && !(clear && !counted(p.targets[row < p.rows ? row : 0], p.ignore, p.vocab));
+    }
+    for (int c = threadIdx.x; c < p.padded; c += kFewThreads)
+    {
+        // all rows' loads before the first store to shared memory, which they could not pass
+        float v[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) v[r] = keep[r] && c < p.dim ? to_f32(x[(r0 + r) * p.ldx + c]) : 0.0f;
+        float* at = xs + (c & 4 ? p.padded / 2 : 0) + (c >> 3) * 4 + (c & 3);
+#pragma unroll
+        for (int r = 0; r < R; ++r) at[r * p.padded] = v[r];
     }
 }
 
@@ -1085,20 +1103,28 @@ __device__ __forceinline__ void own_row(float (&acc)[4][R], int lane, float (&z)
     }
 }
 
-template <typename T, int R, bool VEC>
+// blockIdx.y: which R rows. Q: writes q of the rows instead of their (max, sum) pairs.
+template <typename T, int R, bool VEC, bool Q>
 __global__ void __launch_bounds__(kFewThreads, few_fwd_per_sm(R))
 few_fwd_kernel(const Few p)
 {
     extern __shared__ float few_smem[];
     __shared__ float2 part[kFewWarps][R];
     float* xs = few_smem;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int r0 = static_cast<int>(blockIdx.y) * R, row_ = r0 + lane;
     dep_wait();
     dep_release();
-    stage_rows<T, R>(p, xs, false);
+    if (!Q && p.done != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0)
+    {
+        *p.done = 0;
+    }
+    stage_rows<T, R>(p, r0, xs, false);
     __syncthreads();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t target = lane < p.rows ? p.targets[lane] : -1;
-    const bool valid = lane < p.rows && counted(target, p.ignore, p.vocab);
+    const bool own = lane < R && row_ < p.rows;
+    const int64_t target = own ? p.targets[row_] : -1;
+    const bool valid = own && counted(target, p.ignore, p.vocab);
+    const float lse2 = Q && valid ? p.lse[row_] * kLog2e : 0.0f;
     float m = -INFINITY, s = 0.0f;
     for (int64_t v = (static_cast<int64_t>(blockIdx.x) * kFewWarps + warp) * 4; v < p.vocab;
          v += static_cast<int64_t>(gridDim.x) * kFewWarps * 4)
@@ -1134,87 +1160,51 @@ few_fwd_kernel(const Few p)
         }
         float z[4];
         own_row<R>(acc, lane, z);
-        float top = m;
+        if constexpr (Q)
+        {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-        {
-            if (v + j >= p.vocab) z[j] = -INFINITY;
-            else if (valid && target == v + j) p.target_logit[lane] = z[j];
-            top = fmaxf(top, z[j] * kLog2e);
-        }
-        const float ref = top == -INFINITY ? 0.0f : top;
-        s *= ex2(m - ref);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s += ex2(fmaf(z[j], kLog2e, -ref));
-        m = top;
-    }
-    if (lane < R) part[warp][lane] = make_float2(m, s);
-    __syncthreads();
-    if (threadIdx.x < p.rows)
-    {
-        for (int k = 1; k < kFewWarps; ++k)
-        {
-            const float2 o = part[k][threadIdx.x];
-            const float top = fmaxf(m, o.x);
-            const float ref = top == -INFINITY ? 0.0f : top;
-            s = s * ex2(m - ref) + o.y * ex2(o.x - ref);
-            m = top;
-        }
-        p.parts[static_cast<int64_t>(blockIdx.x) * p.rows + threadIdx.x] = make_float2(m, s);
-    }
-}
-
-// Merges the blocks' pairs of each row (a warp a row, in a fixed order) and takes the mean.
-__global__ void __launch_bounds__(kFewThreads)
-few_merge_kernel(const Few p, int blocks, float* __restrict__ row_loss, float* __restrict__ lse, float* loss)
-{
-    __shared__ float losses[kFewRows];
-    dep_wait();
-    dep_release();
-    const int row = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (row < p.rows)
-    {
-        float m = -INFINITY, s = 0.0f;
-        const auto add = [&](float om, float os) {
-            const float top = fmaxf(m, om);
-            const float ref = top == -INFINITY ? 0.0f : top;
-            s = s * ex2(m - ref) + os * ex2(om - ref);
-            m = top;
-        };
-        for (int b = lane; b < blocks; b += 32)
-        {
-            const float2 o = p.parts[static_cast<int64_t>(b) * p.rows + row];
-            add(o.x, o.y);
-        }
-        for (int d = 16; d > 0; d >>= 1)
-        {
-            const float om = __shfl_down_sync(0xFFFFFFFFu, m, d), os = __shfl_down_sync(0xFFFFFFFFu, s, d);
-            add(om, os);
-        }
-        if (lane == 0)
-        {
-            const float l = (m + log2f(s)) * kLn2;
-            const int64_t t = p.targets[row];
-            if (lse != nullptr) lse[row] = l;
-            losses[row] = counted(t, p.ignore, p.vocab) ? l - p.target_logit[row] : 0.0f;
-            row_loss[row] = losses[row];
-            if (t != p.ignore && !counted(t, p.ignore, p.vocab) && p.status != nullptr) *p.status = VEDA_ERR_OUT_OF_RANGE;
-        }
-    }
-    __syncthreads();
-    if (threadIdx.x == 0 && loss != nullptr)
-    {
-        double sum = 0.0;
-        int n = 0;
-        for (int r = 0; r < p.rows; ++r)
-        {
-            if (counted(p.targets[r], p.ignore, p.vocab))
+            for (int j = 0; j < 4; ++j)
             {
-                sum += static_cast<double>(losses[r]);
-                ++n;
+                if (own && v + j < p.vocab)
+                {
+                    const float q = ex2(fmaf(z[j], kLog2e, -lse2)) - (target == v + j ? 1.0f : 0.0f);
+                    p.q[row_ * p.vocab + v + j] = valid ? q : 0.0f;
+                }
             }
         }
-        *loss = n > 0 ? static_cast<float>(sum / n) : 0.0f;
+        else
+        {
+            float top = m;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+            {
+                if (v + j >= p.vocab) z[j] = -INFINITY;
+                else if (valid && target == v + j) p.target_logit[row_] = z[j];
+                top = fmaxf(top, z[j] * kLog2e);
+            }
+            const float ref = top == -INFINITY ? 0.0f : top;
+            s *= ex2(m - ref);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s += ex2(fmaf(z[j], kLog2e, -ref));
+            m = top;
+        }
+    }
+    if constexpr (!Q)
+    {
+        if (lane < R) part[warp][lane] = make_float2(m, s);
+        __syncthreads();
+        if (warp == 0 && own)
+        {
+            for (int k = 1; k < kFewWarps; ++k)
+            {
+                const float2 o = part[k][lane];
+                const float top = fmaxf(m, o.x);
+                const float ref = top == -INFINITY ? 0.0f : top;
+                s = s * ex2(m - ref) + o.y * ex2(o.x - ref);
+                m = top;
+            }
+            p.parts[static_cast<int64_t>(blockIdx.x) * p.rows + row_] = make_float2(m, s);
+        }
     }
 }
 
@@ -1294,7 +1284,7 @@ few_bwd_kernel(const Few p)
     const int64_t step = static_cast<int64_t>(gridDim.x) * p.chunk;
     int64_t v = static_cast<int64_t>(blockIdx.x) * p.chunk;
     if (v < p.vocab) stage_head<T>(p, stage, v);
-    stage_rows<T, R>(p, xs, true);
+    stage_rows<T, R>(p, 0, xs, true);
     if (threadIdx.x == 0)
     {
         int n = 0;
@@ -1459,6 +1449,148 @@ few_dx_kernel(const Few p, int blocks, T* __restrict__ dx, int64_t lddx)
     }
 }
 
+// ---- small problems: fp32 products on the CUDA cores --------------------------------------------
+// Where rows x vocab x dim is below 2^25 the tensor-core path is all launch latency (the tiny decoder's
+// step: nine launches, 43 us). Such a problem takes four: the pairs and their merge as above, rows in
+// groups of four, then q, kept in fp32, and both products in 32 x 32 tiles.
+// Blocks below gx: tiles of dx = coef q W; the others: of dW = coef q^T x.
+template <typename T>
+__global__ void __launch_bounds__(256)
+small_grads_kernel(const Few p, int gx, int tiles_d)
+{
+    // 128 terms at a time, all their loads under way at once: the time is the latency of these rounds
+    constexpr int K = 128;
+    __shared__ __align__(16) float a[K][36], b[K][36];   // [k][m], [k][n]
+    __shared__ int counts[8];
+    __shared__ bool use[1024];   // rows that are counted
+    dep_wait();
+    dep_release();
+    const int tid = static_cast<int>(threadIdx.x);
+    const bool dw = static_cast<int>(blockIdx.x) >= gx;
+    const int tile = static_cast<int>(blockIdx.x) - (dw ? gx : 0);
+    const int m0 = tile / tiles_d * 32, d0 = tile % tiles_d * 32;
+    const int terms = dw ? p.rows : static_cast<int>(p.vocab), ms = dw ? static_cast<int>(p.vocab) : p.rows;
+    const T* x = static_cast<const T*>(p.x);
+    const T* w = static_cast<const T*>(p.w);
+    const int tx = tid & 31, ty = tid >> 5;   // column; rows 4 ty ..
+    const int vocab = static_cast<int>(p.vocab);
+    // a chunk's operands, into registers: the next chunk's loads run under this one's products
+    float la[K / 8], lb[K / 8];
+    const auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < K / 8; ++i)
+        {
+            const int k = k0 + ty + 8 * i;
+            if (dw)
+            {
+                // q as it lies: k = row, m = vocabulary
+                la[i] = k < terms && m0 + tx < ms ? p.q[k * vocab + m0 + tx] : 0.0f;
+                lb[i] = k < terms && d0 + tx < p.dim ? to_f32(x[k * p.ldx + d0 + tx]) : 0.0f;
+            }
+            else
+            {
+                // 32 rows of q, 128 columns of each
+                const int m = m0 + ty + 8 * (i >> 2), c = k0 + tx + 32 * (i & 3);
+                la[i] = m < ms && c < terms ? p.q[m * vocab + c] : 0.0f;
+                lb[i] = k < terms && d0 + tx < p.dim ? to_f32(w[k * p.ldw + d0 + tx]) : 0.0f;
+            }
+        }
+    };
+    fetch(0);
+    int n = 0, bad = 0;
+    for (int i = tid; i < p.rows; i += 256)
+    {
+        const int64_t t = p.targets[i];
+        use[i] = counted(t, p.ignore, p.vocab);
+        if (use[i]) ++n;
+        else if (t != p.ignore) ++bad;
+    }
+    n = __reduce_add_sync(0xFFFFFFFFu, n);
+    if (blockIdx.x == 0 && __any_sync(0xFFFFFFFFu, bad != 0) && (tid & 31) == 0 && p.status != nullptr)
+    {
+        *p.status = VEDA_ERR_OUT_OF_RANGE;
+    }
+    if ((tid & 31) == 0) counts[tid >> 5] = n;
+    __syncthreads();
+    n = 0;
+    for (int k = 0; k < 8; ++k) n += counts[k];
+    const float coef = n > 0 ? (p.upstream != nullptr ? *p.upstream : 1.0f) / static_cast<float>(n) : 0.0f;
+
+    // four slices of the terms, 64 threads each, a thread 4 x 4 of the tile
+    const int slice = tid >> 6, om = (tid >> 3 & 7) * 4, on = (tid & 7) * 4;
+    float acc[4][4] = {};
+    for (int k0 = 0; k0 < terms; k0 += K)
+    {
+#pragma unroll
+        for (int i = 0; i < K / 8; ++i)
+        {
+            const int k = k0 + ty + 8 * i;
+            if (dw)
+            {
+                a[ty + 8 * i][tx] = la[i];
+                // what an ignored row holds (NaN included) meets q = 0 as 0
+                b[ty + 8 * i][tx] = k < terms && use[k] ? lb[i] : 0.0f;
+            }
+            else
+            {
+                a[tx + 32 * (i & 3)][ty + 8 * (i >> 2)] = la[i];
+                b[ty + 8 * i][tx] = lb[i];
+            }
+        }
+        __syncthreads();
+        if (k0 + K < terms) fetch(k0 + K);
+#pragma unroll 8
+        for (int k = slice * (K / 4); k < (slice + 1) * (K / 4); ++k)
+        {
+            const float4 u = *reinterpret_cast<const float4*>(&a[k][om]);
+            const float4 v = *reinterpret_cast<const float4*>(&b[k][on]);
+            const float um[4] = {u.x, u.y, u.z, u.w}, vn[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+#pragma unroll
+                for (int l = 0; l < 4; ++l) acc[i][l] = fmaf(um[i], vn[l], acc[i][l]);
+            }
+        }
+        __syncthreads();
+    }
+    // the slices' sums meet in shared memory, added in order
+    float* const sums = &a[0][0];   // [slice][32][32]
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+#pragma unroll
+        for (int l = 0; l < 4; ++l) sums[(slice * 32 + om + i) * 32 + on + l] = acc[i][l];
+    }
+    __syncthreads();
+    if (d0 + tx >= p.dim)
+    {
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        const int y = ty + 8 * i, m = m0 + y;
+        if (m >= ms) continue;
+        const float* at_sum = sums + y * 32 + tx;
+        const float v = (((at_sum[0] + at_sum[1024]) + at_sum[2048]) + at_sum[3072]) * coef;
+        if (!dw)
+        {
+            static_cast<T*>(p.dx)[m * p.lddx + d0 + tx] = from_f32<T>(v);
+        }
+        else if (p.dw_f32)
+        {
+            float* at = static_cast<float*>(p.dw) + m * p.lddw + d0 + tx;
+            *at = p.dw_beta ? *at + v : v;
+        }
+        else
+        {
+            bf16* at = static_cast<bf16*>(p.dw) + m * p.lddw + d0 + tx;
+            *at = __float2bfloat16_rn(p.dw_beta ? __bfloat162float(*at) + v : v);
+        }
+    }
+}
+
 // ---- host ------------------------------------------------------------------------------------
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
@@ -1499,6 +1631,12 @@ int choose_strip(int num_m, int num_n, int clusters)
 // the tensor tiles take 98 / 288 for 9.
 bool is_few(int64_t rows, int64_t dim) { return rows <= kFewRows && dim <= 2048; }
 
+// Problems whose products the CUDA cores finish within the latency of the tensor-core path's launches.
+bool is_small(int64_t rows, int64_t vocab, int64_t dim)
+{
+    return rows <= 1024 && vocab <= 4096 && dim <= 1024 && rows * vocab * dim <= (1 << 25);
+}
+
 Layout layout(int64_t rows, int64_t vocab, int64_t dim, bool pack_x, bool pack_w, int dtype, bool backward)
 {
     Layout l{};
@@ -1508,12 +1646,14 @@ Layout layout(int64_t rows, int64_t vocab, int64_t dim, bool pack_x, bool pack_w
         at += static_cast<size_t>(round_up(bytes, 256));
         return here;
     };
-    if (is_few(rows, dim))
+    if (is_few(rows, dim) || is_small(rows, vocab, dim))
     {
+        l.done = take(4);
         l.parts = take(kFewBlocks * rows * 8);
         l.target_logit = take(rows * 4);
         l.ld_acc = round_up(dim, 4);
-        l.acc = take(backward ? kFewBlocks * rows * l.ld_acc * 4 : 0);
+        l.acc = take(backward && is_few(rows, dim) ? kFewBlocks * rows * l.ld_acc * 4 : 0);
+        l.q = take(backward && !is_few(rows, dim) ? rows * vocab * 4 : 0);
         l.total = at;
         return l;
     }
@@ -1733,6 +1873,8 @@ Few few_params(const Call& c, const int64_t* targets, int64_t ignore, int* statu
     p.target_logit = reinterpret_cast<float*>(c.ws + c.l.target_logit);
     p.acc = reinterpret_cast<float*>(c.ws + c.l.acc);
     p.ld_acc = c.l.ld_acc;
+    p.q = reinterpret_cast<float*>(c.ws + c.l.q);
+    p.done = reinterpret_cast<unsigned*>(c.ws + c.l.done);
     p.status = status;
     return p;
 }
@@ -1750,23 +1892,26 @@ bool allow_smem(K kernel, int bytes)
     return ok;
 }
 
-// Blocks: what an SM holds of them on every SM, or fewer where there are fewer pieces of the vocabulary.
-int few_blocks(int64_t vocab, int piece, int per_sm)
+// Blocks of a row group: what the SMs hold at once over all groups, or fewer where there are fewer pieces of
+// the vocabulary.
+int few_blocks(int64_t vocab, int piece, int per_sm, int groups)
 {
-    return static_cast<int>(std::min<int64_t>({(vocab + piece - 1) / piece, int64_t{per_sm} * sm_count(), kFewBlocks}));
+    const int64_t room = std::max(1, per_sm * sm_count() / groups);
+    return static_cast<int>(std::min<int64_t>({(vocab + piece - 1) / piece, room, kFewBlocks}));
 }
 
-template <typename T, int R>
+template <typename T, int R, bool Q>
 int launch_few_fwd(const Few& p, int* blocks, cudaStream_t s)
 {
-    *blocks = few_blocks(p.vocab, 4 * kFewWarps, few_fwd_per_sm(R));
+    const int groups = (p.rows + R - 1) / R;
+    *blocks = few_blocks(p.vocab, 4 * kFewWarps, few_fwd_per_sm(R), groups);
     const int smem = R * p.padded * 4;
-    const auto kernel = p.vec ? few_fwd_kernel<T, R, true> : few_fwd_kernel<T, R, false>;
+    const auto kernel = p.vec ? few_fwd_kernel<T, R, true, Q> : few_fwd_kernel<T, R, false, Q>;
     if (!allow_smem(kernel, smem))
     {
-        return fail(VEDA_ERR_CUDA, "veda_linear_cross_entropy_fwd: shared memory");
+        return fail(VEDA_ERR_CUDA, "veda_linear_cross_entropy: shared memory");
     }
-    return launch("veda_linear_cross_entropy_fwd", kernel, dim3(*blocks), dim3(kFewThreads), smem, s, p);
+    return launch("veda_linear_cross_entropy", kernel, dim3(*blocks, groups), dim3(kFewThreads), smem, s, p);
 }
 
 template <typename T, int R>
@@ -1776,7 +1921,7 @@ int launch_few_bwd(Few p, int* blocks, cudaStream_t s)
     const int room = 220 * 1024 / kFewBwdPerSm - 2048 - (R * p.padded + 32 * R) * 4;
     p.chunk = 32;
     while (p.chunk > 4 && 2 * p.chunk * p.padded * static_cast<int>(sizeof(T)) > room) p.chunk /= 2;
-    *blocks = few_blocks(p.vocab, p.chunk, kFewBwdPerSm);
+    *blocks = few_blocks(p.vocab, p.chunk, kFewBwdPerSm, 1);
     const int smem = (R * p.padded + 32 * R) * 4 + 2 * p.chunk * p.padded * static_cast<int>(sizeof(T));
     if (!allow_smem(few_bwd_kernel<T, R>, smem))
     {
@@ -1785,18 +1930,52 @@ int launch_few_bwd(Few p, int* blocks, cudaStream_t s)
     return launch("veda_linear_cross_entropy_bwd", few_bwd_kernel<T, R>, dim3(*blocks), dim3(kFewThreads), smem, s, p);
 }
 
+int launch_merge(const float2* parts, int slots, int64_t rows, int64_t vocab, const int64_t* targets, int64_t ignore,
+                 const float* target_logit, float* row_loss, float* lse, float* loss, unsigned* done, int* status,
+                 cudaStream_t s)
+{
+    // 32 rows a block reads whole lines of pairs; fewer where the rows would not fill the GPU's SMs
+    int width = 32;
+    while (width > 1 && (rows + width - 1) / width < sm_count()) width /= 2;
+    return launch("veda_linear_cross_entropy_fwd (merge)", merge_kernel,
+                  dim3(static_cast<unsigned>((rows + width - 1) / width)), dim3(256), 0, s, parts, slots, rows, vocab,
+                  width, targets, ignore, target_logit, row_loss, lse, loss, done, status);
+}
+
 template <typename T>
 int few_fwd(const Call& c, const int64_t* targets, int64_t ignore, float* row_loss, float* lse, float* loss, int* status,
             cudaStream_t s)
 {
     const Few p = few_params(c, targets, ignore, status);
     int blocks = 0;
-    int rc = p.rows == 1   ? launch_few_fwd<T, 1>(p, &blocks, s)
-             : p.rows == 2 ? launch_few_fwd<T, 2>(p, &blocks, s)
-                           : launch_few_fwd<T, 4>(p, &blocks, s);
+    const int rc = p.rows == 1   ? launch_few_fwd<T, 1, false>(p, &blocks, s)
+                   : p.rows == 2 ? launch_few_fwd<T, 2, false>(p, &blocks, s)
+                                 : launch_few_fwd<T, 4, false>(p, &blocks, s);
     if (rc != VEDA_OK) return rc;
-    return launch("veda_linear_cross_entropy_fwd (merge)", few_merge_kernel, dim3(1), dim3(kFewThreads), 0, s, p, blocks,
-                  row_loss, lse, loss);
+    return launch_merge(p.parts, blocks, c.rows, c.vocab, targets, ignore, p.target_logit, row_loss, lse, loss, p.done,
+                        status, s);
+}
+
+template <typename T>
+int small_bwd(const Call& c, const int64_t* targets, int64_t ignore, const float* lse, const float* upstream, void* dx,
+              int64_t lddx, void* dw, int64_t lddw, int dtype_dw, bool beta, int* status, cudaStream_t s)
+{
+    Few p = few_params(c, targets, ignore, status);
+    p.lse = lse;
+    p.upstream = upstream;
+    p.dx = dx;
+    p.lddx = lddx;
+    p.dw = dw;
+    p.lddw = lddw;
+    p.dw_f32 = dtype_dw == VEDA_F32;
+    p.dw_beta = beta;
+    int blocks = 0;
+    const int rc = launch_few_fwd<T, 4, true>(p, &blocks, s);
+    if (rc != VEDA_OK) return rc;
+    const int tiles_d = (p.dim + 31) / 32;
+    const int gx = dx != nullptr ? (p.rows + 31) / 32 * tiles_d : 0;
+    const int gw = dw != nullptr ? static_cast<int>((c.vocab + 31) / 32) * tiles_d : 0;
+    return launch("veda_linear_cross_entropy_bwd", small_grads_kernel<T>, dim3(gx + gw), dim3(256), 0, s, p, gx, tiles_d);
 }
 
 template <typename T>
@@ -1863,7 +2042,7 @@ extern "C" int veda_linear_cross_entropy_fwd(const void* x, int64_t ldx, const v
     lce::Call c{x, w, ldx, ldw, rows, vocab, dim, dtype};
     int rc = lce::check(c, workspace, workspace_bytes, false, "veda_linear_cross_entropy_fwd");
     if (rc != VEDA_OK) return rc;
-    if (lce::is_few(rows, dim))
+    if (lce::is_few(rows, dim) || lce::is_small(rows, vocab, dim))
     {
         return dtype == VEDA_BF16
                    ? lce::few_fwd<bf16>(c, targets, ignore_index, row_loss, lse, loss, status, stream)
@@ -1890,13 +2069,8 @@ extern "C" int veda_linear_cross_entropy_fwd(const void* x, int64_t ldx, const v
     rc = split ? pair::launch_pair<lce::StatsWork, 4, true>("veda_linear_cross_entropy_fwd", p, grid, stream)
                : pair::launch_pair<lce::StatsWork, 4, false>("veda_linear_cross_entropy_fwd", p, grid, stream);
     if (rc != VEDA_OK) return rc;
-    // 32 rows a block reads whole lines of pairs; fewer where the rows would not fill the GPU's SMs
-    int width = 32;
-    while (width > 1 && (rows + width - 1) / width < sm_count()) width /= 2;
-    return launch("veda_linear_cross_entropy_fwd (merge)", lce::merge_kernel,
-                  dim3(static_cast<unsigned>((rows + width - 1) / width)), dim3(256), 0, stream,
-                  static_cast<const float2*>(p.parts), c.l.slots, rows, vocab, width, targets, ignore_index,
-                  static_cast<const float*>(p.target_logit), row_loss, lse, loss, p.done, status);
+    return lce::launch_merge(p.parts, c.l.slots, rows, vocab, targets, ignore_index, p.target_logit, row_loss, lse, loss,
+                             p.done, status, stream);
 }
 
 extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
@@ -1937,6 +2111,13 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
                                                        dtype_dw, beta_dw != 0.0f, status, stream)
                                   : lce::few_bwd<float>(c, targets, ignore_index, lse, upstream, dx, lddx, dw, lddw,
                                                         dtype_dw, beta_dw != 0.0f, status, stream);
+    }
+    if (lce::is_small(rows, vocab, dim))
+    {
+        return dtype == VEDA_BF16 ? lce::small_bwd<bf16>(c, targets, ignore_index, lse, upstream, dx, lddx, dw, lddw,
+                                                         dtype_dw, beta_dw != 0.0f, status, stream)
+                                  : lce::small_bwd<float>(c, targets, ignore_index, lse, upstream, dx, lddx, dw, lddw,
+                                                          dtype_dw, beta_dw != 0.0f, status, stream);
     }
     const bool split = dtype == VEDA_F32;
     const int clusters = std::min(lce::kMaxClusters, split ? pair::clusters_available<lce::GradWork, 8, true>()
