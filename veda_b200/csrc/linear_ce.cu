@@ -132,10 +132,11 @@ __device__ __forceinline__ int counted_target(const Params& p, int row)
 }
 
 // ---- forward: running (max, sum) per row over strips of logit tiles ---------------------------
+template <int TN_>
 struct StatsWork
 {
     using Params = lce::Params;
-    static constexpr int TN = pair::kTile;
+    static constexpr int TN = TN_;
     struct Tile
     {
         bool skip, first, last, a_mn, b_mn;
@@ -164,7 +165,7 @@ struct StatsWork
         t.last = sub == strip - 1 || t.nb == p.num_n - 1;
         t.kbs = (p.dim + pair::kBK - 1) / pair::kBK;
         t.a_mn = t.b_mn = false;
-        t.idesc = pair::idesc(p.is_bf16 != 0, false, false);
+        t.idesc = pair::idesc<TN>(p.is_bf16 != 0, false, false);
         return true;
     }
 
@@ -172,7 +173,7 @@ struct StatsWork
                                                     pair::Piece& b)
     {
         a = {&p.x, 0, t.mb * pair::kTile + rank * 128, 0};
-        b = {&p.w, 0, p.v0 + t.nb * pair::kTile + rank * 128, 0};
+        b = {&p.w, 0, p.v0 + t.nb * TN + rank * (TN / 2), 0};
     }
     static __device__ __forceinline__ void ready(const Params&, const Tile&, volatile int*) {}
     static __device__ __forceinline__ void after(const Params&, const Tile&, int) {}
@@ -206,7 +207,7 @@ struct StatsWork
             return;
         }
         const int row = t.mb * pair::kTile + row0 + lane;
-        const int first = p.v0 + t.nb * pair::kTile + col0;
+        const int first = p.v0 + t.nb * TN + col0;
         const float zs = p.split ? p.scalars->z : 1.0f;
 #pragma unroll 1
         for (int c = 0; c < COLS; c += 32)
@@ -259,18 +260,20 @@ struct StatsWork
         }
         if (t.last && row < p.rows)
         {
-            const int halves = pair::kTile / COLS;
+            const int halves = TN / COLS;
             p.parts[static_cast<int64_t>(t.slot * halves + col0 / COLS) * p.rows + row] = make_float2(s.m, s.s);
         }
     }
 };
 
 // ---- backward: the next piece of q beside the current piece's two products --------------------
+enum GradKind { kDw, kDx, kQ };
+
+template <int TN_>
 struct GradWork
 {
     using Params = lce::Params;
-    static constexpr int TN = pair::kTile;
-    enum Kind { kDw, kDx, kQ };
+    static constexpr int TN = TN_;
     struct Tile
     {
         bool skip, a_mn, b_mn;
@@ -298,7 +301,7 @@ struct GradWork
             t.mb = p.by_d.div(u, t.nb);
             t.kbs = (p.rows + pair::kBK - 1) / pair::kBK;
             t.a_mn = t.b_mn = true;
-            t.idesc = pair::idesc(bf, true, true);
+            t.idesc = pair::idesc<TN>(bf, true, true);
             return true;
         }
         u = p.shares.first[kDx][cid] + (u - end);
@@ -311,7 +314,7 @@ struct GradWork
             t.kbs = min(p.dx_kbs, (p.gcols + pair::kBK - 1) / pair::kBK - t.split * p.dx_kbs);
             t.a_mn = false;
             t.b_mn = true;
-            t.idesc = pair::idesc(bf, false, true);
+            t.idesc = pair::idesc<TN>(bf, false, true);
             return true;
         }
         u = p.shares.first[kQ][cid] + (u - end);
@@ -324,14 +327,14 @@ struct GradWork
         t.nb = p.by_m.div(u, t.mb);
         t.kbs = (p.dim + pair::kBK - 1) / pair::kBK;
         t.a_mn = t.b_mn = false;
-        t.idesc = pair::idesc(bf, false, false);
+        t.idesc = pair::idesc<TN>(bf, false, false);
         return true;
     }
 
     static __device__ __forceinline__ void operands(const Params& p, const Tile& t, int rank, pair::Piece& a,
                                                     pair::Piece& b)
     {
-        const int m = t.mb * pair::kTile + rank * 128, n = t.nb * pair::kTile + rank * 128;
+        const int m = t.mb * pair::kTile + rank * 128, n = t.nb * TN + rank * (TN / 2);
         if (t.kind == kDw)
         {
             a = {&p.q_mn, m, 0, 0};
@@ -402,7 +405,7 @@ struct GradWork
 #pragma unroll 1
         for (int c = 0; c < COLS; c += 64)
         {
-            const int col = t.nb * pair::kTile + col0 + c;   // within the piece
+            const int col = t.nb * TN + col0 + c;   // within the piece
             const int left = p.vocab - p.v0 - col;
             uint32_t hi[32], lo[32];
 #pragma unroll
@@ -488,7 +491,7 @@ struct GradWork
 #pragma unroll 1
         for (int c = 0; c < COLS; c += step)
         {
-            const int col = t.nb * pair::kTile + col0 + c;
+            const int col = t.nb * TN + col0 + c;
             if (col >= p.dim)
             {
                 break;
@@ -867,10 +870,11 @@ merge_kernel(const float2* __restrict__ parts, int slots, int64_t rows, int64_t 
     }
 }
 
-// dx = coef x the fp32 sums. One set of them: eight columns a thread, where rows allow it.
+// dx = coef x the fp32 sums, those of the splits added in their order: eight columns a thread, where
+// rows allow it.
 template <typename T>
 __global__ void __launch_bounds__(256)
-finish_dx_kernel(const float* __restrict__ acc, int64_t lda, T* __restrict__ dx, int64_t lddx, int64_t rows,
+finish_dx_kernel(const float* __restrict__ acc, int64_t lda, int splits, T* __restrict__ dx, int64_t lddx, int64_t rows,
                  int64_t dim, bool vec, const Scalars* __restrict__ scalars)
 {
     dep_wait();
@@ -890,6 +894,13 @@ finish_dx_kernel(const float* __restrict__ acc, int64_t lda, T* __restrict__ dx,
             {
                 float a[4];
                 load16(from + k, a);
+                for (int q = 1; q < splits; ++q)
+                {
+                    float more[4];
+                    load16(from + q * rows * lda + k, more);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) a[i] += more[i];
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[k + i] = a[i] * unit * coef;
             }
@@ -905,12 +916,17 @@ finish_dx_kernel(const float* __restrict__ acc, int64_t lda, T* __restrict__ dx,
         }
         else
         {
-            for (int k = 0; k < 8 && c + k < dim; ++k) to[k] = from_f32<T>(from[k] * unit * coef);
+            for (int k = 0; k < 8 && c + k < dim; ++k)
+            {
+                float a = from[k];
+                for (int q = 1; q < splits; ++q) a += from[q * rows * lda + k];
+                to[k] = from_f32<T>(a * unit * coef);
+            }
         }
     }
 }
 
-// The same of several sets, added in a fixed order: 32 columns of a row per block, a warp an eighth.
+// The same for a small dx of many splits: 32 columns of a row per block, a warp an eighth of the splits.
 template <typename T>
 __global__ void __launch_bounds__(256)
 finish_splits_kernel(const float* __restrict__ acc, int64_t lda, int splits, T* __restrict__ dx, int64_t lddx, int64_t rows,
@@ -1626,6 +1642,9 @@ int choose_strip(int num_m, int num_n, int clusters)
     return best;
 }
 
+// Columns of a tile: split products fold their accumulators under the next ones with narrow tiles only.
+int tile_width(int dtype) { return dtype == VEDA_F32 ? 128 : 256; }
+
 // Up to four rows of at most 2048 columns (a thread holds eight) go past the tensor cores. Against
 // 151936 x 1024, forward / backward: 1 row 51 / 143 us, 2 rows 52 / 167, 4 rows 66 / 231, 8 rows 101 / 359;
 // the tensor tiles take 98 / 288 for 9.
@@ -1664,7 +1683,7 @@ Layout layout(int64_t rows, int64_t vocab, int64_t dim, bool pack_x, bool pack_w
     l.part = take(2 * kMaxBlocks * 4);
     l.px = take(pack_x ? l.planes * rows * l.ldp * 2 : 0);
     l.pw = take(pack_w ? l.planes * vocab * l.ldp * 2 : 0);
-    const int num_n = static_cast<int>((vocab + 255) / 256), num_m = static_cast<int>((rows + 255) / 256);
+    const int tn = tile_width(dtype), num_n = static_cast<int>((vocab + tn - 1) / tn), num_m = static_cast<int>((rows + 255) / 256);
     if (!backward)
     {
         // at most 74 clusters on a B200; fewer (reserved SMs) only change which strip is best
@@ -1684,7 +1703,7 @@ Layout layout(int64_t rows, int64_t vocab, int64_t dim, bool pack_x, bool pack_w
         // Where dx has fewer tiles than the GPU has CTA pairs, its sums over a piece are cut into splits of
         // at least 8 k-blocks, each kept apart: one cluster summing 100000 columns for 16 rows of 768 took
         // 430 us by itself.
-        const int64_t tiles = num_m * ((dim + 255) / 256), kbs = (std::min(l.piece, vocab) + 63) / 64;
+        const int64_t tiles = num_m * ((dim + tn - 1) / tn), kbs = (std::min(l.piece, vocab) + 63) / 64;
         const int64_t want = std::min((74 + tiles - 1) / tiles, (kbs + 7) / 8);
         l.splits = static_cast<int>((kbs + (kbs + want - 1) / want - 1) / ((kbs + want - 1) / want));
         l.ld_acc = round_up(dim, 4);
@@ -1811,8 +1830,8 @@ int prepare(const Call& c, const int64_t* targets, int64_t ignore, const float* 
         }
     }
     const bool bf = c.dtype == VEDA_BF16;
-    if (!pair::make_map3(&p.x, px, 2, bf, c.dim, c.rows, c.l.planes, ldx, c.rows * ldx, 64, 128) ||
-        !pair::make_map3(&p.w, pw, 2, bf, c.dim, c.vocab, c.l.planes, ldw, c.vocab * ldw, 64, 128) ||
+    if (!pair::make_map3(&p.x, px, 2, bf, c.dim, c.rows, c.l.planes, ldx, c.rows * ldx, 64, bf ? 128 : 64) ||
+        !pair::make_map3(&p.w, pw, 2, bf, c.dim, c.vocab, c.l.planes, ldw, c.vocab * ldw, 64, bf ? 128 : 64) ||
         (c.backward &&
          (!pair::make_map3(&p.x_mn, px, 2, bf, c.dim, c.rows, c.l.planes, ldx, c.rows * ldx, 64, 64) ||
           !pair::make_map3(&p.w_mn, pw, 2, bf, c.dim, c.vocab, c.l.planes, ldw, c.vocab * ldw, 64, 64))))
@@ -1825,7 +1844,8 @@ int prepare(const Call& c, const int64_t* targets, int64_t ignore, const float* 
     p.split = !bf;
     p.is_bf16 = bf;
     p.num_m = static_cast<int>((c.rows + 255) / 256);
-    p.num_d = static_cast<int>((c.dim + 255) / 256);
+    const int tn = tile_width(c.dtype);
+    p.num_d = static_cast<int>((c.dim + tn - 1) / tn);
     p.by_m = pair::Divisor(static_cast<uint32_t>(p.num_m));
     p.by_d = pair::Divisor(static_cast<uint32_t>(p.num_d));
     p.scalars = c.scalars();
@@ -2049,8 +2069,8 @@ extern "C" int veda_linear_cross_entropy_fwd(const void* x, int64_t ldx, const v
                    : lce::few_fwd<float>(c, targets, ignore_index, row_loss, lse, loss, status, stream);
     }
     const bool split = dtype == VEDA_F32;
-    const int clusters = split ? pair::clusters_available<lce::StatsWork, 4, true>()
-                               : pair::clusters_available<lce::StatsWork, 4, false>();
+    const int clusters = split ? pair::clusters_available<lce::StatsWork<128>, 4, true>()
+                               : pair::clusters_available<lce::StatsWork<256>, 4, false>();
     if (clusters < 1)
     {
         return fail(VEDA_ERR_UNSUPPORTED, "veda_linear_cross_entropy_fwd: no CTA pair fits on this device");
@@ -2058,7 +2078,7 @@ extern "C" int veda_linear_cross_entropy_fwd(const void* x, int64_t ldx, const v
     lce::Params p{};
     rc = lce::prepare(c, targets, ignore_index, nullptr, nullptr, false, p, stream);
     if (rc != VEDA_OK) return rc;
-    p.num_n = static_cast<int>((vocab + 255) / 256);
+    p.num_n = static_cast<int>((vocab + lce::tile_width(dtype) - 1) / lce::tile_width(dtype));
     while ((1 << p.strip_log2) < c.l.strip) ++p.strip_log2;
     p.parts = reinterpret_cast<float2*>(c.ws + c.l.parts);
     p.target_logit = reinterpret_cast<float*>(c.ws + c.l.target_logit);
@@ -2066,8 +2086,8 @@ extern "C" int veda_linear_cross_entropy_fwd(const void* x, int64_t ldx, const v
     const int64_t units = static_cast<int64_t>(c.l.slots) * p.num_m;
     VEDA_REQUIRE(units <= lce::kLimit, "too many tiles");
     const int grid = static_cast<int>(std::min<int64_t>(units, clusters));
-    rc = split ? pair::launch_pair<lce::StatsWork, 4, true>("veda_linear_cross_entropy_fwd", p, grid, stream)
-               : pair::launch_pair<lce::StatsWork, 4, false>("veda_linear_cross_entropy_fwd", p, grid, stream);
+    rc = split ? pair::launch_pair<lce::StatsWork<128>, 4, true>("veda_linear_cross_entropy_fwd", p, grid, stream)
+               : pair::launch_pair<lce::StatsWork<256>, 4, false>("veda_linear_cross_entropy_fwd", p, grid, stream);
     if (rc != VEDA_OK) return rc;
     return lce::launch_merge(p.parts, c.l.slots, rows, vocab, targets, ignore_index, p.target_logit, row_loss, lse, loss,
                              p.done, status, stream);
@@ -2120,8 +2140,8 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
                                                           dtype_dw, beta_dw != 0.0f, status, stream);
     }
     const bool split = dtype == VEDA_F32;
-    const int clusters = std::min(lce::kMaxClusters, split ? pair::clusters_available<lce::GradWork, 8, true>()
-                                                           : pair::clusters_available<lce::GradWork, 8, false>());
+    const int clusters = std::min(lce::kMaxClusters, split ? pair::clusters_available<lce::GradWork<128>, 8, true>()
+                                                           : pair::clusters_available<lce::GradWork<256>, 8, false>());
     if (clusters < 1)
     {
         return fail(VEDA_ERR_UNSUPPORTED, "veda_linear_cross_entropy_bwd: no CTA pair fits on this device");
@@ -2136,7 +2156,7 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
     for (int b = 0; b < 2; ++b)
     {
         char* q = c.ws + c.l.q + static_cast<size_t>(b) * c.l.planes * plane * 2;
-        ok = ok && pair::make_map3(&q_load[b], q, 2, bf, piece, rows, c.l.planes, piece, plane, 64, 128) &&
+        ok = ok && pair::make_map3(&q_load[b], q, 2, bf, piece, rows, c.l.planes, piece, plane, 64, bf ? 128 : 64) &&
              pair::make_map3(&q_mn[b], q, 2, bf, piece, rows, c.l.planes, piece, plane, 64, 64) &&
              pair::make_map3(&q_store[b], q, 2, bf, piece, rows, c.l.planes, piece, plane, 64, 32);
     }
@@ -2170,7 +2190,8 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
         if (k < pieces)
         {
             p.v0 = static_cast<int>(k * piece);
-            tiles[lce::GradWork::kQ] = (std::min(piece, vocab - k * piece) + 255) / 256 * p.num_m;
+            // q is written up to the next multiple of 256 columns, zero past the vocabulary
+            tiles[lce::kQ] = (std::min(piece, vocab - k * piece) + 255) / 256 * (256 / lce::tile_width(dtype)) * p.num_m;
             p.q_out = q_store[k & 1];
         }
         if (k > 0)
@@ -2179,13 +2200,13 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
             p.gcols = static_cast<int>(std::min(piece, vocab - (k - 1) * piece));
             p.q_in = q_load[(k - 1) & 1];
             p.q_mn = q_mn[(k - 1) & 1];
-            tiles[lce::GradWork::kDw] = dw != nullptr ? static_cast<int64_t>((p.gcols + 255) / 256) * p.num_d : 0;
+            tiles[lce::kDw] = dw != nullptr ? static_cast<int64_t>((p.gcols + 255) / 256) * p.num_d : 0;
             // a short last piece may fill fewer splits; all were stored with the first
             const int kbs = (p.gcols + pair::kBK - 1) / pair::kBK;
             p.dx_tiles = p.num_m * p.num_d;
             p.by_dx = pair::Divisor(static_cast<uint32_t>(p.dx_tiles));
             p.dx_kbs = (kbs + c.l.splits - 1) / c.l.splits;
-            tiles[lce::GradWork::kDx] =
+            tiles[lce::kDx] =
                 dx != nullptr ? static_cast<int64_t>((kbs + p.dx_kbs - 1) / p.dx_kbs) * p.dx_tiles : 0;
             p.dx_add = k > 1;
         }
@@ -2195,8 +2216,8 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
         // k-blocks a tile, and what its epilogue adds
         const int64_t cost[3] = {(rows + 63) / 64 + 4, p.dx_kbs + 2, (dim + 63) / 64 + 2};
         lce::share(tiles, cost, grid, p.shares);
-        rc = split ? pair::launch_pair<lce::GradWork, 8, true>("veda_linear_cross_entropy_bwd", p, grid, stream)
-                   : pair::launch_pair<lce::GradWork, 8, false>("veda_linear_cross_entropy_bwd", p, grid, stream);
+        rc = split ? pair::launch_pair<lce::GradWork<128>, 8, true>("veda_linear_cross_entropy_bwd", p, grid, stream)
+                   : pair::launch_pair<lce::GradWork<256>, 8, false>("veda_linear_cross_entropy_bwd", p, grid, stream);
         if (rc != VEDA_OK) return rc;
     }
     if (dx == nullptr)
@@ -2205,7 +2226,7 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
     }
     const lce::Scalars* scalars = c.scalars();
     const auto finish = [&](auto* out, auto one, auto several) {
-        if (c.l.splits > 1)
+        if (c.l.splits > 8 && rows * dim < 65536)
         {
             return launch("veda_linear_cross_entropy_bwd (dx)", several,
                           dim3(static_cast<unsigned>((dim + 31) / 32), static_cast<unsigned>(rows)), dim3(256), 0, stream,
@@ -2215,7 +2236,7 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
         const bool vec = aligned16(dx) && lddx * es % 16 == 0;
         const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((rows * ((dim + 7) / 8) + 255) / 256, 8ll * sm_count()));
         return launch("veda_linear_cross_entropy_bwd (dx)", one, dim3(blocks), dim3(256), 0, stream,
-                      static_cast<const float*>(acc), c.l.ld_acc, out, lddx, rows, dim, vec, scalars);
+                      static_cast<const float*>(acc), c.l.ld_acc, c.l.splits, out, lddx, rows, dim, vec, scalars);
     };
     return bf ? finish(static_cast<bf16*>(dx), lce::finish_dx_kernel<bf16>, lce::finish_splits_kernel<bf16>)
               : finish(static_cast<float*>(dx), lce::finish_dx_kernel<float>, lce::finish_splits_kernel<float>);
