@@ -307,6 +307,76 @@ def test_muon_clip_and_scale(cuda, norm, factor):
     check_muon(master, momentum, lowp, want, 1e-2, 1.7)
 
 
+# One matrix cut among the blocks of a cluster: 2 blocks with 1 column in the last, 9 of them (more than
+# the portable 8), 16, the last one short, a smaller side of 1, of fewer rows than blocks, one past the
+# borders on both sides, and more matrices than fit at once.
+CUT = [(1, 128, 257), (2, 257, 128), (1, 100, 512), (1, 1, 300), (1, 7, 2049), (2, 64, 2048), (1, 128, 4096),
+       (2, 4000, 37), (1, 113, 3841), (1, 128, 4097), (1, 129, 4096), (300, 48, 700), (40, 2500, 128)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [V.BF16, V.F32])
+@pytest.mark.parametrize("b,r,c", CUT)
+def test_matrices_cut_among_blocks(cuda, dtype, b, r, c):
+    g = make(b, r, c, dtype, seed=r + c, kind="spiked")
+    got, want = orth(g, dtype=dtype), exact(g)
+    sync()
+    off = fro(got.double() - want)
+    assert bool((off <= bound(g, want, dtype, dtype == V.F32)).all()), (off / fro(want)).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [V.BF16, V.F32])
+@pytest.mark.parametrize("r,c", [(50, 1200), (1203, 70), (128, 2600)])
+def test_matrices_cut_among_blocks_keep_their_place(cuda, dtype, r, c):
+    t = torch()
+    g = make(3, r, c, dtype, seed=14)
+    g[1, 2, 1] = float("nan")
+    want = orth(g, dtype=dtype)
+    wide = t.full((3, r + 2, c + 11), float("nan"), device="cuda", dtype=g.dtype)
+    wide[:, 1:1 + r, 3:3 + c] = g
+    out = t.full((3, r + 5, c + 9), 7.0, device="cuda", dtype=g.dtype)
+    orth(wide[:, 1:1 + r, 3:3 + c], out=out[:, 2:2 + r, 1:1 + c], dtype=dtype, shape=(3, r, c))
+    one = orth(g[2:], dtype=dtype)
+    sync()
+    assert want[1].isnan().any() and not want[::2].isnan().any()
+    part = out[:, 2:2 + r, 1:1 + c]
+    assert bool((part == want)[::2].all()) and bool((one[0] == want[2]).all())
+    part.fill_(7.0)
+    assert bool((out == 7).all())
+    out = empty((3, r, c), dtype)
+    ws = workspace(V.lib().veda_orthogonalize_workspace(3, r, c, dtype))
+    graph = t.cuda.CUDAGraph()
+    with t.cuda.graph(graph):
+        orth(g, out=out, dtype=dtype, ws=ws)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        sync()
+        assert bool((out == want)[::2].all())
+    orth(g, out=g, dtype=dtype)   # in place
+    sync()
+    assert bool((g == want)[::2].all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("b,r,c", [(2, 100, 2300), (3, 515, 33)])
+def test_muon_on_matrices_cut_among_blocks(cuda, bf16, b, r, c):
+    master, momentum, grad, lowp = muon_state(b, r, c, bf16)
+    want = muon_want(master, momentum, grad)
+    kept = [v.clone() for v in (master, momentum)]
+    bad = grad.clone()
+    bad[-1, -1, -1] = float("inf")
+    muon(master, momentum, bad, lowp, (b, r, c), r * c, flags=2,
+         sumsq=torch().full((1,), float("inf"), device="cuda", dtype=torch().float64))
+    sync()
+    assert bool((master == kept[0]).all()) and bool((momentum == kept[1]).all())
+    muon(master, momentum, grad, lowp, (b, r, c), r * c)
+    sync()
+    check_muon(master, momentum, lowp, want, 1e-2, 1.7)
+
+
 @pytest.mark.gpu
 def test_muon_skips_a_step_that_is_not_finite(cuda):
     t = torch()

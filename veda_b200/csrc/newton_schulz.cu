@@ -8,7 +8,7 @@
 // matrix's step before it is stored, which a counter per matrix and step tells. With a few matrices the
 // next step of one runs beside the last tiles of another, so neither the last, partly filled wave of a
 // product nor its epilogue leaves SMs idle. As one launch per product, 28 x 1024 x 1024 took 870 us
-// against @CHAIN28@. A tall matrix is multiplied from the other side (S = X^T X, X <- X M) by operand
+// against 760. A tall matrix is multiplied from the other side (S = X^T X, X <- X M) by operand
 // order alone, so nothing is transposed. S and M are symmetric: the tiles on and above the diagonal are
 // computed, and each one above it is written a second time, transposed.
 //
@@ -28,6 +28,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace veda::cuda
@@ -848,7 +849,14 @@ init_kernel(Source s, int rows, int cols, const double* __restrict__ partials, f
 // of columns that is K-major for S = X X^T is MN-major for M X without moving a byte. Products are split
 // (hi lo + lo hi + hi hi) for either dtype: what such a matrix costs is the latency of its 15 products
 // one after the other, not their size. As 17 launches of the tiled kernels the two 192 x 64 matrices
-// took 81 us on the GPU; in one block each, 27 us.
+// took 81 us on the GPU; in one block each, 28.7 us. At this size fetching instructions that run once costs
+// as much as what they do: passes that stop where the whole block has nothing left, one copy of each, and shifts
+// for divisions took the fp32 Muon step of 2 x 64 x 64 from 24.7 to 19 us.
+// CLUSTER: a longer side of up to 4096 is cut among the up to 16 blocks of a cluster. Each multiplies its
+// columns of X; only S needs them all, and its parts meet in the blocks' shared memory: every block adds
+// some rows and hands their sums to the others. M, one product of the small side, is formed by each. An
+// iteration then takes 8 (64 x 4096) to 15 us (128 x 4096, 16 blocks), 3 to 7 of them for the exchange;
+// 128 x 1024 in fp32 went from 142 us (tiled) to 75, 64 x 4096 from 277 to 49.
 struct Small
 {
     Source src;
@@ -858,24 +866,56 @@ struct Small
     int64_t ldo, stride_o;
     bf16* lowp;
     float decay, step;
-    int vec;                 // source rows can be read four elements at a time
+    int vec, vec_out;        // source rows can be read, result rows written, four elements at a time
     int* status;
+    // how the longer side is cut: blocks of a matrix, columns each (the last may have fewer), rows of S
+    // that each adds up, bytes for S
+    int ranks, share, band, s_bytes;
+    // log2 of the items that a row (in; tall: a quarter of it) and a result's row (out) take in a block's count:
+    // padded to powers of two, since dividing costs more than the idle turns
+    int in_log, out_log, s_log;
 };
 
+constexpr int kMaxRanks = 16;
 constexpr int kSmallSide = 128, kSmallLong = 256;
 constexpr int kSmallThreads = 512;
 constexpr int kBlockBytes = 128 * 128;   // 128 rows of 64 fp16
 
-inline int small_smem(int m, int n)
+// Fills in the cut; the shared memory of a block.
+inline int small_smem(Small& p)
 {
-    const int nb = (n + 63) / 64, sb = (m + 63) / 64;
-    return (2 * nb + 2 * sb) * kBlockBytes + 1024 + 256;
+    const int m = std::min(p.rows, p.cols), n = std::max(p.rows, p.cols), m16 = (m + 15) / 16 * 16;
+    p.ranks = (n + kSmallLong - 1) / kSmallLong;
+    p.share = ((n + p.ranks - 1) / p.ranks + 15) / 16 * 16;
+    p.band = (m16 + p.ranks - 1) / p.ranks;
+    const auto log_of = [](int items) {
+        int k = 0;
+        while ((1 << k) < items) ++k;
+        return k;
+    };
+    const int own_cols = p.rows > p.cols ? p.cols : p.ranks > 1 ? p.share : p.cols;
+    const int in = p.vec ? own_cols / 4 : own_cols;
+    p.in_log = log_of(p.rows > p.cols ? (in + 3) / 4 : in);
+    p.out_log = log_of(p.vec_out ? own_cols / 4 : own_cols);
+    p.s_log = log_of(m16 / 4);
+    p.s_bytes = std::max(2 * ((m + 63) / 64) * kBlockBytes, p.ranks > 1 ? m16 * (m16 + 4) * 4 : 0);
+    return 2 * ((p.share + 63) / 64) * kBlockBytes + p.s_bytes + 1024 + 256;
 }
 
 // Byte offset of element (row, col) of a plane.
 __device__ __forceinline__ uint32_t plane_at(int row, int col)
 {
     return static_cast<uint32_t>((col >> 6) * kBlockBytes) + tc::sw128_offset(row, (col & 63) >> 3) + (col & 7) * 2;
+}
+
+__device__ __forceinline__ void store_four(float* p, const float (&v)[4])
+{
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store_four(bf16* p, const float (&v)[4])
+{
+    alignas(8) __nv_bfloat162 b[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(b);
 }
 
 // 32 columns from `col` of the lane's row as hi and lo: 1024 x value = v.
@@ -900,7 +940,7 @@ __device__ __forceinline__ void put_planes(uint8_t* hi, uint8_t* lo, int row, in
     }
 }
 
-template <typename T, bool MUON>
+template <typename T, bool MUON, bool CLUSTER>
 __global__ void __launch_bounds__(kSmallThreads, 1)
 small_kernel(const Small p)
 {
@@ -909,18 +949,25 @@ small_kernel(const Small p)
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const bool tall = p.rows > p.cols;
-    const int m = tall ? p.cols : p.rows, n = tall ? p.rows : p.cols;
+    // this block's matrix, and its part of the longer side: n columns from `from` on
+    const int ranks = CLUSTER ? p.ranks : 1;
+    const int rank = CLUSTER ? static_cast<int>(pair::cluster_rank()) : 0;
+    const int matrix = static_cast<int>(blockIdx.x) / ranks;
+    const int m = tall ? p.cols : p.rows, from = rank * p.share;
+    const int n = min((tall ? p.rows : p.cols) - from, p.share);
+    const int own_rows = tall ? n : p.rows, own_cols = tall ? p.cols : n;
     const int m16 = (m + 15) & ~15, n16 = (n + 15) & ~15;
-    const int nb = (n + 63) >> 6, sb = (m + 63) >> 6;
+    const int nb = (p.share + 63) >> 6, sb = (m + 63) >> 6;   // the same layout in every block of a cluster
     uint8_t* const xh = smem;
     uint8_t* const xl = xh + nb * kBlockBytes;
     uint8_t* const sh = xl + nb * kBlockBytes;
     uint8_t* const sl = sh + sb * kBlockBytes;
-    uint64_t* const done = reinterpret_cast<uint64_t*>(sl + sb * kBlockBytes);
+    uint64_t* const done = reinterpret_cast<uint64_t*>(sh + p.s_bytes);
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
     volatile int* const abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
     __shared__ double part[kSmallThreads / 32];
     __shared__ float shared_scale;
+    __shared__ double shares[kMaxRanks];
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0)
@@ -940,6 +987,7 @@ small_kernel(const Small p)
     }
     fence_before();
     __syncthreads();
+    if constexpr (CLUSTER) pair::cluster_sync();   // every block runs: its shared memory may be written
     fence_after();
     const uint32_t tmem = *tmem_slot;
     dep_wait();
@@ -951,86 +999,177 @@ small_kernel(const Small p)
         // the norm (and the momentum), then X
         const Source& s = p.src;
         const float clip = clip_scale(s.sumsq, s.max_norm, s.grad_scale);
-        const T* g = static_cast<const T*>(s.g) + s.stride * blockIdx.x;
-        float* mom = MUON ? s.momentum + s.stride * blockIdx.x : nullptr;
-        const int step = p.vec ? 4 : 1, per_row = p.cols / step, total = p.rows * per_row;
-        const auto value = [&](int64_t at, float (&u)[4], bool first) {
-            if (p.vec) load_n<T, 4>(g + at, u);
-            else u[0] = to_f32(g[at]);
-            if constexpr (MUON)
-            {
-                float o[4];
-                if (p.vec) load_n<float, 4>(mom + at, o);
-                else o[0] = mom[at];
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                {
-                    if (k < step)
-                    {
-                        u[k] = seen(u[k], s.grad_scale, clip);
-                        if (first) o[k] = fmaf(s.beta, o[k], u[k]);
-                        u[k] = s.nesterov ? fmaf(s.beta, o[k], u[k]) : o[k];
-                    }
-                }
-                if (first)
-                {
-                    if (p.vec) *reinterpret_cast<float4*>(mom + at) = make_float4(o[0], o[1], o[2], o[3]);
-                    else mom[at] = o[0];
-                }
-            }
+        const int64_t first = s.stride * matrix + (tall ? from * s.ld : from);
+        const T* g = static_cast<const T*>(s.g) + first;
+        float* mom = MUON ? s.momentum + first : nullptr;
+        const auto advance = [&](float& x, float& o) {
+            x = seen(x, s.grad_scale, clip);
+            o = fmaf(s.beta, o, x);
+            x = s.nesterov ? fmaf(s.beta, o, x) : o;
         };
-        const auto store = [&](int e, const float (&u)[4], float scale) {
-            const int r = e / per_row, c = (e - r * per_row) * step;
+        // An item is four elements of a row where they can be read together, else one. A wide matrix's items go
+        // to the threads along its rows; a tall one's in tiles of 8 rows x 4 items a warp, since a row of it
+        // becomes a column here and lanes side by side would write to the same banks.
+        const int step = p.vec ? 4 : 1, in_log = p.in_log;
+        const auto place = [&](int e, int& r, int& c) {
+            if (tall)
+            {
+                const int tile = e >> 5;
+                r = (tile >> in_log) * 8 + ((e >> 2) & 7);
+                c = ((tile & ((1 << in_log) - 1)) * 4 + (e & 3)) * step;
+            }
+            else
+            {
+                r = e >> in_log;
+                c = (e & ((1 << in_log) - 1)) * step;
+            }
+            return r < own_rows && c < own_cols;
+        };
+        const auto store = [&](int r, int c, const float (&u)[4], float scale) {
+            alignas(8) __half h[4], l[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+            {
+                const float v = u[k] * scale;
+                h[k] = __float2half_rn(v);
+                l[k] = __float2half_rn(v - __half2float(h[k]));
+            }
+            if (!tall && p.vec)
+            {
+                const uint32_t at = plane_at(r, c);   // 8 bytes of a 16-byte group
+                *reinterpret_cast<uint2*>(xh + at) = *reinterpret_cast<const uint2*>(h);
+                *reinterpret_cast<uint2*>(xl + at) = *reinterpret_cast<const uint2*>(l);
+                return;
+            }
 #pragma unroll
             for (int k = 0; k < 4; ++k)
             {
                 if (k < step)
                 {
-                    const float v = u[k] * scale;
-                    const __half h = __float2half_rn(v);
                     const uint32_t at = tall ? plane_at(c + k, r) : plane_at(r, c + k);
-                    *reinterpret_cast<__half*>(xh + at) = h;
-                    *reinterpret_cast<__half*>(xl + at) = __float2half_rn(v - __half2float(h));
+                    *reinterpret_cast<__half*>(xh + at) = h[k];
+                    *reinterpret_cast<__half*>(xl + at) = l[k];
                 }
             }
         };
-        // the first kKept values of a thread stay in registers from one pass to the other; the rest are
-        // read again (by the thread that wrote them, for Muon)
-        constexpr int kKept = 8;
-        float kept[kKept][4];
+        // Up to 32768 elements, 64 a thread: the last half (or all) stays in registers until the norm is known, what
+        // comes before it waits in the place of S, 64 KB where there is a first half. All loads of a
+        // round before the first store: Muon's momentum could alias what is read.
+        constexpr int kItems = 8;
+        const int count = tall ? ((own_rows + 7) / 8) << (in_log + 5) : own_rows << in_log;
+        const int each = kItems * (p.vec ? 1 : 4) * kSmallThreads;   // items of a round
+        float* const waiting = reinterpret_cast<float*>(sh);
+        float u[kItems][4];
         double sum = 0.0;
+        const auto round = [&](int base) {
 #pragma unroll
-        for (int q = 0; q < kKept; ++q)
-        {
-            const int e = threadIdx.x + q * kSmallThreads;
-            if (e < total)
+            for (int q = 0; q < kItems; ++q)
             {
-                const int r = e / per_row, c = (e - r * per_row) * step;
-                value(r * s.ld + c, kept[q], true);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) u[q][k] = 0.0f;
             }
-        }
-#pragma unroll
-        for (int q = 0; q < kKept; ++q)
-        {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
+            if (p.vec)
             {
-                if (static_cast<int>(threadIdx.x) + q * kSmallThreads < total && k < step)
+                float o[MUON ? kItems : 1][4];
+#pragma unroll
+                for (int q = 0; q < kItems; ++q)
                 {
-                    sum += static_cast<double>(kept[q][k]) * kept[q][k];
+                    int r, c;
+                    const int e = base + static_cast<int>(threadIdx.x) + q * kSmallThreads;
+                    if (base + q * kSmallThreads >= count) break;   // the whole block: what is not run is not fetched
+                    if (e < count && place(e, r, c))
+                    {
+                        load_n<T, 4>(g + (r * s.ld + c), u[q]);
+                        if constexpr (MUON) load_n<float, 4>(mom + (r * s.ld + c), o[q]);
+                    }
+                }
+                if constexpr (MUON)
+                {
+#pragma unroll
+                    for (int q = 0; q < kItems; ++q)
+                    {
+                        int r, c;
+                        const int e = base + static_cast<int>(threadIdx.x) + q * kSmallThreads;
+                        if (base + q * kSmallThreads >= count) break;
+                        if (e < count && place(e, r, c))
+                        {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) advance(u[q][k], o[q][k]);
+                            *reinterpret_cast<float4*>(mom + (r * s.ld + c)) = make_float4(o[q][0], o[q][1], o[q][2], o[q][3]);
+                        }
+                    }
                 }
             }
-        }
-#pragma unroll 4
-        for (int e = threadIdx.x + kKept * kSmallThreads; e < total; e += kSmallThreads)
-        {
-            const int r = e / per_row, c = (e - r * per_row) * step;
-            float u[4];
-            value(r * s.ld + c, u, true);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
+            else
             {
-                if (k < step) sum += static_cast<double>(u[k]) * u[k];
+                float o[MUON ? kItems : 1][4];
+#pragma unroll
+                for (int q = 0; q < kItems * 4; ++q)
+                {
+                    int r, c;
+                    const int e = base + static_cast<int>(threadIdx.x) + q * kSmallThreads;
+                    const bool in = e < count && place(e, r, c);
+                    u[q / 4][q % 4] = in ? to_f32(g[r * s.ld + c]) : 0.0f;
+                    if constexpr (MUON) o[q / 4][q % 4] = in ? mom[r * s.ld + c] : 0.0f;
+                }
+                if constexpr (MUON)
+                {
+#pragma unroll
+                    for (int q = 0; q < kItems * 4; ++q)
+                    {
+                        int r, c;
+                        const int e = base + static_cast<int>(threadIdx.x) + q * kSmallThreads;
+                        if (e < count && place(e, r, c))
+                        {
+                            advance(u[q / 4][q % 4], o[q / 4][q % 4]);
+                            mom[r * s.ld + c] = o[q / 4][q % 4];
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < kItems; ++q)
+            {
+                if (base + q * kSmallThreads >= count) break;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sum += static_cast<double>(u[q][k]) * u[q][k];
+            }
+        };
+        const auto planes = [&](int base, float scale) {
+#pragma unroll
+            for (int q = 0; q < kItems; ++q)
+            {
+                const int t = static_cast<int>(threadIdx.x);
+                int r, c;
+                if (p.vec)
+                {
+                    const int e = base + t + q * kSmallThreads;
+                    if (base + q * kSmallThreads >= count) break;
+                    if (e < count && place(e, r, c)) store(r, c, u[q], scale);
+                    continue;
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                {
+                    const int e = base + t + (q * 4 + k) * kSmallThreads;
+                    const float one[4] = {u[q][k], 0.0f, 0.0f, 0.0f};
+                    if (base + (q * 4 + k) * kSmallThreads >= count) break;
+                    if (e < count && place(e, r, c)) store(r, c, one, scale);
+                }
+            }
+        };
+        const bool twice = count > each;
+#pragma unroll 1
+        for (int base = 0; base < count; base += each)
+        {
+            round(base);
+            if (base + each < count)
+            {
+#pragma unroll
+                for (int q = 0; q < kItems; ++q)
+                {
+                    reinterpret_cast<float4*>(waiting)[q * kSmallThreads + threadIdx.x] = make_float4(u[q][0], u[q][1], u[q][2], u[q][3]);
+                }
             }
         }
         sum = warp_sum(sum);
@@ -1039,26 +1178,44 @@ small_kernel(const Small p)
         if (warp == 0)
         {
             sum = warp_sum(lane < kSmallThreads / 32 ? part[lane] : 0.0);
+            if constexpr (CLUSTER)
+            {
+                // every block gets every block's sum and adds them in rank order
+                if (lane < ranks)
+                {
+                    const uint32_t to = pair::peer_addr(&shares[rank], lane);
+                    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(sum) : "memory");
+                }
+                pair::cluster_arrive();
+                pair::cluster_wait();
+                sum = 0.0;
+                for (int k = 0; k < ranks; ++k) sum += shares[k];
+            }
             if (lane == 0)
             {
                 shared_scale = static_cast<float>(static_cast<double>(kUnit) / (sqrt(sum) + static_cast<double>(p.eps)));
             }
         }
+        else if constexpr (CLUSTER)
+        {
+            pair::cluster_arrive();
+            pair::cluster_wait();
+        }
         __syncthreads();
         const float scale = shared_scale;
+#pragma unroll 1
+        for (int base = twice ? each : 0; base >= 0; base -= each)
+        {
+            planes(base, scale);
+            if (base > 0)
+            {
 #pragma unroll
-        for (int q = 0; q < kKept; ++q)
-        {
-            const int e = threadIdx.x + q * kSmallThreads;
-            if (e < total) store(e, kept[q], scale);
-        }
-#pragma unroll 4
-        for (int e = threadIdx.x + kKept * kSmallThreads; e < total; e += kSmallThreads)
-        {
-            const int r = e / per_row, c = (e - r * per_row) * step;
-            float u[4];
-            value(r * s.ld + c, u, false);
-            store(e, u, scale);
+                for (int q = 0; q < kItems; ++q)
+                {
+                    const float4 w = reinterpret_cast<const float4*>(waiting)[q * kSmallThreads + threadIdx.x];
+                    u[q][0] = w.x, u[q][1] = w.y, u[q][2] = w.z, u[q][3] = w.w;
+                }
+            }
         }
     }
 
@@ -1113,8 +1270,11 @@ small_kernel(const Small p)
         fence_after();
     };
 
+    // decoupled decay, then the step along the orthogonalised update
+    const auto stepped = [&](float w, float o) { return __fsub_rn(__fsub_rn(w, __fmul_rn(p.decay, w)), __fmul_rn(p.step, o)); };
     for (int k = 0; k < p.steps; ++k)
     {
+        // a block's own columns of S = X X^T
         product(ts, xh, xl, xh, xl, std::false_type{}, m16, n16);
         const int c0 = half * 32;
         float v[32];
@@ -1125,10 +1285,93 @@ small_kernel(const Small p)
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) * f;
         };
-        if (c0 < m16)
+        if constexpr (!CLUSTER)
         {
-            fetch(ts + lanes + c0, 1.0f / kUnit);
-            if (row < m16) put_planes(sh, sl, row, c0, v);
+            if (c0 < m16)
+            {
+                fetch(ts + lanes + c0, 1.0f / kUnit);
+                if (row < m16) put_planes(sh, sl, row, c0, v);
+            }
+        }
+        else
+        {
+            // The blocks' sums meet: each block leaves its own in the place of S, and after all have, each reads
+            // `band` rows of all of them, adds them in rank order and hands their hi and lo to every block.
+            const int band = p.band, pitch = m16 + 4;   // lanes write a row each: 16-byte pieces in all banks
+            float* const mine = reinterpret_cast<float*>(sh);
+            if (c0 < m16)
+            {
+                fetch(ts + lanes + c0, 1.0f / kUnit);
+                if (row < m16)
+                {
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                    {
+                        if (c0 + 4 * q < m16)
+                        {
+                            *reinterpret_cast<float4*>(mine + row * pitch + c0 + 4 * q) =
+                                make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                        }
+                    }
+                }
+            }
+            pair::cluster_arrive();
+            pair::cluster_wait();
+            // groups of four columns of this block's rows; at most 4 a thread (64 x 128 / 4 / 512)
+            const int rows_here = min(band, m16 - rank * band), s_log = p.s_log, groups = max(0, rows_here) << s_log;
+            float sums[4][4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+            {
+                const int e = static_cast<int>(threadIdx.x) + q * kSmallThreads;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sums[q][i] = 0.0f;
+                const int r = e >> s_log, c = (e & ((1 << s_log) - 1)) * 4;
+                if (e < groups && c < m16)
+                {
+                    const float* at = mine + (rank * band + r) * pitch + c;
+#pragma unroll 8
+                    for (int b = 0; b < ranks; ++b)
+                    {
+                        float w[4];
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(w[0]), "=f"(w[1]), "=f"(w[2]), "=f"(w[3])
+                                     : "r"(pair::peer_addr(at, b)));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sums[q][i] += w[i];
+                    }
+                }
+            }
+            pair::cluster_arrive();   // all have read
+            pair::cluster_wait();
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+            {
+                const int e = static_cast<int>(threadIdx.x) + q * kSmallThreads;
+                const int r = e >> s_log, c = (e & ((1 << s_log) - 1)) * 4;
+                if (e < groups && c < m16)
+                {
+                    uint32_t h[2], l[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                    {
+                        h[i] = pack_f16(sums[q][2 * i], sums[q][2 * i + 1]);
+                        const float2 back = unpack_f16(h[i]);
+                        l[i] = pack_f16(sums[q][2 * i] - back.x, sums[q][2 * i + 1] - back.y);
+                    }
+                    const uint32_t at = plane_at(rank * band + r, c);
+                    for (int b = 0; b < ranks; ++b)
+                    {
+                        const uint32_t to = pair::peer_addr(sh + at, b);
+                        asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(h[0]), "r"(h[1]) : "memory");
+                        asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(to + sb * kBlockBytes), "r"(l[0]), "r"(l[1])
+                                     : "memory");
+                    }
+                }
+            }
+            asm volatile("fence.proxy.async;" ::: "memory");   // the products read S through the other proxy
+            pair::cluster_arrive();   // S is everywhere
+            pair::cluster_wait();
         }
         product(ts, sh, sl, sh, sl, std::false_type{}, m16, m16);
         if (c0 < m16)
@@ -1164,36 +1407,105 @@ small_kernel(const Small p)
             {
                 if (row < m16) put_planes(xh, xl, row, c, v);
             }
-            else if (row < m && !skip)
+            else if (row < m)
             {
-                const int64_t base = p.stride_o * blockIdx.x + (tall ? row : row * p.ldo);
-                const int64_t by = tall ? p.ldo : 1;
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
+                // the result waits as fp32 in X's place, rows as the caller's; a wide one's 16-byte groups
+                // are turned by their row, since each lane writes to its own
+                float* const out = reinterpret_cast<float*>(xh);
+                if (tall)
                 {
-                    if (c + i < n)
+                    float* const to = out + c * m16 + row;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
                     {
-                        const int64_t at = base + (c + i) * by;
-                        const float o = v[i] * (1.0f / kUnit);
-                        if constexpr (MUON)
-                        {
-                            float* w = static_cast<float*>(p.dst) + at;
-                            float x = __fsub_rn(*w, __fmul_rn(p.decay, *w));
-                            x = __fsub_rn(x, __fmul_rn(p.step, o));
-                            *w = x;
-                            if (p.lowp != nullptr) p.lowp[at] = __float2bfloat16_rn(x);
-                        }
-                        else
-                        {
-                            static_cast<T*>(p.dst)[at] = from_f32<T>(o);
-                        }
+                        if (c + i < n) to[i * m16] = v[i] * (1.0f / kUnit);
                     }
+                }
+                else
+                {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                    {
+                        const int at = row * nb * 64 + (((c + i) / 4) ^ (row & 7)) * 4;
+                        *reinterpret_cast<float4*>(out + at) = make_float4(v[i] * (1.0f / kUnit), v[i + 1] * (1.0f / kUnit),
+                                                                           v[i + 2] * (1.0f / kUnit), v[i + 3] * (1.0f / kUnit));
+                    }
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (!skip)
+    {
+        const float* const out = reinterpret_cast<const float*>(xh);
+        const int step = p.vec_out ? 4 : 1, out_log = p.out_log, count = own_rows << out_log;
+        const int64_t base = p.stride_o * matrix + (tall ? from * p.ldo : from);
+        constexpr int kItems = 8;
+        for (int e0 = threadIdx.x; e0 < count; e0 += kItems * kSmallThreads)
+        {
+            float w[MUON ? kItems : 1][4];
+            if constexpr (MUON)
+            {
+#pragma unroll
+                for (int q = 0; q < kItems; ++q)
+                {
+                    const int e = e0 + q * kSmallThreads, r = e >> out_log, c = (e & ((1 << out_log) - 1)) * step;
+                    if (e < count && c < own_cols)
+                    {
+                        const float* at = static_cast<const float*>(p.dst) + base + r * p.ldo + c;
+                        if (p.vec_out) load_n<float, 4>(at, w[q]);
+                        else w[q][0] = *at;
+                    }
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < kItems; ++q)
+            {
+                const int e = e0 + q * kSmallThreads, r = e >> out_log, c = (e & ((1 << out_log) - 1)) * step;
+                if (q * kSmallThreads >= count - e0) break;
+                if (c >= own_cols) continue;
+                const int64_t at = base + r * p.ldo + c;
+                const float* x = out + (tall ? r * m16 + c : r * nb * 64 + ((c / 4) ^ (r & 7)) * 4 + c % 4);
+                float o[4];
+                if (p.vec_out)
+                {
+                    const float4 x4 = *reinterpret_cast<const float4*>(x);
+                    o[0] = x4.x, o[1] = x4.y, o[2] = x4.z, o[3] = x4.w;
+                }
+                else
+                {
+                    o[0] = *x;
+                }
+                if constexpr (MUON)
+                {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                    {
+                        if (k < step) o[k] = stepped(w[q][k], o[k]);
+                    }
+                    float* to = static_cast<float*>(p.dst) + at;
+                    if (p.vec_out) store_four(to, o);
+                    else *to = o[0];
+                    if (p.lowp != nullptr)
+                    {
+                        if (p.vec_out) store_four(p.lowp + at, o);
+                        else p.lowp[at] = __float2bfloat16_rn(o[0]);
+                    }
+                }
+                else if (p.vec_out)
+                {
+                    store_four(static_cast<T*>(p.dst) + at, o);
+                }
+                else
+                {
+                    static_cast<T*>(p.dst)[at] = from_f32<T>(o[0]);
                 }
             }
         }
     }
     fence_before();
     __syncthreads();
+    if constexpr (CLUSTER) pair::cluster_sync();   // no block leaves while another may still write to it
     if (warp == 1)
     {
         fence_after();
@@ -1245,33 +1557,80 @@ Layout layout(int64_t batch, int64_t rows, int64_t cols, bool split, int steps)
 
 bool is_small(int64_t rows, int64_t cols)
 {
-    return std::min(rows, cols) <= kSmallSide && std::max(rows, cols) <= kSmallLong;
+    return std::min(rows, cols) <= kSmallSide && std::max(rows, cols) <= kMaxRanks * kSmallLong;
 }
 
+// Launches the small form; `*taken` stays false where the tiled form is faster, or the device cannot hold a
+// cluster of that many blocks.
 template <typename T, bool MUON>
-int launch_small(const char* what, const Small& p, int64_t batch, cudaStream_t stream)
+int launch_small(const char* what, Small p, int64_t batch, bool split, cudaStream_t stream, bool* taken)
 {
-    auto kernel = small_kernel<T, MUON>;
+    const int smem = small_smem(p);
+    const bool cluster = p.ranks > 1;
+    const auto kernel = cluster ? small_kernel<T, MUON, true> : small_kernel<T, MUON, false>;
+    // per device and cluster size: 0 not asked yet, else 1 + the clusters that run at a time
     constexpr int kDevices = 64;
-    static std::atomic<bool> configured[kDevices];
+    static std::atomic<int> known[kDevices][kMaxRanks + 1];
     int device = 0;
     cudaGetDevice(&device);
     if (device < 0 || device >= kDevices)
     {
         return fail(VEDA_ERR_UNSUPPORTED, std::string(what) + ": no such device");
     }
-    if (!configured[device].load(std::memory_order_acquire))
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(batch * p.ranks));
+    cfg.blockDim = dim3(kSmallThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attrs[2]{};
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim.x = static_cast<unsigned>(p.ranks);
+    attrs[0].val.clusterDim.y = 1;
+    attrs[0].val.clusterDim.z = 1;
+    cfg.attrs = attrs;
+    cfg.numAttrs = 1;
+    int room = known[device][p.ranks].load(std::memory_order_acquire);
+    if (room == 0)
     {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 small_smem(kSmallSide, kSmallLong)) != cudaSuccess)
+        constexpr int kMost = 224 * 1024;   // dynamic; a block also has some static shared memory
+        bool ok = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) == cudaSuccess;
+        if (ok && p.ranks > 8)
         {
-            cudaGetLastError();
-            return fail(VEDA_ERR_CUDA, std::string(what) + ": shared memory for small matrices");
+            ok = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
         }
-        configured[device].store(true, std::memory_order_release);
+        int clusters = 1;
+        if (ok && cluster)
+        {
+            cfg.dynamicSmemBytes = kMost;
+            ok = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters > 0;
+            cfg.dynamicSmemBytes = smem;
+        }
+        cudaGetLastError();
+        room = ok ? 1 + clusters : 1;
+        known[device][p.ranks].store(room, std::memory_order_release);
     }
-    return launch(what, kernel, dim3(static_cast<unsigned>(batch)), dim3(kSmallThreads),
-                  small_smem(std::min(p.rows, p.cols), std::max(p.rows, p.cols)), stream, p);
+    // One block a matrix, or smaller sides of at most 64, are always worth it. Of larger ones the
+    // tiled form, which fills the device, does more matrices in the time (the more so in bf16, where
+    // its products are not split): bf16 64 x 128 x 1024 158 us here and 182 us tiled, 200 of them 570
+    // and 505; 8 x 128 x 4096 181 and 205, 64 of them 947 and 618; fp32 32 x 128 x 4096 460 and 565,
+    // 64 x 4096 x 128 946 and 694. In all of these the longer side is cut in more than two.
+    const int few = split ? 4 : 2;
+    *taken = room > 1 && (std::min(p.rows, p.cols) <= 64 || p.ranks <= few || batch <= static_cast<int64_t>(few) * (room - 1));
+    if (!*taken)
+    {
+        return VEDA_OK;
+    }
+    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = overlapped_launches() ? 2 : 1;
+    count_launch();
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, p);
+    if (err != cudaSuccess)
+    {
+        cudaGetLastError();
+        return fail(VEDA_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(err));
+    }
+    return check_launch(what);
 }
 
 // Whether four elements at a time can be read of every row of every matrix.
@@ -1281,6 +1640,15 @@ bool reads_four(const Source& src, int64_t batch, int64_t cols)
     const uintptr_t bases = reinterpret_cast<uintptr_t>(src.g) | reinterpret_cast<uintptr_t>(src.momentum);
     return (bases & (src.momentum != nullptr ? 15u : 4 * sizeof(T) - 1)) == 0 && cols % 4 == 0 && src.ld % 4 == 0 &&
            (batch == 1 || src.stride % 4 == 0);
+}
+
+// Whether four elements at a time can be written of every row of the result.
+template <typename T>
+bool writes_four(const Params& p, int64_t batch, int64_t cols, bool muon)
+{
+    const uintptr_t size = muon ? 4 : sizeof(T);
+    return (reinterpret_cast<uintptr_t>(p.dst) & (4 * size - 1)) == 0 && (reinterpret_cast<uintptr_t>(p.lowp) & 7) == 0 &&
+           cols % 4 == 0 && p.ldo % 4 == 0 && (batch == 1 || p.stride_o % 4 == 0);
 }
 
 // Tiles of one matrix: of S or M (on and right of the diagonal), and of X.
@@ -1378,10 +1746,13 @@ int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, in
 {
     if (is_small(rows, cols))
     {
-        const Small q{src,   static_cast<int>(rows), static_cast<int>(cols), steps,   a,      b,
-                      c,     eps,                    p.dst,                  p.ldo,   p.stride_o, p.lowp,
-                      p.decay, p.step,               reads_four<T>(src, batch, cols), device_status_ptr()};
-        return launch_small<T, LAST == kMuon>(what, q, batch, stream);
+        const Small q{src,     static_cast<int>(rows), static_cast<int>(cols), steps,        a,          b,
+                      c,       eps,                    p.dst,                  p.ldo,        p.stride_o, p.lowp,
+                      p.decay, p.step,                 reads_four<T>(src, batch, cols), writes_four<T>(p, batch, cols, LAST == kMuon),
+                      device_status_ptr()};
+        bool taken = false;
+        const int rc = launch_small<T, LAST == kMuon>(what, q, batch, SPLIT, stream, &taken);
+        if (rc != VEDA_OK || taken) return rc;
     }
     const Layout l = layout(batch, rows, cols, SPLIT, kMaxSteps);
     double* partials = reinterpret_cast<double*>(ws + l.partials);
