@@ -411,7 +411,7 @@ struct Part
     }
 
     // The last product's result: written out, or applied to the weights, through the staging where TMA
-    // can describe the destination, else element by element.
+    // can describe the destination, else by rows of 32 elements.
     static __device__ __forceinline__ void finish(const Params& p, const View& w, const Tile& t, int trow, int col, uint8_t* in,
                                                   uint8_t* out, uint8_t* stage, int lane, float (&v)[kChunk])
     {
@@ -419,7 +419,14 @@ struct Part
         for (int i = 0; i < kChunk; ++i) v[i] *= 1.0f / kUnit;
         if (!p.vec)
         {
-            finish_direct(p, w, t, trow + lane, col, v);
+            // two units, 4 KB: a set of the split forms, else units 2 and 3, which only stores use that are
+            // not made here
+            uint8_t* tile = !SPLIT ? stage + 2 * kUnitBytes : KIND == kMuon ? in : out;
+            put_f32(tile, lane, v);
+            __syncwarp();
+            finish_direct(p, w, t, trow, col + lane, tile, lane);
+            __syncwarp();
+            if (lane == 0) tc::bulk_commit_group();   // empty: the waits above count groups
             return;
         }
         uint32_t w16[16];
@@ -471,32 +478,48 @@ struct Part
         }
     }
 
-    static __device__ __forceinline__ void finish_direct(const Params& p, const View& w, const Tile& t, int row, int col,
-                                                         float (&v)[kChunk])
+    // The staged chunk row by row, a column a lane: whole lines of rows that start anywhere. With a row a
+    // lane, each store to 32 lines, Muon on 3 x 1111 x 2222 took 670 us instead of 495.
+    static __device__ __forceinline__ void finish_direct(const Params& p, const View& w, const Tile& t, int trow, int col,
+                                                         const uint8_t* tile, int lane)
     {
-        if (row >= w.nrows)
+        if (col >= w.ncols)
         {
             return;
         }
-        const int64_t at = p.stride_o * t.b + static_cast<int64_t>(row) * p.ldo + col;
-#pragma unroll
-        for (int i = 0; i < kChunk; ++i)
+        const int n = min(32, w.nrows - trow);
+        const int64_t at = p.stride_o * t.b + static_cast<int64_t>(trow) * p.ldo + col;
+#pragma unroll 1
+        for (int i0 = 0; i0 < n; i0 += 8)
         {
-            if (col + i < w.ncols)
+            float old[8];
+            if constexpr (KIND == kMuon)
             {
-                if constexpr (KIND == kMuon)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) old[i] = i0 + i < n ? static_cast<const float*>(p.dst)[at + (i0 + i) * p.ldo] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+            {
+                const int r = i0 + i;
+                if (r < n)
                 {
-                    float* weight = static_cast<float*>(p.dst) + at + i;
-                    *weight = update(p, *weight, v[i]);
-                    if (p.lowp != nullptr) p.lowp[at + i] = __float2bfloat16_rn(*weight);
-                }
-                else if (p.out_f32)
-                {
-                    static_cast<float*>(p.dst)[at + i] = v[i];
-                }
-                else
-                {
-                    static_cast<bf16*>(p.dst)[at + i] = __float2bfloat16_rn(v[i]);
+                    const int64_t here = at + r * p.ldo;
+                    const float v = *reinterpret_cast<const float*>(tile + tc::sw128_offset(r, lane >> 2) + (lane & 3) * 4);
+                    if constexpr (KIND == kMuon)
+                    {
+                        const float x = update(p, old[i], v);
+                        static_cast<float*>(p.dst)[here] = x;
+                        if (p.lowp != nullptr) p.lowp[here] = __float2bfloat16_rn(x);
+                    }
+                    else if (p.out_f32)
+                    {
+                        static_cast<float*>(p.dst)[here] = v;
+                    }
+                    else
+                    {
+                        static_cast<bf16*>(p.dst)[here] = __float2bfloat16_rn(v);
+                    }
                 }
             }
         }
