@@ -129,9 +129,11 @@ SHAPES = [(1, 1, 8), (1, 300, 64), (3, 2, 16), (31, 255, 24), (128, 512, 64), (2
           # up to four rows of up to 2048 columns are streamed past; one past each border
           (2, 700, 2048), (3, 601, 1000), (4, 9001, 776), (5, 4100, 64), (4, 50, 2056), (1, 20000, 40), (4, 33, 1),
           (8, 9001, 776),
-          # the tensor-core form: over 1024 rows, 4096 words or 2^25 products
+          # the tensor-core form: over 1024 rows, 4096 words (bf16: 1024) or 2^23 products (bf16: 2^22)
           (31, 4355, 24), (128, 5000, 64), (257, 4353, 40), (300, 4097, 72), (512, 6145, 128), (1025, 255, 16),
-          (9, 4111, 8), (700, 4000, 100), (1024, 4096, 8)]
+          (9, 4111, 8), (700, 4000, 100), (1024, 4096, 8),
+          # small gradients cut into 1, 2, 4 and 8 parts, the last parts short or empty
+          (5, 129, 40), (130, 257, 33), (300, 40, 64), (513, 150, 90), (1024, 33, 100), (9, 1153, 500)]
 
 
 @pytest.mark.gpu
@@ -146,6 +148,29 @@ def test_loss_and_gradients(cuda, dtype, rows, vocab, dim):
 def test_many_pieces_of_the_vocabulary(cuda, dtype, rows, vocab, dim):
     # the pieces of q are 64 MB: 6656 columns at 5000 bf16 rows or 2500 split ones
     run_and_check(*make(rows, vocab, dim, dtype, seed=5, ignored=0.1), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [V.BF16, V.F32])
+@pytest.mark.parametrize("rows,vocab,dim", [(1, 3001, 116), (2, 1037, 102), (3, 515, 101), (4, 40, 260), (1, 9, 2046),
+                                             (4, 2000, 1999), (1, 200, 4), (20, 511, 118), (9, 300, 61)])
+def test_rows_of_every_alignment(cuda, dtype, rows, vocab, dim):
+    # head and dW in groups of 8, 4, 2 and single elements: by dim, by pitch, by base
+    t = torch()
+    x, w, tg = make(rows, vocab, dim, dtype, seed=dim)
+    for pitch, base in ((dim, 0), (dim + dim % 2, 0), ((dim + 7) // 8 * 8, 0), ((dim + 7) // 8 * 8, 4), (dim + 6, 2), (dim + 1, 1)):
+        ww = t.full((vocab * pitch + base + 8,), float("nan"), device="cuda", dtype=w.dtype)
+        wv = ww[base:base + vocab * pitch].view(vocab, pitch)[:, :dim]
+        wv.copy_(w)
+        run_and_check(x, wv, tg, dtype)
+    # dW in rows of 16-byte pitch whose last columns are no whole group, its padding untouched
+    pitch = (dim + 7) // 8 * 8 + 8
+    _, lse, _ = fwd(x, w, tg, dtype)
+    want, wide = empty(w.shape, dtype), t.full((vocab, pitch), 7.0, device="cuda", dtype=w.dtype)
+    bwd(x, w, tg, lse, dtype, dx=None, dw=want, dtype_dw=dtype)
+    bwd(x, w, tg, lse, dtype, dx=None, dw=wide[:, :dim], dtype_dw=dtype)
+    sync()
+    assert bool((wide[:, :dim] == want).all()) and bool((wide[:, dim:] == 7).all())
 
 
 @pytest.mark.gpu

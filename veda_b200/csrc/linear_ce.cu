@@ -504,10 +504,10 @@ struct GradWork
             }
             if (mode == 0)
             {
-                store_direct(p, r, orow + lane, col, trow + lane, unit, coef);
+                store_direct(p, r, orow, col, p.gcols - trow, unit, coef, st, lane);
                 if (!f32)
                 {
-                    store_direct(p, r2, orow + lane, col + 32, trow + lane, unit, coef);
+                    store_direct(p, r2, orow, col + 32, p.gcols - trow, unit, coef, st, lane);
                 }
                 continue;
             }
@@ -562,33 +562,52 @@ struct GradWork
         }
     }
 
-    // A dW row piece whose pitch or base TMA cannot describe, or bf16 accumulation.
-    static __device__ __forceinline__ void store_direct(const Params& p, const uint32_t (&r)[32], int row,
-                                                        int col, int piece_row, float unit, float coef)
+    // Up to 32 rows of dW whose pitch or base TMA cannot describe, or bf16 accumulation: through the staging, row
+    // by row, a column a lane. (A row a lane, each store to 32 lines, took 700 x 9001 x 333's gradients @DD@.)
+    static __device__ __forceinline__ void store_direct(const Params& p, const uint32_t (&r)[32], int row, int col, int rows,
+                                                        float unit, float coef, pair::Staging& st, int lane)
     {
-        if (piece_row >= p.gcols)
-        {
-            return;
-        }
-        const int64_t at = static_cast<int64_t>(row) * p.lddw + col;
+        uint8_t* buf = st.buffer(lane);
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
+        for (int k = 0; k < 8; ++k)
         {
-            if (col + j < p.dim)
+            *reinterpret_cast<float4*>(buf + tc::sw128_offset(lane, k)) =
+                make_float4(__uint_as_float(r[4 * k]) * unit * coef, __uint_as_float(r[4 * k + 1]) * unit * coef,
+                            __uint_as_float(r[4 * k + 2]) * unit * coef, __uint_as_float(r[4 * k + 3]) * unit * coef);
+        }
+        __syncwarp();
+        const int n = col + lane < p.dim ? min(32, rows) : 0;
+        const int64_t at = static_cast<int64_t>(row) * p.lddw + col + lane;
+#pragma unroll 1
+        for (int i0 = 0; i0 < n; i0 += 8)
+        {
+            float old[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
             {
-                float v = __uint_as_float(r[j]) * unit * coef;
-                if (p.dw_f32)
+                old[i] = 0.0f;
+                if (p.dw_beta && i0 + i < n)
                 {
-                    float* d = static_cast<float*>(p.dw_ptr) + at + j;
-                    *d = p.dw_beta ? *d + v : v;
+                    const int64_t here = at + (i0 + i) * p.lddw;
+                    old[i] = p.dw_f32 ? static_cast<const float*>(p.dw_ptr)[here] : __bfloat162float(static_cast<const bf16*>(p.dw_ptr)[here]);
                 }
-                else
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+            {
+                if (i0 + i < n)
                 {
-                    bf16* d = static_cast<bf16*>(p.dw_ptr) + at + j;
-                    *d = __float2bfloat16_rn(p.dw_beta ? __bfloat162float(*d) + v : v);
+                    const int64_t here = at + (i0 + i) * p.lddw;
+                    const float v = *reinterpret_cast<const float*>(buf + tc::sw128_offset(i0 + i, lane >> 2) + (lane & 3) * 4);
+                    const float o = p.dw_beta ? old[i] + v : v;
+                    if (p.dw_f32) static_cast<float*>(p.dw_ptr)[here] = o;
+                    else static_cast<bf16*>(p.dw_ptr)[here] = __float2bfloat16_rn(o);
                 }
             }
         }
+        __syncwarp();
+        if (lane == 0) tc::bulk_commit_group();   // empty: the staging counts groups
+        st.sent();
     }
 };
 
@@ -974,7 +993,7 @@ struct Few
     int64_t vocab;
     const int64_t* targets;
     int64_t ignore;
-    int vec;                 // head rows can be read 16 bytes at a time
+    int grain;               // elements of a head row that can be read at a time: 8, or up to 16 bytes of 4, 2 or 1
     // forward
     float2* parts;           // [block][rows]
     float* target_logit;
@@ -984,7 +1003,7 @@ struct Few
     int chunk;               // vocabulary rows held at a time
     void* dw;
     int64_t lddw;
-    int dw_f32, dw_beta, dw_vec;
+    int dw_f32, dw_beta, dw_grain;   // dw_grain: as grain, of dW's rows; 8 does not ask for whole groups of columns
     float* acc;              // [block][rows][ld_acc] sums of dx, or null
     int64_t ld_acc;
     // small problems
@@ -1016,12 +1035,29 @@ struct Eight
 #pragma unroll
         for (int k = 0; k < static_cast<int>(sizeof(T) / 2); ++k) q[k] = reinterpret_cast<const uint4*>(p)[k];
     }
+    // G elements at a time, the first `left` (a multiple of G)
+    template <int G>
     __device__ __forceinline__ void gather(const T* p, int left)
     {
-        T v[8];
+        struct alignas(G * sizeof(T)) Group
+        {
+            T v[G];
+        };
+        Group g[8 / G];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = k < left ? p[k] : from_f32<T>(0.0f);
-        memcpy(q, v, sizeof(v));
+        for (int k = 0; k < 8 / G; ++k)
+        {
+            if (k * G < left)
+            {
+                g[k] = reinterpret_cast<const Group*>(p)[k];
+            }
+            else
+            {
+#pragma unroll
+                for (int i = 0; i < G; ++i) g[k].v[i] = from_f32<T>(0.0f);
+            }
+        }
+        memcpy(q, g, sizeof(g));
     }
     __device__ __forceinline__ void zero()
     {
@@ -1119,8 +1155,8 @@ __device__ __forceinline__ void own_row(float (&acc)[4][R], int lane, float (&z)
     }
 }
 
-// blockIdx.y: which R rows. Q: writes q of the rows instead of their (max, sum) pairs.
-template <typename T, int R, bool VEC, bool Q>
+// blockIdx.y: which R rows. G: the head's grain. Q: writes q of the rows instead of their (max, sum) pairs.
+template <typename T, int R, int G, bool Q>
 __global__ void __launch_bounds__(kFewThreads, few_fwd_per_sm(R))
 few_fwd_kernel(const Few p)
 {
@@ -1160,14 +1196,14 @@ few_fwd_kernel(const Few p)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                 {
-                    if constexpr (VEC)
+                    if constexpr (G == 8)
                     {
                         w[h][j].zero();
                         if (at < p.dim) w[h][j].stream(row[j] + at);
                     }
                     else
                     {
-                        w[h][j].gather(row[j] + at, p.dim - at);
+                        w[h][j].template gather<G>(row[j] + at, p.dim - at);
                     }
                 }
             }
@@ -1224,65 +1260,114 @@ few_fwd_kernel(const Few p)
     }
 }
 
-// Copies vocabulary rows v .. v + chunk - 1 into `stage` (rows of `padded` elements), 16 bytes at a time
-// and asynchronously where the head allows it. What lies past dim or the vocabulary is zero.
+// Copies vocabulary rows v .. v + chunk - 1, as far as there are, into `stage` (rows of `padded` elements), a
+// row a warp at a time: asynchronously by 16, 8 or 4 bytes. Single bf16 elements, which nothing copies
+// asynchronously, go through registers, 16 loads of a lane at a time. Columns past dim stay as they are.
+template <typename T, int BYTES>
+__device__ __forceinline__ void stage_async(const Few& p, T* stage, int64_t v)
+{
+    constexpr int G = BYTES / sizeof(T);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int r = warp; r < p.chunk && v + r < p.vocab; r += kFewWarps)
+    {
+        const T* row = static_cast<const T*>(p.w) + (v + r) * p.ldw;
+        const uint32_t to = tc::smem_u32(stage + r * p.padded);
+        for (int c = lane * G; c < p.dim; c += 32 * G)
+        {
+            if constexpr (BYTES == 16)
+            {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + c * static_cast<int>(sizeof(T))), "l"(row + c) : "memory");
+            }
+            else
+            {
+                asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to + c * static_cast<int>(sizeof(T))), "l"(row + c), "n"(BYTES)
+                             : "memory");
+            }
+        }
+    }
+}
+
 template <typename T>
 __device__ __forceinline__ void stage_head(const Few& p, T* stage, int64_t v)
 {
-    constexpr int V = 16 / sizeof(T);
-    const T* w = static_cast<const T*>(p.w);
-    if (p.vec)
+    const int bytes = p.grain * static_cast<int>(sizeof(T));
+    if (bytes >= 16)
     {
-        const int per = p.padded / V;
-        for (int i = threadIdx.x; i < p.chunk * per; i += kFewThreads)
-        {
-            const int r = i / per, c = (i - r * per) * V;
-            const bool in = v + r < p.vocab && c < p.dim;   // dim is a multiple of V here
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(stage + r * p.padded + c)),
-                         "l"(in ? w + (v + r) * p.ldw + c : w), "r"(in ? 16u : 0u)
-                         : "memory");
-        }
+        stage_async<T, 16>(p, stage, v);
+    }
+    else if (bytes == 8)
+    {
+        stage_async<T, 8>(p, stage, v);
+    }
+    else if (bytes == 4)
+    {
+        stage_async<T, 4>(p, stage, v);
     }
     else
     {
-        for (int i = threadIdx.x; i < p.chunk * p.padded; i += kFewThreads)
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        for (int r0 = warp; r0 < p.chunk; r0 += 4 * kFewWarps)
         {
-            const int r = i / p.padded, c = i - r * p.padded;
-            stage[i] = v + r < p.vocab && c < p.dim ? w[(v + r) * p.ldw + c] : from_f32<T>(0.0f);
+            for (int c0 = lane; c0 < p.dim; c0 += 128)
+            {
+                T e[4][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                {
+                    const int r = r0 + i * kFewWarps;
+                    const T* row = static_cast<const T*>(p.w) + (v + r) * p.ldw;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                    {
+                        const bool in = r < p.chunk && v + r < p.vocab && c0 + 32 * k < p.dim;
+                        e[i][k] = in ? row[c0 + 32 * k] : from_f32<T>(0.0f);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                    {
+                        const int r = r0 + i * kFewWarps;
+                        if (r < p.chunk && c0 + 32 * k < p.dim) stage[r * p.padded + c0 + 32 * k] = e[i][k];
+                    }
+                }
+            }
         }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
 // Eight columns of a dW row (the first `left` of them), accumulated with beta.
+template <int G, typename U>
+__device__ __forceinline__ void store_dw_by(U* at, const float (&o)[8], int beta, int left)
+{
+    struct alignas(G * sizeof(U)) Group
+    {
+        U v[G];
+    };
+#pragma unroll
+    for (int k = 0; k < 8; k += G)
+    {
+        if (k < left)
+        {
+            Group g;
+            if (beta) g = *reinterpret_cast<const Group*>(at + k);
+#pragma unroll
+            for (int i = 0; i < G; ++i) g.v[i] = from_f32<U>(beta ? to_f32(g.v[i]) + o[k + i] : o[k + i]);
+            *reinterpret_cast<Group*>(at + k) = g;
+        }
+    }
+}
 template <typename U>
-__device__ __forceinline__ void store_dw(U* at, float (&o)[8], int vec, int beta, int left)
+__device__ __forceinline__ void store_dw(U* at, const float (&o)[8], int grain, int beta, int left)
 {
     constexpr int V = 16 / sizeof(U);
-    if (vec && left >= 8)
-    {
-#pragma unroll
-        for (int k = 0; k < 8; k += V)
-        {
-            float part[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) part[i] = o[k + i];
-            if (beta)
-            {
-                float old[V];
-                load16(at + k, old);
-#pragma unroll
-                for (int i = 0; i < V; ++i) part[i] += old[i];
-            }
-            store16(at + k, part);
-        }
-        return;
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-    {
-        if (k < left) at[k] = from_f32<U>(beta ? to_f32(at[k]) + o[k] : o[k]);
-    }
+    if (grain == 8 && left >= 8) store_dw_by<V>(at, o, beta, left);
+    else if (grain == 4) store_dw_by<4>(at, o, beta, left);
+    else if (grain == 2) store_dw_by<2>(at, o, beta, left);
+    else store_dw_by<1>(at, o, beta, left);
 }
 
 template <typename T, int R>
@@ -1299,6 +1384,10 @@ few_bwd_kernel(const Few p)
     dep_release();
     const int64_t step = static_cast<int64_t>(gridDim.x) * p.chunk;
     int64_t v = static_cast<int64_t>(blockIdx.x) * p.chunk;
+    for (int r = warp; r < 2 * p.chunk; r += kFewWarps)
+    {
+        for (int c = p.dim + lane; c < p.padded; c += 32) stage[r * p.padded + c] = from_f32<T>(0.0f);
+    }
     if (v < p.vocab) stage_head<T>(p, stage, v);
     stage_rows<T, R>(p, 0, xs, true);
     if (threadIdx.x == 0)
@@ -1398,8 +1487,8 @@ few_bwd_kernel(const Few p)
                         o[i] = sum * coef;
                     }
                     const int64_t at = (v + k) * p.lddw + col;
-                    if (p.dw_f32) store_dw(static_cast<float*>(p.dw) + at, o, p.dw_vec, p.dw_beta, p.dim - col);
-                    else store_dw(static_cast<bf16*>(p.dw) + at, o, p.dw_vec, p.dw_beta, p.dim - col);
+                    if (p.dw_f32) store_dw(static_cast<float*>(p.dw) + at, o, p.dw_grain, p.dw_beta, p.dim - col);
+                    else store_dw(static_cast<bf16*>(p.dw) + at, o, p.dw_grain, p.dw_beta, p.dim - col);
                 }
             }
         }
@@ -1469,13 +1558,18 @@ few_dx_kernel(const Few p, int blocks, T* __restrict__ dx, int64_t lddx)
 // Where rows x vocab x dim is below 2^25 the tensor-core path is all launch latency (the tiny decoder's
 // step: nine launches, 43 us). Such a problem takes four: the pairs and their merge as above, rows in
 // groups of four, then q, kept in fp32, and both products in 32 x 32 tiles.
-// Blocks below gx: tiles of dx = coef q W; the others: of dW = coef q^T x.
+constexpr int kSmallTerms = 128;
+
+// Blocks below gx: tiles of dx = coef q W; the others: of dW = coef q^T x. Each chunk of 128 terms costs a round
+// trip (5 us), so the terms of a tile are cut among parts_x or parts_w blocks of a cluster of up to eight, and
+// each adds up, in the blocks' order, the rows of the tile that fall to it: 6 x 812 x 128 in one block a
+// tile took 38 us, @SG@ cut.
 template <typename T>
 __global__ void __launch_bounds__(256)
-small_grads_kernel(const Few p, int gx, int tiles_d)
+small_grads_kernel(const Few p, int gx, int tiles_d, int parts_x, int parts_w)
 {
     // 128 terms at a time, all their loads under way at once: the time is the latency of these rounds
-    constexpr int K = 128;
+    constexpr int K = kSmallTerms;
     __shared__ __align__(16) float a[K][36], b[K][36];   // [k][m], [k][n]
     __shared__ int counts[8];
     __shared__ bool use[1024];   // rows that are counted
@@ -1483,9 +1577,13 @@ small_grads_kernel(const Few p, int gx, int tiles_d)
     dep_release();
     const int tid = static_cast<int>(threadIdx.x);
     const bool dw = static_cast<int>(blockIdx.x) >= gx;
-    const int tile = static_cast<int>(blockIdx.x) - (dw ? gx : 0);
+    const int parts = dw ? parts_w : parts_x;
+    const int block = static_cast<int>(blockIdx.x) - (dw ? gx : 0), tile = block / parts, part = block - tile * parts;
+    // blocks that fill the last cluster have rows past the end
     const int m0 = tile / tiles_d * 32, d0 = tile % tiles_d * 32;
-    const int terms = dw ? p.rows : static_cast<int>(p.vocab), ms = dw ? static_cast<int>(p.vocab) : p.rows;
+    const int all = dw ? p.rows : static_cast<int>(p.vocab), ms = dw ? static_cast<int>(p.vocab) : p.rows;
+    const int each = ((all + K - 1) / K + parts - 1) / parts * K, begin = part * each;
+    const int terms = m0 < ms ? min(all, begin + each) : 0;
     const T* x = static_cast<const T*>(p.x);
     const T* w = static_cast<const T*>(p.w);
     const int tx = tid & 31, ty = tid >> 5;   // column; rows 4 ty ..
@@ -1512,7 +1610,7 @@ small_grads_kernel(const Few p, int gx, int tiles_d)
             }
         }
     };
-    fetch(0);
+    if (begin < terms) fetch(begin);
     int n = 0, bad = 0;
     for (int i = tid; i < p.rows; i += 256)
     {
@@ -1535,7 +1633,7 @@ small_grads_kernel(const Few p, int gx, int tiles_d)
     // four slices of the terms, 64 threads each, a thread 4 x 4 of the tile
     const int slice = tid >> 6, om = (tid >> 3 & 7) * 4, on = (tid & 7) * 4;
     float acc[4][4] = {};
-    for (int k0 = 0; k0 < terms; k0 += K)
+    for (int k0 = begin; k0 < terms; k0 += K)
     {
 #pragma unroll
         for (int i = 0; i < K / 8; ++i)
@@ -1579,17 +1677,27 @@ small_grads_kernel(const Few p, int gx, int tiles_d)
         for (int l = 0; l < 4; ++l) sums[(slice * 32 + om + i) * 32 + on + l] = acc[i][l];
     }
     __syncthreads();
-    if (d0 + tx >= p.dim)
-    {
-        return;
-    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
     {
-        const int y = ty + 8 * i, m = m0 + y;
-        if (m >= ms) continue;
-        const float* at_sum = sums + y * 32 + tx;
-        const float v = (((at_sum[0] + at_sum[1024]) + at_sum[2048]) + at_sum[3072]) * coef;
+        float* at = sums + (ty + 8 * i) * 32 + tx;
+        at[0] = ((at[0] + at[1024]) + at[2048]) + at[3072];
+    }
+    pair::cluster_arrive();   // the blocks' sums are there
+    pair::cluster_wait();
+    const int first = static_cast<int>(pair::cluster_rank()) - part, share = 32 / parts;
+    for (int y = part * share + ty; y < (part + 1) * share; y += 8)
+    {
+        const int m = m0 + y;
+        if (m >= ms || d0 + tx >= p.dim) continue;
+        float v = 0.0f;
+        for (int b = 0; b < parts; ++b)
+        {
+            float o;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o) : "r"(pair::peer_addr(sums + y * 32 + tx, first + b)));
+            v += o;
+        }
+        v *= coef;
         if (!dw)
         {
             static_cast<T*>(p.dx)[m * p.lddx + d0 + tx] = from_f32<T>(v);
@@ -1605,6 +1713,7 @@ small_grads_kernel(const Few p, int gx, int tiles_d)
             *at = __float2bfloat16_rn(p.dw_beta ? __bfloat162float(*at) + v : v);
         }
     }
+    pair::cluster_sync();   // no block leaves while another may still read its sums
 }
 
 // ---- host ------------------------------------------------------------------------------------
@@ -1650,10 +1759,22 @@ int tile_width(int dtype) { return dtype == VEDA_F32 ? 128 : 256; }
 // the tensor tiles take 98 / 288 for 9.
 bool is_few(int64_t rows, int64_t dim) { return rows <= kFewRows && dim <= 2048; }
 
-// Problems whose products the CUDA cores finish within the latency of the tensor-core path's launches.
-bool is_small(int64_t rows, int64_t vocab, int64_t dim)
+// Problems whose products the CUDA cores finish within the latency of the tensor-core path's launches, which
+// is longer in fp32 and for odd widths (operands to lay out). Steps, here / tensor cores: bf16 16 x 1000 x 64
+// 18.7 / 25.3 us, 8 x 4000 x 64 38 / 26, 5 x 600 x 1000 43 / 33, 128 x 512 x 64 25.7 / 25.6; fp32 128 x 512 x 64
+// 23.3 / 34, 207 x 766 x 64 32.8 / 34.6, 500 x 500 x 64 42.5 / 36.5, 32 x 2000 x 256 39.0 / 37.8.
+bool is_small(int64_t rows, int64_t vocab, int64_t dim, int dtype)
 {
-    return rows <= 1024 && vocab <= 4096 && dim <= 1024 && rows * vocab * dim <= (1 << 25);
+    if (rows > 1024 || vocab > 4096 || dim > 1024)
+    {
+        return false;
+    }
+    const int64_t products = rows * vocab * dim;
+    if (dtype == VEDA_BF16 && dim % 8 == 0)
+    {
+        return products <= (1 << 22) && vocab <= 1024 && vocab * dim <= (1 << 18);
+    }
+    return products <= (1 << 23);
 }
 
 Layout layout(int64_t rows, int64_t vocab, int64_t dim, bool pack_x, bool pack_w, int dtype, bool backward)
@@ -1665,7 +1786,7 @@ Layout layout(int64_t rows, int64_t vocab, int64_t dim, bool pack_x, bool pack_w
         at += static_cast<size_t>(round_up(bytes, 256));
         return here;
     };
-    if (is_few(rows, dim) || is_small(rows, vocab, dim))
+    if (is_few(rows, dim) || is_small(rows, vocab, dim, dtype))
     {
         l.done = take(4);
         l.parts = take(kFewBlocks * rows * 8);
@@ -1873,6 +1994,18 @@ int check(Call& c, void* workspace, size_t bytes, bool backward, const char* nam
     return VEDA_OK;
 }
 
+// Elements of a row that can be accessed at a time: 8 (of fp32 by 16 bytes twice), 4, 2 or 1.
+int grain(const void* base, int64_t ld, int dtype)
+{
+    const int64_t size = dtype == VEDA_BF16 ? 2 : 4;
+    for (int64_t g = 8; g > 1; g /= 2)
+    {
+        const int64_t bytes = std::min<int64_t>(16, g * size);
+        if (reinterpret_cast<uintptr_t>(base) % bytes == 0 && ld * size % bytes == 0) return static_cast<int>(g);
+    }
+    return 1;
+}
+
 // ---- few rows, host -----------------------------------------------------------------------------
 Few few_params(const Call& c, const int64_t* targets, int64_t ignore, int* status)
 {
@@ -1887,8 +2020,8 @@ Few few_params(const Call& c, const int64_t* targets, int64_t ignore, int* statu
     p.vocab = c.vocab;
     p.targets = targets;
     p.ignore = ignore;
-    const int64_t v = c.dtype == VEDA_BF16 ? 8 : 4;
-    p.vec = aligned16(c.w) && c.ldw % v == 0 && c.dim % 8 == 0;
+    p.grain = grain(c.w, c.ldw, c.dtype);
+    while (c.dim % p.grain != 0) p.grain /= 2;
     p.parts = reinterpret_cast<float2*>(c.ws + c.l.parts);
     p.target_logit = reinterpret_cast<float*>(c.ws + c.l.target_logit);
     p.acc = reinterpret_cast<float*>(c.ws + c.l.acc);
@@ -1926,7 +2059,10 @@ int launch_few_fwd(const Few& p, int* blocks, cudaStream_t s)
     const int groups = (p.rows + R - 1) / R;
     *blocks = few_blocks(p.vocab, 4 * kFewWarps, few_fwd_per_sm(R), groups);
     const int smem = R * p.padded * 4;
-    const auto kernel = p.vec ? few_fwd_kernel<T, R, true, Q> : few_fwd_kernel<T, R, false, Q>;
+    const auto kernel = p.grain == 8   ? few_fwd_kernel<T, R, 8, Q>
+                        : p.grain == 4 ? few_fwd_kernel<T, R, 4, Q>
+                        : p.grain == 2 ? few_fwd_kernel<T, R, 2, Q>
+                                       : few_fwd_kernel<T, R, 1, Q>;
     if (!allow_smem(kernel, smem))
     {
         return fail(VEDA_ERR_CUDA, "veda_linear_cross_entropy: shared memory");
@@ -1948,6 +2084,34 @@ int launch_few_bwd(Few p, int* blocks, cudaStream_t s)
         return fail(VEDA_ERR_CUDA, "veda_linear_cross_entropy_bwd: shared memory");
     }
     return launch("veda_linear_cross_entropy_bwd", few_bwd_kernel<T, R>, dim3(*blocks), dim3(kFewThreads), smem, s, p);
+}
+
+// As launch(), in clusters of `cluster` blocks.
+template <typename... Params, typename... Args>
+int launch_clusters(const char* what, void (*kernel)(Params...), int blocks, int threads, int cluster, cudaStream_t s,
+                    Args&&... args)
+{
+    cudaLaunchAttribute attrs[2]{};
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attrs[0].val.clusterDim.y = 1;
+    attrs[0].val.clusterDim.z = 1;
+    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.stream = s;
+    cfg.attrs = attrs;
+    cfg.numAttrs = overlapped_launches() ? 2 : 1;
+    count_launch();
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+    if (err != cudaSuccess)
+    {
+        cudaGetLastError();
+        return fail(VEDA_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(err));
+    }
+    return check_launch(what);
 }
 
 int launch_merge(const float2* parts, int slots, int64_t rows, int64_t vocab, const int64_t* targets, int64_t ignore,
@@ -1993,9 +2157,18 @@ int small_bwd(const Call& c, const int64_t* targets, int64_t ignore, const float
     const int rc = launch_few_fwd<T, 4, true>(p, &blocks, s);
     if (rc != VEDA_OK) return rc;
     const int tiles_d = (p.dim + 31) / 32;
-    const int gx = dx != nullptr ? (p.rows + 31) / 32 * tiles_d : 0;
-    const int gw = dw != nullptr ? static_cast<int>((c.vocab + 31) / 32) * tiles_d : 0;
-    return launch("veda_linear_cross_entropy_bwd", small_grads_kernel<T>, dim3(gx + gw), dim3(256), 0, s, p, gx, tiles_d);
+    const auto parts_of = [](int64_t terms) {
+        int k = 1;
+        while (k < 8 && k * kSmallTerms < terms) k *= 2;
+        return k;
+    };
+    const int parts_x = parts_of(c.vocab), parts_w = parts_of(p.rows);
+    const int cluster = std::max(dx != nullptr ? parts_x : 1, dw != nullptr ? parts_w : 1);
+    const auto whole = [&](int64_t blocks) { return static_cast<int>(round_up(blocks, cluster)); };
+    const int gx = dx != nullptr ? whole((p.rows + 31) / 32 * tiles_d * parts_x) : 0;
+    const int gw = dw != nullptr ? whole((c.vocab + 31) / 32 * tiles_d * parts_w) : 0;
+    if (gx + gw == 0) return VEDA_OK;
+    return launch_clusters("veda_linear_cross_entropy_bwd", small_grads_kernel<T>, gx + gw, 256, cluster, s, p, gx, tiles_d, parts_x, parts_w);
 }
 
 template <typename T>
@@ -2009,7 +2182,9 @@ int few_bwd(const Call& c, const int64_t* targets, int64_t ignore, const float* 
     p.lddw = lddw;
     p.dw_f32 = dtype_dw == VEDA_F32;
     p.dw_beta = beta;
-    p.dw_vec = aligned16(dw) && lddw % (p.dw_f32 ? 4 : 8) == 0;
+    // groups of 4 or 2 have to end with the row; where groups of 8 do not, the last columns are written singly
+    p.dw_grain = grain(dw, lddw, dtype_dw);
+    while (p.dw_grain < 8 && c.dim % p.dw_grain != 0) p.dw_grain /= 2;
     if (dx == nullptr) p.acc = nullptr;
     int blocks = 0;
     int rc = p.rows == 1   ? launch_few_bwd<T, 1>(p, &blocks, s)
@@ -2062,7 +2237,7 @@ extern "C" int veda_linear_cross_entropy_fwd(const void* x, int64_t ldx, const v
     lce::Call c{x, w, ldx, ldw, rows, vocab, dim, dtype};
     int rc = lce::check(c, workspace, workspace_bytes, false, "veda_linear_cross_entropy_fwd");
     if (rc != VEDA_OK) return rc;
-    if (lce::is_few(rows, dim) || lce::is_small(rows, vocab, dim))
+    if (lce::is_few(rows, dim) || lce::is_small(rows, vocab, dim, dtype))
     {
         return dtype == VEDA_BF16
                    ? lce::few_fwd<bf16>(c, targets, ignore_index, row_loss, lse, loss, status, stream)
@@ -2132,7 +2307,7 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
                                   : lce::few_bwd<float>(c, targets, ignore_index, lse, upstream, dx, lddx, dw, lddw,
                                                         dtype_dw, beta_dw != 0.0f, status, stream);
     }
-    if (lce::is_small(rows, vocab, dim))
+    if (lce::is_small(rows, vocab, dim, dtype))
     {
         return dtype == VEDA_BF16 ? lce::small_bwd<bf16>(c, targets, ignore_index, lse, upstream, dx, lddx, dw, lddw,
                                                          dtype_dw, beta_dw != 0.0f, status, stream)
