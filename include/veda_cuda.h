@@ -245,15 +245,16 @@ int veda_mean_f64(const float* v, int64_t n, float* out, double* out_f64, veda_s
 /*        device float, NULL = 1), dx = coef q w in dtype (overwritten) and dw = coef q^T x + */
 /*        beta_dw dw in dtype_dw (VEDA_F32, or VEDA_BF16 for bf16 operands; beta_dw 0 or 1).  */
 /*        lse is the forward's. dx or dw may be NULL. In bf16, q is rounded to bf16 before    */
-/*        the gradient products, as veda_cross_entropy's dlogits are.                         */
+/*        the gradient products, as veda_cross_entropy's dlogits are (not where there are up  */
+/*        to four rows or few products, which run in fp32 without the tensor cores).          */
 /* Operands: any pitch >= dim and any element-aligned base; where a base is not 16-byte       */
 /* aligned or a pitch no multiple of 8 (bf16; always for fp32) an operand is laid out in the  */
 /* workspace first. The workspace (256-byte aligned, contents undefined before and after) is  */
 /* sized by veda_linear_cross_entropy_workspace; pass a pitch of 1 for an operand whose base  */
 /* is not 16-byte aligned. The largest size with backward = 0 and 1 serves both calls. Results */
-/* repeat bit for bit. fp32 operands are multiplied on the tensor cores as pairs of fp16      */
-/* values (22 bits); magnitudes below 2^-39 of an operand's largest, and of q below 2^-38,    */
-/* are lost.                                                                                  */
+/* repeat bit for bit. Where the tensor cores run, fp32 operands are multiplied as pairs of   */
+/* fp16 values (22 bits); magnitudes below 2^-39 of an operand's largest, and of q below      */
+/* 2^-38, are lost.                                                                           */
 /* ---------------------------------------------------------------------------------------- */
 size_t veda_linear_cross_entropy_workspace(int64_t rows, int64_t vocab, int64_t dim, int64_t ldx,
                                            int64_t ldw, int dtype, int backward);
@@ -341,15 +342,17 @@ int veda_adamw_step_dev(float* master, float* m, float* v, float* g, void* lowp,
 /* reference, whose optimiser is AdamW).                                                      */
 /* ---------------------------------------------------------------------------------------- */
 /* Per matrix of the batch: X = g / (|g|_F + eps), then `steps` times X <- a X + (b S + c S^2) X
- * with S = X X^T, taken on the smaller side; out = X. dtype is that of g and out. The usual
+ * with S = X X^T, taken on the smaller side; out = X. dtype is that of g and out; 1 <= steps <= 64. The usual
  * coefficients are 3.4445, -4.7750, 2.0315 with 5 steps, which bring every singular value that is
  * not tiny to about 1; others must keep the singular values of X, and |a|, |b| + |c|, below 16.
- * bf16 matrices are multiplied in fp16 from an X held in two fp16 values (22 bits); fp32 ones as
- * pairs of fp16 values throughout. Row r, column c of matrix k is g[k stride_g + r ldg + c], any
+ * bf16 matrices are multiplied in fp16 from an X held in two fp16 values (22 bits); fp32 ones, and most with a
+ * side of at most 128, as pairs of fp16 values throughout. Row r, column c of matrix k is g[k stride_g + r ldg + c], any
  * alignment; out may be g. A zero matrix stays zero; a matrix that is not finite gives NaN in
  * itself alone. The workspace (256-byte aligned, contents undefined before and after) is sized by
  * veda_orthogonalize_workspace (0 for an empty or refused shape). batch <= 2^15, rows and cols <=
- * 2^20. Results repeat bit for bit and do not depend on the batch a matrix is in. */
+ * 2^20. Results repeat bit for bit. They do not depend on the batch a matrix is in, unless its smaller side is
+ * 65 to 128 and its longer one above 512: a batch that fills the GPU then takes another form, which rounds
+ * otherwise. */
 size_t veda_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, int dtype);
 int veda_orthogonalize(const void* g, int64_t ldg, int64_t stride_g, void* out, int64_t ldo,
                        int64_t stride_o, int64_t batch, int64_t rows, int64_t cols, int steps,
