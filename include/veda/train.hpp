@@ -218,7 +218,8 @@ public:
     // The loss as autograd::linear_cross_entropy_device (on) instead of the LM head's logits and
     // their cross-entropy (off, the default): the step never holds the [B*T, V] logits and their
     // gradient, in exchange for forming the logits twice. Targets of autograd::kIgnoreTarget are then
-    // not counted. A captured step graph is dropped and captured again.
+    // not counted; the mean is over a rank's own counted targets. A captured step graph is dropped and captured
+    // again.
     void set_linear_loss(bool on);
     // Muon for the hidden matrices (q/k/v/o, gate/up/down of every layer), AdamW for the rest. Their
     // momentum is the optimizer's first moment, so checkpoints keep it. Not with a sharded optimizer.

@@ -202,6 +202,9 @@ int main()
         bad = {};
         bad.steps = 0;
         report("muon_refuses_no_steps", throws<std::invalid_argument>([&] { optim::Muon m(ps, bad); }));
+        bad.steps = 65;
+        report("muon_refuses_too_many_steps", throws<std::invalid_argument>([&] { optim::Muon m(ps, bad); }));
+        report("muon_refuses_a_parameter_twice", throws<std::invalid_argument>([&] { optim::Muon m({ps[0], ps[0]}); }));
     }
     {
         // beside AdamW: a taken parameter is left to Muon, and given back with it
@@ -223,6 +226,7 @@ int main()
             muon.launch(adam.sumsq(), 100.0f, 1.0f);
             report("muon_updates_taken", b.value().to_host() != b0);
             report("refuses_taken_twice", throws<std::invalid_argument>([&] { optim::Muon again(adam, {1}); }));
+            report("refuses_an_index_twice", throws<std::invalid_argument>([&] { optim::Muon again(adam, {0, 0}); }));
             report("refuses_index", throws<std::invalid_argument>([&] { optim::Muon again(adam, {2}); }));
         }
         const std::vector<float> b1 = b.value().to_host();

@@ -10,6 +10,7 @@
 #include <cstdint>
 #include <stdexcept>
 #include <string>
+#include <unordered_set>
 
 namespace veda::optim
 {
@@ -289,12 +290,17 @@ void Muon::check_config() const
     {
         throw std::invalid_argument("Muon: momentum must lie in [0, 1)");
     }
-    if (c.steps == 0)
+    if (c.steps == 0 || c.steps > 64)   // veda_muon_step's range, refused before a step is half made
     {
-        throw std::invalid_argument("Muon: at least one Newton-Schulz step");
+        throw std::invalid_argument("Muon: 1 to 64 Newton-Schulz steps");
     }
+    std::unordered_set<const void*> seen;
     for (const auto& p : parameters_)
     {
+        if (!seen.insert(p.node().get()).second)
+        {
+            throw std::invalid_argument("Muon: a parameter is given twice");
+        }
         if (p.value().rank() != 2)
         {
             throw std::invalid_argument("Muon: a parameter of shape " + p.value().shape().to_string() +

@@ -1677,6 +1677,7 @@ small_grads_kernel(const Few p, int gx, int tiles_d, int parts_x, int parts_w)
         __syncthreads();
     }
     // the slices' sums meet in shared memory, added in order
+    constexpr int kSum = 32 * 32;
     float* const sums = &a[0][0];   // [slice][32][32]
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -1689,7 +1690,7 @@ small_grads_kernel(const Few p, int gx, int tiles_d, int parts_x, int parts_w)
     for (int i = 0; i < 4; ++i)
     {
         float* at = sums + (ty + 8 * i) * 32 + tx;
-        at[0] = ((at[0] + at[1024]) + at[2048]) + at[3072];
+        at[0] = ((at[0] + at[kSum]) + at[2 * kSum]) + at[3 * kSum];
     }
     pair::cluster_arrive();   // the blocks' sums are there
     pair::cluster_wait();
