@@ -143,7 +143,7 @@ template <int TN_>
 struct StatsWork
 {
     using Params = lce::Params;
-    static constexpr int TN = TN_;
+    static constexpr int TN = TN_, CHAIN = 4;
     struct Tile
     {
         bool skip, first, last, a_mn, b_mn;
@@ -280,7 +280,7 @@ template <int TN_>
 struct GradWork
 {
     using Params = lce::Params;
-    static constexpr int TN = TN_;
+    static constexpr int TN = TN_, CHAIN = 4;
     struct Tile
     {
         bool skip, a_mn, b_mn;

@@ -16,12 +16,13 @@
 // SPLIT: operands are pairs of fp16 planes, value = hi + lo, and a product is hi lo + lo hi + hi hi.
 // The tensor core truncates as it adds into its accumulator, an error of some 2^-25 of the running
 // sum per 16 terms and always towards zero: sums of 10000 terms came out 3e-5 short. So the small
-// products go first, and every kChain k-blocks the accumulator is folded into a running sum kept in
-// another part of TMEM, rounded to nearest (1e-6 and less). With TN = 128 two accumulators and the sum
-// fit, and a fold runs under the next chain's products; with TN = 256 the accumulator has no second
-// buffer then, and the products wait for it.
+// products go first, and every CHAIN k-blocks the accumulator is folded into a running sum kept in
+// another part of TMEM, rounded to nearest (some 3e-7 of the sum remain for chains of 4 k-blocks). With
+// TN = 128 two accumulators and the sum fit, and a fold runs under the next chain's products; with TN = 256
+// the accumulator has no second buffer then, and the products wait for it.
 //
 // Work provides
+//   int TN, CHAIN                      columns of a tile; SPLIT: k-blocks between folds
 //   struct Params                      the kernel's argument (tensor maps, pointers, sizes, status)
 //   struct Tile { bool skip; int kbs; uint32_t idesc; bool a_mn, b_mn; ... }
 //   bool tile(p, cid, clusters, i, t)  the i-th tile of cluster cid; false at the end of its list
@@ -41,7 +42,6 @@ namespace veda::cuda::pair
 
 constexpr int kTile = 256;   // tile rows of a CTA pair, and columns unless the Work has TN = 128
 constexpr int kBK = 64;      // k-block: 64 16-bit values, one 128-byte swizzle row
-constexpr int kChain = 4;    // SPLIT: k-blocks between folds
 
 template <int EPI_WARPS_, int TN = kTile>
 struct Cfg
@@ -310,9 +310,9 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
                 }
                 else
                 {
-                    for (int k0 = 0; k0 < t.kbs; k0 += kChain)
+                    for (int k0 = 0; k0 < t.kbs; k0 += Work::CHAIN)
                     {
-                        const int k1 = min(t.kbs, k0 + kChain);
+                        const int k1 = min(t.kbs, k0 + Work::CHAIN);
                         for (int kb = k0; kb < k1; ++kb) load(kb, 0, 1);
                         for (int kb = k0; kb < k1; ++kb) load(kb, 1, 0);
                         for (int kb = k0; kb < k1; ++kb) load(kb, 0, 0);
@@ -339,9 +339,9 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
             }
             const uint32_t astep = (t.a_mn ? 2048 : 32) / 16, bstep = (t.b_mn ? 2048 : 32) / 16;   // 16 terms on
             const uint32_t albo = t.a_mn ? kBK * 128 : 16, blbo = t.b_mn ? kBK * 128 : 16;
-            for (int k0 = 0; !t.skip && k0 < t.kbs; k0 += SPLIT ? kChain : t.kbs)
+            for (int k0 = 0; !t.skip && k0 < t.kbs; k0 += SPLIT ? Work::CHAIN : t.kbs)
             {
-                const int blocks = SPLIT ? 3 * (min(t.kbs, k0 + kChain) - k0) : t.kbs;
+                const int blocks = SPLIT ? 3 * (min(t.kbs, k0 + Work::CHAIN) - k0) : t.kbs;
                 const int buf = TWO ? it & 1 : 0;
                 mbar_wait(&tempty[buf], ((TWO ? it >> 1 : it) & 1) ^ 1, p.status, abort);
                 __syncwarp();
@@ -399,17 +399,17 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
                 Work::before(p, t, state, row0, col0, st, lane, abort);
             }
             const bool more_next = Work::tile(p, cid, clusters, ++i, next);
-            for (int k0 = 0; !t.skip && k0 < t.kbs; k0 += SPLIT ? kChain : t.kbs)
+            for (int k0 = 0; !t.skip && k0 < t.kbs; k0 += SPLIT ? Work::CHAIN : t.kbs)
             {
                 const int buf = TWO ? it & 1 : 0;
                 mbar_wait(&tfull[buf], (TWO ? it >> 1 : it) & 1, p.status, abort);
                 fence_after();
                 const uint32_t base = tmem + static_cast<uint32_t>(buf * TN + col0) +
                                       (static_cast<uint32_t>(quarter * 32) << 16);
-                const bool last = !SPLIT || k0 + kChain >= t.kbs;
+                const bool last = !SPLIT || k0 + Work::CHAIN >= t.kbs;
                 if constexpr (SPLIT)
                 {
-                    if (t.kbs > kChain)
+                    if (t.kbs > Work::CHAIN)
                     {
                         fold<COLS>(base, base - buf * TN + (TWO ? 2 : 1) * TN, k0 == 0, last);
                     }
