@@ -365,8 +365,8 @@ int veda_orthogonalize(const void* g, int64_t ldg, int64_t stride_g, void* out, 
  *   momentum <- beta momentum + g;  u = nesterov ? g + beta momentum : momentum;
  *   master <- master - lr weight_decay master - lr update_scale orthogonalize(u);
  *   lowp <- bf16(master).
- * The products run as for bf16 matrices when lowp is given, else as for fp32 ones
- * (veda_orthogonalize). flags: VEDA_ADAMW_SKIP_NONFINITE leaves everything untouched when the norm
+ * The products run as for bf16 matrices when lowp is given and both sides are above 64, else as for fp32
+ * ones (veda_orthogonalize). flags: VEDA_ADAMW_SKIP_NONFINITE leaves everything untouched when the norm
  * is not finite. grad is not written. The workspace's dtype is VEDA_BF16 when lowp is given, else
  * VEDA_F32. */
 size_t veda_muon_step_workspace(int64_t batch, int64_t rows, int64_t cols, int dtype);

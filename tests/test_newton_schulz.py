@@ -378,6 +378,20 @@ def test_muon_on_matrices_cut_among_blocks(cuda, bf16, b, r, c):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("b,r,c", [(1, 32, 4200), (2, 4203, 40)])
+def test_muon_of_thin_matrices_keeps_the_weights_exact(cuda, b, r, c):
+    # 30 to 50 singular values amplify what fp16 products round most: beside bf16 weights, too, such matrices
+    # are multiplied as fp32 ones, within their bound
+    master, momentum, grad, lowp = muon_state(b, r, c, True, seed=9)
+    w, m, u, o, _ = muon_want(master, momentum, grad)
+    muon(master, momentum, grad, lowp, (b, r, c), r * c)
+    sync()
+    tol = 1e-2 * 1.7 * (bound(u, o, V.F32, True) + 310 * 3 * 2.0 ** -24 * fro(o)) + 4 * 2.0 ** -24 * fro(w)
+    assert bool((fro(master.double() - w) <= tol).all())
+    assert bool((lowp == master.to(torch().bfloat16)).all())
+
+
+@pytest.mark.gpu
 def test_muon_skips_a_step_that_is_not_finite(cuda):
     t = torch()
     state = muon_state(2, 48, 80, True, seed=3)

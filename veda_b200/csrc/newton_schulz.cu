@@ -1765,6 +1765,11 @@ int products(const char* what, int64_t batch, int64_t rows, int64_t cols, int st
     return pair::launch_together<W, 8, SPLIT>(what, p, static_cast<int>(std::min<int64_t>(most, clusters)), stream);
 }
 
+// Whether Muon's products are split: for fp32 weights, and for matrices of some 30 to 50 rows or columns
+// whose other side is too long for a cluster, on which fp16 products come out least exact (fp32 weights off by
+// 1.1e-5 at 32 x 4200, 3e-6 at 64; split 4e-8).
+bool muon_split(int64_t rows, int64_t cols, bool lowp) { return !lowp || std::min(rows, cols) <= 64; }
+
 // norm, X, then the products of every step; p's destination says what the last one (LAST) writes.
 template <typename T, bool SPLIT, int LAST>
 int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, int64_t cols, int steps, float a,
@@ -1790,7 +1795,8 @@ int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, in
     const int64_t stride = batch == 1 ? rows * p.ldo : p.stride_o;
     const bool f32 = LAST == kMuon || SPLIT;
     p.out_f32 = f32;
-    p.vec = fits(p.dst, f32 ? 4 : 2) && (p.lowp == nullptr || fits(p.lowp, 2)) &&
+    // the split form's chunks leave no room to stage the bf16 weights in
+    p.vec = !(SPLIT && p.lowp != nullptr) && fits(p.dst, f32 ? 4 : 2) && (p.lowp == nullptr || fits(p.lowp, 2)) &&
             pair::make_map3(&p.dst_out, p.dst, f32 ? 4 : 2, !f32, cols, rows, batch, p.ldo, stride, 32, 32,
                             f32 ? pair::Swizzle::k128 : pair::Swizzle::k64) &&
             (p.lowp == nullptr || pair::make_map3(&p.lowp_out, p.lowp, 2, true, cols, rows, batch, p.ldo, stride, 32, 32,
@@ -1850,7 +1856,8 @@ extern "C" size_t veda_orthogonalize_workspace(int64_t batch, int64_t rows, int6
 
 extern "C" size_t veda_muon_step_workspace(int64_t batch, int64_t rows, int64_t cols, int dtype)
 {
-    return veda_orthogonalize_workspace(batch, rows, cols, dtype);
+    return veda_orthogonalize_workspace(batch, rows, cols,
+                                        dtype == VEDA_BF16 && ns::muon_split(rows, cols, true) ? VEDA_F32 : dtype);
 }
 
 extern "C" int veda_orthogonalize(const void* g, int64_t ldg, int64_t stride_g, void* out, int64_t ldo,
@@ -1904,7 +1911,7 @@ extern "C" int veda_muon_step(float* master, float* momentum, const float* grad,
         return VEDA_OK;
     }
     VEDA_REQUIRE(master != nullptr && momentum != nullptr && grad != nullptr, "null pointer");
-    const bool split = lowp == nullptr;
+    const bool split = ns::muon_split(rows, cols, lowp != nullptr);
     int rc = ns::check_workspace("veda_muon_step", workspace, workspace_bytes,
                                  ns::layout(batch, rows, cols, split, ns::kMaxSteps).total);
     if (rc != VEDA_OK) return rc;
