@@ -1628,12 +1628,15 @@ int launch_small(const char* what, Small p, int64_t batch, bool split, cudaStrea
         if (ok && cluster)
         {
             cfg.dynamicSmemBytes = kMost;
-            ok = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters > 0;
+            ok = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess;
             cfg.dynamicSmemBytes = smem;
         }
         cudaGetLastError();
         room = ok ? 1 + clusters : 1;
-        known[device][p.ranks].store(room, std::memory_order_release);
+        if (ok)   // an error is not an answer: asked again at the next call
+        {
+            known[device][p.ranks].store(room, std::memory_order_release);
+        }
     }
     // One block a matrix, or smaller sides of at most 64, are always worth it. Of larger ones the
     // tiled form, which fills the device, does more matrices in the time (the more so in bf16, where
