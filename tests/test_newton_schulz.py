@@ -423,6 +423,26 @@ def test_muon_steps_from_a_graph(cuda):
     assert all(bool((a == b).all()) for a, b in zip(state, other))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [V.BF16, V.F32])
+@pytest.mark.parametrize("b,r,c", [(20, 260, 520), (2, 519, 267)])
+def test_ragged_tiles_repeat_bit_for_bit(cuda, dtype, b, r, c):
+    # warps with rows or columns past the end leave a tile early, and their next one may be of another product
+    g = make(b, r, c, dtype, seed=r, kind="spiked")
+    first, want = orth(g, dtype=dtype), exact(g)
+    assert bool((fro(first.double() - want) <= bound(g, want, dtype, dtype == V.F32)).all())
+    for _ in range(8):
+        assert bool((orth(g, dtype=dtype) == first).all())
+    state = muon_state(b, r, c, dtype == V.BF16, seed=c)
+    other = [None if v is None else v.clone() for v in state]
+    muon(*state, (b, r, c), r * c)
+    for _ in range(4):
+        again = [None if v is None else v.clone() for v in other]
+        muon(*again, (b, r, c), r * c)
+        assert all(a is None or bool((a == o).all()) for a, o in zip(again, state))
+    sync()
+
+
 def test_workspaces_and_refusals_without_a_gpu():
     lib = V.lib()
     size = lib.veda_orthogonalize_workspace

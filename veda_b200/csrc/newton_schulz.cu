@@ -212,9 +212,6 @@ struct Part
     {
         if constexpr (AHEAD > 0)
         {
-            // the last tile's copies have landed (its stores are complete)
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            __syncwarp();
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j)
             {
@@ -277,6 +274,7 @@ struct Part
         const int trow = t.mb * pair::kTile + row0, tcol = t.nb * TN + col0;
         if (trow >= w.nrows || (KIND == kMuon && skipped_step(p.flags, p.sumsq, p.grad_scale)))
         {
+            landed();
             return;
         }
         const bool mirror = SYM && t.nb >= (pair::kTile / TN) * (t.mb + 1);   // right of the diagonal tiles
@@ -377,6 +375,19 @@ struct Part
                 __syncwarp();
                 next_chunk<COLS>(p, w, t, j, trow, tcol, stage, lane);
             }
+        }
+        landed();
+    }
+
+    // Chunks of rows or columns past the end are copied in (as zeros) and not used: they have landed before
+    // the warp leaves the tile, since the next one's kind may write to their units without copies of its own
+    // to wait for.
+    static __device__ __forceinline__ void landed()
+    {
+        if constexpr (AHEAD > 0)
+        {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();
         }
     }
 
