@@ -1601,11 +1601,15 @@ Variable linear_cross_entropy_impl(const LinearSaved& l, const Variable& x, cons
         {
             dx = Tensor::empty(l.xin->value.shape(), d);
         }
-        float* dw = nullptr;
+        // a weight that is no leaf may hold a gradient of its own type already
+        void* dw = nullptr;
+        DType dw_type = DType::F32;
         bool fresh = false;
         if (l.win->requires_grad)
         {
-            dw = static_cast<float*>(grad_target(*l.win, &fresh, DType::F32).data_ptr());
+            Tensor& gw = grad_target(*l.win, &fresh, DType::F32);
+            dw = gw.data_ptr();
+            dw_type = gw.dtype();
         }
         const Tensor up = as_dtype(g, DType::F32);
         const size_t bytes = veda_linear_cross_entropy_workspace(rows, V, D, l.ldx, D, dt(d), 1);
@@ -1617,7 +1621,7 @@ Variable linear_cross_entropy_impl(const LinearSaved& l, const Variable& x, cons
                                                 static_cast<const int64_t*>(targets.data_ptr()), ignore,
                                                 static_cast<const float*>(lse.data_ptr()),
                                                 static_cast<const float*>(up.data_ptr()),
-                                                dx.defined() ? dx.data_ptr() : nullptr, D, dw, D, VEDA_F32,
+                                                dx.defined() ? dx.data_ptr() : nullptr, D, dw, D, dt(dw_type),
                                                 fresh ? 0.0f : 1.0f, rows, V, D, ws.data_ptr(), bytes, flag,
                                                 dt(d), S()),
                   "linear_cross_entropy backward");
