@@ -1102,23 +1102,27 @@ void Trainer::step_impl(const Tensor& ids, const Tensor& targets)
         dp_->finish();
     }
     {
+        // every gradient is read for the norm; a Muon updates its parameters in a class of its own
         const double n = static_cast<double>(model_->parameter_count()) /
                          static_cast<double>(sharded() ? world() : 1);
-        profile::Scope scope("adamw", 0.0,
-                             n * (4.0 + 16.0 + 12.0 + (model_->dtype() == DType::BF16 ? 2.0 : 0.0)));
+        const double updated = n - (muon_ ? static_cast<double>(muon_->elements()) : 0.0);
+        const double lowp = model_->dtype() == DType::BF16 ? 2.0 : 0.0;
+        profile::Scope scope("adamw", 0.0, n * 4.0 + updated * (16.0 + 12.0 + lowp));
         if (sharded())
         {
             dp_->update(opt_->config(), max_norm_);
         }
         else
         {
-            const float scale = 1.0f / static_cast<float>(world());
-            opt_->launch_clipped(max_norm_, scale);
-            if (muon_)
-            {
-                muon_->launch(opt_->sumsq(), max_norm_, scale);
-            }
+            opt_->launch_clipped(max_norm_, 1.0f / static_cast<float>(world()));
         }
+    }
+    if (muon_)
+    {
+        // gradient read, momentum and master read and written, weights written
+        profile::Scope scope("muon", muon_->flops(),
+                             static_cast<double>(muon_->elements()) * (20.0 + (model_->dtype() == DType::BF16 ? 2.0 : 0.0)));
+        muon_->launch(opt_->sumsq(), max_norm_, 1.0f / static_cast<float>(world()));
     }
     cuda_check(cudaMemcpyAsync(loss_.data_ptr(), loss.value().data_ptr(), sizeof(float),
                                cudaMemcpyDeviceToDevice, cs()),
@@ -1136,10 +1140,6 @@ std::vector<uint8_t> to_host_bytes(const void* device, size_t count)
 }
 } // namespace
 
-void Trainer::save_checkpoint(const std::string& dir)
-{
-    sync();
-    const size_t n = model_->parameter_count();
 namespace
 {
 // "a,b=3" of a checkpoint's metadata as {a: "", b: "3"}; empty where there is no such entry.
@@ -1157,6 +1157,10 @@ std::map<std::string, std::string> listed(const std::map<std::string, std::strin
 }
 } // namespace
 
+void Trainer::save_checkpoint(const std::string& dir)
+{
+    sync();
+    const size_t n = model_->parameter_count();
     const bool bf16 = model_->dtype() == DType::BF16;
     float* master = master_weights();
     const float* m = static_cast<const float*>(opt_->first_moments().data_ptr());
@@ -1282,10 +1286,6 @@ void Trainer::load_checkpoint(const std::string& dir)
         }
         steps = static_cast<size_t>(std::stoull(it->second));
     }
-    float* dmaster = master_weights();
-    cuda_check(cudaMemcpyAsync(dmaster, master.data(), n * sizeof(float), cudaMemcpyHostToDevice, cs()),
-               "checkpoint write");
-    if (model_->dtype() == DType::BF16)
     // A Muon's momentum goes on as one where a Muon has the parameter; AdamW, which has no use for it, begins anew.
     std::vector<size_t> starts(model_->parameters().size(), 0);
     const std::map<std::string, std::string> muon = listed(state.metadata, "muon"), later = listed(state.metadata, "start");
@@ -1313,6 +1313,10 @@ void Trainer::load_checkpoint(const std::string& dir)
         ++i;
     }
     drop_step_graph();   // AdamW's runs and corrections may be others now
+    float* dmaster = master_weights();
+    cuda_check(cudaMemcpyAsync(dmaster, master.data(), n * sizeof(float), cudaMemcpyHostToDevice, cs()),
+               "checkpoint write");
+    if (model_->dtype() == DType::BF16)
     {
         check(veda_f32_to_bf16(dmaster, model_->value_arena().data_ptr(), static_cast<int64_t>(n), cs()),
               "checkpoint write");
@@ -1324,11 +1328,11 @@ void Trainer::load_checkpoint(const std::string& dir)
                                cudaMemcpyHostToDevice, cs()),
                "checkpoint write");
     opt_->set_steps(steps);
+    opt_->set_starts(starts);
     if (sharded())
     {
         dp_->load_master(dmaster);
         dp_->load_moments(static_cast<const float*>(opt_->first_moments().data_ptr()),
-    opt_->set_starts(starts);
                           static_cast<const float*>(opt_->second_moments().data_ptr()), steps);
     }
     cuda_check(cudaStreamSynchronize(cs()), "checkpoint write");
