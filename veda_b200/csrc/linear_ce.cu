@@ -58,6 +58,10 @@ __device__ __forceinline__ float ex2(float x)
     return y;
 }
 
+// A logit as a reference in log2 units, rounded up: z log2 e - reference, in one fused operation, is at most 0 then.
+// Rounded to nearest, it could be positive by 2^-24 of its size, and 2 to that power infinite above 2^31.
+__device__ __forceinline__ float log2_units(float z) { return __fmul_ru(z, kLog2e); }
+
 // Device scalars of a call: what turns a tile's sum into a logit, and the gradients' factors. The
 // powers of two stay apart from coef: their product with it could be subnormal where dx is not.
 struct Scalars
@@ -104,11 +108,11 @@ struct Params
     const int64_t* targets;
     int64_t ignore;
     const float* lse;
+    const float* row_scale;  // forward, split: 2^ex of each row of x
     float2* parts;           // [strip slots][rows] running (max, sum)
     float* target_logit;     // [rows]
     unsigned* done;          // cleared for the merge's blocks to count themselves
     int* status;
-    const float* row_scale;  // forward, split: 2^ex of each row of x
 };
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b)
@@ -260,7 +264,7 @@ struct StatsWork
             float mx[4] = {z[0], z[1], z[2], z[3]};
 #pragma unroll
             for (int j = 4; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], z[j]);
-            const float m = fmaxf(s.m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e);
+            const float m = fmaxf(s.m, log2_units(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))));
             // a row of -inf so far: any finite reference gives exponentials of 0, and NaN stays NaN
             const float ref = m == -INFINITY ? 0.0f : m;
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -631,10 +635,6 @@ __device__ __forceinline__ bool counted(int64_t t, int64_t ignore, int64_t vocab
     return t != ignore && t >= 0 && t < vocab;
 }
 
-// Largest finite magnitude of the counted rows of x (blocks below gx) and of w (the others) as one
-// partial per block; with row_scale, the scale of every row of x instead of x's partials.
-__global__ void __launch_bounds__(256)
-absmax_kernel(const float* __restrict__ x, int64_t ldx, int64_t rows, const float* __restrict__ w, int64_t ldw,
 // 2^e that brings a largest magnitude into [2^13, 2^14), clamped so that 2^e and 2^-e are normal
 // (a tensor of magnitudes below 2^-113 keeps fewer bits).
 __device__ __forceinline__ float split_scale(float top)
@@ -649,6 +649,10 @@ __device__ __forceinline__ float split_scale(float top)
     return ldexpf(1.0f, e < -120 ? -120 : e > 120 ? 120 : e);
 }
 
+// Largest finite magnitude of the counted rows of x (blocks below gx) and of w (the others) as one
+// partial per block; with row_scale, the scale of every row of x instead of x's partials.
+__global__ void __launch_bounds__(256)
+absmax_kernel(const float* __restrict__ x, int64_t ldx, int64_t rows, const float* __restrict__ w, int64_t ldw,
               int64_t vocab, int64_t dim, const int64_t* __restrict__ targets, int64_t ignore, int gx,
               float* __restrict__ part, float* __restrict__ row_scale)
 {
@@ -659,11 +663,11 @@ __device__ __forceinline__ float split_scale(float top)
     const float* m = is_w ? w : x;
     const int64_t ld = is_w ? ldw : ldx, n = is_w ? vocab : rows;
     const int64_t b = is_w ? blockIdx.x - gx : blockIdx.x, blocks = is_w ? gridDim.x - gx : gx;
+    const bool by_row = !is_w && row_scale != nullptr;
     float top = 0.0f;
     for (int64_t r = b * 8 + threadIdx.x / 32; r < n; r += blocks * 8)
     {
         if (!is_w && !by_row && !counted(targets[r], ignore, vocab))
-    const bool by_row = !is_w && row_scale != nullptr;
         {
             continue;
         }
@@ -672,10 +676,6 @@ __device__ __forceinline__ float split_scale(float top)
             const float v = fabsf(m[r * ld + c]);
             top = v <= FLT_MAX ? fmaxf(top, v) : top;
         }
-    }
-    top = warp_max(top);
-    if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = top;
-    __syncthreads();
         if (by_row)
         {
             top = warp_max(top);
@@ -686,6 +686,10 @@ __device__ __forceinline__ float split_scale(float top)
     if (by_row)
     {
         return;
+    }
+    top = warp_max(top);
+    if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = top;
+    __syncthreads();
     if (threadIdx.x == 0)
     {
         for (int k = 1; k < 8; ++k) top = fmaxf(top, warp_part[k]);
@@ -773,11 +777,11 @@ pack_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, const T* __restr
     const int64_t ld = is_w ? ldw : ldx, n = is_w ? vocab : rows;
     const int64_t b = is_w ? block - gx : block, blocks = is_w ? gw : gx;
     const float scale = part != nullptr ? scale_shared[is_w ? 1 : 0] : 1.0f;
+    const bool by_row = !is_w && row_scale != nullptr;
     const bool vec = is_w ? vw : vx;
     const int64_t per_row = ldp / 8, groups = n * per_row;   // of eight columns
 #pragma unroll 2
     for (int64_t g = b * 256 + threadIdx.x; g < groups; g += blocks * 256)
-    const bool by_row = !is_w && row_scale != nullptr;
     {
         const int64_t r = g / per_row, c = (g - r * per_row) * 8;
         const int left = static_cast<int>(dim - c < 8 ? dim - c : 8);
@@ -808,11 +812,11 @@ pack_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, const T* __restr
             for (int k = 0; k < 8; ++k) v[k] = k < left ? to_f32(m[r * ld + c + k]) : 0.0f;
         }
         uint32_t hi[4], lo[4];
+        const float own = by_row ? row_scale[r] : scale;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
         {
             if constexpr (sizeof(T) == 2)
-        const float own = by_row ? row_scale[r] : scale;
             {
                 hi[k] = pack_bf16(v[2 * k], v[2 * k + 1]);   // bf16 values: exact
             }
@@ -870,7 +874,9 @@ merge_kernel(const float2* __restrict__ parts, int slots, int64_t rows, int64_t 
     }
     if (slice == 0 && row < rows)
     {
-        const float l = (m + log2f(s)) * kLn2;
+        // a sum of 0: every term vanished against the rounding of a maximum past 2^31, whose logarithm the sum's
+        // could not change
+        const float l = (s == 0.0f ? m : m + log2f(s)) * kLn2;
         if (lse != nullptr) lse[row] = l;
         const int64_t t = targets[row];
         const bool inside = t >= 0 && t < vocab;
@@ -1258,7 +1264,7 @@ few_fwd_kernel(const Few p)
             {
                 if (v + j >= p.vocab) z[j] = -INFINITY;
                 else if (valid && target == v + j) p.target_logit[row_] = z[j];
-                top = fmaxf(top, z[j] * kLog2e);
+                top = fmaxf(top, log2_units(z[j]));
             }
             const float ref = top == -INFINITY ? 0.0f : top;
             s *= ex2(m - ref);
@@ -1829,13 +1835,13 @@ Layout layout(int64_t rows, int64_t vocab, int64_t dim, bool pack_x, bool pack_w
     l.scalars = take(sizeof(Scalars));
     l.done = take(4);
     l.part = take(2 * kMaxBlocks * 4);
+    l.row_scale = take(!backward && dtype == VEDA_F32 ? rows * 4 : 0);
     l.px = take(pack_x ? l.planes * rows * l.ldp * 2 : 0);
     l.pw = take(pack_w ? l.planes * vocab * l.ldp * 2 : 0);
     const int tn = tile_width(dtype), num_n = static_cast<int>((vocab + tn - 1) / tn), num_m = static_cast<int>((rows + 255) / 256);
     if (!backward)
     {
         // at most 74 clusters on a B200; fewer (reserved SMs) only change which strip is best
-    l.row_scale = take(!backward && dtype == VEDA_F32 ? rows * 4 : 0);
         l.strip = choose_strip(num_m, num_n, 74);
         l.slots = (num_n + l.strip - 1) / l.strip;
         l.parts = take(static_cast<int64_t>(l.slots) * 2 * rows * 8);
@@ -1940,13 +1946,13 @@ int prepare(const Call& c, const int64_t* targets, int64_t ignore, const float* 
     if (c.dtype == VEDA_F32)
     {
         part = reinterpret_cast<float*>(c.ws + c.l.part);
+        if (!c.backward) row_scale = reinterpret_cast<float*>(c.ws + c.l.row_scale);
         const int rc = launch("veda_linear_cross_entropy", absmax_kernel, dim3(gx + gw), dim3(256), 0, s,
                               static_cast<const float*>(c.x), c.ldx, c.rows, static_cast<const float*>(c.w), c.ldw,
                               c.vocab, c.dim, targets, ignore, static_cast<int>(gx), part, row_scale);
         if (rc != VEDA_OK) return rc;
     }
     const void *px = c.x, *pw = c.w;
-        if (!c.backward) row_scale = reinterpret_cast<float*>(c.ws + c.l.row_scale);
     int64_t ldx = c.ldx, ldw = c.ldw;
     if (scalars || part != nullptr || c.pack_x || c.pack_w)
     {
@@ -2000,13 +2006,13 @@ int prepare(const Call& c, const int64_t* targets, int64_t ignore, const float* 
     p.by_m = pair::Divisor(static_cast<uint32_t>(p.num_m));
     p.by_d = pair::Divisor(static_cast<uint32_t>(p.num_d));
     p.scalars = c.scalars();
+    p.row_scale = row_scale;
     p.targets = targets;
     p.ignore = ignore;
     p.status = device_status_ptr();
     return VEDA_OK;
 }
 
-    p.row_scale = row_scale;
 // Common checks; fills c and its layout.
 int check(Call& c, void* workspace, size_t bytes, bool backward, const char* name)
 {
