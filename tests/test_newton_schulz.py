@@ -443,75 +443,6 @@ def test_ragged_tiles_repeat_bit_for_bit(cuda, dtype, b, r, c):
     sync()
 
 
-@pytest.mark.gpu
-@pytest.mark.parametrize("dtype", [V.BF16, V.F32])
-@pytest.mark.parametrize("r,c", [(20, 30), (40, 600), (300, 280), (135, 50)])
-def test_zero_matrices_without_eps(cuda, dtype, r, c):
-    # eps = 0 leaves nothing to divide by; in one block, cut among blocks and tiled
-    t = torch()
-    g = make(3, r, c, dtype, seed=21)
-    g[1] = 0
-    got = orth(g, dtype=dtype, eps=0.0)
-    want = exact(g[::2], eps=0.0)
-    sync()
-    assert not bool(got[1].any()) and not bool(got.isnan().any())
-    off = fro(got[::2].double() - want)
-    assert bool((off <= bound(g[::2], want, dtype, dtype == V.F32)).all())
-    master, momentum, grad, lowp = muon_state(3, r, c, dtype == V.BF16, seed=22)
-    momentum[1], grad[1] = 0, 0
-    before = master.clone()
-    ws = workspace(V.lib().veda_muon_step_workspace(3, r, c, dtype))
-    call("veda_muon_step", ptr(master), ptr(momentum), ptr(grad), ptr(lowp), 3, r, c, r * c, 1e-2, 0.9, 1, 0.1, 1.7, 5,
-         *NS, 0.0, None, 1.0, 1.0, 0, ptr(ws), ws.numel(), stream())
-    sync()
-    # lr, the decay and their product in fp32, and the two roundings of w - (lr decay) w
-    want = before[1].double() * (1 - 1e-2 * 0.1)
-    assert bool(((master[1].double() - want).abs() <= 2 * 2.0 ** -24 * before[1].double().abs()).all())
-    assert not bool(momentum[1].any()) and not bool(master.isnan().any())
-
-
-@pytest.mark.gpu
-@pytest.mark.parametrize("dtype", [V.BF16, V.F32])
-@pytest.mark.parametrize("r,c", [(20, 30), (40, 600), (300, 280), (1001, 523)])
-@pytest.mark.parametrize("power", [-128, -110, -90, 90, 125])
-def test_norms_of_any_size_without_eps(cuda, dtype, r, c, power):
-    # powers of two leave every mantissa as it is, so the result has the same bits: whole numbers below 8,
-    # which stay exact down to the smallest subnormals of either type and up to its largest values
-    t = torch()
-    g = t.randint(-7, 8, (2, r, c), device="cuda", generator=t.Generator(device="cuda").manual_seed(23))
-    base = orth(g.to(dt(dtype)), dtype=dtype, eps=0.0)
-    got = orth(t.ldexp(g.double(), t.tensor(float(power), device="cuda", dtype=t.float64)).to(dt(dtype)), dtype=dtype, eps=0.0)
-    sync()
-    assert not bool(base.isnan().any()) and bool((got == base).all())
-
-
-@pytest.mark.gpu
-def test_long_fp32_sums_are_as_exact_as_one_chain(cuda):
-    # The tensor core truncates as it adds: a chain of two k-blocks (128 terms) of one sign falls short of its sum by a
-    # constant share, and the folds that join chains round to nearest and add none. One step with a = c = 0, b = 1 is
-    # S X: 64 copies of a matrix side by side have its S (the copies are scaled by 1/8, exactly) and, in every
-    # copy, its S X / 8, out of 64 times the chains. What the planes of X, S and M round is formed here, so the products
-    # alone are compared, in the mean over 129 x 129 elements: S and M X add one chain's share each (129 terms of M X,
-    # the same in both), and a fold's 2^-24 of random sign vanishes in the mean. A quarter is allowed; with chains of
-    # twice the length the share of S doubles, half as much again in all, and without folds it grows 64 times.
-    t = torch()
-    n = 129
-    u = t.rand(1, n, n, device="cuda", generator=t.Generator(device="cuda").manual_seed(24)) + 0.5
-    h = lambda v: v.to(t.float16).double()
-    two = lambda v: h(v) + h(v - h(v))
-    short = []
-    for k in (1, 64):
-        g = u.repeat(1, 1, k)
-        got = orth(g, dtype=V.F32, steps=1, coef=(0.0, 1.0, 0.0), eps=0.0)
-        sync()
-        scale = (1024.0 / g.double().square().sum().sqrt()).float()
-        x = two((g * scale).double())[0]
-        m = two(x @ x.mT / 1024)
-        want = m @ x / 1024 / 1024
-        short.append(-float(((got[0].double() - want) / want).mean()))
-    assert 0 <= short[1] <= 1.25 * short[0], short
-
-
 def test_workspaces_and_refusals_without_a_gpu():
     lib = V.lib()
     size = lib.veda_orthogonalize_workspace

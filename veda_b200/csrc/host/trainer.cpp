@@ -18,13 +18,10 @@
 
 #include "watchdog.hpp"
 
-#include <algorithm>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <filesystem>
-#include <map>
-#include <sstream>
 #include <stdexcept>
 #include <unordered_map>
 
@@ -744,19 +741,6 @@ Trainer::~Trainer()
     }
 }
 
-namespace
-{
-// Whether some of AdamW's parameters count their steps from a later one than the first.
-bool restarted(const optim::AdamW& opt)
-{
-    for (size_t i = 0; i < opt.parameters().size(); ++i)
-    {
-        if (opt.start(i) > 0) return true;
-    }
-    return false;
-}
-} // namespace
-
 void Trainer::init_data_parallel(const void* nccl_unique_id, int rank, int world,
                                  size_t bucket_bytes, bool sharded)
 {
@@ -774,11 +758,6 @@ void Trainer::init_data_parallel(const void* nccl_unique_id, int rank, int world
     if (sharded && muon_)
     {
         throw std::invalid_argument("Trainer: a sharded optimizer does not run Muon");
-    }
-    if (sharded && restarted(*opt_))
-    {
-        throw std::invalid_argument("Trainer: a sharded optimizer has one step count for all parameters, and Muon "
-                                    "has given some of them back");
     }
     dp_ = std::make_unique<DataParallel>(nccl_unique_id, rank, world, sharded);
     dp_->attach(*model_, bucket_bytes, master_weights(), opt_->steps(), batch_ * length_);
@@ -888,13 +867,18 @@ void Trainer::use_muon(const optim::MuonConfig& config)
         }
     }
     drop_step_graph();
-    if (muon_)
-    {
-        muon_->set_config(config);   // the momentum stays
-    }
-    else
+    // an earlier Muon hands its parameters back first, and takes them again if this one is refused
+    const bool had = muon_ != nullptr;
+    const optim::MuonConfig before = had ? muon_->config() : config;
+    muon_.reset();
+    try
     {
         muon_ = std::make_unique<optim::Muon>(*opt_, hidden, config);
+    }
+    catch (...)
+    {
+        if (had) muon_ = std::make_unique<optim::Muon>(*opt_, hidden, before);
+        throw;
     }
 }
 
@@ -1102,27 +1086,23 @@ void Trainer::step_impl(const Tensor& ids, const Tensor& targets)
         dp_->finish();
     }
     {
-        // every gradient is read for the norm; a Muon updates its parameters in a class of its own
         const double n = static_cast<double>(model_->parameter_count()) /
                          static_cast<double>(sharded() ? world() : 1);
-        const double updated = n - (muon_ ? static_cast<double>(muon_->elements()) : 0.0);
-        const double lowp = model_->dtype() == DType::BF16 ? 2.0 : 0.0;
-        profile::Scope scope("adamw", 0.0, n * 4.0 + updated * (16.0 + 12.0 + lowp));
+        profile::Scope scope("adamw", 0.0,
+                             n * (4.0 + 16.0 + 12.0 + (model_->dtype() == DType::BF16 ? 2.0 : 0.0)));
         if (sharded())
         {
             dp_->update(opt_->config(), max_norm_);
         }
         else
         {
-            opt_->launch_clipped(max_norm_, 1.0f / static_cast<float>(world()));
+            const float scale = 1.0f / static_cast<float>(world());
+            opt_->launch_clipped(max_norm_, scale);
+            if (muon_)
+            {
+                muon_->launch(opt_->sumsq(), max_norm_, scale);
+            }
         }
-    }
-    if (muon_)
-    {
-        // gradient read, momentum and master read and written, weights written
-        profile::Scope scope("muon", muon_->flops(),
-                             static_cast<double>(muon_->elements()) * (20.0 + (model_->dtype() == DType::BF16 ? 2.0 : 0.0)));
-        muon_->launch(opt_->sumsq(), max_norm_, 1.0f / static_cast<float>(world()));
     }
     cuda_check(cudaMemcpyAsync(loss_.data_ptr(), loss.value().data_ptr(), sizeof(float),
                                cudaMemcpyDeviceToDevice, cs()),
@@ -1136,23 +1116,6 @@ std::vector<uint8_t> to_host_bytes(const void* device, size_t count)
 {
     std::vector<uint8_t> out(count * sizeof(T));
     cuda_check(cudaMemcpyAsync(out.data(), device, out.size(), cudaMemcpyDeviceToHost, cs()), "checkpoint read");
-    return out;
-}
-} // namespace
-
-namespace
-{
-// "a,b=3" of a checkpoint's metadata as {a: "", b: "3"}; empty where there is no such entry.
-std::map<std::string, std::string> listed(const std::map<std::string, std::string>& metadata, const std::string& key)
-{
-    std::map<std::string, std::string> out;
-    const auto it = metadata.find(key);
-    std::stringstream items(it == metadata.end() ? "" : it->second);
-    for (std::string item; std::getline(items, item, ',');)
-    {
-        const size_t eq = item.find('=');
-        out[item.substr(0, eq)] = eq == std::string::npos ? "" : item.substr(eq + 1);
-    }
     return out;
 }
 } // namespace
@@ -1202,25 +1165,8 @@ void Trainer::save_checkpoint(const std::string& dir)
         throw std::logic_error("save_checkpoint: parameters do not tile the arena");
     }
     io::write_safetensors(dir + "/model.safetensors", weights, {{"format", "pt"}});
-    // Which first moments are a Muon's momentum, and where AdamW's moments began later than its first step.
-    std::map<std::string, std::string> metadata{{"format", "pt"}, {"step", std::to_string(steps)}};
-    std::string muon, starts;
-    size_t i = 0;
-    for (const auto& [name, value] : model_->named_parameters())
-    {
-        if (!sharded() && opt_->taken(i))
-        {
-            muon += (muon.empty() ? "" : ",") + name;
-        }
-        else if (!sharded() && opt_->start(i) > 0)
-        {
-            starts += (starts.empty() ? "" : ",") + name + "=" + std::to_string(opt_->start(i));
-        }
-        ++i;
-    }
-    if (!muon.empty()) metadata["muon"] = muon;
-    if (!starts.empty()) metadata["start"] = starts;
-    io::write_safetensors(dir + "/optimizer.safetensors", state, metadata);
+    io::write_safetensors(dir + "/optimizer.safetensors", state,
+                          {{"format", "pt"}, {"step", std::to_string(steps)}});
 }
 
 void Trainer::load_checkpoint(const std::string& dir)
@@ -1286,33 +1232,6 @@ void Trainer::load_checkpoint(const std::string& dir)
         }
         steps = static_cast<size_t>(std::stoull(it->second));
     }
-    // A Muon's momentum goes on as one where a Muon has the parameter; AdamW, which has no use for it, begins anew.
-    std::vector<size_t> starts(model_->parameters().size(), 0);
-    const std::map<std::string, std::string> muon = listed(state.metadata, "muon"), later = listed(state.metadata, "start");
-    if (sharded() && (!muon.empty() || !later.empty()))
-    {
-        throw std::invalid_argument("load_checkpoint: a sharded optimizer has one step count for all parameters, and " + dir +
-                                    " holds a Muon's");
-    }
-    size_t i = 0;
-    at = 0;
-    for (const auto& [name, value] : model_->named_parameters())
-    {
-        const size_t count = value.numel();
-        if (const auto it = later.find(name); it != later.end())
-        {
-            starts[i] = static_cast<size_t>(std::stoull(it->second));
-        }
-        if (muon.contains(name) && !opt_->taken(i))
-        {
-            std::fill_n(m.begin() + at, count, 0.0f);
-            std::fill_n(v.begin() + at, count, 0.0f);
-            starts[i] = steps;
-        }
-        at += count;
-        ++i;
-    }
-    drop_step_graph();   // AdamW's runs and corrections may be others now
     float* dmaster = master_weights();
     cuda_check(cudaMemcpyAsync(dmaster, master.data(), n * sizeof(float), cudaMemcpyHostToDevice, cs()),
                "checkpoint write");
@@ -1328,7 +1247,6 @@ void Trainer::load_checkpoint(const std::string& dir)
                                cudaMemcpyHostToDevice, cs()),
                "checkpoint write");
     opt_->set_steps(steps);
-    opt_->set_starts(starts);
     if (sharded())
     {
         dp_->load_master(dmaster);

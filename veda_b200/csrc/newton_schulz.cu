@@ -752,21 +752,6 @@ __device__ __forceinline__ void load_n(const T* p, float (&v)[N])
     }
 }
 
-// What X's stored values are made with: kUnit u / (|u| + eps) = (u lift) scale, from the sum of squares. lift is a
-// power of two that keeps scale a normal number for norms below 2^-100 and above 2^100 (a scale of 2^10 / |u| in fp32
-// would be infinite below 2^-118). 0 where norm and eps both are: such a matrix is zero and stays so.
-struct Unit
-{
-    float lift, scale;
-    __device__ __forceinline__ float operator()(float u) const { return u * lift * scale; }
-};
-__device__ __forceinline__ Unit unit_of(double sum, float eps)
-{
-    const double d = sqrt(sum) + static_cast<double>(eps);
-    const double lift = d < 0x1p-100 ? 0x1p64 : d > 0x1p100 ? 0x1p-64 : 1.0;
-    return {static_cast<float>(lift), d == 0.0 ? 0.0f : static_cast<float>(static_cast<double>(kUnit) / (d * lift))};
-}
-
 // A block takes every gridDim.x-th group of eight rows of matrix blockIdx.y, a warp a row, N elements
 // a lane at a time (4 where rows and bases allow 16-byte accesses of fp32).
 // Updates the momentum (Muon) and leaves the block's sum of squares of what is orthogonalised: G, the
@@ -845,7 +830,7 @@ init_kernel(Source s, int rows, int cols, const double* __restrict__ partials, f
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = total;
     __syncthreads();
     total = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
-    const Unit unit = unit_of(total, eps);
+    const float scale = static_cast<float>(static_cast<double>(kUnit) / (sqrt(total) + static_cast<double>(eps)));
     const float clip = clip_scale(s.sumsq, s.max_norm, s.grad_scale);
     const T* g = static_cast<const T*>(s.g);
     for (int r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8)
@@ -874,7 +859,7 @@ init_kernel(Source s, int rows, int cols, const double* __restrict__ partials, f
 #pragma unroll
             for (int k = 0; k < N; ++k)
             {
-                const float v = unit(u[k]);
+                const float v = u[k] * scale;
                 const __half h = __float2half_rn(v);
                 hi[k] = __half_as_ushort(h);
                 lo[k] = __half_as_ushort(__float2half_rn(v - __half2float(h)));
@@ -1018,7 +1003,7 @@ small_kernel(const Small p)
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
     volatile int* const abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
     __shared__ double part[kSmallThreads / 32];
-    __shared__ Unit shared_unit;
+    __shared__ float shared_scale;
     __shared__ double shares[kMaxRanks];
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
@@ -1077,12 +1062,12 @@ small_kernel(const Small p)
             }
             return r < own_rows && c < own_cols;
         };
-        const auto store = [&](int r, int c, const float (&u)[4], const Unit& unit) {
+        const auto store = [&](int r, int c, const float (&u)[4], float scale) {
             alignas(8) __half h[4], l[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
             {
-                const float v = unit(u[k]);
+                const float v = u[k] * scale;
                 h[k] = __float2half_rn(v);
                 l[k] = __float2half_rn(v - __half2float(h[k]));
             }
@@ -1187,7 +1172,7 @@ small_kernel(const Small p)
                 for (int k = 0; k < 4; ++k) sum += static_cast<double>(u[q][k]) * u[q][k];
             }
         };
-        const auto planes = [&](int base, const Unit& unit) {
+        const auto planes = [&](int base, float scale) {
 #pragma unroll
             for (int q = 0; q < kItems; ++q)
             {
@@ -1197,7 +1182,7 @@ small_kernel(const Small p)
                 {
                     const int e = base + t + q * kSmallThreads;
                     if (base + q * kSmallThreads >= count) break;
-                    if (e < count && place(e, r, c)) store(r, c, u[q], unit);
+                    if (e < count && place(e, r, c)) store(r, c, u[q], scale);
                     continue;
                 }
 #pragma unroll
@@ -1206,7 +1191,7 @@ small_kernel(const Small p)
                     const int e = base + t + (q * 4 + k) * kSmallThreads;
                     const float one[4] = {u[q][k], 0.0f, 0.0f, 0.0f};
                     if (base + (q * 4 + k) * kSmallThreads >= count) break;
-                    if (e < count && place(e, r, c)) store(r, c, one, unit);
+                    if (e < count && place(e, r, c)) store(r, c, one, scale);
                 }
             }
         };
@@ -1245,7 +1230,7 @@ small_kernel(const Small p)
             }
             if (lane == 0)
             {
-                shared_unit = unit_of(sum, p.eps);
+                shared_scale = static_cast<float>(static_cast<double>(kUnit) / (sqrt(sum) + static_cast<double>(p.eps)));
             }
         }
         else if constexpr (CLUSTER)
@@ -1254,11 +1239,11 @@ small_kernel(const Small p)
             pair::cluster_wait();
         }
         __syncthreads();
-        const Unit unit = shared_unit;
+        const float scale = shared_scale;
 #pragma unroll 1
         for (int base = twice ? each : 0; base >= 0; base -= each)
         {
-            planes(base, unit);
+            planes(base, scale);
             if (base > 0)
             {
 #pragma unroll
@@ -1787,7 +1772,7 @@ int products(const char* what, int64_t batch, int64_t rows, int64_t cols, int st
     const int clusters = pair::clusters_available<W, 8, SPLIT>();
     if (clusters < 1)
     {
-        return pair::none_available(what, clusters);
+        return fail(VEDA_ERR_UNSUPPORTED, std::string(what) + ": no CTA pair fits on this device");
     }
     // more clusters than a step of the batch has tiles would only wait
     const int64_t most = std::max(half, whole) * batch;
