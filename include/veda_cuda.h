@@ -253,8 +253,8 @@ int veda_mean_f64(const float* v, int64_t n, float* out, double* out_f64, veda_s
 /* sized by veda_linear_cross_entropy_workspace; pass a pitch of 1 for an operand whose base  */
 /* is not 16-byte aligned. The largest size with backward = 0 and 1 serves both calls. Results */
 /* repeat bit for bit. Where the tensor cores run, fp32 operands are multiplied as pairs of   */
-/* fp16 values (22 bits); magnitudes below 2^-39 of an operand's largest, and of q below      */
-/* 2^-38, are lost.                                                                           */
+/* fp16 values (22 bits); magnitudes below 2^-39 of an operand's largest (in the forward, of a */
+/* row of x's own largest), and of q below 2^-38, are lost.                                   */
 /* ---------------------------------------------------------------------------------------- */
 size_t veda_linear_cross_entropy_workspace(int64_t rows, int64_t vocab, int64_t dim, int64_t ldx,
                                            int64_t ldw, int dtype, int backward);

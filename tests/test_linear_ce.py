@@ -394,6 +394,35 @@ def test_repeats_bit_for_bit_on_other_streams_and_from_a_graph(cuda):
     assert bool((l3 == lse).all()) and bool((a == dx).all()) and bool((b == dw).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [V.BF16, V.F32])
+@pytest.mark.parametrize("scale", [2.0 ** 7, 1e6, 1e-30])
+@pytest.mark.parametrize("rows,vocab,dim", [(4, 300, 64), (60, 300, 64), (60, 4300, 64), (300, 5001, 40)])
+@pytest.mark.parametrize("counted", [0.5, 0.0])
+def test_lse_of_rows_that_are_not_counted(cuda, dtype, scale, rows, vocab, dim, counted):
+    # lse is every row's, whatever the others hold: rows that are not counted far above or below the counted
+    # ones in size, and no counted row at all
+    t = torch()
+    x, w, tg = make(rows, vocab, dim, dtype, seed=15)
+    clean = x.clone()
+    if counted:
+        tg[1::2] = IGN
+    else:
+        tg[:] = IGN
+    x[1::2] = (x[1::2].float() * scale).to(x.dtype)
+    row, lse, loss = fwd(x, w, tg, dtype)
+    row0, lse0, loss0 = fwd(clean, w, tg, dtype)
+    sync()
+    # the module's bounds, every row's own
+    z = x.double() @ w.double().t()
+    seg, drop = (3, 3 * 2.0 ** -22) if dtype == V.F32 else (1, 0.0)
+    dz = ((seg * dim / 16 + 4) * 2.0 ** -23 + drop) * (x.double().abs() @ w.double().abs().t()).amax(1)
+    want = t.logsumexp(z, 1)
+    within(lse, want, dz + 2.0 ** -21 + 4 * 2.0 ** -24 * want.abs(), "lse")
+    assert bool((row[tg == IGN] == 0).all())
+    assert bool((row == row0).all()) and float(loss) == float(loss0) and bool((lse[::2] == lse0[::2]).all())
+
+
 def test_workspace_sizes_and_refusals_without_a_gpu():
     lib = V.lib()
     size = lib.veda_linear_cross_entropy_workspace

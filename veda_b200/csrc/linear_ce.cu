@@ -21,8 +21,10 @@
 // element within a launch, so results repeat bit for bit. Where dx has few tiles its sums are cut among
 // clusters, one fp32 plane a cut, added in order at the end.
 //
-// fp32 operands: each is split into two fp16 planes, value 2^e = hi + lo (22 bits, e chosen from
-// the tensor's largest finite value), and a product becomes hi lo + lo hi + hi hi on 256 x 128 tiles
+// fp32 operands: each is split into two fp16 planes, value 2^e = hi + lo (22 bits, e chosen from the
+// largest finite value: of w; of the counted rows of x in the backward; of each row of x in the forward, whose
+// lse is every row's, so that a row far larger than the counted ones neither overflows nor costs them
+// bits), and a product becomes hi lo + lo hi + hi hi on 256 x 128 tiles
 // with three times the k-blocks (pair_mma.cuh); lo lo is below the 22nd bit. fp32 CUDA-core products run at a
 // twentieth of the tensor cores' rate, so three tensor products are still far cheaper: 1000 x 10007 x 320
 // takes 147 us, forward and backward.
@@ -60,7 +62,7 @@ __device__ __forceinline__ float ex2(float x)
 // powers of two stay apart from coef: their product with it could be subnormal where dx is not.
 struct Scalars
 {
-    float z;                // 2^-(ex + ew) of split operands, else 1
+    float z;                // 2^-(ex + ew) of split operands (forward: 2^-ew, ex being each row's own), else 1
     float coef;             // upstream / counted rows
     float unit_dx, unit_dw; // 2^-(13 + ew), 2^-(13 + ex) of split operands, else 1
     float x, w;             // 2^ex, 2^ew of split operands
@@ -102,6 +104,7 @@ struct Params
     const int64_t* targets;
     int64_t ignore;
     const float* lse;
+    const float* row_scale;  // forward, split: 2^ex of each row of x
     float2* parts;           // [strip slots][rows] running (max, sum)
     float* target_logit;     // [rows]
     unsigned* done;          // cleared for the merge's blocks to count themselves
@@ -152,7 +155,7 @@ struct StatsWork
     };
     struct State
     {
-        float m, s;
+        float m, s, zs;
         int target;
     };
 
@@ -201,7 +204,9 @@ struct StatsWork
             }
             s.m = -INFINITY;
             s.s = 0.0f;
-            s.target = counted_target(p, t.mb * pair::kTile + row0 + lane);
+            const int row = t.mb * pair::kTile + row0 + lane;
+            s.target = counted_target(p, row);
+            s.zs = p.split && row < p.rows ? p.scalars->z / p.row_scale[row] : 1.0f;
         }
     }
 
@@ -215,7 +220,6 @@ struct StatsWork
         }
         const int row = t.mb * pair::kTile + row0 + lane;
         const int first = p.v0 + t.nb * TN + col0;
-        const float zs = p.split ? p.scalars->z : 1.0f;
 #pragma unroll 1
         for (int c = 0; c < COLS; c += 32)
         {
@@ -235,7 +239,7 @@ struct StatsWork
             if (p.split)
             {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) z[j] *= zs;
+                for (int j = 0; j < 32; ++j) z[j] *= s.zs;
             }
             if (left < 32)
             {
@@ -627,43 +631,6 @@ __device__ __forceinline__ bool counted(int64_t t, int64_t ignore, int64_t vocab
     return t != ignore && t >= 0 && t < vocab;
 }
 
-// Largest finite magnitude of the counted rows of x (blocks below gx) and of w (the others) as one
-// partial per block.
-__global__ void __launch_bounds__(256)
-absmax_kernel(const float* __restrict__ x, int64_t ldx, int64_t rows, const float* __restrict__ w, int64_t ldw,
-              int64_t vocab, int64_t dim, const int64_t* __restrict__ targets, int64_t ignore, int gx,
-              float* __restrict__ part)
-{
-    __shared__ float warp_part[8];
-    dep_wait();
-    dep_release();
-    const bool is_w = static_cast<int>(blockIdx.x) >= gx;
-    const float* m = is_w ? w : x;
-    const int64_t ld = is_w ? ldw : ldx, n = is_w ? vocab : rows;
-    const int64_t b = is_w ? blockIdx.x - gx : blockIdx.x, blocks = is_w ? gridDim.x - gx : gx;
-    float top = 0.0f;
-    for (int64_t r = b * 8 + threadIdx.x / 32; r < n; r += blocks * 8)
-    {
-        if (!is_w && !counted(targets[r], ignore, vocab))
-        {
-            continue;
-        }
-        for (int64_t c = threadIdx.x & 31; c < dim; c += 32)
-        {
-            const float v = fabsf(m[r * ld + c]);
-            top = v <= FLT_MAX ? fmaxf(top, v) : top;
-        }
-    }
-    top = warp_max(top);
-    if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = top;
-    __syncthreads();
-    if (threadIdx.x == 0)
-    {
-        for (int k = 1; k < 8; ++k) top = fmaxf(top, warp_part[k]);
-        part[blockIdx.x] = top;
-    }
-}
-
 // 2^e that brings a largest magnitude into [2^13, 2^14), clamped so that 2^e and 2^-e are normal
 // (a tensor of magnitudes below 2^-113 keeps fewer bits).
 __device__ __forceinline__ float split_scale(float top)
@@ -678,17 +645,66 @@ __device__ __forceinline__ float split_scale(float top)
     return ldexpf(1.0f, e < -120 ? -120 : e > 120 ? 120 : e);
 }
 
+// Largest finite magnitude of the counted rows of x (blocks below gx) and of w (the others) as one
+// partial per block; with row_scale, the scale of every row of x instead of x's partials.
+__global__ void __launch_bounds__(256)
+absmax_kernel(const float* __restrict__ x, int64_t ldx, int64_t rows, const float* __restrict__ w, int64_t ldw,
+              int64_t vocab, int64_t dim, const int64_t* __restrict__ targets, int64_t ignore, int gx,
+              float* __restrict__ part, float* __restrict__ row_scale)
+{
+    __shared__ float warp_part[8];
+    dep_wait();
+    dep_release();
+    const bool is_w = static_cast<int>(blockIdx.x) >= gx;
+    const float* m = is_w ? w : x;
+    const int64_t ld = is_w ? ldw : ldx, n = is_w ? vocab : rows;
+    const int64_t b = is_w ? blockIdx.x - gx : blockIdx.x, blocks = is_w ? gridDim.x - gx : gx;
+    const bool by_row = !is_w && row_scale != nullptr;
+    float top = 0.0f;
+    for (int64_t r = b * 8 + threadIdx.x / 32; r < n; r += blocks * 8)
+    {
+        if (!is_w && !by_row && !counted(targets[r], ignore, vocab))
+        {
+            continue;
+        }
+        for (int64_t c = threadIdx.x & 31; c < dim; c += 32)
+        {
+            const float v = fabsf(m[r * ld + c]);
+            top = v <= FLT_MAX ? fmaxf(top, v) : top;
+        }
+        if (by_row)
+        {
+            top = warp_max(top);
+            if ((threadIdx.x & 31) == 0) row_scale[r] = split_scale(top);
+            top = 0.0f;
+        }
+    }
+    if (by_row)
+    {
+        return;
+    }
+    top = warp_max(top);
+    if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x == 0)
+    {
+        for (int k = 1; k < 8; ++k) top = fmaxf(top, warp_part[k]);
+        part[blockIdx.x] = top;
+    }
+}
+
 // What comes before the tensor-core launches, in one: the call's scalars (the last block: split scales
 // from the partial maxima, upstream / counted rows) and the operand planes of x (blocks below gx) and w
 // (the next gw) with a pitch of a multiple of 8 elements: a bf16 copy, or the two fp16 halves of an fp32
 // operand. clear: rows of x that are not counted become zeros, so that what padding holds (NaN
-// included) meets q = 0 in dW's product as 0. vx, vw: eight elements of a row can be read at a time.
+// included) meets q = 0 in dW's product as 0. vx, vw: eight elements of a row can be read at a time. row_scale: the
+// scales of the rows of x, if each has its own (parts_x is 0 then).
 template <typename T>
 __global__ void __launch_bounds__(256)
 pack_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, const T* __restrict__ w, int64_t ldw, int64_t vocab,
             int64_t dim, const int64_t* __restrict__ targets, int64_t ignore, bool clear, bool vx, bool vw, int gx, int gw,
-            uint16_t* __restrict__ px, uint16_t* __restrict__ pw, int64_t ldp, const float* __restrict__ part, int parts_x,
-            int parts_w, const float* __restrict__ upstream, Scalars* __restrict__ scalars, int* status)
+            uint16_t* __restrict__ px, uint16_t* __restrict__ pw, int64_t ldp, const float* __restrict__ part, int first_w,
+            int parts_x, int parts_w, const float* __restrict__ row_scale, const float* __restrict__ upstream, Scalars* __restrict__ scalars, int* status)
 {
     __shared__ int counts[8];
     __shared__ float tops[2][8];
@@ -701,7 +717,7 @@ pack_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, const T* __restr
     {
         float tx = 0.0f, tw = 0.0f;
         for (int i = threadIdx.x; i < parts_x; i += 256) tx = fmaxf(tx, part[i]);
-        for (int i = threadIdx.x; i < parts_w; i += 256) tw = fmaxf(tw, part[parts_x + i]);
+        for (int i = threadIdx.x; i < parts_w; i += 256) tw = fmaxf(tw, part[first_w + i]);
         tx = warp_max(tx);
         tw = warp_max(tw);
         if (lane == 0) tops[0][warp] = tx, tops[1][warp] = tw;
@@ -757,6 +773,7 @@ pack_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, const T* __restr
     const int64_t ld = is_w ? ldw : ldx, n = is_w ? vocab : rows;
     const int64_t b = is_w ? block - gx : block, blocks = is_w ? gw : gx;
     const float scale = part != nullptr ? scale_shared[is_w ? 1 : 0] : 1.0f;
+    const bool by_row = !is_w && row_scale != nullptr;
     const bool vec = is_w ? vw : vx;
     const int64_t per_row = ldp / 8, groups = n * per_row;   // of eight columns
 #pragma unroll 2
@@ -791,6 +808,7 @@ pack_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, const T* __restr
             for (int k = 0; k < 8; ++k) v[k] = k < left ? to_f32(m[r * ld + c + k]) : 0.0f;
         }
         uint32_t hi[4], lo[4];
+        const float own = by_row ? row_scale[r] : scale;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
         {
@@ -800,7 +818,7 @@ pack_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, const T* __restr
             }
             else
             {
-                const float a = v[2 * k] * scale, d = v[2 * k + 1] * scale;
+                const float a = v[2 * k] * own, d = v[2 * k + 1] * own;
                 hi[k] = pack_f16(a, d);
                 lo[k] = pack_f16(a - f16_lo(hi[k]), d - f16_hi(hi[k]));
             }
@@ -1737,7 +1755,7 @@ struct Layout
     int64_t ld_acc;       // pitch of the fp32 dx sums
     int splits;           // of dx's sum over a piece
     int strip, slots;     // forward: tiles a strip, strips
-    size_t scalars, done, part, px, pw, parts, target_logit, q, acc, total;
+    size_t scalars, done, part, row_scale, px, pw, parts, target_logit, q, acc, total;
 };
 
 // Tiles per strip: up to 8, by the number of tile times the busiest of `clusters` clusters runs;
@@ -1811,6 +1829,7 @@ Layout layout(int64_t rows, int64_t vocab, int64_t dim, bool pack_x, bool pack_w
     l.scalars = take(sizeof(Scalars));
     l.done = take(4);
     l.part = take(2 * kMaxBlocks * 4);
+    l.row_scale = take(!backward && dtype == VEDA_F32 ? rows * 4 : 0);
     l.px = take(pack_x ? l.planes * rows * l.ldp * 2 : 0);
     l.pw = take(pack_w ? l.planes * vocab * l.ldp * 2 : 0);
     const int tn = tile_width(dtype), num_n = static_cast<int>((vocab + tn - 1) / tn), num_m = static_cast<int>((rows + 255) / 256);
@@ -1916,14 +1935,15 @@ unsigned pack_blocks(int64_t rows)
 int prepare(const Call& c, const int64_t* targets, int64_t ignore, const float* upstream, int* status,
             bool scalars, Params& p, cudaStream_t s)
 {
-    float* part = nullptr;
+    float *part = nullptr, *row_scale = nullptr;
     const unsigned gx = pack_blocks(c.rows), gw = pack_blocks(c.vocab);
     if (c.dtype == VEDA_F32)
     {
         part = reinterpret_cast<float*>(c.ws + c.l.part);
+        if (!c.backward) row_scale = reinterpret_cast<float*>(c.ws + c.l.row_scale);
         const int rc = launch("veda_linear_cross_entropy", absmax_kernel, dim3(gx + gw), dim3(256), 0, s,
                               static_cast<const float*>(c.x), c.ldx, c.rows, static_cast<const float*>(c.w), c.ldw,
-                              c.vocab, c.dim, targets, ignore, static_cast<int>(gx), part);
+                              c.vocab, c.dim, targets, ignore, static_cast<int>(gx), part, row_scale);
         if (rc != VEDA_OK) return rc;
     }
     const void *px = c.x, *pw = c.w;
@@ -1942,7 +1962,8 @@ int prepare(const Call& c, const int64_t* targets, int64_t ignore, const float* 
             return launch("veda_linear_cross_entropy (operands)", kernel, dim3(bx + bw + 1), dim3(256), 0, s, x, c.ldx,
                           c.rows, w, c.ldw, c.vocab, c.dim, targets, ignore, c.backward, vec(c.x, c.ldx), vec(c.w, c.ldw),
                           bx, bw, ox, ow, c.l.ldp, static_cast<const float*>(part), static_cast<int>(gx),
-                          static_cast<int>(gw), upstream, c.scalars(), status);
+                          row_scale != nullptr ? 0 : static_cast<int>(gx), static_cast<int>(gw),
+                          static_cast<const float*>(row_scale), upstream, c.scalars(), status);
         };
         const int rc = c.dtype == VEDA_F32
                            ? go(static_cast<const float*>(c.x), static_cast<const float*>(c.w), pack_kernel<float>)
@@ -1979,6 +2000,7 @@ int prepare(const Call& c, const int64_t* targets, int64_t ignore, const float* 
     p.by_m = pair::Divisor(static_cast<uint32_t>(p.num_m));
     p.by_d = pair::Divisor(static_cast<uint32_t>(p.num_d));
     p.scalars = c.scalars();
+    p.row_scale = row_scale;
     p.targets = targets;
     p.ignore = ignore;
     p.status = device_status_ptr();
