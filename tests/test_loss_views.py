@@ -25,7 +25,7 @@ def test_compiles(tmp_path):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("part", ["shared"])
+@pytest.mark.parametrize("part", ["shared", "views"])
 def test_cpp_api(cuda, tmp_path, part):
     r = subprocess.run([str(compile_check("loss_views_check", tmp_path)), part], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "FAIL" not in r.stdout, r.stdout + r.stderr

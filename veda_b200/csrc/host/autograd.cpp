@@ -1572,6 +1572,16 @@ Variable linear(const Variable& x, const Variable& w)
 
 namespace
 {
+// The workspace of the loss head for these operands, which are laid out in it where they do not begin on 16 bytes.
+size_t linear_ce_workspace(const LinearSaved& l, int backward)
+{
+    const auto pitch = [](const Tensor& t, int64_t ld) {
+        return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? ld : int64_t{1};
+    };
+    return veda_linear_cross_entropy_workspace(l.rows, l.out, l.in, pitch(l.xs, l.ldx), pitch(l.wc, l.in),
+                                               dt(l.xs.dtype()), backward);
+}
+
 Variable linear_cross_entropy_impl(const LinearSaved& l, const Variable& x, const Variable& w,
                                    const Tensor& targets, int64_t ignore, bool device_check)
 {
@@ -1583,7 +1593,7 @@ Variable linear_cross_entropy_impl(const LinearSaved& l, const Variable& x, cons
     Tensor loss = Tensor::empty(Shape({}), DType::F32);
     int* flag = device_check ? detail::device_flag() : nullptr;
     {
-        const size_t bytes = veda_linear_cross_entropy_workspace(rows, V, D, l.ldx, D, dt(d), 0);
+        const size_t bytes = linear_ce_workspace(l, 0);
         Tensor ws = Tensor::empty(Shape({(bytes + 3) / 4}), DType::F32);
         profile::Scope scope("linear_ce_fwd", 2.0 * rows * V * D,
                              es * (static_cast<double>(rows) * D + static_cast<double>(V) * D));
@@ -1612,7 +1622,7 @@ Variable linear_cross_entropy_impl(const LinearSaved& l, const Variable& x, cons
             dw_type = gw.dtype();
         }
         const Tensor up = as_dtype(g, DType::F32);
-        const size_t bytes = veda_linear_cross_entropy_workspace(rows, V, D, l.ldx, D, dt(d), 1);
+        const size_t bytes = linear_ce_workspace(l, 1);
         Tensor ws = Tensor::empty(Shape({(bytes + 3) / 4}), DType::F32);
         {
             profile::Scope scope("linear_ce_bwd", 6.0 * rows * V * D,
