@@ -443,6 +443,48 @@ def test_ragged_tiles_repeat_bit_for_bit(cuda, dtype, b, r, c):
     sync()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [V.BF16, V.F32])
+@pytest.mark.parametrize("r,c", [(20, 30), (40, 600), (300, 280), (135, 50)])
+def test_zero_matrices_without_eps(cuda, dtype, r, c):
+    # eps = 0 leaves nothing to divide by; in one block, cut among blocks and tiled
+    t = torch()
+    g = make(3, r, c, dtype, seed=21)
+    g[1] = 0
+    got = orth(g, dtype=dtype, eps=0.0)
+    want = exact(g[::2], eps=0.0)
+    sync()
+    assert not bool(got[1].any()) and not bool(got.isnan().any())
+    off = fro(got[::2].double() - want)
+    assert bool((off <= bound(g[::2], want, dtype, dtype == V.F32)).all())
+    master, momentum, grad, lowp = muon_state(3, r, c, dtype == V.BF16, seed=22)
+    momentum[1], grad[1] = 0, 0
+    before = master.clone()
+    ws = workspace(V.lib().veda_muon_step_workspace(3, r, c, dtype))
+    call("veda_muon_step", ptr(master), ptr(momentum), ptr(grad), ptr(lowp), 3, r, c, r * c, 1e-2, 0.9, 1, 0.1, 1.7, 5,
+         *NS, 0.0, None, 1.0, 1.0, 0, ptr(ws), ws.numel(), stream())
+    sync()
+    # lr, the decay and their product in fp32, and the two roundings of w - (lr decay) w
+    want = before[1].double() * (1 - 1e-2 * 0.1)
+    assert bool(((master[1].double() - want).abs() <= 2 * 2.0 ** -24 * before[1].double().abs()).all())
+    assert not bool(momentum[1].any()) and not bool(master.isnan().any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [V.BF16, V.F32])
+@pytest.mark.parametrize("r,c", [(20, 30), (40, 600), (300, 280), (1001, 523)])
+@pytest.mark.parametrize("power", [-128, -110, -90, 90, 125])
+def test_norms_of_any_size_without_eps(cuda, dtype, r, c, power):
+    # powers of two leave every mantissa as it is, so the result has the same bits: whole numbers below 8,
+    # which stay exact down to the smallest subnormals of either type and up to its largest values
+    t = torch()
+    g = t.randint(-7, 8, (2, r, c), device="cuda", generator=t.Generator(device="cuda").manual_seed(23))
+    base = orth(g.to(dt(dtype)), dtype=dtype, eps=0.0)
+    got = orth(t.ldexp(g.double(), t.tensor(float(power), device="cuda", dtype=t.float64)).to(dt(dtype)), dtype=dtype, eps=0.0)
+    sync()
+    assert not bool(base.isnan().any()) and bool((got == base).all())
+
+
 def test_workspaces_and_refusals_without_a_gpu():
     lib = V.lib()
     size = lib.veda_orthogonalize_workspace

@@ -752,6 +752,21 @@ __device__ __forceinline__ void load_n(const T* p, float (&v)[N])
     }
 }
 
+// What X's stored values are made with: kUnit u / (|u| + eps) = (u lift) scale, from the sum of squares. lift is a
+// power of two that keeps scale a normal number for norms below 2^-100 and above 2^100 (a scale of 2^10 / |u| in fp32
+// would be infinite below 2^-118). 0 where norm and eps both are: such a matrix is zero and stays so.
+struct Unit
+{
+    float lift, scale;
+    __device__ __forceinline__ float operator()(float u) const { return u * lift * scale; }
+};
+__device__ __forceinline__ Unit unit_of(double sum, float eps)
+{
+    const double d = sqrt(sum) + static_cast<double>(eps);
+    const double lift = d < 0x1p-100 ? 0x1p64 : d > 0x1p100 ? 0x1p-64 : 1.0;
+    return {static_cast<float>(lift), d == 0.0 ? 0.0f : static_cast<float>(static_cast<double>(kUnit) / (d * lift))};
+}
+
 // A block takes every gridDim.x-th group of eight rows of matrix blockIdx.y, a warp a row, N elements
 // a lane at a time (4 where rows and bases allow 16-byte accesses of fp32).
 // Updates the momentum (Muon) and leaves the block's sum of squares of what is orthogonalised: G, the
@@ -830,7 +845,7 @@ init_kernel(Source s, int rows, int cols, const double* __restrict__ partials, f
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = total;
     __syncthreads();
     total = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
-    const float scale = static_cast<float>(static_cast<double>(kUnit) / (sqrt(total) + static_cast<double>(eps)));
+    const Unit unit = unit_of(total, eps);
     const float clip = clip_scale(s.sumsq, s.max_norm, s.grad_scale);
     const T* g = static_cast<const T*>(s.g);
     for (int r = blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += gridDim.x * 8)
@@ -859,7 +874,7 @@ init_kernel(Source s, int rows, int cols, const double* __restrict__ partials, f
 #pragma unroll
             for (int k = 0; k < N; ++k)
             {
-                const float v = u[k] * scale;
+                const float v = unit(u[k]);
                 const __half h = __float2half_rn(v);
                 hi[k] = __half_as_ushort(h);
                 lo[k] = __half_as_ushort(__float2half_rn(v - __half2float(h)));
@@ -1003,7 +1018,7 @@ small_kernel(const Small p)
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
     volatile int* const abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
     __shared__ double part[kSmallThreads / 32];
-    __shared__ float shared_scale;
+    __shared__ Unit shared_unit;
     __shared__ double shares[kMaxRanks];
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
@@ -1062,12 +1077,12 @@ small_kernel(const Small p)
             }
             return r < own_rows && c < own_cols;
         };
-        const auto store = [&](int r, int c, const float (&u)[4], float scale) {
+        const auto store = [&](int r, int c, const float (&u)[4], const Unit& unit) {
             alignas(8) __half h[4], l[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
             {
-                const float v = u[k] * scale;
+                const float v = unit(u[k]);
                 h[k] = __float2half_rn(v);
                 l[k] = __float2half_rn(v - __half2float(h[k]));
             }
@@ -1172,7 +1187,7 @@ small_kernel(const Small p)
                 for (int k = 0; k < 4; ++k) sum += static_cast<double>(u[q][k]) * u[q][k];
             }
         };
-        const auto planes = [&](int base, float scale) {
+        const auto planes = [&](int base, const Unit& unit) {
 #pragma unroll
             for (int q = 0; q < kItems; ++q)
             {
@@ -1182,7 +1197,7 @@ small_kernel(const Small p)
                 {
                     const int e = base + t + q * kSmallThreads;
                     if (base + q * kSmallThreads >= count) break;
-                    if (e < count && place(e, r, c)) store(r, c, u[q], scale);
+                    if (e < count && place(e, r, c)) store(r, c, u[q], unit);
                     continue;
                 }
 #pragma unroll
@@ -1191,7 +1206,7 @@ small_kernel(const Small p)
                     const int e = base + t + (q * 4 + k) * kSmallThreads;
                     const float one[4] = {u[q][k], 0.0f, 0.0f, 0.0f};
                     if (base + (q * 4 + k) * kSmallThreads >= count) break;
-                    if (e < count && place(e, r, c)) store(r, c, one, scale);
+                    if (e < count && place(e, r, c)) store(r, c, one, unit);
                 }
             }
         };
@@ -1230,7 +1245,7 @@ small_kernel(const Small p)
             }
             if (lane == 0)
             {
-                shared_scale = static_cast<float>(static_cast<double>(kUnit) / (sqrt(sum) + static_cast<double>(p.eps)));
+                shared_unit = unit_of(sum, p.eps);
             }
         }
         else if constexpr (CLUSTER)
@@ -1239,11 +1254,11 @@ small_kernel(const Small p)
             pair::cluster_wait();
         }
         __syncthreads();
-        const float scale = shared_scale;
+        const Unit unit = shared_unit;
 #pragma unroll 1
         for (int base = twice ? each : 0; base >= 0; base -= each)
         {
-            planes(base, scale);
+            planes(base, unit);
             if (base > 0)
             {
 #pragma unroll
