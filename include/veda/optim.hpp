@@ -56,6 +56,14 @@ public:
     const core::Tensor& second_moments() const noexcept { return v_arena_; }
     // Restores the step count (the bias corrections of the next step use steps + 1).
     void set_steps(size_t steps) noexcept { steps_ = steps; }
+    // Steps that had been made when the moments of parameter i began: its bias corrections count from
+    // there. 0 but for parameters that restart() was called for.
+    size_t start(size_t i) const { return starts_.at(i); }
+    void set_starts(const std::vector<size_t>& starts);
+    // Clears the moments of these parameters; their bias corrections begin anew, as a new AdamW's do.
+    void restart(const std::vector<size_t>& indices);
+    // Whether a Muon has parameter i.
+    bool taken(size_t i) const { return taken_.at(i); }
     // On: a clipped step whose global norm is not finite updates nothing (weights, moments and
     // gradients are left as they were); the caller, who reads the norm, then takes the step back
     // with set_steps(steps() - 1). Off (the default, the reference's behaviour): the step runs.
@@ -80,12 +88,15 @@ private:
         float* m;
         float* v;
         void* lowp;   // bf16 value copy, or null for fp32 parameters
+        size_t start, bias;   // steps before its moments began; its pair in bias_
     };
     friend class Muon;
     void build_runs();
     std::vector<Run> runs_of(bool all) const;
     // Leaves parameters to another optimizer, or takes them back.
     void set_taken(const std::vector<size_t>& indices, bool taken);
+    void build_updates();
+    void upload_bias();
     void launch(const double* sumsq, float max_norm, float grad_scale);
 
     std::vector<autograd::Variable> parameters_;
@@ -94,11 +105,15 @@ private:
     std::vector<Run> runs_;      // every parameter: what the global norm covers
     std::vector<Run> updates_;   // those that step() updates
     std::vector<bool> taken_;
+    std::vector<size_t> starts_;
     AdamWConfig config_;
     size_t steps_ = 0;
     core::Tensor sumsq_;     // device double
-    core::Tensor bias_;      // device double [2]: 1 - beta1^t, 1 - beta2^t of the current step
-    double bias_host_[2] = {1.0, 1.0};
+    // device doubles: 1 - beta1^t, 1 - beta2^t of the current step, a pair for each start in use (room for a
+    // pair a parameter, so that the address stays)
+    core::Tensor bias_;
+    std::vector<size_t> bias_starts_;
+    std::vector<double> bias_host_;
     core::Tensor workspace_;
     float last_scale_ = 1.0f;
 };
@@ -130,7 +145,9 @@ public:
     explicit Muon(std::vector<autograd::Variable> parameters, MuonConfig config = {});
     // Takes over the parameters `indices` of an AdamW: its steps no longer update them (its global
     // norm still counts them), their momentum is their first moment there and their master weights
-    // are its. `base` must outlive this object; what it holds for them is given back then.
+    // are its. `base` must outlive this object, whose end gives them back: the momentum, some 1 / (1 - momentum)
+    // gradients in size and without a second moment beside it, is of no use to AdamW, so its moments for
+    // them are cleared and their bias corrections begin anew (AdamW::restart).
     Muon(AdamW& base, const std::vector<size_t>& indices, MuonConfig config = {});
     ~Muon();
     Muon(const Muon&) = delete;
@@ -145,6 +162,8 @@ public:
     void launch(const double* sumsq, float max_norm, float grad_scale);
     void zero_grad();
     const MuonConfig& config() const noexcept { return config_; }
+    // Other numbers from the next launch on; momentum and master weights stay. A refused one changes nothing.
+    void set_config(const MuonConfig& config);
     const std::vector<autograd::Variable>& parameters() const noexcept { return parameters_; }
     // fp32 momentum and master weights of parameter i (the value itself for fp32 parameters).
     core::Tensor momentum(size_t i) const { return momenta_[i]; }
@@ -162,7 +181,8 @@ private:
         float* grad;
         void* lowp;
     };
-    void check_config() const;
+    static void check_config(const MuonConfig& config);
+    void check_parameters() const;
     void build_batches();
 
     AdamW* base_ = nullptr;

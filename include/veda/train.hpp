@@ -185,7 +185,9 @@ public:
     // or fp32 as the model computes) and dir/optimizer.safetensors (per parameter its fp32
     // master weights, first and second moments as "<name>.master", ".exp_avg", ".exp_avg_sq";
     // metadata "step"). Data-parallel: rank 0 writes; collective when sharded. Loading without
-    // an optimizer file starts the optimizer afresh from the file's weights.
+    // an optimizer file starts the optimizer afresh from the file's weights. Metadata "muon" names the
+    // parameters whose first moment is a Muon's momentum: loaded where no Muon has them, AdamW begins anew
+    // for them (and "start" says from which step, in later files); a sharded optimizer refuses such files.
     void save_checkpoint(const std::string& dir);
     void load_checkpoint(const std::string& dir);
 
@@ -222,8 +224,8 @@ public:
     // again.
     void set_linear_loss(bool on);
     // Muon for the hidden matrices (q/k/v/o, gate/up/down of every layer), AdamW for the rest. Their
-    // momentum is the optimizer's first moment, so checkpoints keep it. Not with a sharded optimizer.
-    // A captured step graph is dropped and captured again.
+    // momentum is the optimizer's first moment, so checkpoints keep it. Called again, the numbers change and
+    // the momentum stays. Not with a sharded optimizer. A captured step graph is dropped and captured again.
     void use_muon(const optim::MuonConfig& config);
 
     TinyTransformer& model() noexcept { return *model_; }

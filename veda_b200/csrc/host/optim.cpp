@@ -91,7 +91,7 @@ AdamW::AdamW(std::vector<autograd::Variable> parameters, AdamWConfig config)
         }
     }
     sumsq_ = Tensor(Shape({2}), DType::F32);   // 8 bytes: one double
-    bias_ = Tensor(Shape({4}), DType::F32);    // two doubles
+    bias_ = Tensor(Shape({4 * (parameters_.size() + 1)}), DType::F32);
     build_runs();
 }
 
@@ -117,11 +117,11 @@ std::vector<AdamW::Run> AdamW::runs_of(bool all) const
         }
         Run r{i, 1, static_cast<int64_t>(n), fptr(g), fptr(masters_[i]), fptr(m_arena_) + offset,
               fptr(v_arena_) + offset,
-              p.value().dtype() == DType::BF16 ? p.value().data_ptr() : nullptr};
+              p.value().dtype() == DType::BF16 ? p.value().data_ptr() : nullptr, starts_[i], 0};
         if (!runs.empty())
         {
             Run& last = runs.back();
-            const bool adjacent = last.first + last.count == i &&
+            const bool adjacent = last.first + last.count == i && (all || last.start == r.start) &&
                                   last.grad + last.n == r.grad && last.master + last.n == r.master &&
                                   last.m + last.n == r.m &&
                                   ((last.lowp == nullptr && r.lowp == nullptr) ||
@@ -145,8 +145,9 @@ std::vector<AdamW::Run> AdamW::runs_of(bool all) const
 void AdamW::build_runs()
 {
     taken_.resize(parameters_.size(), false);
+    starts_.resize(parameters_.size(), 0);
     runs_ = runs_of(true);
-    updates_ = runs_of(false);
+    build_updates();
     int64_t largest = 1;
     for (const Run& r : runs_)
     {
@@ -162,19 +163,83 @@ void AdamW::set_taken(const std::vector<size_t>& indices, bool taken)
     {
         taken_[i] = taken;
     }
-    updates_ = runs_of(false);
+    build_updates();
+}
+
+void AdamW::build_updates()
+{
+    std::vector<Run> updates = runs_of(false);
+    std::vector<size_t> starts;
+    for (Run& r : updates)
+    {
+        const auto at = std::find(starts.begin(), starts.end(), r.start);
+        r.bias = static_cast<size_t>(at - starts.begin());
+        if (at == starts.end())
+        {
+            starts.push_back(r.start);
+        }
+    }
+    bias_host_.resize(2 * starts.size());
+    updates_ = std::move(updates);
+    bias_starts_ = std::move(starts);
+    upload_bias();   // a step that is counted already finds its corrections in the new order
+}
+
+void AdamW::upload_bias()
+{
+    for (size_t k = 0; k < bias_starts_.size(); ++k)
+    {
+        // a count set back to before the start has the first step's corrections
+        const double t = static_cast<double>(steps_ > bias_starts_[k] ? steps_ - bias_starts_[k] : 1);
+        bias_host_[2 * k] = 1.0 - std::pow(static_cast<double>(config_.beta1), t);
+        bias_host_[2 * k + 1] = 1.0 - std::pow(static_cast<double>(config_.beta2), t);
+    }
+    if (!bias_host_.empty() &&
+        cudaMemcpyAsync(bias_.data_ptr(), bias_host_.data(), bias_host_.size() * sizeof(double), cudaMemcpyHostToDevice,
+                        cs()) != cudaSuccess)
+    {
+        throw std::runtime_error("AdamW: bias correction upload failed");
+    }
+}
+
+void AdamW::set_starts(const std::vector<size_t>& starts)
+{
+    if (starts.size() != parameters_.size())
+    {
+        throw std::invalid_argument("AdamW::set_starts: " + std::to_string(starts.size()) + " starts for " +
+                                    std::to_string(parameters_.size()) + " parameters");
+    }
+    starts_ = starts;
+    build_updates();
+}
+
+void AdamW::restart(const std::vector<size_t>& indices)
+{
+    std::vector<size_t> starts = starts_;
+    std::vector<size_t> offsets;
+    size_t at = 0;
+    for (const auto& p : parameters_)
+    {
+        offsets.push_back(at);
+        at += p.value().numel();
+    }
+    for (const size_t i : indices)
+    {
+        const size_t bytes = parameters_.at(i).value().numel() * sizeof(float);
+        if (bytes > 0 && (cudaMemsetAsync(fptr(m_arena_) + offsets[i], 0, bytes, cs()) != cudaSuccess ||
+                          cudaMemsetAsync(fptr(v_arena_) + offsets[i], 0, bytes, cs()) != cudaSuccess))
+        {
+            throw std::runtime_error("AdamW::restart: memset failed");
+        }
+        starts[i] = steps_;
+    }
+    set_starts(starts);
 }
 
 void AdamW::advance()
 {
     ++steps_;
-    bias_host_[0] = 1.0 - std::pow(static_cast<double>(config_.beta1), static_cast<double>(steps_));
-    bias_host_[1] = 1.0 - std::pow(static_cast<double>(config_.beta2), static_cast<double>(steps_));
-    if (cudaMemcpyAsync(bias_.data_ptr(), bias_host_, sizeof(bias_host_), cudaMemcpyHostToDevice, cs()) !=
-        cudaSuccess)
-    {
-        throw std::runtime_error("AdamW: bias correction upload failed");
-    }
+    upload_bias();
 }
 
 void AdamW::launch(const double* sumsq, float max_norm, float grad_scale)
@@ -185,7 +250,7 @@ void AdamW::launch(const double* sumsq, float max_norm, float grad_scale)
     {
         check(veda_adamw_step_dev(r.master, r.m, r.v, r.grad, r.lowp, r.n, config_.learning_rate,
                                   config_.beta1, config_.beta2, config_.eps, config_.weight_decay,
-                                  bias, sumsq, max_norm, grad_scale,
+                                  bias + 2 * r.bias, sumsq, max_norm, grad_scale,
                                   skip_nonfinite_ && sumsq != nullptr ? VEDA_ADAMW_SKIP_NONFINITE : 0,
                                   current_stream()),
               "AdamW::step");
@@ -279,9 +344,8 @@ void clear_grads(const std::vector<autograd::Variable>& parameters, const char* 
 constexpr size_t kMuonWorkspace = size_t{1} << 30;
 } // namespace
 
-void Muon::check_config() const
+void Muon::check_config(const MuonConfig& c)
 {
-    const MuonConfig& c = config_;
     if (!(c.learning_rate >= 0.0f) || !(c.weight_decay >= 0.0f) || !(c.eps >= 0.0f))
     {
         throw std::invalid_argument("Muon: learning rate, eps and weight decay must not be negative");
@@ -294,6 +358,16 @@ void Muon::check_config() const
     {
         throw std::invalid_argument("Muon: 1 to 64 Newton-Schulz steps");
     }
+}
+
+void Muon::set_config(const MuonConfig& config)
+{
+    check_config(config);
+    config_ = config;
+}
+
+void Muon::check_parameters() const
+{
     std::unordered_set<const void*> seen;
     for (const auto& p : parameters_)
     {
@@ -312,7 +386,8 @@ void Muon::check_config() const
 Muon::Muon(std::vector<autograd::Variable> parameters, MuonConfig config)
     : parameters_(std::move(parameters)), config_(config)
 {
-    check_config();
+    check_config(config_);
+    check_parameters();
     // Momentum and masters lie as the gradients do where those are views of one arena, so that equal
     // matrices at a constant distance stay so; back to back where the gradients are scattered.
     size_t total = 0;
@@ -390,7 +465,8 @@ Muon::Muon(AdamW& base, const std::vector<size_t>& indices, MuonConfig config) :
         momenta_.push_back(Tensor::view(base.first_moments().storage(), offsets[i], p.value().shape(), DType::F32));
         masters_.push_back(base.master(i));
     }
-    check_config();
+    check_config(config_);
+    check_parameters();
     build_batches();
     base.set_taken(indices, true);
     base_ = &base;
@@ -401,7 +477,15 @@ Muon::~Muon()
 {
     if (base_ != nullptr)
     {
-        base_->set_taken(taken_, false);
+        try
+        {
+            base_->restart(taken_);
+            base_->set_taken(taken_, false);
+        }
+        catch (...)
+        {
+            // a device that fails here fails the next call too; a destructor has no other way to say so
+        }
     }
 }
 

@@ -18,10 +18,13 @@
 
 #include "watchdog.hpp"
 
+#include <algorithm>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <filesystem>
+#include <map>
+#include <sstream>
 #include <stdexcept>
 #include <unordered_map>
 
@@ -741,6 +744,19 @@ Trainer::~Trainer()
     }
 }
 
+namespace
+{
+// Whether some of AdamW's parameters count their steps from a later one than the first.
+bool restarted(const optim::AdamW& opt)
+{
+    for (size_t i = 0; i < opt.parameters().size(); ++i)
+    {
+        if (opt.start(i) > 0) return true;
+    }
+    return false;
+}
+} // namespace
+
 void Trainer::init_data_parallel(const void* nccl_unique_id, int rank, int world,
                                  size_t bucket_bytes, bool sharded)
 {
@@ -758,6 +774,11 @@ void Trainer::init_data_parallel(const void* nccl_unique_id, int rank, int world
     if (sharded && muon_)
     {
         throw std::invalid_argument("Trainer: a sharded optimizer does not run Muon");
+    }
+    if (sharded && restarted(*opt_))
+    {
+        throw std::invalid_argument("Trainer: a sharded optimizer has one step count for all parameters, and Muon "
+                                    "has given some of them back");
     }
     dp_ = std::make_unique<DataParallel>(nccl_unique_id, rank, world, sharded);
     dp_->attach(*model_, bucket_bytes, master_weights(), opt_->steps(), batch_ * length_);
@@ -867,18 +888,13 @@ void Trainer::use_muon(const optim::MuonConfig& config)
         }
     }
     drop_step_graph();
-    // an earlier Muon hands its parameters back first, and takes them again if this one is refused
-    const bool had = muon_ != nullptr;
-    const optim::MuonConfig before = had ? muon_->config() : config;
-    muon_.reset();
-    try
+    if (muon_)
+    {
+        muon_->set_config(config);   // the momentum stays
+    }
+    else
     {
         muon_ = std::make_unique<optim::Muon>(*opt_, hidden, config);
-    }
-    catch (...)
-    {
-        if (had) muon_ = std::make_unique<optim::Muon>(*opt_, hidden, before);
-        throw;
     }
 }
 
@@ -1120,6 +1136,23 @@ std::vector<uint8_t> to_host_bytes(const void* device, size_t count)
 }
 } // namespace
 
+namespace
+{
+// "a,b=3" of a checkpoint's metadata as {a: "", b: "3"}; empty where there is no such entry.
+std::map<std::string, std::string> listed(const std::map<std::string, std::string>& metadata, const std::string& key)
+{
+    std::map<std::string, std::string> out;
+    const auto it = metadata.find(key);
+    std::stringstream items(it == metadata.end() ? "" : it->second);
+    for (std::string item; std::getline(items, item, ',');)
+    {
+        const size_t eq = item.find('=');
+        out[item.substr(0, eq)] = eq == std::string::npos ? "" : item.substr(eq + 1);
+    }
+    return out;
+}
+} // namespace
+
 void Trainer::save_checkpoint(const std::string& dir)
 {
     sync();
@@ -1165,8 +1198,25 @@ void Trainer::save_checkpoint(const std::string& dir)
         throw std::logic_error("save_checkpoint: parameters do not tile the arena");
     }
     io::write_safetensors(dir + "/model.safetensors", weights, {{"format", "pt"}});
-    io::write_safetensors(dir + "/optimizer.safetensors", state,
-                          {{"format", "pt"}, {"step", std::to_string(steps)}});
+    // Which first moments are a Muon's momentum, and where AdamW's moments began later than its first step.
+    std::map<std::string, std::string> metadata{{"format", "pt"}, {"step", std::to_string(steps)}};
+    std::string muon, starts;
+    size_t i = 0;
+    for (const auto& [name, value] : model_->named_parameters())
+    {
+        if (!sharded() && opt_->taken(i))
+        {
+            muon += (muon.empty() ? "" : ",") + name;
+        }
+        else if (!sharded() && opt_->start(i) > 0)
+        {
+            starts += (starts.empty() ? "" : ",") + name + "=" + std::to_string(opt_->start(i));
+        }
+        ++i;
+    }
+    if (!muon.empty()) metadata["muon"] = muon;
+    if (!starts.empty()) metadata["start"] = starts;
+    io::write_safetensors(dir + "/optimizer.safetensors", state, metadata);
 }
 
 void Trainer::load_checkpoint(const std::string& dir)
@@ -1232,6 +1282,33 @@ void Trainer::load_checkpoint(const std::string& dir)
         }
         steps = static_cast<size_t>(std::stoull(it->second));
     }
+    // A Muon's momentum goes on as one where a Muon has the parameter; AdamW, which has no use for it, begins anew.
+    std::vector<size_t> starts(model_->parameters().size(), 0);
+    const std::map<std::string, std::string> muon = listed(state.metadata, "muon"), later = listed(state.metadata, "start");
+    if (sharded() && (!muon.empty() || !later.empty()))
+    {
+        throw std::invalid_argument("load_checkpoint: a sharded optimizer has one step count for all parameters, and " + dir +
+                                    " holds a Muon's");
+    }
+    size_t i = 0;
+    at = 0;
+    for (const auto& [name, value] : model_->named_parameters())
+    {
+        const size_t count = value.numel();
+        if (const auto it = later.find(name); it != later.end())
+        {
+            starts[i] = static_cast<size_t>(std::stoull(it->second));
+        }
+        if (muon.contains(name) && !opt_->taken(i))
+        {
+            std::fill_n(m.begin() + at, count, 0.0f);
+            std::fill_n(v.begin() + at, count, 0.0f);
+            starts[i] = steps;
+        }
+        at += count;
+        ++i;
+    }
+    drop_step_graph();   // AdamW's runs and corrections may be others now
     float* dmaster = master_weights();
     cuda_check(cudaMemcpyAsync(dmaster, master.data(), n * sizeof(float), cudaMemcpyHostToDevice, cs()),
                "checkpoint write");
@@ -1247,6 +1324,7 @@ void Trainer::load_checkpoint(const std::string& dir)
                                cudaMemcpyHostToDevice, cs()),
                "checkpoint write");
     opt_->set_steps(steps);
+    opt_->set_starts(starts);
     if (sharded())
     {
         dp_->load_master(dmaster);
