@@ -170,6 +170,9 @@ public:
     core::Tensor master(size_t i) const { return masters_[i]; }
     // Batches a step launches.
     size_t batches() const noexcept { return batches_.size(); }
+    // Weights that a step updates, and the operations of its products (symmetric ones counted by halves).
+    size_t elements() const noexcept;
+    double flops() const noexcept;
 
 private:
     struct Batch

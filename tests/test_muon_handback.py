@@ -107,3 +107,28 @@ def test_muon_with_other_numbers_keeps_its_momentum(cuda):
     b.close()
 
 
+@pytest.mark.gpu
+def test_profile_class_of_muon(cuda):
+    from veda_b200 import train_abi as TA
+    cfg, B, T = QWEN, 2, 128
+    params = O.init_params(cfg, 11, bf16=True)
+    ids, tg = O.synthetic_batch(cfg, B, T, 11)
+    t = trainer(cfg, 1, B, T, params)
+    t.use_muon(1e-3)
+    t.step_host(ids, tg)
+    TA.profile_enable(True)
+    try:
+        t.step_host(ids, tg)
+        got = TA.profile_collect()
+    finally:
+        TA.profile_enable(False)
+    t.close()
+    shapes = [shape for name, shape in O.param_specs(cfg) if is_hidden(name, shape)]
+    taken = sum(int(np.prod(s)) for s in shapes)
+    every = sum(int(np.prod(s)) for _, s in O.param_specs(cfg))
+    flops = sum(5.0 * (m * m * n + m ** 3 + 2.0 * m * m * n) for m, n in ((min(s), max(s)) for s in shapes))
+    ms, f, b, n = got["muon"]
+    assert n == 1 and ms > 0 and b == 22.0 * taken and abs(f - flops) <= 1e-9 * flops
+    ms, f, b, n = got["adamw"]
+    # every gradient for the norm; gradient, moments and masters of the rest
+    assert n == 1 and ms > 0 and b == 4.0 * every + 30.0 * (every - taken)

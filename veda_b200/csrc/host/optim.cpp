@@ -591,6 +591,24 @@ void Muon::step_clipped(float max_norm, float grad_scale)
     launch(ss, max_norm, grad_scale);
 }
 
+size_t Muon::elements() const noexcept
+{
+    size_t n = 0;
+    for (const Batch& b : batches_) n += static_cast<size_t>(b.count * b.rows * b.cols);
+    return n;
+}
+
+double Muon::flops() const noexcept
+{
+    double sum = 0.0;
+    for (const Batch& b : batches_)
+    {
+        const double m = static_cast<double>(std::min(b.rows, b.cols)), n = static_cast<double>(std::max(b.rows, b.cols));
+        sum += static_cast<double>(b.count * static_cast<int64_t>(config_.steps)) * (m * m * n + m * m * m + 2.0 * m * m * n);
+    }
+    return sum;
+}
+
 void Muon::zero_grad() { clear_grads(parameters_, "Muon::zero_grad"); }
 
 float clip_gradient_norm(const std::vector<autograd::Variable>& parameters, float max_norm)

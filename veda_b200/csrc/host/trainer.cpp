@@ -1102,23 +1102,27 @@ void Trainer::step_impl(const Tensor& ids, const Tensor& targets)
         dp_->finish();
     }
     {
+        // every gradient is read for the norm; a Muon updates its parameters in a class of its own
         const double n = static_cast<double>(model_->parameter_count()) /
                          static_cast<double>(sharded() ? world() : 1);
-        profile::Scope scope("adamw", 0.0,
-                             n * (4.0 + 16.0 + 12.0 + (model_->dtype() == DType::BF16 ? 2.0 : 0.0)));
+        const double updated = n - (muon_ ? static_cast<double>(muon_->elements()) : 0.0);
+        const double lowp = model_->dtype() == DType::BF16 ? 2.0 : 0.0;
+        profile::Scope scope("adamw", 0.0, n * 4.0 + updated * (16.0 + 12.0 + lowp));
         if (sharded())
         {
             dp_->update(opt_->config(), max_norm_);
         }
         else
         {
-            const float scale = 1.0f / static_cast<float>(world());
-            opt_->launch_clipped(max_norm_, scale);
-            if (muon_)
-            {
-                muon_->launch(opt_->sumsq(), max_norm_, scale);
-            }
+            opt_->launch_clipped(max_norm_, 1.0f / static_cast<float>(world()));
         }
+    }
+    if (muon_)
+    {
+        // gradient read, momentum and master read and written, weights written
+        profile::Scope scope("muon", muon_->flops(),
+                             static_cast<double>(muon_->elements()) * (20.0 + (model_->dtype() == DType::BF16 ? 2.0 : 0.0)));
+        muon_->launch(opt_->sumsq(), max_norm_, 1.0f / static_cast<float>(world()));
     }
     cuda_check(cudaMemcpyAsync(loss_.data_ptr(), loss.value().data_ptr(), sizeof(float),
                                cudaMemcpyDeviceToDevice, cs()),
