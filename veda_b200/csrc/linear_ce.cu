@@ -2279,7 +2279,7 @@ extern "C" int veda_linear_cross_entropy_fwd(const void* x, int64_t ldx, const v
                                : pair::clusters_available<lce::StatsWork<256>, 4, false>();
     if (clusters < 1)
     {
-        return fail(VEDA_ERR_UNSUPPORTED, "veda_linear_cross_entropy_fwd: no CTA pair fits on this device");
+        return pair::none_available("veda_linear_cross_entropy_fwd", clusters);
     }
     lce::Params p{};
     rc = lce::prepare(c, targets, ignore_index, nullptr, nullptr, false, p, stream);
@@ -2350,7 +2350,7 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
                                                            : pair::clusters_available<lce::GradWork<256>, 8, false>());
     if (clusters < 1)
     {
-        return fail(VEDA_ERR_UNSUPPORTED, "veda_linear_cross_entropy_bwd: no CTA pair fits on this device");
+        return pair::none_available("veda_linear_cross_entropy_bwd", clusters);
     }
     lce::Params p{};
     rc = lce::prepare(c, targets, ignore_index, upstream, status, true, p, stream);

@@ -1787,7 +1787,7 @@ int products(const char* what, int64_t batch, int64_t rows, int64_t cols, int st
     const int clusters = pair::clusters_available<W, 8, SPLIT>();
     if (clusters < 1)
     {
-        return fail(VEDA_ERR_UNSUPPORTED, std::string(what) + ": no CTA pair fits on this device");
+        return pair::none_available(what, clusters);
     }
     // more clusters than a step of the batch has tiles would only wait
     const int64_t most = std::max(half, whole) * batch;

@@ -461,7 +461,8 @@ bool make_map3(CUtensorMap* map, const void* base, int es, bool is_bf16, int64_t
                Swizzle swizzle = Swizzle::k128);
 
 // Clusters of the kernel that the current device can hold at once, capped by the SMs that
-// veda_set_reserved_sms leaves (0: none fit). Cached per device.
+// veda_set_reserved_sms leaves (0: none fit; -1: the query failed, and is asked again at the next call).
+// Cached per device.
 template <class Work, int EPI_WARPS, bool SPLIT>
 int clusters_available()
 {
@@ -478,6 +479,7 @@ int clusters_available()
     {
         auto kernel = pair_kernel<Work, EPI_WARPS, SPLIT>;
         int n = 0;
+        bool ok = false;
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<EPI_WARPS, Work::TN>::SMEM) ==
             cudaSuccess)
         {
@@ -492,17 +494,25 @@ int clusters_available()
             attr.val.clusterDim.z = 1;
             cfg.attrs = &attr;
             cfg.numAttrs = 1;
-            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess)
-            {
-                n = 0;
-            }
+            ok = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess;
+        }
+        if (!ok)
+        {
             cudaGetLastError();
+            return -1;
         }
         have = n + 1;
         cached[device].store(have, std::memory_order_release);
     }
     const int cap = compute_sms() / 2;
     return have - 1 < cap ? have - 1 : cap;
+}
+
+// The error of a call whose clusters_available() is below 1.
+inline int none_available(const char* what, int clusters)
+{
+    return clusters < 0 ? fail(VEDA_ERR_CUDA, std::string(what) + ": the query for the device's clusters failed")
+                        : fail(VEDA_ERR_UNSUPPORTED, std::string(what) + ": no CTA pair fits on this device");
 }
 
 template <class Work, int EPI_WARPS, bool SPLIT>
