@@ -423,6 +423,32 @@ def test_lse_of_rows_that_are_not_counted(cuda, dtype, scale, rows, vocab, dim, 
     assert bool((row == row0).all()) and float(loss) == float(loss0) and bool((lse[::2] == lse0[::2]).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [V.BF16, V.F32])
+@pytest.mark.parametrize("scale", [1e9, 1e14, 1e30])
+@pytest.mark.parametrize("rows,vocab,dim", [(1, 300, 64), (4, 300, 64), (60, 300, 64), (60, 4300, 64), (300, 5001, 40)])
+def test_forward_of_huge_logits(cuda, dtype, scale, rows, vocab, dim):
+    # logits whose rounding in log2 units is itself past the exponential's range: the reference of a row's sum lies
+    # above them, so no term overflows, and a sum that vanishes leaves the maximum
+    t = torch()
+    x, w, tg = make(rows, vocab, dim, dtype, seed=19, ignored=0.2)
+    x = (x.float() * scale).to(x.dtype)
+    row, lse, loss = fwd(x, w, tg, dtype)
+    sync()
+    z = x.double() @ w.double().t()
+    seg, drop = (3, 3 * 2.0 ** -22) if dtype == V.F32 else (1, 0.0)
+    dz = ((seg * dim / 16 + 4) * 2.0 ** -23 + drop) * (x.double().abs() @ w.double().abs().t()).amax(1)
+    want = t.logsumexp(z, 1)
+    # beside the module's bounds: a sum of up to `vocab` terms that vanished against the maximum's rounding
+    dlse = dz + 2.0 ** -21 + 4 * 2.0 ** -24 * want.abs() + t.where(want.abs() > 1e9, float(np.log(vocab)), 0.0)
+    within(lse, want, dlse, "lse")
+    used = tg != IGN
+    at = t.where(used, tg, 0)[:, None]
+    drow = dz + dlse + 2.0 ** -23 * (want.abs() + z.gather(1, at)[:, 0].abs())
+    within(row, t.where(used, want - z.gather(1, at)[:, 0], 0.0), t.where(used, drow, 0.0) + 1e-30, "row loss")
+    assert bool(loss.isfinite().all())
+
+
 def test_workspace_sizes_and_refusals_without_a_gpu():
     lib = V.lib()
     size = lib.veda_linear_cross_entropy_workspace

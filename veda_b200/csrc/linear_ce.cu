@@ -58,6 +58,10 @@ __device__ __forceinline__ float ex2(float x)
     return y;
 }
 
+// A logit as a reference in log2 units, rounded up: z log2 e - reference, in one fused operation, is at most 0 then.
+// Rounded to nearest, it could be positive by 2^-24 of its size, and 2 to that power infinite above 2^31.
+__device__ __forceinline__ float log2_units(float z) { return __fmul_ru(z, kLog2e); }
+
 // Device scalars of a call: what turns a tile's sum into a logit, and the gradients' factors. The
 // powers of two stay apart from coef: their product with it could be subnormal where dx is not.
 struct Scalars
@@ -260,7 +264,7 @@ struct StatsWork
             float mx[4] = {z[0], z[1], z[2], z[3]};
 #pragma unroll
             for (int j = 4; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], z[j]);
-            const float m = fmaxf(s.m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kLog2e);
+            const float m = fmaxf(s.m, log2_units(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))));
             // a row of -inf so far: any finite reference gives exponentials of 0, and NaN stays NaN
             const float ref = m == -INFINITY ? 0.0f : m;
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -870,7 +874,9 @@ merge_kernel(const float2* __restrict__ parts, int slots, int64_t rows, int64_t 
     }
     if (slice == 0 && row < rows)
     {
-        const float l = (m + log2f(s)) * kLn2;
+        // a sum of 0: every term vanished against the rounding of a maximum past 2^31, whose logarithm the sum's
+        // could not change
+        const float l = (s == 0.0f ? m : m + log2f(s)) * kLn2;
         if (lse != nullptr) lse[row] = l;
         const int64_t t = targets[row];
         const bool inside = t >= 0 && t < vocab;
@@ -1258,7 +1264,7 @@ few_fwd_kernel(const Few p)
             {
                 if (v + j >= p.vocab) z[j] = -INFINITY;
                 else if (valid && target == v + j) p.target_logit[row_] = z[j];
-                top = fmaxf(top, z[j] * kLog2e);
+                top = fmaxf(top, log2_units(z[j]));
             }
             const float ref = top == -INFINITY ? 0.0f : top;
             s *= ex2(m - ref);
