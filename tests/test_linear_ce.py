@@ -449,6 +449,47 @@ def test_forward_of_huge_logits(cuda, dtype, scale, rows, vocab, dim):
     assert bool(loss.isfinite().all())
 
 
+def _bias(got, want):
+    return float(((got.double() - want) / want).mean())
+
+
+@pytest.mark.gpu
+def test_long_fp32_sums_are_as_exact_as_one_chain(cuda):
+    # The tensor core truncates as it adds, so what a chain of four k-blocks (256 terms) falls short of its sum
+    # is a constant share of it where all terms have one sign; the folds that join the chains round to nearest
+    # and add none. 32 times the same terms therefore fall short by the same share as 256 do: in the mean
+    # over 1024 columns the folds' own roundings (2^-24 each, 32 of them in a sum) leave some 2^-24
+    # sqrt(32 / 1024) = 1e-8 of noise beside the chain's 17 / 2 additions of at least 2^-26 each, 1.3e-7: a
+    # quarter is allowed. A chain of twice the length would double the share, one without folds take it to 32.
+    # lse = 0 and logits of 0 make every q exactly 1, and 0 at the target, whose word or row holds zeros.
+    t = torch()
+    dim, rows, words = 1024, 8192, 256
+    g = t.Generator(device="cuda").manual_seed(16)
+    lse = t.zeros(rows, device="cuda")
+    tg = t.zeros(rows, device="cuda", dtype=t.int64)
+    short = []
+    for k in (1, 32):
+        w = t.rand(words, dim, device="cuda", generator=g.manual_seed(17)) + 0.5
+        w[0] = 0
+        w = w.repeat(k, 1)
+        dx = empty((rows, dim))
+        bwd(t.zeros(rows, dim, device="cuda"), w, tg, lse, V.F32, dx=dx)
+        sync()
+        assert bool((dx == dx[0]).all())
+        short.append(-_bias(dx[0], w.double().sum(0) / rows))
+    assert 0 <= short[1] <= 1.25 * short[0], short
+    short = []
+    for k in (1, 32):
+        n = words * k
+        x = (t.rand(words, dim, device="cuda", generator=g.manual_seed(18)) + 0.5).repeat(k, 1)
+        dw = empty((4500, dim))
+        bwd(x, t.zeros(4500, dim, device="cuda"), tg[:n], lse[:n], V.F32, dw=dw)
+        sync()
+        assert bool((dw[1:] == dw[1]).all()) and not bool(dw[0].any())
+        short.append(-_bias(dw[1], x.double().sum(0) / n))
+    assert 0 <= short[1] <= 1.25 * short[0], short
+
+
 def test_workspace_sizes_and_refusals_without_a_gpu():
     lib = V.lib()
     size = lib.veda_linear_cross_entropy_workspace

@@ -485,6 +485,33 @@ def test_norms_of_any_size_without_eps(cuda, dtype, r, c, power):
     assert not bool(base.isnan().any()) and bool((got == base).all())
 
 
+@pytest.mark.gpu
+def test_long_fp32_sums_are_as_exact_as_one_chain(cuda):
+    # The tensor core truncates as it adds: a chain of two k-blocks (128 terms) of one sign falls short of its sum by a
+    # constant share, and the folds that join chains round to nearest and add none. One step with a = c = 0, b = 1 is
+    # S X: 64 copies of a matrix side by side have its S (the copies are scaled by 1/8, exactly) and, in every
+    # copy, its S X / 8, out of 64 times the chains. What the planes of X, S and M round is formed here, so the products
+    # alone are compared, in the mean over 129 x 129 elements: S and M X add one chain's share each (129 terms of M X,
+    # the same in both), and a fold's 2^-24 of random sign vanishes in the mean. A quarter is allowed; with chains of
+    # twice the length the share of S doubles, half as much again in all, and without folds it grows 64 times.
+    t = torch()
+    n = 129
+    u = t.rand(1, n, n, device="cuda", generator=t.Generator(device="cuda").manual_seed(24)) + 0.5
+    h = lambda v: v.to(t.float16).double()
+    two = lambda v: h(v) + h(v - h(v))
+    short = []
+    for k in (1, 64):
+        g = u.repeat(1, 1, k)
+        got = orth(g, dtype=V.F32, steps=1, coef=(0.0, 1.0, 0.0), eps=0.0)
+        sync()
+        scale = (1024.0 / g.double().square().sum().sqrt()).float()
+        x = two((g * scale).double())[0]
+        m = two(x @ x.mT / 1024)
+        want = m @ x / 1024 / 1024
+        short.append(-float(((got[0].double() - want) / want).mean()))
+    assert 0 <= short[1] <= 1.25 * short[0], short
+
+
 def test_workspaces_and_refusals_without_a_gpu():
     lib = V.lib()
     size = lib.veda_orthogonalize_workspace
