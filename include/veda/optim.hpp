@@ -130,6 +130,9 @@ struct MuonConfig
     // The orthogonalised update is scaled by 0.2 sqrt(max(rows, cols)), which gives its entries the
     // size of AdamW's, so learning rates carry over (false: by sqrt(max(1, rows / cols))).
     bool match_adamw = true;
+    // bf16 parameters with both sides above 64: products as for fp32 ones (VEDA_MUON_FP32_PRODUCTS), which keeps the
+    // master weights exact to fp32 at three times the operations; without, the update is off by some 0.15 %.
+    bool fp32_products = false;
 };
 
 // Momentum orthogonalised by Newton-Schulz products (veda_muon_step) for rank-2 parameters:

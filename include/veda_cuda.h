@@ -365,10 +365,13 @@ int veda_orthogonalize(const void* g, int64_t ldg, int64_t stride_g, void* out, 
  *   momentum <- beta momentum + g;  u = nesterov ? g + beta momentum : momentum;
  *   master <- master - lr weight_decay master - lr update_scale orthogonalize(u);
  *   lowp <- bf16(master).
- * The products run as for bf16 matrices when lowp is given and both sides are above 64, else as for fp32
- * ones (veda_orthogonalize). flags: VEDA_ADAMW_SKIP_NONFINITE leaves everything untouched when the norm
- * is not finite. grad is not written. The workspace's dtype is VEDA_BF16 when lowp is given, else
- * VEDA_F32. */
+ * The products run as for bf16 matrices when lowp is given and both sides are above 64 (the update is off by some
+ * 0.15 % then, which shows in master, not in lowp), else as for fp32 ones (veda_orthogonalize). flags:
+ * VEDA_ADAMW_SKIP_NONFINITE leaves everything untouched when the norm is not finite;
+ * VEDA_MUON_FP32_PRODUCTS runs the products as for fp32 matrices beside lowp, too, three times as many.
+ * grad is not written. The workspace's dtype is VEDA_BF16 when lowp is given without
+ * VEDA_MUON_FP32_PRODUCTS, else VEDA_F32. */
+#define VEDA_MUON_FP32_PRODUCTS 4
 size_t veda_muon_step_workspace(int64_t batch, int64_t rows, int64_t cols, int dtype);
 int veda_muon_step(float* master, float* momentum, const float* grad, void* lowp, int64_t batch,
                    int64_t rows, int64_t cols, int64_t stride, float lr, float beta, int nesterov,

@@ -486,6 +486,31 @@ def test_norms_of_any_size_without_eps(cuda, dtype, r, c, power):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("b,r,c", [(2, 260, 520), (1, 1001, 523), (2, 100, 2300), (1, 4203, 70), (2, 80, 96)])
+def test_muon_with_fp32_products_keeps_master_weights_exact(cuda, b, r, c):
+    # VEDA_MUON_FP32_PRODUCTS beside bf16 weights: the bound of fp32 weights; tiled, cut among blocks and in one
+    master, momentum, grad, lowp = muon_state(b, r, c, True, seed=25)
+    w, m, u, o, _ = muon_want(master, momentum, grad)
+    ws = workspace(V.lib().veda_muon_step_workspace(b, r, c, V.F32))
+    muon(master, momentum, grad, lowp, (b, r, c), r * c, flags=4, ws=ws)
+    sync()
+    tol = 1e-2 * 1.7 * (bound(u, o, V.F32, True) + 310 * 3 * 2.0 ** -24 * fro(o)) + 4 * 2.0 ** -24 * fro(w)
+    assert bool((fro(master.double() - w) <= tol).all()), (fro(master.double() - w) / tol).max()
+    assert bool((lowp == master.to(torch().bfloat16)).all())
+
+
+def test_workspace_of_muon_with_fp32_products_without_a_gpu():
+    # what serves bf16 weights is too small for them
+    lib = V.lib()
+    buf = ctypes.create_string_buffer(1024)
+    a = (ctypes.addressof(buf) + 255) // 256 * 256
+    n = lib.veda_muon_step_workspace(1, 300, 400, V.BF16)
+    rc = lib.veda_muon_step(a, a, a, a, 1, 300, 400, 300 * 400, 1.0, 0.9, 1, 0.0, 1.0, 5, *NS, 1e-7, None, 1.0, 1.0, 4, a, n, None)
+    assert rc == V.ERR_INVALID_ARGUMENT and "workspace" in lib.veda_last_error().decode()
+    assert n < lib.veda_muon_step_workspace(1, 300, 400, V.F32)
+
+
+@pytest.mark.gpu
 def test_long_fp32_sums_are_as_exact_as_one_chain(cuda):
     # The tensor core truncates as it adds: a chain of two k-blocks (128 terms) of one sign falls short of its sum by a
     # constant share, and the folds that join chains round to nearest and add none. One step with a = c = 0, b = 1 is

@@ -363,7 +363,12 @@ void Muon::check_config(const MuonConfig& c)
 void Muon::set_config(const MuonConfig& config)
 {
     check_config(config);
+    const bool other = config.fp32_products != config_.fp32_products;
     config_ = config;
+    if (other)
+    {
+        build_batches();   // their workspace is another
+    }
 }
 
 void Muon::check_parameters() const
@@ -504,6 +509,7 @@ void Muon::build_batches()
                step(masters_[a], masters_[b]) == d && step(momenta_[a], momenta_[b]) == d;
     };
     batches_.clear();
+    workspace_bytes_ = 0;
     std::vector<bool> done(parameters_.size(), false);
     size_t largest = 1;
     for (size_t i = 0; i < parameters_.size(); ++i)
@@ -521,7 +527,7 @@ void Muon::build_batches()
         const Shape& shape = p.value().shape();
         const int64_t rows = static_cast<int64_t>(shape[0]), cols = static_cast<int64_t>(shape[1]);
         const bool lowp = p.value().dtype() == DType::BF16;
-        const int d = lowp ? VEDA_BF16 : VEDA_F32;
+        const int d = lowp && !config_.fp32_products ? VEDA_BF16 : VEDA_F32;
         Batch b{i, 1, rows, cols, 0, fptr(masters_[i]), fptr(momenta_[i]), fptr(g),
                 lowp ? p.value().data_ptr() : nullptr};
         size_t last = i;
@@ -553,7 +559,8 @@ void Muon::launch(const double* sumsq, float max_norm, float grad_scale)
 {
     flush_host_writes(parameters_);
     const MuonConfig& c = config_;
-    const int flags = base_ != nullptr && base_->skip_nonfinite() ? VEDA_ADAMW_SKIP_NONFINITE : 0;
+    const int flags = (base_ != nullptr && base_->skip_nonfinite() ? VEDA_ADAMW_SKIP_NONFINITE : 0) |
+                      (c.fp32_products ? VEDA_MUON_FP32_PRODUCTS : 0);
     for (const Batch& b : batches_)
     {
         const float rows = static_cast<float>(b.rows), cols = static_cast<float>(b.cols);

@@ -1796,7 +1796,8 @@ int products(const char* what, int64_t batch, int64_t rows, int64_t cols, int st
 
 // Whether Muon's products are split: for fp32 weights, and for matrices of some 30 to 50 rows or columns
 // whose other side is too long for a cluster, on which fp16 products come out least exact (fp32 weights off by
-// 1.1e-5 at 32 x 4200, 3e-6 at 64; split 4e-8).
+// 1.1e-5 at 32 x 4200, 3e-6 at 64; split 4e-8). Larger matrices beside bf16 weights are split where the caller asks
+// (VEDA_MUON_FP32_PRODUCTS): their master weights come out 3e-6 off without, and 28 x 2048 x 1024 takes 1.4 against 4.7 ms.
 bool muon_split(int64_t rows, int64_t cols, bool lowp) { return !lowp || std::min(rows, cols) <= 64; }
 
 // norm, X, then the products of every step; p's destination says what the last one (LAST) writes.
@@ -1940,7 +1941,7 @@ extern "C" int veda_muon_step(float* master, float* momentum, const float* grad,
         return VEDA_OK;
     }
     VEDA_REQUIRE(master != nullptr && momentum != nullptr && grad != nullptr, "null pointer");
-    const bool split = ns::muon_split(rows, cols, lowp != nullptr);
+    const bool split = ns::muon_split(rows, cols, lowp != nullptr) || (flags & VEDA_MUON_FP32_PRODUCTS) != 0;
     int rc = ns::check_workspace("veda_muon_step", workspace, workspace_bytes,
                                  ns::layout(batch, rows, cols, split, ns::kMaxSteps).total);
     if (rc != VEDA_OK) return rc;
