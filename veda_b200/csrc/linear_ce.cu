@@ -2298,8 +2298,8 @@ extern "C" int veda_linear_cross_entropy_fwd(const void* x, int64_t ldx, const v
     const int64_t units = static_cast<int64_t>(c.l.slots) * p.num_m;
     VEDA_REQUIRE(units <= lce::kLimit, "too many tiles");
     const int grid = static_cast<int>(std::min<int64_t>(units, clusters));
-    rc = split ? pair::launch_pair<lce::StatsWork<128>, 4, true>("veda_linear_cross_entropy_fwd", p, grid, stream)
-               : pair::launch_pair<lce::StatsWork<256>, 4, false>("veda_linear_cross_entropy_fwd", p, grid, stream);
+    rc = split ? pair::launch_pair<lce::StatsWork<128>, 4, true>("veda_linear_cross_entropy_fwd", p, grid, false, stream)
+               : pair::launch_pair<lce::StatsWork<256>, 4, false>("veda_linear_cross_entropy_fwd", p, grid, false, stream);
     if (rc != VEDA_OK) return rc;
     return lce::launch_merge(p.parts, c.l.slots, rows, vocab, targets, ignore_index, p.target_logit, row_loss, lse, loss,
                              p.done, status, stream);
@@ -2428,8 +2428,8 @@ extern "C" int veda_linear_cross_entropy_bwd(const void* x, int64_t ldx, const v
         // k-blocks a tile, and what its epilogue adds
         const int64_t cost[3] = {(rows + 63) / 64 + 4, p.dx_kbs + 2, (dim + 63) / 64 + 2};
         lce::share(tiles, cost, grid, p.shares);
-        rc = split ? pair::launch_pair<lce::GradWork<128>, 8, true>("veda_linear_cross_entropy_bwd", p, grid, stream)
-                   : pair::launch_pair<lce::GradWork<256>, 8, false>("veda_linear_cross_entropy_bwd", p, grid, stream);
+        rc = split ? pair::launch_pair<lce::GradWork<128>, 8, true>("veda_linear_cross_entropy_bwd", p, grid, k > 0, stream)
+                   : pair::launch_pair<lce::GradWork<256>, 8, false>("veda_linear_cross_entropy_bwd", p, grid, k > 0, stream);
         if (rc != VEDA_OK) return rc;
     }
     if (dx == nullptr)

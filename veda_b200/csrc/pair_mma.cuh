@@ -460,6 +460,9 @@ bool make_map3(CUtensorMap* map, const void* base, int es, bool is_bf16, int64_t
                int64_t planes, int64_t ld, int64_t plane, uint32_t bx, uint32_t by,
                Swizzle swizzle = Swizzle::k128);
 
+// Shared memory of a launch: all of an SM's, so that no other kernel's blocks run beside it.
+constexpr int kOwnSm = 227 * 1024;
+
 // Clusters of the kernel that the current device can hold at once, capped by the SMs that
 // veda_set_reserved_sms leaves (0: none fit; -1: the query failed, and is asked again at the next call).
 // Cached per device.
@@ -480,13 +483,12 @@ int clusters_available()
         auto kernel = pair_kernel<Work, EPI_WARPS, SPLIT>;
         int n = 0;
         bool ok = false;
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<EPI_WARPS, Work::TN>::SMEM) ==
-            cudaSuccess)
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOwnSm) == cudaSuccess)
         {
             cudaLaunchConfig_t cfg{};
             cfg.gridDim = dim3(2 * (sm_count() / 2));
             cfg.blockDim = dim3(Cfg<EPI_WARPS, Work::TN>::THREADS);
-            cfg.dynamicSmemBytes = Cfg<EPI_WARPS, Work::TN>::SMEM;
+            cfg.dynamicSmemBytes = kOwnSm;
             cudaLaunchAttribute attr{};
             attr.id = cudaLaunchAttributeClusterDimension;
             attr.val.clusterDim.x = 2;
@@ -515,11 +517,33 @@ inline int none_available(const char* what, int clusters)
                         : fail(VEDA_ERR_UNSUPPORTED, std::string(what) + ": no CTA pair fits on this device");
 }
 
+// overlapped: may start while the kernel ahead is running (launch()), which has to be of this kind too: its blocks own
+// their SMs as these do. Behind others the tensor memory would be allocated beside their last blocks, and there one
+// cluster's allocation never came back, its SMs long empty and every other cluster finished: once in some 7000 calls
+// of the loss head of 2048 x 32000 x 1024 in fp32, behind the launch that lays operands out. With both kept apart,
+// 109000 calls ran through.
 template <class Work, int EPI_WARPS, bool SPLIT>
-int launch_pair(const char* what, const typename Work::Params& p, int clusters, cudaStream_t s)
+int launch_pair(const char* what, const typename Work::Params& p, int clusters, bool overlapped, cudaStream_t s)
 {
-    return launch(what, pair_kernel<Work, EPI_WARPS, SPLIT>, dim3(2 * clusters), dim3(Cfg<EPI_WARPS, Work::TN>::THREADS),
-                  Cfg<EPI_WARPS, Work::TN>::SMEM, s, p);
+    const auto kernel = pair_kernel<Work, EPI_WARPS, SPLIT>;
+    const dim3 grid(2 * clusters), block(Cfg<EPI_WARPS, Work::TN>::THREADS);
+    if (overlapped)
+    {
+        return launch(what, kernel, grid, block, kOwnSm, s, p);
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = kOwnSm;
+    cfg.stream = s;
+    count_launch();
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, p);
+    if (err != cudaSuccess)
+    {
+        cudaGetLastError();
+        return fail(VEDA_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(err));
+    }
+    return check_launch(what);
 }
 
 // The same with all clusters on the device at once (a cooperative launch), for a Work whose tiles wait
@@ -530,7 +554,7 @@ int launch_together(const char* what, const typename Work::Params& p, int cluste
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(2 * clusters);
     cfg.blockDim = dim3(Cfg<EPI_WARPS, Work::TN>::THREADS);
-    cfg.dynamicSmemBytes = Cfg<EPI_WARPS, Work::TN>::SMEM;
+    cfg.dynamicSmemBytes = kOwnSm;
     cfg.stream = s;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeCooperative;
