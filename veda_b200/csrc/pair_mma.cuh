@@ -120,6 +120,18 @@ __device__ __forceinline__ void cluster_sync()
 {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
+// A whole warp's bounded wait, converged afterwards (the elected lane issues for all, and tensor memory is read by
+// whole warps); false once a wait of the CTA has given up.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t phase, int* status, volatile int* abort)
+{
+    bool ok = tc::mbar_try_wait(tc::smem_u32(bar), phase);
+    if (!ok)
+    {
+        tc::mbar_wait(bar, phase, status, abort);
+        ok = *abort == 0;
+    }
+    return __all_sync(0xFFFFFFFFu, ok);
+}
 __device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z)
 {
     asm volatile(
@@ -278,8 +290,10 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
                 const int adx = t.a_mn ? 0 : kBK, ady = t.a_mn ? kBK : 0;
                 const int bdx = t.b_mn ? 0 : kBK, bdy = t.b_mn ? kBK : 0;
                 auto load = [&](int kb, int za, int zb) {
-                    mbar_wait(&empty[stage], phase ^ 1, p.status, abort);
-                    __syncwarp();
+                    if (!warp_wait(&empty[stage], phase ^ 1, p.status, abort))
+                    {
+                        return;   // nothing frees the stages any more
+                    }
                     const uint32_t bar = peer_addr(&full[stage], 0);
                     uint8_t* ad = sa + stage * C_::A_BYTES;
                     uint8_t* bd = sb + stage * C_::B_BYTES;
@@ -321,6 +335,17 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
             }
             more = Work::tile(p, cid, clusters, ++i, t);   // the ring is full of this tile's blocks
         }
+        // The last release of every stage arrives before the CTA leaves: its signals cross CTAs on their own, and
+        // the next kernel's barriers take these barriers' place.
+        for (int s = 0; s < C_::STAGES; ++s)
+        {
+            warp_wait(&empty[stage], phase ^ 1, p.status, abort);
+            if (++stage == C_::STAGES)
+            {
+                stage = 0;
+                phase ^= 1;
+            }
+        }
     }
     else if (warp == 1 && rank == 0)
     {
@@ -343,14 +368,15 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
             {
                 const int blocks = SPLIT ? 3 * (min(t.kbs, k0 + Work::CHAIN) - k0) : t.kbs;
                 const int buf = TWO ? it & 1 : 0;
-                mbar_wait(&tempty[buf], ((TWO ? it >> 1 : it) & 1) ^ 1, p.status, abort);
-                __syncwarp();
+                warp_wait(&tempty[buf], ((TWO ? it >> 1 : it) & 1) ^ 1, p.status, abort);
                 fence_after();
                 const uint32_t d = tmem + static_cast<uint32_t>(buf * TN);
                 for (int kb = 0; kb < blocks; ++kb)
                 {
-                    mbar_wait(&full[stage], phase, p.status, abort);
-                    __syncwarp();
+                    if (!warp_wait(&full[stage], phase, p.status, abort))
+                    {
+                        break;
+                    }
                     fence_after();
                     const uint64_t ad = smem_desc(smem_u32(sa + stage * C_::A_BYTES), albo, 1024);
                     const uint64_t bd = smem_desc(smem_u32(sb + stage * C_::B_BYTES), blbo, 1024);
@@ -402,7 +428,7 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
             for (int k0 = 0; !t.skip && k0 < t.kbs; k0 += SPLIT ? Work::CHAIN : t.kbs)
             {
                 const int buf = TWO ? it & 1 : 0;
-                mbar_wait(&tfull[buf], (TWO ? it >> 1 : it) & 1, p.status, abort);
+                warp_wait(&tfull[buf], (TWO ? it >> 1 : it) & 1, p.status, abort);
                 fence_after();
                 const uint32_t base = tmem + static_cast<uint32_t>(buf * TN + col0) +
                                       (static_cast<uint32_t>(quarter * 32) << 16);
@@ -443,7 +469,15 @@ pair_kernel(const __grid_constant__ typename Work::Params p)
     }
     fence_before();
     __syncthreads();
+    if (*abort != 0)
+    {
+        // a wait gave up: half a millisecond, in which the loads and products in flight end
+        for (const long long start = clock64(); clock64() - start < (1ll << 20);)
+        {
+        }
+    }
     cluster_sync();   // no CTA leaves while its peer may still read its operands or barriers
+    __syncwarp();
     if (warp == 1)
     {
         fence_after();
