@@ -139,8 +139,12 @@ struct MuonConfig
 //   m <- momentum m + g;  u = nesterov ? g + momentum m : m;
 //   w <- w - lr weight_decay w - lr scale orthogonalize(u).
 // Momentum and, for bf16 parameters, master weights are fp32. Parameters of one shape that lie a
-// constant distance apart (the same matrix of every layer of train::TinyTransformer) are updated as
-// one batch. Not part of the reference, whose optimizer is AdamW.
+// constant distance apart are updated as one batch: from each on, the next of its shape sets the distance and those
+// that follow at it join. In train::TinyTransformer that makes one batch of a matrix that is the only one of its shape
+// in a layer (down of every layer), and a pair a layer of two neighbours of one shape (k and v, gate and up).
+// Not part of the reference, whose optimizer is AdamW. The method and the quintic's coefficients: K. Jordan et al.,
+// "Muon: An optimizer for hidden layers in neural networks" (2024); the scale 0.2 sqrt(max(rows, cols)): J. Liu et
+// al., "Muon is Scalable for LLM Training" (2025).
 class Muon
 {
 public:

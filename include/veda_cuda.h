@@ -240,13 +240,14 @@ int veda_mean_f64(const float* v, int64_t n, float* out, double* out_f64, veda_s
 /* be NULL) to VEDA_ERR_OUT_OF_RANGE. With no counted row the loss and the gradients are 0.   */
 /*   fwd: lse[r] = log sum_v exp z[r, v], row_loss[r] = lse[r] - z[r, t_r], loss[0] = the mean  */
 /*        over the counted rows, all fp32; lse and loss may be NULL. What a row that is not     */
-/*        counted holds (NaN included) reaches no other row and no gradient.                    */
+/*        counted holds (NaN included) reaches no other row and no gradient; its lse is there.  */
 /*   bwd: with q = exp(z - lse) - onehot(t) and coef = upstream[0] / counted rows (upstream:  */
 /*        device float, NULL = 1), dx = coef q w in dtype (overwritten) and dw = coef q^T x + */
 /*        beta_dw dw in dtype_dw (VEDA_F32, or VEDA_BF16 for bf16 operands; beta_dw 0 or 1).  */
-/*        lse is the forward's. dx or dw may be NULL. In bf16, q is rounded to bf16 before    */
-/*        the gradient products, as veda_cross_entropy's dlogits are (not where there are up  */
-/*        to four rows or few products, which run in fp32 without the tensor cores).          */
+/*        lse is the forward's; its rounding in fp32, 2^-24 of its size, is q's relative one. */
+/*        dx or dw may be NULL. In bf16, q is rounded to bf16 before the gradient products,   */
+/*        as veda_cross_entropy's dlogits are (not where there are up to four rows or few     */
+/*        products, which run in fp32 without the tensor cores).                              */
 /* Operands: any pitch >= dim and any element-aligned base; where a base is not 16-byte       */
 /* aligned or a pitch no multiple of 8 (bf16; always for fp32) an operand is laid out in the  */
 /* workspace first. The workspace (256-byte aligned, contents undefined before and after) is  */
@@ -347,7 +348,7 @@ int veda_adamw_step_dev(float* master, float* m, float* v, float* g, void* lowp,
  * not tiny to about 1; others must keep the singular values of X, and |a|, |b| + |c|, below 16.
  * bf16 matrices are multiplied in fp16 from an X held in two fp16 values (22 bits); fp32 ones, and most with a
  * side of at most 128, as pairs of fp16 values throughout. Row r, column c of matrix k is g[k stride_g + r ldg + c], any
- * alignment; out may be g. A zero matrix stays zero; a matrix that is not finite gives NaN in
+ * alignment; out may be g, of the same pitch and stride. A zero matrix stays zero; a matrix that is not finite gives NaN in
  * itself alone. The workspace (256-byte aligned, contents undefined before and after) is sized by
  * veda_orthogonalize_workspace (0 for an empty or refused shape). batch <= 2^15, rows and cols <=
  * 2^20. Results repeat bit for bit. They do not depend on the batch a matrix is in, unless its smaller side is

@@ -69,7 +69,9 @@ int veda_trainer_init_dp_sharded(veda_trainer* t, const void* unique_id128, int 
  * dir/model.safetensors holds the weights under the reference's parameter names
  * (Model.cpp:120-140) in the model's dtype; dir/optimizer.safetensors holds per parameter the fp32
  * master weights, first and second moments ("<name>.master", ".exp_avg", ".exp_avg_sq") and the
- * step count (metadata "step"). Loading restores all of it, so training resumes bit-exactly; a
+ * step count (metadata "step"; "muon" names the parameters whose first moment is a Muon's momentum: a trainer
+ * without Muon begins AdamW anew for them, at the "start" that later files give, and a sharded one refuses the
+ * file). Loading restores all of it, so training resumes bit-exactly; a
  * directory without optimizer.safetensors loads the weights and starts the optimizer afresh.
  * Data-parallel: rank 0 writes; with a sharded optimizer both calls are collective. */
 int veda_trainer_save_checkpoint(veda_trainer* t, const char* dir);
@@ -147,17 +149,18 @@ int veda_trainer_set_recompute_attention(veda_trainer* t, int on);
 
 /* on = 1: the LM head and its cross-entropy as one operator that never stores the [batch*seq_len,
  * vocab] logits or their gradient (veda_linear_cross_entropy_*); targets of -100 are then not counted
- * in the mean. Default off. */
+ * in the mean. Data-parallel, each rank takes the mean over its own counted targets and the ranks' gradients are
+ * averaged with equal weight: not the gradient of the joined batch where the ranks' counts differ. Default off. */
 int veda_trainer_set_linear_loss(veda_trainer* t, int on);
 /* Muon (veda_muon_step) for every layer's q/k/v/o and gate/up/down matrices from the next step on,
  * AdamW for the rest; the clip covers all of them. The update is scaled by 0.2 sqrt(max(rows, cols)),
- * so AdamW's learning rates carry over. Momentum is kept in the first moments, checkpoints included. Not
- * with a sharded optimizer. */
+ * so AdamW's learning rates carry over. Momentum is kept in the first moments, checkpoints included; called again,
+ * the numbers change and the momentum stays. Not with a sharded optimizer. */
 int veda_trainer_use_muon(veda_trainer* t, float lr, float momentum, int nesterov, float weight_decay,
                           int steps);
 
 /* Device-time profile of kernel classes (gemm_fwd, gemm_dx, gemm_dw, attn_fwd, attn_bwd,
- * cross_entropy, rmsnorm_bwd, swiglu_bwd, adamw), recorded with CUDA events while enabled. */
+ * cross_entropy, linear_ce_fwd, linear_ce_bwd, rmsnorm_bwd, swiglu_bwd, adamw, muon), recorded with CUDA events while enabled. */
 int veda_profile_enable(int on);
 /* Writes up to `cap` entries; returns the number of classes (synchronises; resets the totals). */
 int veda_profile_collect(char (*names)[32], double* ms, double* flops, double* bytes,

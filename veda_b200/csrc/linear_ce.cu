@@ -8,13 +8,15 @@
 //   forward   loss_n = lse_n - z_n[t_n], loss = mean over the counted rows. One pass over 256 x 256
 //             logit tiles in tensor memory; a thread owns a row and keeps the running maximum and
 //             the running sum of exponentials (fp32, log2 units) over a strip of tiles, so a row
-//             leaves (max, sum) pairs only, which a second launch merges. Bound by the products: bf16
-//             8192 x 151936 x 1024 1.47 ms, 1729 TFLOP/s, the epilogue under the next tile's products.
+//             leaves (max, sum) pairs only, which a second launch merges. Bound by the products, the
+//             epilogue under the next tile's: bf16 8192 x 151936 x 1024 1.50 ms (1700 TFLOP/s) called by
+//             itself at full clocks, 1.75 ms (1457) in runs, which the power cap holds at some 1400 MHz.
 //   backward  q = exp(z - lse) - onehot(t), formed piece by piece of the vocabulary from z computed
 //             again (the price of not keeping it), dx = coef q W, dW = coef q^T x with
 //             coef = upstream / counted rows. A piece of q stays in L2: the launch that multiplies
 //             piece c into dx and dW computes piece c + 1 beside it. Bound by the products too (three
-//             of them, one more than with stored logits): the same size 5.85 ms, 1307 TFLOP/s.
+//             of them, one more than with stored logits): the same size 5.8 to 6.2 ms called by itself,
+//             6.1 to 6.4 in runs (1260 to 1200 TFLOP/s); forward and backward 7.8 to 8.1 ms.
 // q is stored without coef, so its largest entry, about -1 at the target, keeps its bits when
 // rounded to bf16 whatever the row count; coef is applied to the fp32 sums. The sums over the
 // vocabulary (dx) are held in an fp32 buffer, added piece by piece in order: no atomics meet on an
@@ -27,7 +29,7 @@
 // bits), and a product becomes hi lo + lo hi + hi hi on 256 x 128 tiles
 // with three times the k-blocks (pair_mma.cuh); lo lo is below the 22nd bit. fp32 CUDA-core products run at a
 // twentieth of the tensor cores' rate, so three tensor products are still far cheaper: 1000 x 10007 x 320
-// takes 147 us, forward and backward.
+// takes 161 us, forward and backward.
 //
 // A few rows, which only stream the head, and small problems, which only wait for launches, are computed in fp32
 // on the CUDA cores (below), for either dtype.
@@ -1788,14 +1790,15 @@ int choose_strip(int num_m, int num_n, int clusters)
 int tile_width(int dtype) { return dtype == VEDA_F32 ? 128 : 256; }
 
 // Up to four rows of at most 2048 columns (a thread holds eight) go past the tensor cores. Against
-// 151936 x 1024, forward / backward: 1 row 51 / 143 us, 2 rows 52 / 167, 4 rows 66 / 231, 8 rows 101 / 359;
-// the tensor tiles take 98 / 288 for 9.
+// 151936 x 1024, forward / backward in runs: 1 row 53 / 128 us, 2 rows 53 / 151, 4 rows 67 / 213; the tensor tiles
+// take 86 / 225 for 9 (8 rows on the CUDA cores: 101 / 359).
 bool is_few(int64_t rows, int64_t dim) { return rows <= kFewRows && dim <= 2048; }
 
 // Problems whose products the CUDA cores finish within the latency of the tensor-core path's launches, which
 // is longer in fp32 and for odd widths (operands to lay out). Steps, here / tensor cores: bf16 16 x 1000 x 64
 // 18.7 / 25.3 us, 8 x 4000 x 64 38 / 26, 5 x 600 x 1000 43 / 33, 128 x 512 x 64 25.7 / 25.6; fp32 128 x 512 x 64
-// 23.3 / 34, 207 x 766 x 64 32.8 / 34.6, 500 x 500 x 64 42.5 / 36.5, 32 x 2000 x 256 39.0 / 37.8.
+// 23.3 / 34, 207 x 766 x 64 32.8 / 34.6, 500 x 500 x 64 42.5 / 36.5, 32 x 2000 x 256 39.0 / 37.8. (The tensor cores'
+// times are of launches that overlapped; apart, as they are now, they take some 5 us more.)
 bool is_small(int64_t rows, int64_t vocab, int64_t dim, int dtype)
 {
     if (rows > 1024 || vocab > 4096 || dim > 1024)

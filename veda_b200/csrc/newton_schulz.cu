@@ -8,7 +8,7 @@
 // matrix's step before it is stored, which a counter per matrix and step tells. With a few matrices the
 // next step of one runs beside the last tiles of another, so neither the last, partly filled wave of a
 // product nor its epilogue leaves SMs idle. As one launch per product, 28 x 1024 x 1024 took 870 us
-// against 760. A tall matrix is multiplied from the other side (S = X^T X, X <- X M) by operand
+// against 760, both in short runs at full clocks (long ones, under the power cap: 850). A tall matrix is multiplied from the other side (S = X^T X, X <- X M) by operand
 // order alone, so nothing is transposed. S and M are symmetric: the tiles on and above the diagonal are
 // computed, and each one above it is written a second time, transposed.
 //
@@ -1843,7 +1843,7 @@ int iterate(const char* what, const Source& src, int64_t batch, int64_t rows, in
     // Narrow tiles (256 x 128) have half the latency and one and a half times the operand traffic a flop:
     // they win while the wide ones of X leave the 74 CTA pairs at most about one and a half each (1024 x
     // 1024: 136 against 176 us; 8 x 500 x 1500, 96 wide tiles: 362 against 457; 2048 x 4096, 128: 420
-    // against 414; 28 x 1024 x 1024, 448: 992 against 843). Split products take them always: with wide
+    // against 414; 28 x 1024 x 1024, 448: 992 against 843, both under the power cap). Split products take them always: with wide
     // tiles their folds are not overlapped.
     if constexpr (!SPLIT)
     {

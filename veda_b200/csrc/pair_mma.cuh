@@ -14,10 +14,10 @@
 // of products for k = 1024), and a k-block costs the loading thread additions only.
 //
 // SPLIT: operands are pairs of fp16 planes, value = hi + lo, and a product is hi lo + lo hi + hi hi.
-// The tensor core truncates as it adds into its accumulator, an error of some 2^-25 of the running
-// sum per 16 terms and always towards zero: sums of 10000 terms came out 3e-5 short. So the small
-// products go first, and every CHAIN k-blocks the accumulator is folded into a running sum kept in
-// another part of TMEM, rounded to nearest (some 3e-7 of the sum remain for chains of 4 k-blocks). With
+// The tensor core truncates as it adds into its accumulator, always towards zero: sums of 10000 terms came out 3e-5
+// short. So the small products go first, and every CHAIN k-blocks the accumulator is folded into a running sum kept
+// in another part of TMEM, rounded to nearest: where all terms have one sign, 1.5e-6 of the sum are missing with
+// chains of 4 k-blocks, whatever its length, and 3.2e-6 with chains of 8. With
 // TN = 128 two accumulators and the sum fit, and a fold runs under the next chain's products; with TN = 256
 // the accumulator has no second buffer then, and the products wait for it.
 //
