@@ -54,8 +54,9 @@ public:
     // First and second moments of every parameter, fp32, back to back in parameter order.
     const core::Tensor& first_moments() const noexcept { return m_arena_; }
     const core::Tensor& second_moments() const noexcept { return v_arena_; }
-    // Restores the step count (the bias corrections of the next step use steps + 1).
-    void set_steps(size_t steps) noexcept { steps_ = steps; }
+    // Restores the step count (the bias corrections of the next step use steps + 1, or what has been made since a
+    // restart(), which lies no later than the count).
+    void set_steps(size_t steps);
     // Steps that had been made when the moments of parameter i began: its bias corrections count from
     // there. 0 but for parameters that restart() was called for.
     size_t start(size_t i) const { return starts_.at(i); }

@@ -149,10 +149,41 @@ void run(const std::string& name, DType type)
     report(name + "_others_are_still_not_touched",
            a.value().to_host() == a2.value().to_host() && c.value().to_host() == c2.value().to_host());
 }
+
+// A step count set back to before the hand-back counts from there.
+void counted_back()
+{
+    const optim::AdamWConfig config{0.01f, 0.9f, 0.999f, 1e-8f, 0.1f};
+    Variable a = Variable::leaf(matrix(5, DType::F32));
+    optim::AdamW adam({a}, config);
+    {
+        optim::Muon muon(adam, {0});
+        for (uint32_t k = 0; k < 5; ++k)
+        {
+            fill(a, 300 + k);
+            adam.step();
+            muon.step();
+        }
+    }
+    report("starts_at_the_hand_back", adam.start(0) == 5 && !adam.taken(0));
+    adam.set_steps(2);
+    report("start_follows_the_count", adam.start(0) == 2 && adam.steps() == 2);
+    Variable b = Variable::leaf(core::contiguous(a.value()));
+    optim::AdamW anew({b}, config);
+    for (uint32_t k = 0; k < 6; ++k)
+    {
+        fill(a, 400 + k);
+        fill(b, 400 + k);
+        adam.step();
+        anew.step();
+    }
+    report("goes_on_from_the_count", a.value().to_host() == b.value().to_host());
+}
 } // namespace
 
 int main()
 {
+    counted_back();
     run("f32", DType::F32);
     run("bf16", DType::BF16);
     std::printf("%d failures\n", failures);

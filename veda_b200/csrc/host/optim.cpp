@@ -189,7 +189,7 @@ void AdamW::upload_bias()
 {
     for (size_t k = 0; k < bias_starts_.size(); ++k)
     {
-        // a count set back to before the start has the first step's corrections
+        // before the first step there is nothing to correct
         const double t = static_cast<double>(steps_ > bias_starts_[k] ? steps_ - bias_starts_[k] : 1);
         bias_host_[2 * k] = 1.0 - std::pow(static_cast<double>(config_.beta1), t);
         bias_host_[2 * k + 1] = 1.0 - std::pow(static_cast<double>(config_.beta2), t);
@@ -199,6 +199,21 @@ void AdamW::upload_bias()
                         cs()) != cudaSuccess)
     {
         throw std::runtime_error("AdamW: bias correction upload failed");
+    }
+}
+
+void AdamW::set_steps(size_t steps)
+{
+    steps_ = steps;
+    bool changed = false;
+    for (size_t& start : starts_)
+    {
+        changed = changed || start > steps;
+        start = std::min(start, steps);
+    }
+    if (changed)
+    {
+        build_updates();
     }
 }
 

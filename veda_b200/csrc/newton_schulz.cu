@@ -1612,6 +1612,8 @@ bool is_small(int64_t rows, int64_t cols)
     return std::min(rows, cols) <= kSmallSide && std::max(rows, cols) <= kMaxRanks * kSmallLong;
 }
 
+// A block of the small form takes all of an SM's registers (512 threads of more than 120), so no other kernel's blocks
+// run beside the allocation of its tensor memory, though its launches overlap.
 // Launches the small form; `*taken` stays false where the tiled form is faster, or the device cannot hold a
 // cluster of that many blocks.
 template <typename T, bool MUON>
