@@ -194,6 +194,10 @@ def run_reference(args):
     rank = int(os.environ.get("RANK", "0"))
     if rank != 0:
         return 0
+    from oracle import ref as R
+    if not R.available():
+        emit({"impl": "reference", "unavailable": "oracle/_ref/libveda_ref.so is not built"})
+        return 0
     c, B, T, _ = WORKLOADS[args.workload]
     threads = os.cpu_count() or 1
     vals, desc, spent = [], "", 0.0
